@@ -44,6 +44,36 @@ class ModelInfo(C.Structure):
     ]
 
 
+_u32, _u64 = C.c_uint32, C.c_uint64
+
+
+class PagePlanArgs(C.Structure):
+    _fields_ = [(n, _u64) for n in ("lens", "news", "free_pages", "table", "depths", "starts",
+                                    "positions", "slots", "owners", "used")] + \
+               [(n, _u32) for n in ("n_req", "page_size", "max_pages", "n_free", "max_tokens")]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", _u32), ("trained", _u32), ("factor", C.c_float), ("low", C.c_float),
+                ("high", C.c_float), ("amplitude", C.c_float)]
+
+
+class RopeAppendArgs(C.Structure):
+    _fields_ = [(n, _u64) for n in ("plan", "positions", "q", "k", "v", "slots", "q_out",
+                                    "k_cache", "v_cache", "q_off", "k_off", "v_off", "q_stride",
+                                    "k_stride", "v_stride")] + \
+               [(n, _u32) for n in ("type", "layout", "n_tokens", "n_heads", "n_kv", "head_dim",
+                                    "page_size", "n_pages")]
+
+
+class TreeAttnArgs(C.Structure):
+    _fields_ = [(n, _u64) for n in ("q", "k_cache", "v_cache", "table", "lens", "starts", "mask",
+                                    "positions", "out", "q_off", "q_stride")] + \
+               [(n, _u32) for n in ("type", "n_req", "n_rows", "max_nodes", "n_heads", "n_kv",
+                                    "head_dim", "page_size", "n_pages", "max_pages", "window")] + \
+               [("scale", C.c_float), ("softcap", C.c_float)]
+
+
 _vp = C.c_void_p
 _sz = C.c_size_t
 _buf = C.c_uint64
@@ -55,6 +85,7 @@ SIGNATURES = {
     "cw_last_error": [],
     "cw_abi_version": [],
     "cw_ctx_create": [C.c_int, C.POINTER(_vp)],
+    "cw_ctx_create_on_stream": [C.c_int, _vp, C.POINTER(_vp)],
     "cw_ctx_destroy": [_vp],
     "cw_ctx_backend": [_vp, C.c_char_p, _sz],
     "cw_ctx_device": [_vp, C.POINTER(C.c_int)],
@@ -65,6 +96,7 @@ SIGNATURES = {
     "cw_storage_bytes": [_vp, _vp, _sz, _pbuf],
     "cw_empty": [_vp, _sz, _pbuf],
     "cw_empty_persistent": [_vp, _sz, _pbuf],
+    "cw_buf_wrap": [_vp, _vp, _sz, _pbuf],
     "cw_buf_release": [_vp, _buf],
     "cw_buf_nbytes": [_vp, _buf, C.POINTER(_sz)],
     "cw_buf_device_ptr": [_vp, _buf, C.POINTER(_vp)],
@@ -103,6 +135,10 @@ SIGNATURES = {
     "cw_q8_0_gemv": [_vp, _buf, _buf, _sz, _sz, _pbuf],
     "cw_q4_0_gemv_bench": [_vp, _buf, C.POINTER(C.c_uint64), _sz, _sz, _sz, _sz,
                            C.POINTER(C.c_double)],
+    "cw_page_plan": [_vp, C.POINTER(PagePlanArgs)],
+    "cw_rope_plan": [_vp, _sz, C.c_double, C.POINTER(RopeScaling), _pbuf],
+    "cw_rope_append": [_vp, C.POINTER(RopeAppendArgs)],
+    "cw_tree_attention": [_vp, C.POINTER(TreeAttnArgs)],
     "cw_model_load_gguf": [_vp, C.c_char_p, C.POINTER(_vp)],
     "cw_model_free": [_vp],
     "cw_model_get_info": [_vp, C.POINTER(ModelInfo)],
@@ -173,11 +209,15 @@ def load(path: str | None = None):
 
 def call(name: str, *args) -> None:
     """Call `name` and raise CwError on a non-zero status."""
-    L = load()
-    rc = getattr(L, name)(*args)
+    rc = getattr(load(), name)(*args)
     if rc != CW_OK:
-        msg = L.cw_last_error()
-        raise CwError(rc, name, msg.decode(errors="replace") if msg else "")
+        fail(rc, name)
+
+
+def fail(rc: int, name: str) -> None:
+    """Raise the CwError of a call that returned `rc`."""
+    msg = load().cw_last_error()
+    raise CwError(rc, name, msg.decode(errors="replace") if msg else "")
 
 
 def exported_symbols() -> list[str]:

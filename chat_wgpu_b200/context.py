@@ -20,11 +20,12 @@ from . import _lib
 class Buffer:
     """A device buffer handle (the analogue of wgpu::Buffer)."""
 
-    __slots__ = ("ctx", "handle")
+    __slots__ = ("ctx", "handle", "owner")
 
-    def __init__(self, ctx: "GpuContext", handle: int):
+    def __init__(self, ctx: "GpuContext", handle: int, owner=None):
         self.ctx = ctx
         self.handle = int(handle)
+        self.owner = owner  # what keeps a wrapped buffer's memory alive
 
     @property
     def nbytes(self) -> int:
@@ -50,12 +51,17 @@ def _np(a, dtype) -> np.ndarray:
 
 
 class GpuContext:
-    """GpuContext::new (context.rs:60-104) on CUDA device `device`."""
+    """GpuContext::new (context.rs:60-104) on CUDA device `device`.  With
+    `stream` (a cudaStream_t as an int, 0 = the legacy default stream) ops are
+    enqueued on the caller's stream instead of one of the context's own."""
 
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream: int | None = None):
         _lib.load()
         h = C.c_void_p()
-        _lib.call("cw_ctx_create", int(device), C.byref(h))
+        if stream is None:
+            _lib.call("cw_ctx_create", int(device), C.byref(h))
+        else:
+            _lib.call("cw_ctx_create_on_stream", int(device), int(stream), C.byref(h))
         self._h = h
         # models (and through them sessions) made on this context: released
         # before the context itself, whatever order Python drops them in
@@ -120,6 +126,20 @@ class GpuContext:
     def empty_persistent(self, length: int) -> Buffer:
         """GpuContext::empty_persistent (context.rs:229-232), zero-filled."""
         return self._new("cw_empty_persistent", int(length))
+
+    def wrap(self, tensor) -> Buffer:
+        """A device tensor of another library as a buffer, without a copy: any
+        object with data_ptr(), element_size(), shape and stride() (a torch
+        tensor on the context's device).  The buffer reaches from the tensor's
+        first element to its last, whatever its strides, and keeps the tensor
+        alive; its address must be 16-byte aligned."""
+        n = 0
+        if all(int(d) > 0 for d in tensor.shape):
+            n = 1 + sum((int(d) - 1) * int(st) for d, st in zip(tensor.shape, tensor.stride()))
+        b = C.c_uint64()
+        _lib.call("cw_buf_wrap", self._h, int(tensor.data_ptr()), n * int(tensor.element_size()),
+                  C.byref(b))
+        return Buffer(self, b.value, tensor)
 
     def copy(self, src: Buffer, src_off: int, dst: Buffer, dst_off: int, length: int) -> None:
         """GpuContext::copy (context.rs:252-269); offsets/length in f32 elements."""

@@ -49,7 +49,8 @@ void clear_error();
 // Device-side status word written by bounded waits (never a trap).
 enum DeviceStatus : int { DEV_OK = 0, DEV_TIMEOUT = 1, DEV_BAD_INPUT = 2 };
 
-enum BufKind : int { BUF_STORAGE = 0, BUF_PERSISTENT = 1, BUF_ARENA = 2 };
+// BUF_WRAPPED: memory of the caller (cw_buf_wrap), never freed here.
+enum BufKind : int { BUF_STORAGE = 0, BUF_PERSISTENT = 1, BUF_ARENA = 2, BUF_WRAPPED = 3 };
 
 struct BufEntry {
     void* ptr = nullptr;
@@ -65,6 +66,10 @@ struct BufEntry {
     // Set for a Q8_0 weight split for the streaming GEMV (cw_q8_0_split):
     // [rows][in_f/32][32] codes, f16 scale plane at scale_off.
     bool q8_split = false;
+    // Set for a rotary plan (cw_rope_plan): [rope_dim/2] u64 turns per position
+    // as a fraction of 2^64; cos and sin are scaled by rope_amp.
+    uint32_t rope_dim = 0;
+    float rope_amp = 1.f;
 };
 
 struct ProfRec {
@@ -77,6 +82,7 @@ struct ProfRec {
 struct cw_ctx {
     int device = 0;
     cudaStream_t stream = nullptr;
+    bool own_stream = true;  // false: the caller's (cw_ctx_create_on_stream)
     int sm_count = 0;
     int clock_khz = 1;  // max SM clock (profile cycle conversion)
     int max_smem_optin = 0;
@@ -110,6 +116,10 @@ struct cw_ctx {
     // grow-only scratch of the prefill GEMM op (split f16 operands)
     void* gemm_scratch = nullptr;
     size_t gemm_scratch_bytes = 0;
+
+    // grow-only scratch of the tree attention (partial states of split keys)
+    void* tree_scratch = nullptr;
+    size_t tree_scratch_bytes = 0;
 };
 
 namespace cw {

@@ -193,7 +193,7 @@ const char* cw_last_error(void) { return g_err.c_str(); }
 
 int cw_abi_version(void) { return CW_ABI_VERSION; }
 
-int cw_ctx_create(int device, cw_ctx** out) {
+static int ctx_create(int device, cudaStream_t stream, bool own, cw_ctx** out) {
     clear_error();
     CW_CHECK(out, CW_ERR_INVALID_ARG, "cw_ctx_create: out is NULL");
     *out = nullptr;
@@ -221,7 +221,11 @@ int cw_ctx_create(int device, cw_ctx** out) {
     char b[320];
     snprintf(b, sizeof b, "CUDA sm_%d%da (%s)", prop.major, prop.minor, prop.name);
     c->backend = b;
-    cudaError_t e1 = cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking);
+    c->own_stream = own;
+    c->stream = stream;
+    cudaError_t e1 = own ? cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking)
+                         : cudaStreamQuery(stream);
+    if (e1 == cudaErrorNotReady) e1 = cudaSuccess;
     cudaError_t e2 = cudaMalloc(&c->d_status, sizeof(int));
     if (e1 != cudaSuccess || e2 != cudaSuccess) {
         delete c;
@@ -238,11 +242,18 @@ int cw_ctx_create(int device, cw_ctx** out) {
     return CW_OK;
 }
 
+int cw_ctx_create(int device, cw_ctx** out) { return ctx_create(device, nullptr, true, out); }
+
+int cw_ctx_create_on_stream(int device, void* stream, cw_ctx** out) {
+    return ctx_create(device, (cudaStream_t)stream, false, out);
+}
+
 int cw_ctx_destroy(cw_ctx* ctx) {
     if (!ctx) return CW_OK;
     cudaSetDevice(ctx->device);
-    if (ctx->stream) cudaStreamSynchronize(ctx->stream);
-    for (auto& kv : ctx->bufs) cudaFree(kv.second.ptr);
+    if (ctx->stream || !ctx->own_stream) cudaStreamSynchronize(ctx->stream);
+    for (auto& kv : ctx->bufs)
+        if (kv.second.kind != BUF_WRAPPED) cudaFree(kv.second.ptr);
     for (auto& kv : ctx->rope_tables) cudaFree(kv.second);
     for (auto& p : ctx->prof) {
         cudaEventDestroy(p.start);
@@ -252,7 +263,8 @@ int cw_ctx_destroy(cw_ctx* ctx) {
     if (ctx->d_status) cudaFree(ctx->d_status);
     if (ctx->d_counters) cudaFree(ctx->d_counters);
     if (ctx->gemm_scratch) cudaFree(ctx->gemm_scratch);
-    if (ctx->stream) cudaStreamDestroy(ctx->stream);
+    if (ctx->tree_scratch) cudaFree(ctx->tree_scratch);
+    if (ctx->stream && ctx->own_stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
     return CW_OK;
 }
@@ -326,6 +338,31 @@ int cw_empty_persistent(cw_ctx* ctx, size_t len, cw_buf* out) {
     return CW_OK;
 }
 
+int cw_buf_wrap(cw_ctx* ctx, void* dptr, size_t nbytes, cw_buf* out) {
+    clear_error();
+    CW_CHECK(ctx && out && dptr, CW_ERR_INVALID_ARG, "cw_buf_wrap: bad arguments");
+    CW_CHECK(((uintptr_t)dptr & 15) == 0, CW_ERR_INVALID_ARG,
+             "cw_buf_wrap: the address must be 16-byte aligned");
+    cudaSetDevice(ctx->device);
+    cudaPointerAttributes at;
+    CW_CUDA(cudaPointerGetAttributes(&at, dptr));
+    CW_CHECK((at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged) &&
+                 at.device == ctx->device,
+             CW_ERR_INVALID_ARG, "cw_buf_wrap: not memory of device %d", ctx->device);
+    BufEntry e;
+    e.ptr = dptr;
+    e.nbytes = nbytes;
+    e.kind = BUF_WRAPPED;
+    const uint64_t id = ctx->next_id++;
+    try {
+        ctx->bufs[id] = e;
+    } catch (...) {
+        return set_error(CW_ERR_OOM, "cw_buf_wrap: out of host memory");
+    }
+    *out = id;
+    return CW_OK;
+}
+
 int cw_buf_release(cw_ctx* ctx, cw_buf buf) {
     clear_error();
     CW_CHECK(ctx, CW_ERR_INVALID_ARG, "cw_buf_release: ctx is NULL");
@@ -333,9 +370,11 @@ int cw_buf_release(cw_ctx* ctx, cw_buf buf) {
     CW_TRY(buf_get(ctx, buf, &e, 0, "cw_buf_release"));
     CW_CHECK(e->kind != BUF_ARENA, CW_ERR_INVALID_ARG,
              "cw_buf_release: arena buffers belong to the context");
-    cudaSetDevice(ctx->device);
-    CW_CUDA(cudaStreamSynchronize(ctx->stream));
-    cudaFree(e->ptr);
+    if (e->kind != BUF_WRAPPED) {
+        cudaSetDevice(ctx->device);
+        CW_CUDA(cudaStreamSynchronize(ctx->stream));
+        cudaFree(e->ptr);
+    }
     ctx->bufs.erase(buf);
     return CW_OK;
 }

@@ -2,4 +2,4 @@
 src/kernels/ (q4, attention, norm, rope, activation, argmax).  Each function
 takes a GpuContext plus buffers and dimensions and returns a new arena
 buffer, like its Rust counterpart."""
-from . import activation, argmax, attention, norm, q4, rope  # noqa: F401
+from . import activation, argmax, attention, norm, pages, q4, rope, tree  # noqa: F401

@@ -66,6 +66,12 @@ int cw_abi_version(void);
  * non-blocking stream.  Fails with CW_ERR_NO_DEVICE if the device is not an
  * sm_100 part. */
 int cw_ctx_create(int device, cw_ctx** out);
+/* The same context on the caller's stream (a cudaStream_t of that device; NULL
+ * = the legacy default stream) instead of one of its own: ops are ordered with
+ * the caller's other work there, and the caller keeps the stream alive until
+ * the context is destroyed.  Sessions capture their steps as CUDA graphs,
+ * which CUDA does not allow on the legacy default stream. */
+int cw_ctx_create_on_stream(int device, void* stream, cw_ctx** out);
 int cw_ctx_destroy(cw_ctx* ctx);
 /* GpuContext.backend (context.rs:28,70): e.g. "CUDA sm_100a (NVIDIA B200)". */
 int cw_ctx_backend(cw_ctx* ctx, char* buf, size_t cap);
@@ -89,6 +95,12 @@ int cw_storage_bytes(cw_ctx* ctx, const void* data, size_t nbytes, cw_buf* out);
 int cw_empty(cw_ctx* ctx, size_t len, cw_buf* out);
 /* GpuContext::empty_persistent (context.rs:229-232): never recycled. */
 int cw_empty_persistent(cw_ctx* ctx, size_t len, cw_buf* out);
+/* Register device memory that the caller owns (another library's tensor) as a
+ * buffer: nbytes at dptr, memory of the context's device, 16-byte aligned.  As
+ * in the library's own buffers, vector loads may touch (never use) the bytes up
+ * to the next multiple of 256.  The caller keeps the memory until the buffer is
+ * released and every op on it has run; cw_buf_release forgets it. */
+int cw_buf_wrap(cw_ctx* ctx, void* dptr, size_t nbytes, cw_buf* out);
 /* Drop a storage / persistent buffer (wgpu frees on Drop).  Arena buffers
  * are owned by the context and are rejected here. */
 int cw_buf_release(cw_ctx* ctx, cw_buf buf);
@@ -264,6 +276,122 @@ int cw_q6_k_gemv(cw_ctx* ctx, cw_buf x, cw_buf w, size_t in_f, size_t out_f, cw_
  * relative of the f32 dequantised product). */
 int cw_q8_0_split(cw_ctx* ctx, cw_buf w, size_t rows, size_t in_f, cw_buf* out);
 int cw_q8_0_gemv(cw_ctx* ctx, cw_buf x, cw_buf w, size_t in_f, size_t out_f, cw_buf* out);
+
+/* ---- drafted tokens over a paged cache -------------------------------------
+ * No counterpart in the reference, whose cache is one contiguous row per
+ * position and whose step is one query.  A server that verifies several drafted
+ * tokens of several requests in one step calls, in this order:
+ *   cw_page_plan       pages, slots and positions of the step's tokens
+ *   cw_rope_append     (per layer) rotate q and k, write k and v to their slots
+ *   cw_tree_attention  (per layer) every drafted node attends its request's
+ *                      cached tokens and its own ancestors
+ * A request r has lens[r] cached tokens and news[r] new ones, its nodes; token
+ * rows are ragged, request r owning rows [starts[r], starts[r+1]).  The cache of
+ * a layer is two buffers [n_pages][n_kv][page_size][head_dim] of one type (f32,
+ * f16 or bf16: CW_GGUF_F32, CW_GGUF_F16, CW_GGUF_BF16), each page holding
+ * page_size consecutive positions of one request; table[r][i] is the page of its
+ * positions [i*page_size, (i+1)*page_size).  The node i of request r is stored
+ * at position lens[r] + i whatever its depth; a caller that accepts a path
+ * feeds the accepted tokens again as the first nodes of the next step and adds
+ * to lens only what is then stored in order.
+ *
+ * Arguments come as a struct, so a program fills it once per buffer set and
+ * calls with it every step.  Every cw_buf is a whole buffer; *_off and *_stride
+ * count elements.  Index buffers are i32.  Lengths, page ids and slots are
+ * device data: a value out of range is never followed out of a buffer; it is
+ * skipped and reported by the next synchronising call as CW_ERR_INVALID_ARG
+ * unless the entry says otherwise. */
+typedef struct {
+    cw_buf lens;        /* [n_req] cached tokens (negative counts as 0)            */
+    cw_buf news;        /* [n_req] new tokens (negative counts as 0)               */
+    cw_buf free_pages;  /* [n_free] ids of free pages, taken from the front        */
+    cw_buf table;       /* [n_req][max_pages], updated in place                    */
+    cw_buf depths;      /* [max_tokens] depth of each token row in its tree, or 0  */
+    cw_buf starts;      /* out [n_req + 1] first token row of each request         */
+    cw_buf positions;   /* out [max_tokens] lens + depth (no depths: lens + index) */
+    cw_buf slots;       /* out [max_tokens] page * page_size + offset, or -1       */
+    cw_buf owners;      /* out [max_tokens] request of each row, or -1             */
+    cw_buf used;        /* out [1] pages taken (more than n_free: that many lack)  */
+    uint32_t n_req, page_size, max_pages, n_free, max_tokens;
+} cw_page_plan_args;
+/* Block tables and slots of one step from the request lengths, on the device.
+ * Request r needs pages ceil(lens/page_size) .. ceil((lens+news)/page_size);
+ * these are given out in request order and written to its table row.  Rows past
+ * the last token get position 0, slot -1, owner -1.  A token without a page
+ * (the free list ran out, the table row is full, the table holds a negative id)
+ * gets slot -1 and is no error: compare used with n_free.  n_req <= 16384. */
+int cw_page_plan(cw_ctx* ctx, const cw_page_plan_args* args);
+
+/* Rotary frequencies of rot_dim / 2 pairs with base theta, stretched for
+ * contexts longer than the trained one.  The rate of pair i is
+ * f_i = theta^(-2i/rot_dim) radians per position, then
+ *   LINEAR  f / factor
+ *   BANDED  pairs turning more than `high` times within `trained` positions keep
+ *           f, fewer than `low` times take f / factor, linear in the turns between
+ *   YARN    the same between the pair indices that turn `high` and `low` times,
+ *           linear in the index; cos and sin times `amplitude`, or with
+ *           amplitude 0 times 0.1 ln(factor) + 1 */
+#define CW_ROPE_PLAIN 0
+#define CW_ROPE_LINEAR 1
+#define CW_ROPE_BANDED 2
+#define CW_ROPE_YARN 3
+typedef struct {
+    uint32_t kind, trained;
+    float factor, low, high, amplitude;
+} cw_rope_scaling;
+/* scaling may be NULL (CW_ROPE_PLAIN).  *plan is a persistent buffer: the turns
+ * per position of each pair as 64-bit fixed point, so that position times rate
+ * is reduced modulo a turn exactly at any position. */
+int cw_rope_plan(cw_ctx* ctx, size_t rot_dim, double theta, const cw_rope_scaling* scaling,
+                 cw_buf* plan);
+#define CW_ROPE_HALF 0         /* pair i = elements i and i + rot_dim/2 */
+#define CW_ROPE_INTERLEAVED 1  /* pair i = elements 2i and 2i + 1       */
+typedef struct {
+    cw_buf plan, positions;        /* positions [n_tokens]                           */
+    cw_buf q, k, v;                /* rows of n_heads / n_kv / n_kv heads            */
+    cw_buf slots;                  /* [n_tokens]; -1: k and v of the row not written */
+    cw_buf q_out;                  /* [n_tokens][n_heads * head_dim]                 */
+    cw_buf k_cache, v_cache;       /* [n_pages][n_kv][page_size][head_dim]           */
+    uint64_t q_off, k_off, v_off;  /* first element of row 0 in its buffer           */
+    uint64_t q_stride, k_stride, v_stride; /* elements from row to row               */
+    uint32_t type, layout, n_tokens, n_heads, n_kv, head_dim, page_size, n_pages;
+} cw_rope_append_args;
+/* q_out = rotated q; the cache rows of the slots = rotated k, and v.  All of one
+ * type, rotated in f32 and rounded once.  The plan's rot_dim <= head_dim: later
+ * elements pass through.  n_heads = 0 leaves q out, n_kv = 0 k, v and the cache
+ * (their buffers may be 0).  q_out may be q itself where q's rows are contiguous.
+ * Rows whose slots are equal are written in no particular order. */
+int cw_rope_append(cw_ctx* ctx, const cw_rope_append_args* args);
+
+typedef struct {
+    cw_buf q;                  /* [n_rows] rows of n_heads * head_dim                  */
+    cw_buf k_cache, v_cache;   /* [n_pages][n_kv][page_size][head_dim]                 */
+    cw_buf table;              /* [n_req][max_pages]                                   */
+    cw_buf lens;               /* [n_req] cached tokens before the nodes               */
+    cw_buf starts;             /* [n_req + 1]                                          */
+    cw_buf mask;               /* [n_rows][mask_words] bit j: the row sees node j of its
+                                  request (itself among them); 0: node i sees j <= i   */
+    cw_buf positions;          /* [n_rows], at least lens; used with a window only     */
+    cw_buf out;                /* [n_rows][n_heads * head_dim]                         */
+    uint64_t q_off, q_stride;  /* elements                                             */
+    uint32_t type, n_req, n_rows, max_nodes, n_heads, n_kv, head_dim, page_size, n_pages,
+        max_pages, window;
+    float scale, softcap;      /* scale 0: head_dim^-0.5; softcap 0: none              */
+} cw_tree_attn_args;
+/* out = softmax(cap(scale * q . k) over the keys a row sees) v.  A row sees every
+ * cached token of its request and the nodes of its mask; with a window only keys
+ * whose position is less than `window` before its own.  A row that sees nothing
+ * gives zeros; what a row does not see does not reach it, non-finite values
+ * included.  mask_words is ceil(max_nodes / 32); a request has at most max_nodes
+ * (<= 1024) nodes.  Query head h reads kv head h / (n_heads / n_kv); head_dim <=
+ * 256.  Rows of out past starts[n_req] keep their contents.  q, cache and out are
+ * of one type; sums and the softmax are f32.  16-bit types with head_dim a
+ * multiple of 8 and page_size 8, 16, 32 or a multiple of 64 run on the tcgen05
+ * tensor cores (there the softmax weights are rounded to the type before the
+ * product with v), everything else on warp-level tensor-core products at f32
+ * accuracy.  Uses a context-owned scratch that grows on demand, which
+ * synchronises. */
+int cw_tree_attention(cw_ctx* ctx, const cw_tree_attn_args* args);
 
 /* ---- model: src/model/{mod,qwen3,layers,cache}.rs --------------------------------------------- */
 typedef struct {
