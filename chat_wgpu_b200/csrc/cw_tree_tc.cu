@@ -1,8 +1,668 @@
-// cw_tree_tc.cu -- the tcgen05 kernel of cw_tree_attention takes no shape yet.
+// cw_tree_tc.cu -- cw_tree_attention over 16-bit caches on the 5th-generation
+// tensor cores (tcgen05, operands staged by TMA, accumulators in TMEM).
+//
+// Per 64-key tile and 128 query rows (one TMEM lane a row):
+//
+//   S [128 x 64]  = Q K^T   both from shared memory (128-byte swizzled)
+//   P [128 x 64]  = 2^(c S - ref), rounded to the type, over S's own columns
+//   O [128 x D]  += P V     P from TMEM, V as it lies in memory (keys x dims)
+//
+// The cache is read once: all G query heads of a kv head and all nodes of the
+// request share a tile (up to 128 rows, or 256 with two row blocks per CTA).  A
+// tile of 64 keys at D = 128 is 32 KB and takes an SM's share of the memory
+// bandwidth 0.75 us; its two products with all 128 rows take about 0.15 us of
+// tensor time and its exponentials 0.3 us, so the kernel is bound by memory up to
+// those rows and padding short row blocks costs nothing.
+//
+// Warps: 4 (or 2 x 4) softmax warps, a thread per row, so row maxima and sums need
+// no exchange; one TMA warp; one MMA thread.  S has two TMEM buffers: the scores of
+// tile i + 1 are formed while the weights of tile i are.  O is rescaled only when a
+// row's maximum has grown by 2^8 since its last reference (weights then stay below
+// 256, far inside both types); the final division makes the reference drop out.
+// Weights are rounded to the cache's type for the second product; the row's sum is
+// taken over the rounded weights, so a constant v comes out exact.
+//
+// Keys that not every row sees lie in the tiles of the nodes, the last tile and,
+// with a window, those at its edge.  There each thread forms its row's 64-bit set
+// of seen keys, v rows past the end are zeroed, and a tile whose v holds values
+// that are not finite is mended: those values are taken out of the product and
+// added to the rows that see them.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "cw_gemm.cuh"
 #include "cw_tree.cuh"
+
 namespace cw {
-bool tree_tc_takes(const cw_tree_attn_args&, const void*, const void*, const void*) { return false; }
-int tree_tc_rows(const TreeArgs&) { return 128; }
-int tree_tc_grid(cw_ctx*, const TreeArgs&) { return 1; }
-int tree_tc_launch(cw_ctx*, const TreeArgs&, uint32_t, int) { return CW_ERR_UNSUPPORTED; }
+
+constexpr int TT_STAGES = 16;  // most stages of the ring (one K or V tile each)
+constexpr uint64_t TT_WAIT_NS = 2000000000ull;
+
+// A parity wait tells a phase from the one before it only, so a barrier that is
+// waited on once per tile is doubled by tile parity: when tile n - 1's phase is
+// waited for, tile n - 3's is known to be over (scores of tile n - 1 come after it).
+struct TtBars {
+    uint64_t full[TT_STAGES], empty[TT_STAGES];
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], pv[2][2], done;  // [row block][tile % 2]
+    uint32_t tmem, failed;
+};
+
+__device__ __forceinline__ void tt_ld32(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+        "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
 }
+__device__ __forceinline__ void tt_st32(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+        "%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// Waits for this thread's TMEM loads; the values pass through, so no use of them can
+// be moved before it.
+__device__ __forceinline__ void tt_wait_ld32(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]),
+                   "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ uint32_t tt_ld1(uint32_t addr) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ void tt_st1(uint32_t addr, uint32_t r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(addr), "r"(r)
+                 : "memory");
+}
+__device__ __forceinline__ void tt_wait_st() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tt_fence_async() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+// D[tmem] += A[tmem] B[shared]
+__device__ __forceinline__ void tt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc)
+        : "memory");
+}
+// Matrix descriptor of an operand whose contraction index is the row (V: keys x
+// dims) in 128-byte swizzled 64-element columns: column blocks `block` bytes apart,
+// 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t tt_desc_rows(uint32_t saddr, uint32_t block) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(block >> 4) << 16) |
+           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+template <bool BF> __host__ __device__ constexpr uint32_t tt_idesc(int n, bool b_rows) {
+    return (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | (b_rows ? 1u << 16 : 0u) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ float tt_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// Two weights rounded and packed (first in the low half), their rounded values added.
+template <bool BF> __device__ __forceinline__ uint32_t tt_pack(float x, float y, float& sum) {
+    uint32_t r;
+    if (BF) {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+        sum += __uint_as_float(r << 16) + __uint_as_float(r & 0xffff0000u);
+    } else {
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+        const float2 f = __half22float2(*(const __half2*)&r);
+        sum += f.x + f.y;
+    }
+    return r;
+}
+template <bool BF> __device__ __forceinline__ float tt_value(uint32_t bits16) {
+    if (BF) return __uint_as_float(bits16 << 16);
+    return __half2float(__ushort_as_half((unsigned short)bits16));
+}
+template <bool BF> __device__ __forceinline__ bool tt_odd(uint32_t bits16) {
+    const uint32_t e = BF ? 0x7f80u : 0x7c00u;
+    return (bits16 & e) == e;
+}
+template <bool BF> __device__ __forceinline__ bool tt_odd8(const uint4& x) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) odd |= tt_odd<BF>(w[i] & 0xffffu) | tt_odd<BF>(w[i] >> 16);
+    return odd;
+}
+// Barrier and OR over the threads of the item's active row blocks (one named barrier
+// for each count: a block may run ahead through items that are not its own).
+__device__ __forceinline__ bool tt_any(bool x, int blocks) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)x), "r"(blocks), "r"(blocks * 128)
+        : "memory");
+    return r != 0;
+}
+
+// Sequence numbers of an item's tiles in the ring: K0, then K(i+1), V(i) in turn.
+__device__ __forceinline__ int tt_k_at(int i) { return i == 0 ? 0 : 2 * i - 1; }
+__device__ __forceinline__ int tt_v_at(int i, int tiles) { return min(2 * i + 2, 2 * tiles - 1); }
+
+template <bool BF, int HD, int NB>
+__global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
+    k_tree_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+              const __grid_constant__ TreeArgs a, int stages, int q_rows) {
+    constexpr int COLS = HD / 64;             // 64-element column blocks of a row
+    constexpr int STAGE = COLS * TR_TILE * 128;
+    constexpr int TCOLS = 128 + HD;           // TMEM columns of a row block: S0, S1, O
+    constexpr uint32_t TMEM = NB * TCOLS <= 256 ? 256 : 512;
+    constexpr int THREADS = NB * 128 + 64;
+    extern __shared__ uint8_t tt_raw[];
+    uint8_t* sm = (uint8_t*)(((uintptr_t)tt_raw + 1023) & ~(uintptr_t)1023);
+    const int q_block = q_rows * 128;         // bytes of a column block of the queries
+    uint8_t* s_q = sm;                        // [NB][COLS][q_rows][128]
+    uint8_t* ring = sm + NB * COLS * q_block;
+    TtBars* bars = (TtBars*)(ring + stages * STAGE);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_trigger();
+    if (warp == 0) tmem_alloc(&bars->tmem, TMEM);
+    if (tid == 32) {
+        for (int s = 0; s < stages; s++) {
+            mbar_init(&bars->full[s], 1);
+            mbar_init(&bars->empty[s], 1);
+        }
+        for (int b = 0; b < NB; b++) {
+            mbar_init(&bars->q_full[b], 4);
+            for (int i = 0; i < 2; i++) {
+                mbar_init(&bars->pv[b][i], 1);
+                mbar_init(&bars->s_full[b][i], 1);
+                mbar_init(&bars->p_full[b][i], 4);
+            }
+        }
+        mbar_init(&bars->done, 1);
+        bars->failed = 0;
+        fence_mbar_init();
+    }
+    TreeRun run = tree_run<THREADS>(a);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars->tmem;
+    // A wait that gives up sets `failed`, and later waits return at once: the TMA and
+    // MMA loops end, the softmax warps (which meet at barriers) run through their
+    // items without waiting.
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        if (mbar_try_wait(bar, parity & 1)) return true;
+        if (*(volatile uint32_t*)&bars->failed) return false;
+        if (mbar_wait(bar, parity & 1, TT_WAIT_NS)) return true;
+        gm_fail(a.status);
+        *(volatile uint32_t*)&bars->failed = 1;
+        return false;
+    };
+    TreeItem it;
+    bool any = false, ok = true;
+    long long seq = 0;  // ring position of the item's first tile
+
+    if (warp == NB * 4) {  // ---- TMA: all lanes, a box each
+        const int per = a.page < TR_TILE ? TR_TILE / a.page : 1;  // pages of a tile
+        const int box = min(a.page, TR_TILE);
+        const int pi = lane / COLS, col = lane - pi * COLS;
+        if (lane == 0) {
+            tma_prefetch_desc(&map_k);
+            tma_prefetch_desc(&map_v);
+        }
+        long long issued = 0;
+        while (run.left > 0 && ok) {
+            it = tree_next(a, run);
+            const int key0 = (it.q.tile0 + it.tile) * TR_TILE + pi * box;
+            const int* row = a.table + (size_t)it.r * a.max_pages;
+            // row of the lane's box of tile i in the cache as [rows][D], or -1
+            auto place = [&](int i) -> int {
+                const int key = key0 + i * TR_TILE;
+                if (pi >= per || i >= it.tiles || key >= it.q.keys) return -1;
+                const int p = key / a.page, id = row[p];
+                if (id < 0 || id >= a.n_pages) {
+                    tree_bad(a);
+                    return -1;
+                }
+                return (id * a.K + it.head) * a.page + (key - p * a.page);
+            };
+            auto load = [&](const CUtensorMap* map, int at, long long n) -> bool {
+                const int s = (int)(n % stages);
+                if (n >= stages &&
+                    !__all_sync(FULL, wait(&bars->empty[s], (uint32_t)(n / stages - 1))))
+                    return false;
+                const uint32_t live = __ballot_sync(FULL, at >= 0);
+                if (lane == 0) mbar_expect_tx(&bars->full[s], __popc(live) * box * 128);
+                __syncwarp();
+                if (at >= 0)
+                    tma_load_2d(ring + s * STAGE + col * (TR_TILE * 128) + pi * box * 128, map,
+                                col * 64, at, &bars->full[s]);
+                issued++;
+                return true;
+            };
+            int now = place(0), next = place(1);
+            ok = load(&map_k, now, seq);
+            for (int i = 0; i < it.tiles && ok; i++) {
+                const int later = place(i + 2);
+                if (i + 1 < it.tiles) ok = load(&map_k, next, seq + tt_k_at(i + 1));
+                ok = ok && load(&map_v, now, seq + tt_v_at(i, it.tiles));
+                now = next;
+                next = later;
+            }
+            seq += 2 * it.tiles;
+        }
+        if (!ok)  // copies in flight land before the block may end
+            for (long long i = issued > stages ? issued - stages : 0; i < issued; i++)
+                (void)mbar_wait(&bars->full[i % stages], (uint32_t)(i / stages) & 1, TT_WAIT_NS);
+    } else if (warp == NB * 4 + 1) {  // ---- MMA: one thread
+        if (lane == 0) {
+            constexpr uint32_t id_s = tt_idesc<BF>(TR_TILE, false);
+            constexpr uint32_t id_o = tt_idesc<BF>(HD, true);
+            const uint32_t q0 = smem_addr(s_q), r0 = smem_addr(ring);
+            uint32_t n[2] = {0, 0}, items[2] = {0, 0};  // tiles and items of each row block
+            const int steps = (a.D + 15) / 16;
+            while (run.left > 0 && ok) {
+                it = tree_next(a, run);
+                const int blocks = it.rows > 128 ? NB : 1;
+                for (int b = 0; b < blocks && ok; b++) ok = wait(&bars->q_full[b], items[b]++);
+                if (!ok) break;
+                tc_fence_after();
+                auto scores = [&](int i) -> bool {
+                    const long long at = seq + tt_k_at(i);
+                    const int s = (int)(at % stages);
+                    if (!wait(&bars->full[s], (uint32_t)(at / stages))) return false;
+                    for (int b = 0; b < blocks; b++) {
+                        const uint32_t m = n[b] + i;
+                        // this buffer's weights went into the product of tile i - 2
+                        if (i >= 2 && !wait(&bars->pv[b][m & 1], (m - 2) >> 1)) return false;
+                        tc_fence_after();
+                        const uint32_t d = tmem + b * TCOLS + (m & 1) * 64;
+                        const uint64_t dq = umma_desc_sw128(q0 + b * COLS * q_block),
+                                       dk = umma_desc_sw128(r0 + s * STAGE);
+                        for (int k = 0; k < steps; k++) {
+                            const uint32_t in = (k & 3) * 32;
+                            umma_f16(d, dq + (((k >> 2) * q_block + in) >> 4),
+                                     dk + (((k >> 2) * (TR_TILE * 128) + in) >> 4), id_s, k > 0);
+                        }
+                        tc_commit(&bars->s_full[b][m & 1]);
+                    }
+                    tc_commit(&bars->empty[s]);
+                    return true;
+                };
+                ok = scores(0);
+                for (int i = 0; i < it.tiles && ok; i++) {
+                    if (i + 1 < it.tiles) ok = scores(i + 1);
+                    const long long at = seq + tt_v_at(i, it.tiles);
+                    const int s = (int)(at % stages);
+                    ok = ok && wait(&bars->full[s], (uint32_t)(at / stages));
+                    for (int b = 0; b < blocks && ok; b++) {
+                        const uint32_t m = n[b] + i;
+                        ok = wait(&bars->p_full[b][m & 1], m >> 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t p = tmem + b * TCOLS + (m & 1) * 64;
+                        const uint64_t dv = tt_desc_rows(r0 + s * STAGE, TR_TILE * 128);
+#pragma unroll
+                        for (int k = 0; k < TR_TILE / 16; k++)
+                            tt_mma_ts(tmem + b * TCOLS + 128, p + 8 * k,
+                                      dv + ((k * 16 * 128) >> 4), id_o);
+                        tc_commit(&bars->pv[b][m & 1]);
+                    }
+                    if (ok) tc_commit(&bars->empty[s]);
+                }
+                for (int b = 0; b < blocks; b++) n[b] += it.tiles;
+                seq += 2 * it.tiles;
+            }
+            // every product issued has ended before the block frees its TMEM
+            tc_commit(&bars->done);
+            (void)mbar_wait(&bars->done, 0, TT_WAIT_NS);
+        }
+        __syncwarp();
+    } else {  // ---- softmax: a thread per row
+        const int b = warp >> 2, m = tid & 127;
+        const uint32_t lanes = tmem + b * TCOLS + ((uint32_t)(warp & 3) << 21);
+        const uint32_t t_o = lanes + 128;
+        uint32_t n = 0;
+        const float log2e = 1.44269504088896341f;
+        const float c2 = a.softcap > 0.f ? log2e : a.scale * log2e;
+        uint8_t* q_sm = s_q + b * COLS * q_block;
+        while (run.left > 0) {
+            it = tree_next(a, run);
+            any = true;
+            const int blocks = it.rows > 128 ? NB : 1;
+            const long long at0 = seq;
+            seq += 2 * it.tiles;
+            if (b >= blocks) continue;
+            const int m0 = it.block * a.bm + b * 128;       // row 0 of the request's rows
+            const int rows = min(it.rows - b * 128, 128);
+            const bool work = (warp & 3) * 32 < rows;       // the warp has rows
+            const int key0 = (it.q.tile0 + it.tile) * TR_TILE;
+            // ---- queries, and this row's window
+            for (int i = m; i < rows * COLS * 8; i += 128) {
+                const int r = i / (COLS * 8), c = i % (COLS * 8);
+                const int node = (m0 + r) / a.G, gi = (m0 + r) - node * a.G;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (c * 8 < a.D)
+                    x = *(const uint4*)((const uint16_t*)a.q +
+                                        (long long)(it.q.row0 + node) * a.q_stride +
+                                        (long long)(it.head * a.G + gi) * a.D + c * 8);
+                *(uint4*)(q_sm + (c >> 3) * q_block + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+            }
+            int edge = 0, edge_max = 0;  // this row's, and the largest of the item's rows
+            if (a.window > 0) {
+                if (m < rows) edge = tree_edge(a, it.q, m0 + m);
+                const int last = (it.block * a.bm + it.rows - 1) / a.G;
+                for (int node = it.block * a.bm / a.G + lane; node <= last; node += 32)
+                    edge_max = max(edge_max, tree_edge(a, it.q, node * a.G));
+                edge_max = __reduce_max_sync(FULL, edge_max);
+            }
+            if (work) {
+                uint32_t z[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) z[i] = 0;
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) tt_st32(t_o + c, z);
+                tt_wait_st();
+            }
+            tt_fence_async();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->q_full[b]);
+            float top = -INFINITY, ref_m = -INFINITY, sum = 0.f;
+            for (int i = 0; i < it.tiles; i++, n++) {
+                const int kt = key0 + i * TR_TILE;
+                const bool part = tree_partial(it.q, edge_max, kt);
+                uint64_t sees = ~0ull;
+                if (part && work && (kt < edge || kt + TR_TILE > it.q.len))
+                    sees = m < rows ? tree_sees(a, it.q, m0 + m, kt) : 0;
+                wait(&bars->s_full[b][n & 1], n >> 1);
+                __syncwarp();
+                tc_fence_after();
+                const uint32_t t_s = lanes + (n & 1) * 64;
+                if (work) {
+                    float s[64];
+                    tt_ld32(t_s, (uint32_t*)s);
+                    tt_ld32(t_s + 32, (uint32_t*)s + 32);
+                    tt_wait_ld32((uint32_t*)s);
+                    tt_wait_ld32((uint32_t*)s + 32);
+                    if (a.softcap > 0.f) {
+                        // tanh(y) = 1 - 2 / (1 + e^2y): off by 2^-22, times softcap a
+                        // score error far below one rounding of the weight
+                        const float y2 = 2.f * log2e * a.scale / a.softcap;
+#pragma unroll
+                        for (int j = 0; j < 64; j++) {
+                            const float y = s[j] * y2;
+                            s[j] = a.softcap - __fdividef(2.f * a.softcap,
+                                                          1.f + tt_exp2(y > 120.f ? 120.f : y));
+                        }
+                    }
+                    if (part) {
+#pragma unroll
+                        for (int j = 0; j < 64; j++)
+                            if (!(sees >> j & 1)) s[j] = -INFINITY;
+                    }
+                    float t0 = top, t1 = s[1], t2 = s[2], t3 = s[3];
+                    t0 = fmaxf(t0, s[0]);
+#pragma unroll
+                    for (int j = 4; j < 64; j += 4) {
+                        t0 = fmaxf(t0, s[j]);
+                        t1 = fmaxf(t1, s[j + 1]);
+                        t2 = fmaxf(t2, s[j + 2]);
+                        t3 = fmaxf(t3, s[j + 3]);
+                    }
+                    top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+                    if (i == 0) {
+                        ref_m = top;
+                    } else if (__any_sync(FULL, m < rows && (top - ref_m) * c2 > 8.f)) {
+                        const float fix = ref_m == -INFINITY ? 0.f : tt_exp2((ref_m - top) * c2);
+                        wait(&bars->pv[b][(n - 1) & 1], (n - 1) >> 1);  // O holds the tiles before this one
+                        __syncwarp();
+                        tc_fence_after();
+                        if (top > ref_m) {
+                            sum *= fix;
+                            ref_m = top;
+                        }
+#pragma unroll
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t o[32];
+                            tt_ld32(t_o + c, o);
+                            tt_wait_ld32(o);
+#pragma unroll
+                            for (int j = 0; j < 32; j++)
+                                o[j] = __float_as_uint(__uint_as_float(o[j]) * fix);
+                            tt_st32(t_o + c, o);
+                        }
+                    }
+                    const float ref = ref_m == -INFINITY ? 0.f : ref_m * c2;
+                    uint32_t p[32];
+                    float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        p[j] = tt_pack<BF>(tt_exp2(fmaf(s[2 * j], c2, -ref)),
+                                           tt_exp2(fmaf(s[2 * j + 1], c2, -ref)), l0);
+                        p[j + 1] = tt_pack<BF>(tt_exp2(fmaf(s[2 * j + 2], c2, -ref)),
+                                               tt_exp2(fmaf(s[2 * j + 3], c2, -ref)), l1);
+                    }
+                    sum += l0 + l1;
+                    tt_st32(t_s, p);
+                    tt_wait_st();
+                }
+                if (part) {  // v rows past the end, and values that are not finite
+                    const long long at = at0 + tt_v_at(i, it.tiles);
+                    const int sv = (int)(at % stages);
+                    wait(&bars->full[sv], (uint32_t)(at / stages));
+                    uint8_t* v = ring + sv * STAGE;
+                    const int live = min(it.q.keys - kt, TR_TILE);
+                    bool odd = false;
+                    for (int x = b * 128 + m; x < COLS * TR_TILE * 8; x += blocks * 128) {
+                        uint4* w = (uint4*)(v + x * 16);  // row (x / 8) % 64 of its column block
+                        if ((x >> 3) % TR_TILE >= live) *w = make_uint4(0, 0, 0, 0);
+                        else odd |= tt_odd8<BF>(*w);
+                    }
+                    if (tt_any(odd, blocks)) {
+                        if (work) {
+                            if (i > 0) wait(&bars->pv[b][(n - 1) & 1], (n - 1) >> 1);
+                            __syncwarp();
+                            tc_fence_after();
+                            for (int j = 0; j < live; j++)
+                                for (int c = 0; c < COLS * 8; c++) {
+                                    const uint4 x = *(const uint4*)(v + (c >> 3) * (TR_TILE * 128) +
+                                                                    j * 128 +
+                                                                    (((c & 7) ^ (j & 7)) << 4));
+                                    if (!tt_odd8<BF>(x)) continue;
+                                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                                    for (int e = 0; e < 8; e++) {
+                                        const uint32_t bits = e & 1 ? w[e >> 1] >> 16
+                                                                    : w[e >> 1] & 0xffffu;
+                                        if (!tt_odd<BF>(bits)) continue;
+                                        uint32_t pj = tt_ld1(t_s + (j >> 1));
+                                        uint32_t oj = tt_ld1(t_o + c * 8 + e);
+                                        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                                                     : "+r"(pj), "+r"(oj)::"memory");
+                                        float o = __uint_as_float(oj);
+                                        if (sees >> j & 1)
+                                            o = fmaf(tt_value<BF>(j & 1 ? pj >> 16 : pj & 0xffffu),
+                                                     tt_value<BF>(bits), o);
+                                        __syncwarp();
+                                        tt_st1(t_o + c * 8 + e, __float_as_uint(o));
+                                        tt_wait_st();
+                                    }
+                                }
+                        }
+                        (void)tt_any(false, blocks);  // all have read them
+                        for (int x = b * 128 + m; x < COLS * TR_TILE * 8; x += blocks * 128) {
+                            uint16_t* w = (uint16_t*)(v + x * 16);
+                            for (int e = 0; e < 8; e++)
+                                if (tt_odd<BF>(w[e])) w[e] = 0;
+                        }
+                    }
+                    tt_fence_async();
+                    // both row blocks read the mended tile
+                    if (NB > 1) (void)tt_any(false, blocks);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->p_full[b][n & 1]);
+            }
+            // ---- the item's end
+            wait(&bars->pv[b][(n - 1) & 1], (n - 1) >> 1);
+            __syncwarp();
+            tc_fence_after();
+            if (work) {
+                const bool mine = m < rows;
+                const size_t piece =
+                    ((size_t)blockIdx.x * 2 + tree_slot(run, it)) * a.bm + b * 128 + m;
+                const int node = (m0 + m) / a.G, gi = (m0 + m) - node * a.G;
+                uint16_t* out = (uint16_t*)a.out +
+                                ((long long)(it.q.row0 + node) * a.H + it.head * a.G + gi) * a.D;
+                const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+                if (mine && !it.whole)
+                    a.ml[piece] =
+                        make_float2(ref_m == -INFINITY ? -INFINITY : ref_m * c2, sum);
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t o[32];
+                    __syncwarp();
+                    tt_ld32(t_o + c, o);
+                    tt_wait_ld32(o);
+                    if (!mine) {
+                    } else if (it.whole) {
+                        float unused = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8) {
+                            if (c + j >= a.D) break;
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                w[e] = tt_pack<BF>(__uint_as_float(o[j + 2 * e]) * inv,
+                                                   __uint_as_float(o[j + 2 * e + 1]) * inv, unused);
+                            if (inv == 0.f) w[0] = w[1] = w[2] = w[3] = 0;
+                            *(uint4*)(out + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            if (c + j >= a.D) break;
+                            *(uint4*)(a.part + piece * a.dp + c + j) =
+                                make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0) tree_record(a, run, it, any);
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, TMEM);
+    }
+}
+
+static PFN_cuTensorMapEncodeTiled_v12000 tt_encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+                cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (PFN_cuTensorMapEncodeTiled_v12000)p;
+    });
+    return fn;
+}
+
+// The cache as [n_pages * K * page rows][D], boxes of one page (64 rows at most) by
+// 64 elements; columns past D read zeros.
+static int tt_map(CUtensorMap* map, const void* base, const TreeArgs& a, bool bf) {
+    auto enc = tt_encode_fn();
+    CW_CHECK(enc, CW_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    cuuint64_t dims[2] = {(cuuint64_t)a.D, (cuuint64_t)a.n_pages * a.K * a.page};
+    cuuint64_t strides[1] = {(cuuint64_t)a.D * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)std::min(a.page, TR_TILE)};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                     const_cast<void*>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CW_CHECK(r == CUDA_SUCCESS, CW_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return CW_OK;
+}
+
+bool tree_tc_takes(const cw_tree_attn_args& p, const void* q, const void* k, const void* v) {
+    const bool pages = p.page_size == 8 || p.page_size == 16 || p.page_size == 32 ||
+                       p.page_size % TR_TILE == 0;
+    return p.type != CW_GGUF_F32 && p.head_dim % 8 == 0 && pages && p.q_off % 8 == 0 &&
+           p.q_stride % 8 == 0 && (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0 &&
+           (uint64_t)p.n_pages * p.n_kv * p.page_size < (1ull << 31);
+}
+// Two row blocks to a CTA where a request can have more than 128 rows, so that its
+// keys are still read once (their TMEM, 2 x (128 + 256) columns, does not fit at 256).
+int tree_tc_rows(const TreeArgs& a) { return a.max_nodes * a.G > 128 && a.D <= 128 ? 256 : 128; }
+static int tt_per_sm(const TreeArgs& a) { return a.bm == 128 && a.D <= 128 ? 2 : 1; }
+int tree_tc_grid(cw_ctx* ctx, const TreeArgs& a) { return ctx->sm_count * tt_per_sm(a); }
+
+template <bool BF, int HD, int NB>
+static int tt_go(cw_ctx* ctx, const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv,
+                 int grid) {
+    auto kern = k_tree_tc<BF, HD, NB>;
+    // the ring takes what the queries leave of the SM's shared memory (two CTAs of
+    // 114 KB or one of 227 KB); products read rows past q_rows as whatever follows
+    const int q_rows = std::min(128, (a.max_nodes * a.G + 7) / 8 * 8);
+    const size_t q = (size_t)NB * (HD / 64) * q_rows * 128, stage = (HD / 64) * TR_TILE * 128;
+    const size_t cap = tt_per_sm(a) == 2 ? 115200 : 230400, fixed = 1024 + sizeof(TtBars);
+    const int stages = (int)std::min<size_t>((cap - fixed - q) / stage, TT_STAGES);
+    const size_t smem = fixed + q + stages * stage;
+    static bool set[64] = {};
+    if (!set[ctx->device & 63]) {
+        CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cap));
+        set[ctx->device & 63] = true;
+    }
+    return launch_pdl(ctx, false, kern, dim3(grid), dim3(NB * 128 + 64), smem, mk, mv, a, stages,
+                      q_rows);
+}
+template <bool BF>
+static int tt_dims(cw_ctx* ctx, const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv,
+                   int grid) {
+    if (a.D > 128) return tt_go<BF, 256, 1>(ctx, a, mk, mv, grid);
+    if (a.bm == 256)
+        return a.D <= 64 ? tt_go<BF, 64, 2>(ctx, a, mk, mv, grid)
+                         : tt_go<BF, 128, 2>(ctx, a, mk, mv, grid);
+    return a.D <= 64 ? tt_go<BF, 64, 1>(ctx, a, mk, mv, grid)
+                     : tt_go<BF, 128, 1>(ctx, a, mk, mv, grid);
+}
+
+int tree_tc_launch(cw_ctx* ctx, const TreeArgs& a, uint32_t type, int grid) {
+    const bool bf = type == CW_GGUF_BF16;
+    CUtensorMap mk, mv;
+    CW_TRY(tt_map(&mk, a.k, a, bf));
+    CW_TRY(tt_map(&mv, a.v, a, bf));
+    return bf ? tt_dims<true>(ctx, a, mk, mv, grid) : tt_dims<false>(ctx, a, mk, mv, grid);
+}
+
+}  // namespace cw
