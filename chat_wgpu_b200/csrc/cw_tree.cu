@@ -28,7 +28,7 @@
 namespace cw {
 
 constexpr int TR_THREADS = 256;
-constexpr size_t TR_SMEM_CAP = 226 * 1024 + 512;  // dynamic; the kernel also has static
+constexpr size_t TR_SMEM_CAP = 226 * 1024 + 384;  // dynamic; the kernel also has static
 
 __device__ __forceinline__ void tr_cp16(void* dst, const void* src, bool live) {
     const int n = live ? 16 : 0;
@@ -96,10 +96,11 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
     long long* s_row = (long long*)(s_sees + BM);  // [2][64] element offset of a key row, or -1
     float2* s_ml = (float2*)(s_row + 2 * TR_TILE); // [WK][BM]
     __shared__ int s_edge;
+    __shared__ TreeShared s_run;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int wm = warp % WM, wk = warp / WM, g = lane >> 2, t4 = lane & 3;
     pdl_trigger();
-    TreeRun run = tree_run<TR_THREADS>(a);
+    TreeRun run = tree_run<TR_THREADS>(a, &s_run);
     TreeItem it;
     bool any = false;
     while (run.left > 0) {

@@ -90,11 +90,16 @@ struct TreeItem {
     bool whole;
 };
 
-// All threads (NT of them, a multiple of 32).
+// All threads (NT of them, a multiple of 32); sh is shared memory.
+struct TreeShared {
+    long long w[16], off;
+    int r;
+};
 template <int NT>
-__device__ TreeRun tree_run(const TreeArgs& a) {
-    __shared__ long long s_w[NT / 32], s_off;
-    __shared__ int s_r;
+__device__ TreeRun tree_run(const TreeArgs& a, TreeShared* sh) {
+    long long* s_w = sh->w;
+    long long& s_off = sh->off;
+    int& s_r = sh->r;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const bool one = a.n_req <= NT;
     long long mine = 0;

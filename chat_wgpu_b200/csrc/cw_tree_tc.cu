@@ -48,6 +48,8 @@ struct TtBars {
     uint64_t full[TT_STAGES], empty[TT_STAGES];
     uint64_t q_full[2], s_full[2][2], p_full[2][2], pv[2][2], done;  // [row block][tile % 2]
     uint32_t tmem, failed;
+    TreeShared run;
+    float2 ml[128];  // maximum (times log2 e) and sum of each lane's part of a row
 };
 
 __device__ __forceinline__ void tt_ld32(uint32_t addr, uint32_t* r) {
@@ -74,6 +76,24 @@ __device__ __forceinline__ void tt_st32(uint32_t addr, const uint32_t* r) {
         "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+template <int N> __device__ __forceinline__ void tt_st(uint32_t addr, const uint32_t* r) {
+    if constexpr (N == 32) {
+        tt_st32(addr, r);
+    } else if constexpr (N == 16) {
+        asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+            "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+            "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+            "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+            "r"(r[15])
+            : "memory");
+    } else {
+        asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
+            "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+            : "memory");
+    }
+}
 // Waits for this thread's TMEM loads; the values pass through, so no use of them can
 // be moved before it.
 __device__ __forceinline__ void tt_wait_ld32(uint32_t* r) {
@@ -84,6 +104,24 @@ __device__ __forceinline__ void tt_wait_ld32(uint32_t* r) {
                    "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
                    "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]),
                    "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+// N columns, waited for.
+template <int N> __device__ __forceinline__ void tt_load(uint32_t addr, uint32_t* r) {
+    if constexpr (N == 64) {
+        tt_ld32(addr, r);
+        tt_ld32(addr + 32, r + 32);
+        tt_wait_ld32(r);
+        tt_wait_ld32(r + 32);
+    } else if constexpr (N == 32) {
+        tt_ld32(addr, r);
+        tt_wait_ld32(r);
+    } else {
+        tmem_ld16(addr, *(uint32_t(*)[16])r);
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                       "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                       "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+    }
 }
 __device__ __forceinline__ uint32_t tt_ld1(uint32_t addr) {
     uint32_t r;
@@ -100,12 +138,15 @@ __device__ __forceinline__ void tt_wait_st() {
 __device__ __forceinline__ void tt_fence_async() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-// D[tmem] += A[tmem] B[shared]
-__device__ __forceinline__ void tt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+// D[tmem] += A[tmem] B[shared], in the TMEM lanes whose bits in off0 (lanes 0-31) ..
+// off3 (lanes 96-127) are 0.
+__device__ __forceinline__ void tt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t off0, uint32_t off1, uint32_t off2,
+                                          uint32_t off3) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%4, %5, %6, %7}, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(off0), "r"(off1), "r"(off2), "r"(off3)
         : "memory");
 }
 // Matrix descriptor of an operand whose contraction index is the row (V: keys x
@@ -165,11 +206,34 @@ __device__ __forceinline__ bool tt_any(bool x, int blocks) {
     return r != 0;
 }
 
-// Sequence numbers of an item's tiles in the ring: K0, then K(i+1), V(i) in turn.
-__device__ __forceinline__ int tt_k_at(int i) { return i == 0 ? 0 : 2 * i - 1; }
-__device__ __forceinline__ int tt_v_at(int i, int tiles) { return min(2 * i + 2, 2 * tiles - 1); }
+// A place in the ring.  An item's tiles pass through it in the order K0, then K(i+1),
+// V(i) in turn: 2 * tiles places.
+struct TtPlace {
+    int stage;
+    uint32_t phase;
+    __device__ __forceinline__ void next(int stages) {
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+    __device__ __forceinline__ void skip(int n, int stages) {
+        stage += n;
+        while (stage >= stages) {
+            stage -= stages;
+            phase ^= 1;
+        }
+    }
+};
+__device__ __forceinline__ bool tt_elect() {  // one lane of a converged warp
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
 
-template <bool BF, int HD, int NB>
+template <bool BF, int HD, int NB, int SPLIT>
 __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
     k_tree_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
               const __grid_constant__ TreeArgs a, int stages, int q_rows) {
@@ -178,14 +242,21 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
     constexpr int TCOLS = 128 + HD;           // TMEM columns of a row block: S0, S1, O
     constexpr uint32_t TMEM = NB * TCOLS <= 256 ? 256 : 512;
     constexpr int THREADS = NB * 128 + 64;
-    extern __shared__ uint8_t tt_raw[];
-    uint8_t* sm = (uint8_t*)(((uintptr_t)tt_raw + 1023) & ~(uintptr_t)1023);
+    constexpr int KEYS = TR_TILE / SPLIT;     // keys of a tile that a thread weighs
+    constexpr int LANES = 128 / SPLIT;        // rows of a row block
+    static_assert(NB == 1 || SPLIT == 1, "a split row block is the only one");
+    extern __shared__ __align__(1024) uint8_t sm[];
     const int q_block = q_rows * 128;         // bytes of a column block of the queries
     uint8_t* s_q = sm;                        // [NB][COLS][q_rows][128]
     uint8_t* ring = sm + NB * COLS * q_block;
     TtBars* bars = (TtBars*)(ring + stages * STAGE);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_trigger();
+    // the swizzle counts from 1024-byte boundaries; no static shared memory precedes
+    if (smem_addr(sm) & 1023) {
+        if (tid == 0) tree_bad(a);
+        return;
+    }
     if (warp == 0) tmem_alloc(&bars->tmem, TMEM);
     if (tid == 32) {
         for (int s = 0; s < stages; s++) {
@@ -204,7 +275,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
         bars->failed = 0;
         fence_mbar_init();
     }
-    TreeRun run = tree_run<THREADS>(a);
+    TreeRun run = tree_run<THREADS>(a, &bars->run);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -215,14 +286,18 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
         if (mbar_try_wait(bar, parity & 1)) return true;
         if (*(volatile uint32_t*)&bars->failed) return false;
-        if (mbar_wait(bar, parity & 1, TT_WAIT_NS)) return true;
+        const uint64_t from = global_ns();
+        do {
+            for (int i = 0; i < 256; i++)  // reading the clock would delay the wake-up
+                if (mbar_try_wait(bar, parity & 1)) return true;
+        } while (global_ns() - from < TT_WAIT_NS);
         gm_fail(a.status);
         *(volatile uint32_t*)&bars->failed = 1;
         return false;
     };
     TreeItem it;
     bool any = false, ok = true;
-    long long seq = 0;  // ring position of the item's first tile
+    TtPlace at = {0, 0};
 
     if (warp == NB * 4) {  // ---- TMA: all lanes, a box each
         const int per = a.page < TR_TILE ? TR_TILE / a.page : 1;  // pages of a tile
@@ -232,116 +307,137 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
             tma_prefetch_desc(&map_k);
             tma_prefetch_desc(&map_v);
         }
-        long long issued = 0;
+        const int shift = (a.page & (a.page - 1)) == 0 ? __ffs(a.page) - 1 : -1;
+        bool full = false;  // every stage has been filled once
         while (run.left > 0 && ok) {
             it = tree_next(a, run);
             const int key0 = (it.q.tile0 + it.tile) * TR_TILE + pi * box;
             const int* row = a.table + (size_t)it.r * a.max_pages;
-            // row of the lane's box of tile i in the cache as [rows][D], or -1
-            auto place = [&](int i) -> int {
+            // the page of the lane's box of tile i, read a tile ahead of its use
+            auto page_of = [&](int i) -> int {
                 const int key = key0 + i * TR_TILE;
                 if (pi >= per || i >= it.tiles || key >= it.q.keys) return -1;
-                const int p = key / a.page, id = row[p];
+                return row[shift >= 0 ? key >> shift : key / a.page];
+            };
+            // that box's row in the cache as [rows][D], or -1
+            auto place = [&](int i, int id) -> int {
+                const int key = key0 + i * TR_TILE;
+                if (pi >= per || i >= it.tiles || key >= it.q.keys) return -1;
                 if (id < 0 || id >= a.n_pages) {
                     tree_bad(a);
                     return -1;
                 }
-                return (id * a.K + it.head) * a.page + (key - p * a.page);
+                const int in = shift >= 0 ? key & (a.page - 1) : key % a.page;
+                return (id * a.K + it.head) * a.page + in;
             };
-            auto load = [&](const CUtensorMap* map, int at, long long n) -> bool {
-                const int s = (int)(n % stages);
-                if (n >= stages &&
-                    !__all_sync(FULL, wait(&bars->empty[s], (uint32_t)(n / stages - 1))))
-                    return false;
-                const uint32_t live = __ballot_sync(FULL, at >= 0);
+            auto load = [&](const CUtensorMap* map, int at_row) -> bool {
+                const int s = at.stage;
+                if (full && !__all_sync(FULL, wait(&bars->empty[s], at.phase ^ 1))) return false;
+                const uint32_t live = __ballot_sync(FULL, at_row >= 0);
                 if (lane == 0) mbar_expect_tx(&bars->full[s], __popc(live) * box * 128);
                 __syncwarp();
-                if (at >= 0)
+                if (at_row >= 0)
                     tma_load_2d(ring + s * STAGE + col * (TR_TILE * 128) + pi * box * 128, map,
-                                col * 64, at, &bars->full[s]);
-                issued++;
+                                col * 64, at_row, &bars->full[s]);
+                at.next(stages);
+                full |= at.stage == 0;
                 return true;
             };
-            int now = place(0), next = place(1);
-            ok = load(&map_k, now, seq);
+            int id = page_of(1), now = place(0, page_of(0));
+            ok = load(&map_k, now);
             for (int i = 0; i < it.tiles && ok; i++) {
-                const int later = place(i + 2);
-                if (i + 1 < it.tiles) ok = load(&map_k, next, seq + tt_k_at(i + 1));
-                ok = ok && load(&map_v, now, seq + tt_v_at(i, it.tiles));
+                const int next = place(i + 1, id);
+                id = page_of(i + 2);
+                if (i + 1 < it.tiles) ok = load(&map_k, next);
+                ok = ok && load(&map_v, now);
                 now = next;
-                next = later;
             }
-            seq += 2 * it.tiles;
         }
         if (!ok)  // copies in flight land before the block may end
-            for (long long i = issued > stages ? issued - stages : 0; i < issued; i++)
-                (void)mbar_wait(&bars->full[i % stages], (uint32_t)(i / stages) & 1, TT_WAIT_NS);
-    } else if (warp == NB * 4 + 1) {  // ---- MMA: one thread
-        if (lane == 0) {
-            constexpr uint32_t id_s = tt_idesc<BF>(TR_TILE, false);
-            constexpr uint32_t id_o = tt_idesc<BF>(HD, true);
-            const uint32_t q0 = smem_addr(s_q), r0 = smem_addr(ring);
-            uint32_t n[2] = {0, 0}, items[2] = {0, 0};  // tiles and items of each row block
-            const int steps = (a.D + 15) / 16;
-            while (run.left > 0 && ok) {
-                it = tree_next(a, run);
-                const int blocks = it.rows > 128 ? NB : 1;
-                for (int b = 0; b < blocks && ok; b++) ok = wait(&bars->q_full[b], items[b]++);
-                if (!ok) break;
-                tc_fence_after();
-                auto scores = [&](int i) -> bool {
-                    const long long at = seq + tt_k_at(i);
-                    const int s = (int)(at % stages);
-                    if (!wait(&bars->full[s], (uint32_t)(at / stages))) return false;
-                    for (int b = 0; b < blocks; b++) {
-                        const uint32_t m = n[b] + i;
-                        // this buffer's weights went into the product of tile i - 2
-                        if (i >= 2 && !wait(&bars->pv[b][m & 1], (m - 2) >> 1)) return false;
-                        tc_fence_after();
-                        const uint32_t d = tmem + b * TCOLS + (m & 1) * 64;
-                        const uint64_t dq = umma_desc_sw128(q0 + b * COLS * q_block),
-                                       dk = umma_desc_sw128(r0 + s * STAGE);
-                        for (int k = 0; k < steps; k++) {
-                            const uint32_t in = (k & 3) * 32;
-                            umma_f16(d, dq + (((k >> 2) * q_block + in) >> 4),
-                                     dk + (((k >> 2) * (TR_TILE * 128) + in) >> 4), id_s, k > 0);
-                        }
-                        tc_commit(&bars->s_full[b][m & 1]);
-                    }
-                    tc_commit(&bars->empty[s]);
-                    return true;
-                };
-                ok = scores(0);
-                for (int i = 0; i < it.tiles && ok; i++) {
-                    if (i + 1 < it.tiles) ok = scores(i + 1);
-                    const long long at = seq + tt_v_at(i, it.tiles);
-                    const int s = (int)(at % stages);
-                    ok = ok && wait(&bars->full[s], (uint32_t)(at / stages));
-                    for (int b = 0; b < blocks && ok; b++) {
-                        const uint32_t m = n[b] + i;
-                        ok = wait(&bars->p_full[b][m & 1], m >> 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t p = tmem + b * TCOLS + (m & 1) * 64;
-                        const uint64_t dv = tt_desc_rows(r0 + s * STAGE, TR_TILE * 128);
+            for (int s = 0; s < stages; s++)
+                if (full || s < at.stage)  // the last filling of stage s
+                    (void)mbar_wait(&bars->full[s], s < at.stage ? at.phase : at.phase ^ 1,
+                                    TT_WAIT_NS);
+    } else if (warp == NB * 4 + 1) {  // ---- MMA: the warp waits, one lane issues
+        constexpr uint32_t id_s = tt_idesc<BF>(TR_TILE, false);
+        constexpr uint32_t id_o = tt_idesc<BF>(HD, true);
+        const uint64_t q0 = umma_desc_sw128(smem_addr(s_q)), k0 = umma_desc_sw128(smem_addr(ring)),
+                       v0 = tt_desc_rows(smem_addr(ring), TR_TILE * 128);
+        const bool one = tt_elect();
+        auto all = [&](uint64_t* bar, uint32_t parity) {
+            return __all_sync(FULL, wait(bar, parity)) != 0;
+        };
+        uint32_t n[2] = {0, 0}, items[2] = {0, 0};  // tiles and items of each row block
+        while (run.left > 0 && ok) {
+            it = tree_next(a, run);
+            const int blocks = it.rows > 128 ? NB : 1;
+            for (int b = 0; b < blocks && ok; b++) ok = all(&bars->q_full[b], items[b]++);
+            auto scores = [&](int i) {
+                const int s = at.stage;
+                ok = ok && all(&bars->full[s], at.phase);
+                at.next(stages);
 #pragma unroll
-                        for (int k = 0; k < TR_TILE / 16; k++)
-                            tt_mma_ts(tmem + b * TCOLS + 128, p + 8 * k,
-                                      dv + ((k * 16 * 128) >> 4), id_o);
-                        tc_commit(&bars->pv[b][m & 1]);
+                for (int b = 0; b < NB; b++) {
+                    if (b >= blocks) break;
+                    const uint32_t m = n[b] + i;
+                    // this buffer's weights went into the product of tile i - 2
+                    if (i >= 2) ok = ok && all(&bars->pv[b][m & 1], (m - 2) >> 1);
+                    tc_fence_after();
+                    if (one && ok) {
+                        const uint32_t d = tmem + b * TCOLS + (m & 1) * 64;
+                        const uint64_t dq = q0 + ((b * COLS * q_block) >> 4),
+                                       dk = k0 + ((s * STAGE) >> 4);
+#pragma unroll
+                        for (int k = 0; k < HD / 16; k++)
+                            umma_f16(d, dq + (((k >> 2) * q_block + (k & 3) * 32) >> 4),
+                                     dk + (((k >> 2) * (TR_TILE * 128) + (k & 3) * 32) >> 4), id_s,
+                                     k > 0);
+                        tc_commit(&bars->s_full[b][m & 1]);
+                        if (b + 1 == blocks) tc_commit(&bars->empty[s]);
                     }
-                    if (ok) tc_commit(&bars->empty[s]);
+                    __syncwarp();
                 }
-                for (int b = 0; b < blocks; b++) n[b] += it.tiles;
-                seq += 2 * it.tiles;
+            };
+            scores(0);
+            for (int i = 0; i < it.tiles && ok; i++) {
+                if (i + 1 < it.tiles) scores(i + 1);
+                const int s = at.stage;
+                ok = ok && all(&bars->full[s], at.phase);
+                at.next(stages);
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    if (b >= blocks) break;
+                    const uint32_t m = n[b] + i;
+                    ok = ok && all(&bars->p_full[b][m & 1], m >> 1);
+                    tc_fence_after();
+                    if (one && ok) {
+                        const uint32_t p = tmem + b * TCOLS + (m & 1) * 64;
+                        const uint64_t dv = v0 + ((s * STAGE) >> 4);
+                        // keys 16k..16k+15 go to the lanes that weigh them
+#pragma unroll
+                        for (int k = 0; k < TR_TILE / 16; k++) {
+                            auto off = [&](int quad) {
+                                return k * 16 / KEYS == quad * 32 / LANES ? 0u : ~0u;
+                            };
+                            tt_mma_ts(tmem + b * TCOLS + 128, p + 8 * k,
+                                      dv + ((k * 16 * 128) >> 4), id_o, off(0), off(1), off(2),
+                                      off(3));
+                        }
+                        tc_commit(&bars->pv[b][m & 1]);
+                        if (b + 1 == blocks) tc_commit(&bars->empty[s]);
+                    }
+                    __syncwarp();
+                }
             }
-            // every product issued has ended before the block frees its TMEM
-            tc_commit(&bars->done);
-            (void)mbar_wait(&bars->done, 0, TT_WAIT_NS);
+            for (int b = 0; b < blocks; b++) n[b] += it.tiles;
         }
+        // every product issued has ended before the block frees its TMEM
+        if (one) tc_commit(&bars->done);
+        (void)mbar_wait(&bars->done, 0, TT_WAIT_NS);
         __syncwarp();
     } else {  // ---- softmax: a thread per row
-        const int b = warp >> 2, m = tid & 127;
+        // lane m weighs keys [part * KEYS, ..+KEYS) of each tile for row r
+        const int b = warp >> 2, m = tid & 127, r = m % LANES, part = m / LANES;
         const uint32_t lanes = tmem + b * TCOLS + ((uint32_t)(warp & 3) << 21);
         const uint32_t t_o = lanes + 128;
         uint32_t n = 0;
@@ -352,27 +448,31 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
             it = tree_next(a, run);
             any = true;
             const int blocks = it.rows > 128 ? NB : 1;
-            const long long at0 = seq;
-            seq += 2 * it.tiles;
+            TtPlace at_v = at;  // of the item's first V tile
+            at_v.skip(it.tiles > 1 ? 2 : 1, stages);
+            at.skip(2 * it.tiles % (2 * stages), stages);
             if (b >= blocks) continue;
             const int m0 = it.block * a.bm + b * 128;       // row 0 of the request's rows
             const int rows = min(it.rows - b * 128, 128);
-            const bool work = (warp & 3) * 32 < rows;       // the warp has rows
+            const bool work = (warp & 3) * 32 % LANES < rows;  // the warp has rows
             const int key0 = (it.q.tile0 + it.tile) * TR_TILE;
             // ---- queries, and this row's window
             for (int i = m; i < rows * COLS * 8; i += 128) {
-                const int r = i / (COLS * 8), c = i % (COLS * 8);
-                const int node = (m0 + r) / a.G, gi = (m0 + r) - node * a.G;
+                const int qr = i / (COLS * 8), c = i % (COLS * 8);
+                const int node = (m0 + qr) / a.G, gi = (m0 + qr) - node * a.G;
                 uint4 x = make_uint4(0, 0, 0, 0);
                 if (c * 8 < a.D)
                     x = *(const uint4*)((const uint16_t*)a.q +
                                         (long long)(it.q.row0 + node) * a.q_stride +
                                         (long long)(it.head * a.G + gi) * a.D + c * 8);
-                *(uint4*)(q_sm + (c >> 3) * q_block + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+#pragma unroll
+                for (int s = 0; s < SPLIT; s++)  // once for each part's lanes
+                    *(uint4*)(q_sm + (c >> 3) * q_block + (qr + s * LANES) * 128 +
+                              (((c & 7) ^ (qr & 7)) << 4)) = x;
             }
             int edge = 0, edge_max = 0;  // this row's, and the largest of the item's rows
             if (a.window > 0) {
-                if (m < rows) edge = tree_edge(a, it.q, m0 + m);
+                if (r < rows) edge = tree_edge(a, it.q, m0 + r);
                 const int last = (it.block * a.bm + it.rows - 1) / a.G;
                 for (int node = it.block * a.bm / a.G + lane; node <= last; node += 32)
                     edge_max = max(edge_max, tree_edge(a, it.q, node * a.G));
@@ -393,40 +493,37 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
             float top = -INFINITY, ref_m = -INFINITY, sum = 0.f;
             for (int i = 0; i < it.tiles; i++, n++) {
                 const int kt = key0 + i * TR_TILE;
-                const bool part = tree_partial(it.q, edge_max, kt);
+                const bool mixed = tree_partial(it.q, edge_max, kt);
                 uint64_t sees = ~0ull;
-                if (part && work && (kt < edge || kt + TR_TILE > it.q.len))
-                    sees = m < rows ? tree_sees(a, it.q, m0 + m, kt) : 0;
+                if (mixed && work && (kt < edge || kt + TR_TILE > it.q.len))
+                    sees = r < rows ? tree_sees(a, it.q, m0 + r, kt) : 0;
                 wait(&bars->s_full[b][n & 1], n >> 1);
                 __syncwarp();
                 tc_fence_after();
                 const uint32_t t_s = lanes + (n & 1) * 64;
                 if (work) {
-                    float s[64];
-                    tt_ld32(t_s, (uint32_t*)s);
-                    tt_ld32(t_s + 32, (uint32_t*)s + 32);
-                    tt_wait_ld32((uint32_t*)s);
-                    tt_wait_ld32((uint32_t*)s + 32);
+                    float s[KEYS];
+                    tt_load<KEYS>(t_s + part * KEYS, (uint32_t*)s);
                     if (a.softcap > 0.f) {
                         // tanh(y) = 1 - 2 / (1 + e^2y): off by 2^-22, times softcap a
                         // score error far below one rounding of the weight
                         const float y2 = 2.f * log2e * a.scale / a.softcap;
 #pragma unroll
-                        for (int j = 0; j < 64; j++) {
+                        for (int j = 0; j < KEYS; j++) {
                             const float y = s[j] * y2;
                             s[j] = a.softcap - __fdividef(2.f * a.softcap,
                                                           1.f + tt_exp2(y > 120.f ? 120.f : y));
                         }
                     }
-                    if (part) {
+                    if (mixed) {
 #pragma unroll
-                        for (int j = 0; j < 64; j++)
-                            if (!(sees >> j & 1)) s[j] = -INFINITY;
+                        for (int j = 0; j < KEYS; j++)
+                            if (!(sees >> (part * KEYS + j) & 1)) s[j] = -INFINITY;
                     }
                     float t0 = top, t1 = s[1], t2 = s[2], t3 = s[3];
                     t0 = fmaxf(t0, s[0]);
 #pragma unroll
-                    for (int j = 4; j < 64; j += 4) {
+                    for (int j = 4; j < KEYS; j += 4) {
                         t0 = fmaxf(t0, s[j]);
                         t1 = fmaxf(t1, s[j + 1]);
                         t2 = fmaxf(t2, s[j + 2]);
@@ -435,7 +532,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
                     top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
                     if (i == 0) {
                         ref_m = top;
-                    } else if (__any_sync(FULL, m < rows && (top - ref_m) * c2 > 8.f)) {
+                    } else if (__any_sync(FULL, r < rows && (top - ref_m) * c2 > 8.f)) {
                         const float fix = ref_m == -INFINITY ? 0.f : tt_exp2((ref_m - top) * c2);
                         wait(&bars->pv[b][(n - 1) & 1], (n - 1) >> 1);  // O holds the tiles before this one
                         __syncwarp();
@@ -456,24 +553,22 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
                         }
                     }
                     const float ref = ref_m == -INFINITY ? 0.f : ref_m * c2;
-                    uint32_t p[32];
+                    uint32_t p[KEYS / 2];
                     float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
+                    for (int j = 0; j < KEYS / 2; j += 2) {
                         p[j] = tt_pack<BF>(tt_exp2(fmaf(s[2 * j], c2, -ref)),
                                            tt_exp2(fmaf(s[2 * j + 1], c2, -ref)), l0);
                         p[j + 1] = tt_pack<BF>(tt_exp2(fmaf(s[2 * j + 2], c2, -ref)),
                                                tt_exp2(fmaf(s[2 * j + 3], c2, -ref)), l1);
                     }
                     sum += l0 + l1;
-                    tt_st32(t_s, p);
+                    tt_st<KEYS / 2>(t_s + part * (KEYS / 2), p);
                     tt_wait_st();
                 }
-                if (part) {  // v rows past the end, and values that are not finite
-                    const long long at = at0 + tt_v_at(i, it.tiles);
-                    const int sv = (int)(at % stages);
-                    wait(&bars->full[sv], (uint32_t)(at / stages));
-                    uint8_t* v = ring + sv * STAGE;
+                if (mixed) {  // v rows past the end, and values that are not finite
+                    wait(&bars->full[at_v.stage], at_v.phase);
+                    uint8_t* v = ring + at_v.stage * STAGE;
                     const int live = min(it.q.keys - kt, TR_TILE);
                     bool odd = false;
                     for (int x = b * 128 + m; x < COLS * TR_TILE * 8; x += blocks * 128) {
@@ -502,7 +597,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
                                         asm volatile("tcgen05.wait::ld.sync.aligned;"
                                                      : "+r"(pj), "+r"(oj)::"memory");
                                         float o = __uint_as_float(oj);
-                                        if (sees >> j & 1)
+                                        if ((sees >> j & 1) && j / KEYS == part)
                                             o = fmaf(tt_value<BF>(j & 1 ? pj >> 16 : pj & 0xffffu),
                                                      tt_value<BF>(bits), o);
                                         __syncwarp();
@@ -525,50 +620,93 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars->p_full[b][n & 1]);
+                at_v.skip(i + 2 < it.tiles ? 2 : 1, stages);
             }
             // ---- the item's end
             wait(&bars->pv[b][(n - 1) & 1], (n - 1) >> 1);
             __syncwarp();
             tc_fence_after();
-            if (work) {
-                const bool mine = m < rows;
-                const size_t piece =
-                    ((size_t)blockIdx.x * 2 + tree_slot(run, it)) * a.bm + b * 128 + m;
-                const int node = (m0 + m) / a.G, gi = (m0 + m) - node * a.G;
-                uint16_t* out = (uint16_t*)a.out +
-                                ((long long)(it.q.row0 + node) * a.H + it.head * a.G + gi) * a.D;
+            const size_t piece =
+                ((size_t)blockIdx.x * 2 + tree_slot(run, it)) * a.bm + b * 128 + r;
+            const int node = (m0 + r) / a.G, gi = (m0 + r) - node * a.G;
+            uint16_t* out = (uint16_t*)a.out +
+                            ((long long)(it.q.row0 + node) * a.H + it.head * a.G + gi) * a.D;
+            const float top2 = ref_m == -INFINITY ? -INFINITY : ref_m * c2;
+            // N f32 sums of columns c.. of this row: the result, or the partial state
+            auto put = [&](const float* o, int c, float inv) {
+                if (it.whole) {
+                    float unused = 0.f;
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        w[e] = inv == 0.f ? 0u : tt_pack<BF>(o[2 * e] * inv, o[2 * e + 1] * inv, unused);
+                    *(uint4*)(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                    *(float4*)(a.part + piece * a.dp + c) = make_float4(o[0], o[1], o[2], o[3]);
+                    *(float4*)(a.part + piece * a.dp + c + 4) = make_float4(o[4], o[5], o[6], o[7]);
+                }
+            };
+            if constexpr (SPLIT == 1) {
                 const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-                if (mine && !it.whole)
-                    a.ml[piece] =
-                        make_float2(ref_m == -INFINITY ? -INFINITY : ref_m * c2, sum);
+                if (r < rows && !it.whole) a.ml[piece] = make_float2(top2, sum);
+                if (work) {
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
-                    uint32_t o[32];
-                    __syncwarp();
-                    tt_ld32(t_o + c, o);
-                    tt_wait_ld32(o);
-                    if (!mine) {
-                    } else if (it.whole) {
-                        float unused = 0.f;
+                    for (int c = 0; c < HD; c += 32) {
+                        float o[32];
+                        __syncwarp();
+                        tt_load<32>(t_o + c, (uint32_t*)o);
 #pragma unroll
-                        for (int j = 0; j < 32; j += 8) {
-                            if (c + j >= a.D) break;
-                            uint32_t w[4];
+                        for (int j = 0; j < 32; j += 8)
+                            if (r < rows && c + j < a.D) put(o + j, c + j, inv);
+                    }
+                }
+            } else {
+                // join the SPLIT parts of each row: 32 columns at a time through the
+                // queries' place, 16-byte chunks exclusive-ored with the lane
+                bars->ml[m] = make_float2(top2, sum);
+                (void)tt_any(false, 1);
+                float top = -INFINITY, l = 0.f;
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                w[e] = tt_pack<BF>(__uint_as_float(o[j + 2 * e]) * inv,
-                                                   __uint_as_float(o[j + 2 * e + 1]) * inv, unused);
-                            if (inv == 0.f) w[0] = w[1] = w[2] = w[3] = 0;
-                            *(uint4*)(out + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                    } else {
+                for (int s = 0; s < SPLIT; s++) top = fmaxf(top, bars->ml[s * LANES + r].x);
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            if (c + j >= a.D) break;
-                            *(uint4*)(a.part + piece * a.dp + c + j) =
-                                make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                for (int s = 0; s < SPLIT; s++) {
+                    const float2 x = bars->ml[s * LANES + r];
+                    if (x.x != -INFINITY) l += x.y * tt_exp2(x.x - top);
+                }
+                const float own = top2 == -INFINITY ? 0.f : tt_exp2(top2 - top);
+                const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+                if (r < rows && part == 0 && !it.whole) a.ml[piece] = make_float2(top, l);
+#pragma unroll 1
+                for (int c = 0; c < HD && c < a.D; c += 32) {
+                    if (work) {
+                        float o[32];
+                        tt_load<32>(t_o + c, (uint32_t*)o);
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            *(float4*)(q_sm + m * 128 + ((j ^ (m & 7)) << 4)) =
+                                make_float4(own == 0.f ? 0.f : o[4 * j] * own,
+                                            own == 0.f ? 0.f : o[4 * j + 1] * own,
+                                            own == 0.f ? 0.f : o[4 * j + 2] * own,
+                                            own == 0.f ? 0.f : o[4 * j + 3] * own);
+                    }
+                    (void)tt_any(false, 1);
+                    if (r < rows) {  // this thread: 32 / SPLIT of the columns
+#pragma unroll
+                        for (int j = 0; j < 8 / SPLIT; j += 2) {
+                            const int at = part * (8 / SPLIT) + j;
+                            float o[8] = {};
+#pragma unroll
+                            for (int s = 0; s < SPLIT; s++) {
+                                const uint8_t* from = q_sm + (s * LANES + r) * 128;
+                                const float4 x = *(const float4*)(from + ((at ^ (r & 7)) << 4));
+                                const float4 y = *(const float4*)(from + (((at + 1) ^ (r & 7)) << 4));
+                                o[0] += x.x, o[1] += x.y, o[2] += x.z, o[3] += x.w;
+                                o[4] += y.x, o[5] += y.y, o[6] += y.z, o[7] += y.w;
+                            }
+                            if (c + at * 4 < a.D) put(o, c + at * 4, inv);
                         }
                     }
+                    (void)tt_any(false, 1);
                 }
             }
             tc_fence_before();
@@ -627,15 +765,16 @@ int tree_tc_rows(const TreeArgs& a) { return a.max_nodes * a.G > 128 && a.D <= 1
 static int tt_per_sm(const TreeArgs& a) { return a.bm == 128 && a.D <= 128 ? 2 : 1; }
 int tree_tc_grid(cw_ctx* ctx, const TreeArgs& a) { return ctx->sm_count * tt_per_sm(a); }
 
-template <bool BF, int HD, int NB>
+template <bool BF, int HD, int NB, int SPLIT>
 static int tt_go(cw_ctx* ctx, const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv,
                  int grid) {
-    auto kern = k_tree_tc<BF, HD, NB>;
+    auto kern = k_tree_tc<BF, HD, NB, SPLIT>;
     // the ring takes what the queries leave of the SM's shared memory (two CTAs of
-    // 114 KB or one of 227 KB); products read rows past q_rows as whatever follows
-    const int q_rows = std::min(128, (a.max_nodes * a.G + 7) / 8 * 8);
+    // 113 KB or one of 227 KB); without a split, products read rows past q_rows as
+    // whatever follows
+    const int q_rows = SPLIT > 1 ? 128 : std::min(128, (a.max_nodes * a.G + 7) / 8 * 8);
     const size_t q = (size_t)NB * (HD / 64) * q_rows * 128, stage = (HD / 64) * TR_TILE * 128;
-    const size_t cap = tt_per_sm(a) == 2 ? 115200 : 230400, fixed = 1024 + sizeof(TtBars);
+    const size_t cap = tt_per_sm(a) == 2 ? 115712 : 232448, fixed = sizeof(TtBars);
     const int stages = (int)std::min<size_t>((cap - fixed - q) / stage, TT_STAGES);
     const size_t smem = fixed + q + stages * stage;
     static bool set[64] = {};
@@ -646,15 +785,22 @@ static int tt_go(cw_ctx* ctx, const TreeArgs& a, const CUtensorMap& mk, const CU
     return launch_pdl(ctx, false, kern, dim3(grid), dim3(NB * 128 + 64), smem, mk, mv, a, stages,
                       q_rows);
 }
+template <bool BF, int HD>
+static int tt_split(cw_ctx* ctx, const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv,
+                    int grid) {
+    if constexpr (HD <= 128)
+        if (a.bm == 256) return tt_go<BF, HD, 2, 1>(ctx, a, mk, mv, grid);
+    const int most = a.max_nodes * a.G;
+    if (most <= 32) return tt_go<BF, HD, 1, 4>(ctx, a, mk, mv, grid);
+    if (most <= 64) return tt_go<BF, HD, 1, 2>(ctx, a, mk, mv, grid);
+    return tt_go<BF, HD, 1, 1>(ctx, a, mk, mv, grid);
+}
 template <bool BF>
 static int tt_dims(cw_ctx* ctx, const TreeArgs& a, const CUtensorMap& mk, const CUtensorMap& mv,
                    int grid) {
-    if (a.D > 128) return tt_go<BF, 256, 1>(ctx, a, mk, mv, grid);
-    if (a.bm == 256)
-        return a.D <= 64 ? tt_go<BF, 64, 2>(ctx, a, mk, mv, grid)
-                         : tt_go<BF, 128, 2>(ctx, a, mk, mv, grid);
-    return a.D <= 64 ? tt_go<BF, 64, 1>(ctx, a, mk, mv, grid)
-                     : tt_go<BF, 128, 1>(ctx, a, mk, mv, grid);
+    if (a.D <= 64) return tt_split<BF, 64>(ctx, a, mk, mv, grid);
+    if (a.D <= 128) return tt_split<BF, 128>(ctx, a, mk, mv, grid);
+    return tt_split<BF, 256>(ctx, a, mk, mv, grid);
 }
 
 int tree_tc_launch(cw_ctx* ctx, const TreeArgs& a, uint32_t type, int grid) {

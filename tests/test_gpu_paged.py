@@ -297,6 +297,14 @@ TREE = [  # dtype, heads, kv, dim, page, lens, nodes, options
     ("bf16", 16, 2, 64, 256, [1000], [200], {}),
     ("bf16", 24, 8, 80, 32, [333], [12], {}),
     ("bf16", 1, 1, 8, 8, [9, 0, 2], [1, 0, 3], {}),
+    # several tiles to a block's run, for each way a tile's keys are dealt to the lanes
+    ("bf16", 8, 8, 128, 64, [6000], [1], {}),
+    ("bf16", 32, 8, 128, 16, [4000, 900], [8, 3], {}),
+    ("bf16", 32, 8, 128, 64, [5000], [9], {}),
+    ("f16", 32, 8, 64, 32, [4500, 40], [16, 12], dict(softcap=10.0)),
+    ("f16", 32, 8, 64, 8, [4500], [33], dict(window=1000)),
+    ("f16", 8, 4, 256, 64, [6000], [40], {}),
+    ("f32", 16, 8, 128, 16, [3000, 700], [9, 30], {}),
 ]
 
 
