@@ -82,6 +82,8 @@ struct TreeRun {
     long long u;      // next unit, of all
     long long off;    // next unit, within request r
     int r, left;      // units left in the run
+    int seen;         // the request whose lengths q holds, or -1
+    TreeReq q;
 };
 struct TreeItem {
     TreeReq q;
@@ -157,6 +159,7 @@ __device__ TreeRun tree_run(const TreeArgs& a, TreeShared* sh) {
     __syncthreads();
     t.r = s_r;
     t.off = s_off;
+    t.seen = -1;
     return t;
 }
 
@@ -164,11 +167,15 @@ __device__ TreeRun tree_run(const TreeArgs& a, TreeShared* sh) {
 __device__ __forceinline__ TreeItem tree_next(const TreeArgs& a, TreeRun& t) {
     TreeItem it;
     while (true) {
-        it.q = tree_req(a, t.r, false);
-        if (t.off < tree_units(a, it.q)) break;
+        if (t.seen != t.r) {  // an item of the request before it needs no loads
+            t.q = tree_req(a, t.r, false);
+            t.seen = t.r;
+        }
+        if (t.off < tree_units(a, t.q)) break;
         t.r++;
         t.off = 0;
     }
+    it.q = t.q;
     const int item = (int)(t.off / it.q.tiles);
     it.r = t.r;
     it.tile = (int)(t.off - (long long)item * it.q.tiles);

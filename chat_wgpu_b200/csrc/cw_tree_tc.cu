@@ -27,19 +27,12 @@
 // of seen keys, v rows past the end are zeroed, and a tile whose v holds values
 // that are not finite is mended: those values are taken out of the product and
 // added to the rows that see them.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
 #include <algorithm>
 #include <mutex>
 
-#include "cw_gemm.cuh"
-#include "cw_tree.cuh"
+#include "cw_tree_tc.cuh"
 
 namespace cw {
-
-constexpr int TT_STAGES = 16;  // most stages of the ring (one K or V tile each)
-constexpr uint64_t TT_WAIT_NS = 2000000000ull;
 
 // A parity wait tells a phase from the one before it only, so a barrier that is
 // waited on once per tile is doubled by tile parity: when tile n - 1's phase is
@@ -49,150 +42,8 @@ struct TtBars {
     uint64_t q_full[2], s_full[2][2], p_full[2][2], pv[2][2], done;  // [row block][tile % 2]
     uint32_t tmem, failed;
     TreeShared run;
-    float2 ml[128];  // maximum (times log2 e) and sum of each lane's part of a row
 };
 
-__device__ __forceinline__ void tt_ld32(uint32_t addr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
-        "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(addr));
-}
-__device__ __forceinline__ void tt_st32(uint32_t addr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
-        "%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-        "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-template <int N> __device__ __forceinline__ void tt_st(uint32_t addr, const uint32_t* r) {
-    if constexpr (N == 32) {
-        tt_st32(addr, r);
-    } else if constexpr (N == 16) {
-        asm volatile(
-            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-            "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
-            "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-            "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-            "r"(r[15])
-            : "memory");
-    } else {
-        asm volatile(
-            "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
-            "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-            : "memory");
-    }
-}
-// Waits for this thread's TMEM loads; the values pass through, so no use of them can
-// be moved before it.
-__device__ __forceinline__ void tt_wait_ld32(uint32_t* r) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
-                   "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
-                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]),
-                   "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
-}
-// N columns, waited for.
-template <int N> __device__ __forceinline__ void tt_load(uint32_t addr, uint32_t* r) {
-    if constexpr (N == 64) {
-        tt_ld32(addr, r);
-        tt_ld32(addr + 32, r + 32);
-        tt_wait_ld32(r);
-        tt_wait_ld32(r + 32);
-    } else if constexpr (N == 32) {
-        tt_ld32(addr, r);
-        tt_wait_ld32(r);
-    } else {
-        tmem_ld16(addr, *(uint32_t(*)[16])r);
-        asm volatile("tcgen05.wait::ld.sync.aligned;"
-                     : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
-                       "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                       "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
-    }
-}
-__device__ __forceinline__ uint32_t tt_ld1(uint32_t addr) {
-    uint32_t r;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(addr));
-    return r;
-}
-__device__ __forceinline__ void tt_st1(uint32_t addr, uint32_t r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(addr), "r"(r)
-                 : "memory");
-}
-__device__ __forceinline__ void tt_wait_st() {
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tt_fence_async() {
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-}
-// D[tmem] += A[tmem] B[shared], in the TMEM lanes whose bits in off0 (lanes 0-31) ..
-// off3 (lanes 96-127) are 0.
-__device__ __forceinline__ void tt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                          uint32_t off0, uint32_t off1, uint32_t off2,
-                                          uint32_t off3) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, 1, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%4, %5, %6, %7}, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(off0), "r"(off1), "r"(off2), "r"(off3)
-        : "memory");
-}
-// Matrix descriptor of an operand whose contraction index is the row (V: keys x
-// dims) in 128-byte swizzled 64-element columns: column blocks `block` bytes apart,
-// 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t tt_desc_rows(uint32_t saddr, uint32_t block) {
-    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(block >> 4) << 16) |
-           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-template <bool BF> __host__ __device__ constexpr uint32_t tt_idesc(int n, bool b_rows) {
-    return (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | (b_rows ? 1u << 16 : 0u) |
-           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
-__device__ __forceinline__ float tt_exp2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-// Two weights rounded and packed (first in the low half), their rounded values added.
-template <bool BF> __device__ __forceinline__ uint32_t tt_pack(float x, float y, float& sum) {
-    uint32_t r;
-    if (BF) {
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
-        sum += __uint_as_float(r << 16) + __uint_as_float(r & 0xffff0000u);
-    } else {
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
-        const float2 f = __half22float2(*(const __half2*)&r);
-        sum += f.x + f.y;
-    }
-    return r;
-}
-template <bool BF> __device__ __forceinline__ float tt_value(uint32_t bits16) {
-    if (BF) return __uint_as_float(bits16 << 16);
-    return __half2float(__ushort_as_half((unsigned short)bits16));
-}
-template <bool BF> __device__ __forceinline__ bool tt_odd(uint32_t bits16) {
-    const uint32_t e = BF ? 0x7f80u : 0x7c00u;
-    return (bits16 & e) == e;
-}
-template <bool BF> __device__ __forceinline__ bool tt_odd8(const uint4& x) {
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < 4; i++) odd |= tt_odd<BF>(w[i] & 0xffffu) | tt_odd<BF>(w[i] >> 16);
-    return odd;
-}
 // Barrier and OR over the threads of the item's active row blocks (one named barrier
 // for each count: a block may run ahead through items that are not its own).
 __device__ __forceinline__ bool tt_any(bool x, int blocks) {
@@ -206,50 +57,43 @@ __device__ __forceinline__ bool tt_any(bool x, int blocks) {
     return r != 0;
 }
 
-// A place in the ring.  An item's tiles pass through it in the order K0, then K(i+1),
-// V(i) in turn: 2 * tiles places.
-struct TtPlace {
-    int stage;
-    uint32_t phase;
-    __device__ __forceinline__ void next(int stages) {
-        if (++stage == stages) {
-            stage = 0;
-            phase ^= 1;
-        }
-    }
-    __device__ __forceinline__ void skip(int n, int stages) {
-        stage += n;
-        while (stage >= stages) {
-            stage -= stages;
-            phase ^= 1;
-        }
-    }
+// The shapes of one instance.  HD: head dims rounded up; a thread's keys of a tile
+// are KEYS consecutive ones, so SPLIT lanes share a row.
+template <int HD, int NB, int SPLIT> struct TtShape {
+    static constexpr int COLS = HD / 64;                // 64-element column blocks
+    static constexpr int TILE = HD <= 128 ? 128 : 64;   // keys of a tile
+    static constexpr int SK = HD <= 64 ? 128 : 64;      // keys of a ring stage
+    static constexpr int HALVES = TILE / SK;            // stages of a K or V tile
+    static constexpr int STAGE = COLS * SK * 128;
+    // TMEM of a row block: SB buffers of scores, then O.  Two fit beside 256 dims (one
+    // CTA per SM, which has to overlap its own steps); below, 128-key tiles with one
+    // buffer halve the hand-overs per key, and the SM's other CTA or row block fills
+    // the gaps.
+    static constexpr int SB = HD <= 128 ? 1 : 2;
+    static constexpr int TCOLS = SB * TILE + HD;
+    static constexpr uint32_t TMEM = NB * TCOLS <= 256 ? 256 : 512;
+    static constexpr int THREADS = NB * 128 + 64;
+    static constexpr int PER_SM = NB == 1 && HD <= 128 ? 2 : 1;
+    static constexpr int KEYS = TILE / SPLIT;
+    static constexpr int LANES = 128 / SPLIT;           // rows of a row block
 };
-__device__ __forceinline__ bool tt_elect() {  // one lane of a converged warp
-    uint32_t r;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(r));
-    return r != 0;
-}
 
 template <bool BF, int HD, int NB, int SPLIT>
-__global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
     k_tree_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
               const __grid_constant__ TreeArgs a, int stages, int q_rows) {
-    constexpr int COLS = HD / 64;             // 64-element column blocks of a row
-    constexpr int STAGE = COLS * TR_TILE * 128;
-    constexpr int TCOLS = 128 + HD;           // TMEM columns of a row block: S0, S1, O
-    constexpr uint32_t TMEM = NB * TCOLS <= 256 ? 256 : 512;
-    constexpr int THREADS = NB * 128 + 64;
-    constexpr int KEYS = TR_TILE / SPLIT;     // keys of a tile that a thread weighs
-    constexpr int LANES = 128 / SPLIT;        // rows of a row block
+    typedef TtShape<HD, NB, SPLIT> Z;
+    constexpr int COLS = Z::COLS, TILE = Z::TILE, SK = Z::SK, HALVES = Z::HALVES, SB = Z::SB;
+    constexpr int STAGE = Z::STAGE, TCOLS = Z::TCOLS, KEYS = Z::KEYS, LANES = Z::LANES;
     static_assert(NB == 1 || SPLIT == 1, "a split row block is the only one");
+    static_assert(SB == 1 || HALVES == 1, "the ring's order");
     extern __shared__ __align__(1024) uint8_t sm[];
     const int q_block = q_rows * 128;         // bytes of a column block of the queries
     uint8_t* s_q = sm;                        // [NB][COLS][q_rows][128]
     uint8_t* ring = sm + NB * COLS * q_block;
     TtBars* bars = (TtBars*)(ring + stages * STAGE);
+    // reference and sum of each lane's part of a row, when the queries are done with
+    float2* s_ml = HD > 64 ? (float2*)(s_q + 128 * 128) : (float2*)(bars + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_trigger();
     // the swizzle counts from 1024-byte boundaries; no static shared memory precedes
@@ -257,7 +101,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
         if (tid == 0) tree_bad(a);
         return;
     }
-    if (warp == 0) tmem_alloc(&bars->tmem, TMEM);
+    if (warp == 0) tmem_alloc(&bars->tmem, Z::TMEM);
     if (tid == 32) {
         for (int s = 0; s < stages; s++) {
             mbar_init(&bars->full[s], 1);
@@ -275,187 +119,179 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
         bars->failed = 0;
         fence_mbar_init();
     }
-    TreeRun run = tree_run<THREADS>(a, &bars->run);
+    TreeRun run = tree_run<Z::THREADS>(a, &bars->run);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = bars->tmem;
-    // A wait that gives up sets `failed`, and later waits return at once: the TMA and
-    // MMA loops end, the softmax warps (which meet at barriers) run through their
-    // items without waiting.
-    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-        if (mbar_try_wait(bar, parity & 1)) return true;
-        if (*(volatile uint32_t*)&bars->failed) return false;
-        const uint64_t from = global_ns();
-        do {
-            for (int i = 0; i < 256; i++)  // reading the clock would delay the wake-up
-                if (mbar_try_wait(bar, parity & 1)) return true;
-        } while (global_ns() - from < TT_WAIT_NS);
-        gm_fail(a.status);
-        *(volatile uint32_t*)&bars->failed = 1;
-        return false;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return tt_wait(bar, parity, &bars->failed, a.status);
     };
+    auto all = [&](uint64_t* bar, uint32_t parity) {  // the same answer for the warp
+        return __all_sync(FULL, wait(bar, parity)) != 0;
+    };
+    // barrier and phase of tile n of a row block, where its scores' buffer is reused
+    auto buf = [](uint32_t n) { return SB == 2 ? n & 1 : 0u; };
+    auto turn = [](uint32_t n) { return SB == 2 ? n >> 1 : n; };
     TreeItem it;
     bool any = false, ok = true;
+    const bool wide = a.D % 64 == 0;
+    const TtTile tile = wide ? TtTile{COLS * 1024, 1024} : TtTile{1024, SK * 128};
     TtPlace at = {0, 0};
 
     if (warp == NB * 4) {  // ---- TMA: all lanes, a box each
-        const int per = a.page < TR_TILE ? TR_TILE / a.page : 1;  // pages of a tile
-        const int box = min(a.page, TR_TILE);
-        const int pi = lane / COLS, col = lane - pi * COLS;
+        TtFeed<COLS, SK> feed(a, ring, bars->full, bars->empty, stages, tile);
         if (lane == 0) {
             tma_prefetch_desc(&map_k);
             tma_prefetch_desc(&map_v);
         }
-        const int shift = (a.page & (a.page - 1)) == 0 ? __ffs(a.page) - 1 : -1;
-        bool full = false;  // every stage has been filled once
+        auto load = [&](const CUtensorMap* map, int group) {
+            ok = ok && feed.load(map, group, all);
+        };
         while (run.left > 0 && ok) {
             it = tree_next(a, run);
-            const int key0 = (it.q.tile0 + it.tile) * TR_TILE + pi * box;
-            const int* row = a.table + (size_t)it.r * a.max_pages;
-            // the page of the lane's box of tile i, read a tile ahead of its use
-            auto page_of = [&](int i) -> int {
-                const int key = key0 + i * TR_TILE;
-                if (pi >= per || i >= it.tiles || key >= it.q.keys) return -1;
-                return row[shift >= 0 ? key >> shift : key / a.page];
-            };
-            // that box's row in the cache as [rows][D], or -1
-            auto place = [&](int i, int id) -> int {
-                const int key = key0 + i * TR_TILE;
-                if (pi >= per || i >= it.tiles || key >= it.q.keys) return -1;
-                if (id < 0 || id >= a.n_pages) {
-                    tree_bad(a);
-                    return -1;
+            feed.begin(it);
+            const int tiles = (it.tiles * TR_TILE + TILE - 1) / TILE;
+            int now[HALVES];
+#pragma unroll
+            for (int h = 0; h < HALVES; h++) now[h] = feed.place(h);
+#pragma unroll
+            for (int h = 0; h < HALVES; h++) load(&map_k, now[h]);
+            for (int i = 0; i < tiles && ok; i++) {
+                int next[HALVES];
+#pragma unroll
+                for (int h = 0; h < HALVES; h++) next[h] = feed.place((i + 1) * HALVES + h);
+                if (SB == 2 && i + 1 < tiles) load(&map_k, next[0]);
+#pragma unroll
+                for (int h = 0; h < HALVES; h++) load(&map_v, now[h]);
+                if (SB == 1 && i + 1 < tiles) {
+#pragma unroll
+                    for (int h = 0; h < HALVES; h++) load(&map_k, next[h]);
                 }
-                const int in = shift >= 0 ? key & (a.page - 1) : key % a.page;
-                return (id * a.K + it.head) * a.page + in;
-            };
-            auto load = [&](const CUtensorMap* map, int at_row) -> bool {
-                const int s = at.stage;
-                if (full && !__all_sync(FULL, wait(&bars->empty[s], at.phase ^ 1))) return false;
-                const uint32_t live = __ballot_sync(FULL, at_row >= 0);
-                if (lane == 0) mbar_expect_tx(&bars->full[s], __popc(live) * box * 128);
-                __syncwarp();
-                if (at_row >= 0)
-                    tma_load_2d(ring + s * STAGE + col * (TR_TILE * 128) + pi * box * 128, map,
-                                col * 64, at_row, &bars->full[s]);
-                at.next(stages);
-                full |= at.stage == 0;
-                return true;
-            };
-            int id = page_of(1), now = place(0, page_of(0));
-            ok = load(&map_k, now);
-            for (int i = 0; i < it.tiles && ok; i++) {
-                const int next = place(i + 1, id);
-                id = page_of(i + 2);
-                if (i + 1 < it.tiles) ok = load(&map_k, next);
-                ok = ok && load(&map_v, now);
-                now = next;
+#pragma unroll
+                for (int h = 0; h < HALVES; h++) now[h] = next[h];
             }
         }
-        if (!ok)  // copies in flight land before the block may end
-            for (int s = 0; s < stages; s++)
-                if (full || s < at.stage)  // the last filling of stage s
-                    (void)mbar_wait(&bars->full[s], s < at.stage ? at.phase : at.phase ^ 1,
-                                    TT_WAIT_NS);
+        if (!ok) feed.drain();
     } else if (warp == NB * 4 + 1) {  // ---- MMA: the warp waits, one lane issues
-        constexpr uint32_t id_s = tt_idesc<BF>(TR_TILE, false);
-        constexpr uint32_t id_o = tt_idesc<BF>(HD, true);
-        const uint64_t q0 = umma_desc_sw128(smem_addr(s_q)), k0 = umma_desc_sw128(smem_addr(ring)),
-                       v0 = tt_desc_rows(smem_addr(ring), TR_TILE * 128);
+        constexpr uint32_t id_s = tt_idesc<BF>(SK, false, false);
+        constexpr uint32_t id_o = tt_idesc<BF>(HD, false, true);
+        const uint64_t q0 = umma_desc_sw128(smem_addr(s_q)), kv0 = tt_desc(smem_addr(ring), tile);
+        const int steps = (a.D + 15) / 16;
         const bool one = tt_elect();
-        auto all = [&](uint64_t* bar, uint32_t parity) {
-            return __all_sync(FULL, wait(bar, parity)) != 0;
-        };
         uint32_t n[2] = {0, 0}, items[2] = {0, 0};  // tiles and items of each row block
         while (run.left > 0 && ok) {
             it = tree_next(a, run);
             const int blocks = it.rows > 128 ? NB : 1;
+            const int tiles = (it.tiles * TR_TILE + TILE - 1) / TILE;
             for (int b = 0; b < blocks && ok; b++) ok = all(&bars->q_full[b], items[b]++);
-            auto scores = [&](int i) {
-                const int s = at.stage;
-                ok = ok && all(&bars->full[s], at.phase);
-                at.next(stages);
+            // S = Q K^T of tile i for row block b; K's stages from place k
+            auto scores = [&](int i, int b, TtPlace k) {
+                const uint32_t m = n[b] + i;
+                // this buffer's weights went into the product of tile i - SB
+                if (i >= SB) ok = ok && all(&bars->pv[b][(m - SB) & 1], (m - SB) >> 1);
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    if (b >= blocks) break;
-                    const uint32_t m = n[b] + i;
-                    // this buffer's weights went into the product of tile i - 2
-                    if (i >= 2) ok = ok && all(&bars->pv[b][m & 1], (m - 2) >> 1);
+                for (int h = 0; h < HALVES; h++, k.next(stages)) {
+                    if (b == 0) ok = ok && all(&bars->full[k.stage], k.phase);
                     tc_fence_after();
                     if (one && ok) {
-                        const uint32_t d = tmem + b * TCOLS + (m & 1) * 64;
+                        const uint32_t d = tmem + b * TCOLS + buf(m) * TILE + h * SK;
                         const uint64_t dq = q0 + ((b * COLS * q_block) >> 4),
-                                       dk = k0 + ((s * STAGE) >> 4);
+                                       dk = kv0 + ((k.stage * STAGE) >> 4);
 #pragma unroll
-                        for (int k = 0; k < HD / 16; k++)
-                            umma_f16(d, dq + (((k >> 2) * q_block + (k & 3) * 32) >> 4),
-                                     dk + (((k >> 2) * (TR_TILE * 128) + (k & 3) * 32) >> 4), id_s,
-                                     k > 0);
-                        tc_commit(&bars->s_full[b][m & 1]);
-                        if (b + 1 == blocks) tc_commit(&bars->empty[s]);
+                        for (int x = 0; x < HD / 16; x++)
+                            if (x < steps)
+                                umma_f16(d, dq + (((x >> 2) * q_block + (x & 3) * 32) >> 4),
+                                         dk + (((x >> 2) * tile.col + (x & 3) * 32) >> 4), id_s,
+                                         x > 0);
+                        if (b + 1 == blocks) tc_commit(&bars->empty[k.stage]);
+                        if (h + 1 == HALVES) tc_commit(&bars->s_full[b][buf(m)]);
                     }
                     __syncwarp();
                 }
             };
-            scores(0);
-            for (int i = 0; i < it.tiles && ok; i++) {
-                if (i + 1 < it.tiles) scores(i + 1);
-                const int s = at.stage;
-                ok = ok && all(&bars->full[s], at.phase);
-                at.next(stages);
+            // O += P V; V's stages from place v
+            auto values = [&](int i, int b, TtPlace v) {
+                const uint32_t m = n[b] + i;
+                ok = ok && all(&bars->p_full[b][buf(m)], turn(m));
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    if (b >= blocks) break;
-                    const uint32_t m = n[b] + i;
-                    ok = ok && all(&bars->p_full[b][m & 1], m >> 1);
+                for (int h = 0; h < HALVES; h++, v.next(stages)) {
+                    if (b == 0) ok = ok && all(&bars->full[v.stage], v.phase);
                     tc_fence_after();
                     if (one && ok) {
-                        const uint32_t p = tmem + b * TCOLS + (m & 1) * 64;
-                        const uint64_t dv = v0 + ((s * STAGE) >> 4);
-                        // keys 16k..16k+15 go to the lanes that weigh them
+                        const uint32_t p = tmem + b * TCOLS + buf(m) * TILE + h * (SK / 2);
+                        const uint64_t dv = kv0 + ((v.stage * STAGE) >> 4);
+                        // 16 keys go to the lanes that weigh them
 #pragma unroll
-                        for (int k = 0; k < TR_TILE / 16; k++) {
+                        for (int x = 0; x < SK / 16; x++) {
                             auto off = [&](int quad) {
-                                return k * 16 / KEYS == quad * 32 / LANES ? 0u : ~0u;
+                                return (h * SK + x * 16) / KEYS == quad * 32 / LANES ? 0u : ~0u;
                             };
-                            tt_mma_ts(tmem + b * TCOLS + 128, p + 8 * k,
-                                      dv + ((k * 16 * 128) >> 4), id_o, off(0), off(1), off(2),
-                                      off(3));
+                            tt_mma_ts(tmem + b * TCOLS + SB * TILE, p + 8 * x,
+                                      dv + ((x * 2 * tile.group) >> 4), id_o, off(0), off(1),
+                                      off(2), off(3));
                         }
-                        tc_commit(&bars->pv[b][m & 1]);
-                        if (b + 1 == blocks) tc_commit(&bars->empty[s]);
+                        if (b + 1 == blocks) tc_commit(&bars->empty[v.stage]);
+                        if (h + 1 == HALVES) tc_commit(&bars->pv[b][m & 1]);
                     }
                     __syncwarp();
                 }
+            };
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+                if (b < blocks) scores(0, b, at);
+            at.skip(HALVES, stages);
+            for (int i = 0; i < tiles && ok; i++) {
+                TtPlace k = at, v = at;
+                const bool more = i + 1 < tiles;
+                if (SB == 2 && more) v.skip(1, stages);  // K(i+1) lies before V(i)
+                if (SB == 1) k.skip(HALVES, stages);
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+                    if (b < blocks) {
+                        if (SB == 2 && more) scores(i + 1, b, k);
+                        values(i, b, v);
+                        if (SB == 1 && more) scores(i + 1, b, k);
+                    }
+                at.skip(more ? 2 * HALVES : HALVES, stages);
             }
-            for (int b = 0; b < blocks; b++) n[b] += it.tiles;
+            for (int b = 0; b < blocks; b++) n[b] += tiles;
         }
         // every product issued has ended before the block frees its TMEM
         if (one) tc_commit(&bars->done);
         (void)mbar_wait(&bars->done, 0, TT_WAIT_NS);
         __syncwarp();
-    } else {  // ---- softmax: a thread per row
+    } else {  // ---- softmax: a thread per row and part of the keys
         // lane m weighs keys [part * KEYS, ..+KEYS) of each tile for row r
         const int b = warp >> 2, m = tid & 127, r = m % LANES, part = m / LANES;
         const uint32_t lanes = tmem + b * TCOLS + ((uint32_t)(warp & 3) << 21);
-        const uint32_t t_o = lanes + 128;
+        const uint32_t t_o = lanes + SB * TILE;
         uint32_t n = 0;
         const float log2e = 1.44269504088896341f;
-        const float c2 = a.softcap > 0.f ? log2e : a.scale * log2e;
+        const bool cap = a.softcap > 0.f;
+        const float c2 = cap ? log2e : a.scale * log2e;
+        const float y2 = cap ? 2.f * log2e * a.scale / a.softcap : 0.f;
+        // a score with the cap: tanh(y) = 1 - 2 / (1 + e^2y), off by 2^-22, times
+        // softcap far below one rounding of the weight
+        auto capped = [&](float s) {
+            const float y = s * y2;
+            return a.softcap - __fdividef(2.f * a.softcap, 1.f + tt_exp2(y > 120.f ? 120.f : y));
+        };
         uint8_t* q_sm = s_q + b * COLS * q_block;
         while (run.left > 0) {
             it = tree_next(a, run);
             any = true;
             const int blocks = it.rows > 128 ? NB : 1;
+            const int tiles = (it.tiles * TR_TILE + TILE - 1) / TILE;
             TtPlace at_v = at;  // of the item's first V tile
-            at_v.skip(it.tiles > 1 ? 2 : 1, stages);
-            at.skip(2 * it.tiles % (2 * stages), stages);
+            at_v.skip(SB == 2 && tiles > 1 ? 2 : HALVES, stages);
+            at.skip(2 * HALVES * tiles % (2 * stages), stages);
             if (b >= blocks) continue;
             const int m0 = it.block * a.bm + b * 128;       // row 0 of the request's rows
             const int rows = min(it.rows - b * 128, 128);
             const bool work = (warp & 3) * 32 % LANES < rows;  // the warp has rows
             const int key0 = (it.q.tile0 + it.tile) * TR_TILE;
+            const int end = min(it.q.keys, key0 + it.tiles * TR_TILE);  // of this piece's keys
             // ---- queries, and this row's window
             for (int i = m; i < rows * COLS * 8; i += 128) {
                 const int qr = i / (COLS * 8), c = i % (COLS * 8);
@@ -490,58 +326,60 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->q_full[b]);
-            float top = -INFINITY, ref_m = -INFINITY, sum = 0.f;
-            for (int i = 0; i < it.tiles; i++, n++) {
-                const int kt = key0 + i * TR_TILE;
-                const bool mixed = tree_partial(it.q, edge_max, kt);
-                uint64_t sees = ~0ull;
-                if (mixed && work && (kt < edge || kt + TR_TILE > it.q.len))
-                    sees = r < rows ? tree_sees(a, it.q, m0 + r, kt) : 0;
-                wait(&bars->s_full[b][n & 1], n >> 1);
+            // running maximum of the scores, the weights' reference (in powers of two),
+            // and the sum of the weights
+            float top = -INFINITY, ref = -INFINITY, sum = 0.f;
+            for (int i = 0; i < tiles; i++, n++) {
+                const int kt = key0 + i * TILE;
+                const bool mixed = kt + TILE > end || kt + TILE > it.q.len || kt < edge_max;
+                uint64_t sees[2] = {~0ull, ~0ull};  // this row's, of all the tile's keys
+                if (mixed) {
+#pragma unroll
+                    for (int h = 0; h < TILE / 64; h++) {
+                        const int k = kt + h * 64;
+                        if (k < edge || k + 64 > it.q.len || k + 64 > end)
+                            sees[h] = r < rows && k < end ? tree_sees(a, it.q, m0 + r, k) : 0;
+                    }
+                }
+                const uint64_t mine = (part * KEYS < 64 ? sees[0] : sees[1]) >> (part * KEYS % 64);
+                wait(&bars->s_full[b][buf(n)], turn(n));
                 __syncwarp();
                 tc_fence_after();
-                const uint32_t t_s = lanes + (n & 1) * 64;
+                const uint32_t t_s = lanes + buf(n) * TILE;
                 if (work) {
-                    float s[KEYS];
-                    tt_load<KEYS>(t_s + part * KEYS, (uint32_t*)s);
-                    if (a.softcap > 0.f) {
-                        // tanh(y) = 1 - 2 / (1 + e^2y): off by 2^-22, times softcap a
-                        // score error far below one rounding of the weight
-                        const float y2 = 2.f * log2e * a.scale / a.softcap;
+                    constexpr int CH = KEYS < 64 ? KEYS : 64;  // scores held at a time
+                    float s[CH];
+                    float t0 = top, t1 = top, t2 = top, t3 = top;
+                    uint64_t seen = mine;
+#pragma unroll 1
+                    for (int h = 0; h < KEYS / CH; h++) {
+                        tt_load<CH>(t_s + part * KEYS + h * CH, (uint32_t*)s);
+                        if (KEYS > 64) seen = h ? sees[1] : sees[0];
+                        if (mixed) {
 #pragma unroll
-                        for (int j = 0; j < KEYS; j++) {
-                            const float y = s[j] * y2;
-                            s[j] = a.softcap - __fdividef(2.f * a.softcap,
-                                                          1.f + tt_exp2(y > 120.f ? 120.f : y));
+                            for (int j = 0; j < CH; j++)
+                                if (!(seen >> j & 1)) s[j] = -INFINITY;
                         }
-                    }
-                    if (mixed) {
 #pragma unroll
-                        for (int j = 0; j < KEYS; j++)
-                            if (!(sees >> (part * KEYS + j) & 1)) s[j] = -INFINITY;
-                    }
-                    float t0 = top, t1 = s[1], t2 = s[2], t3 = s[3];
-                    t0 = fmaxf(t0, s[0]);
-#pragma unroll
-                    for (int j = 4; j < KEYS; j += 4) {
-                        t0 = fmaxf(t0, s[j]);
-                        t1 = fmaxf(t1, s[j + 1]);
-                        t2 = fmaxf(t2, s[j + 2]);
-                        t3 = fmaxf(t3, s[j + 3]);
+                        for (int j = 0; j < CH; j += 4) {
+                            t0 = fmaxf(t0, s[j]);
+                            t1 = fmaxf(t1, s[j + 1]);
+                            t2 = fmaxf(t2, s[j + 2]);
+                            t3 = fmaxf(t3, s[j + 3]);
+                        }
                     }
                     top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+                    const float want = top == -INFINITY ? -INFINITY : (cap ? capped(top) : top) * c2;
                     if (i == 0) {
-                        ref_m = top;
-                    } else if (__any_sync(FULL, r < rows && (top - ref_m) * c2 > 8.f)) {
-                        const float fix = ref_m == -INFINITY ? 0.f : tt_exp2((ref_m - top) * c2);
-                        wait(&bars->pv[b][(n - 1) & 1], (n - 1) >> 1);  // O holds the tiles before this one
+                        ref = want;
+                    } else if (__any_sync(FULL, r < rows && want - ref > 8.f)) {
+                        const float fix = ref == -INFINITY ? 0.f : tt_exp2(ref - want);
+                        wait(&bars->pv[b][(n - 1) & 1], (n - 1) >> 1);  // O: the tiles so far
                         __syncwarp();
                         tc_fence_after();
-                        if (top > ref_m) {
-                            sum *= fix;
-                            ref_m = top;
-                        }
-#pragma unroll
+                        sum *= fix;
+                        ref = want;
+#pragma unroll 1
                         for (int c = 0; c < HD; c += 32) {
                             uint32_t o[32];
                             tt_ld32(t_o + c, o);
@@ -552,28 +390,55 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
                             tt_st32(t_o + c, o);
                         }
                     }
-                    const float ref = ref_m == -INFINITY ? 0.f : ref_m * c2;
-                    uint32_t p[KEYS / 2];
+                    const float from = ref == -INFINITY ? 0.f : ref;
                     float l0 = 0.f, l1 = 0.f;
+#pragma unroll 1
+                    for (int h = 0; h < KEYS / CH; h++) {
+                        if (KEYS > CH) {
+                            tt_load<CH>(t_s + h * CH, (uint32_t*)s);
+                            seen = h ? sees[1] : sees[0];
+                        }
+                        uint32_t p[CH / 2];
+                        if (cap) {
 #pragma unroll
-                    for (int j = 0; j < KEYS / 2; j += 2) {
-                        p[j] = tt_pack<BF>(tt_exp2(fmaf(s[2 * j], c2, -ref)),
-                                           tt_exp2(fmaf(s[2 * j + 1], c2, -ref)), l0);
-                        p[j + 1] = tt_pack<BF>(tt_exp2(fmaf(s[2 * j + 2], c2, -ref)),
-                                               tt_exp2(fmaf(s[2 * j + 3], c2, -ref)), l1);
+                            for (int j = 0; j < CH; j++) s[j] = capped(s[j]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < CH; j++) s[j] = tt_exp2(fmaf(s[j], c2, -from));
+                        if (mixed) {
+#pragma unroll
+                            for (int j = 0; j < CH; j++)
+                                if (!(seen >> j & 1)) s[j] = 0.f;
+                        }
+#pragma unroll
+                        for (int j = 0; j < CH / 2; j += 2) {
+                            p[j] = tt_pack<BF>(s[2 * j], s[2 * j + 1], l0);
+                            p[j + 1] = tt_pack<BF>(s[2 * j + 2], s[2 * j + 3], l1);
+                        }
+                        // over scores that this thread has read (weight j of a part lies
+                        // at half the part's column or before it)
+                        tt_st<CH / 2>(t_s + part * (KEYS / 2) + h * (CH / 2), p);
                     }
                     sum += l0 + l1;
-                    tt_st<KEYS / 2>(t_s + part * (KEYS / 2), p);
                     tt_wait_st();
                 }
                 if (mixed) {  // v rows past the end, and values that are not finite
+                    TtPlace v1 = at_v;
                     wait(&bars->full[at_v.stage], at_v.phase);
-                    uint8_t* v = ring + at_v.stage * STAGE;
-                    const int live = min(it.q.keys - kt, TR_TILE);
+                    if (HALVES == 2) {
+                        v1.next(stages);
+                        wait(&bars->full[v1.stage], v1.phase);
+                    }
+                    __syncwarp();
+                    uint8_t* v[2] = {ring + at_v.stage * STAGE, ring + v1.stage * STAGE};
+                    auto chunk = [&](int j, int c) {
+                        return v[HALVES == 2 ? j / SK : 0] + tile.at(j % SK, c);
+                    };
+                    const int live = end - kt;
                     bool odd = false;
-                    for (int x = b * 128 + m; x < COLS * TR_TILE * 8; x += blocks * 128) {
-                        uint4* w = (uint4*)(v + x * 16);  // row (x / 8) % 64 of its column block
-                        if ((x >> 3) % TR_TILE >= live) *w = make_uint4(0, 0, 0, 0);
+                    for (int x = b * 128 + m; x < COLS * TILE * 8; x += blocks * 128) {
+                        uint4* w = (uint4*)chunk(x / (COLS * 8), x % (COLS * 8));
+                        if (x / (COLS * 8) >= live) *w = make_uint4(0, 0, 0, 0);
                         else odd |= tt_odd8<BF>(*w);
                     }
                     if (tt_any(odd, blocks)) {
@@ -581,23 +446,23 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
                             if (i > 0) wait(&bars->pv[b][(n - 1) & 1], (n - 1) >> 1);
                             __syncwarp();
                             tc_fence_after();
-                            for (int j = 0; j < live; j++)
+#pragma unroll 1
+                            for (int j = 0; j < min(live, TILE); j++)
+#pragma unroll 1
                                 for (int c = 0; c < COLS * 8; c++) {
-                                    const uint4 x = *(const uint4*)(v + (c >> 3) * (TR_TILE * 128) +
-                                                                    j * 128 +
-                                                                    (((c & 7) ^ (j & 7)) << 4));
+                                    const uint4 x = *(const uint4*)chunk(j, c);
                                     if (!tt_odd8<BF>(x)) continue;
-                                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll 1
                                     for (int e = 0; e < 8; e++) {
-                                        const uint32_t bits = e & 1 ? w[e >> 1] >> 16
-                                                                    : w[e >> 1] & 0xffffu;
+                                        const uint32_t bits = ((const uint16_t*)chunk(j, c))[e];
                                         if (!tt_odd<BF>(bits)) continue;
                                         uint32_t pj = tt_ld1(t_s + (j >> 1));
                                         uint32_t oj = tt_ld1(t_o + c * 8 + e);
                                         asm volatile("tcgen05.wait::ld.sync.aligned;"
                                                      : "+r"(pj), "+r"(oj)::"memory");
                                         float o = __uint_as_float(oj);
-                                        if ((sees >> j & 1) && j / KEYS == part)
+                                        const uint64_t see = j < 64 ? sees[0] : sees[1];
+                                        if ((see >> (j & 63) & 1) && j / KEYS == part)
                                             o = fmaf(tt_value<BF>(j & 1 ? pj >> 16 : pj & 0xffffu),
                                                      tt_value<BF>(bits), o);
                                         __syncwarp();
@@ -607,8 +472,8 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
                                 }
                         }
                         (void)tt_any(false, blocks);  // all have read them
-                        for (int x = b * 128 + m; x < COLS * TR_TILE * 8; x += blocks * 128) {
-                            uint16_t* w = (uint16_t*)(v + x * 16);
+                        for (int x = b * 128 + m; x < COLS * TILE * 8; x += blocks * 128) {
+                            uint16_t* w = (uint16_t*)chunk(x / (COLS * 8), x % (COLS * 8));
                             for (int e = 0; e < 8; e++)
                                 if (tt_odd<BF>(w[e])) w[e] = 0;
                         }
@@ -619,8 +484,8 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bars->p_full[b][n & 1]);
-                at_v.skip(i + 2 < it.tiles ? 2 : 1, stages);
+                if (lane == 0) mbar_arrive(&bars->p_full[b][buf(n)]);
+                at_v.skip(SB == 2 ? (i + 2 < tiles ? 2 : 1) : 2 * HALVES, stages);
             }
             // ---- the item's end
             wait(&bars->pv[b][(n - 1) & 1], (n - 1) >> 1);
@@ -631,7 +496,6 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
             const int node = (m0 + r) / a.G, gi = (m0 + r) - node * a.G;
             uint16_t* out = (uint16_t*)a.out +
                             ((long long)(it.q.row0 + node) * a.H + it.head * a.G + gi) * a.D;
-            const float top2 = ref_m == -INFINITY ? -INFINITY : ref_m * c2;
             // N f32 sums of columns c.. of this row: the result, or the partial state
             auto put = [&](const float* o, int c, float inv) {
                 if (it.whole) {
@@ -648,7 +512,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
             };
             if constexpr (SPLIT == 1) {
                 const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-                if (r < rows && !it.whole) a.ml[piece] = make_float2(top2, sum);
+                if (r < rows && !it.whole) a.ml[piece] = make_float2(ref, sum);
                 if (work) {
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 32) {
@@ -663,17 +527,17 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
             } else {
                 // join the SPLIT parts of each row: 32 columns at a time through the
                 // queries' place, 16-byte chunks exclusive-ored with the lane
-                bars->ml[m] = make_float2(top2, sum);
+                s_ml[m] = make_float2(ref, sum);
                 (void)tt_any(false, 1);
                 float top = -INFINITY, l = 0.f;
 #pragma unroll
-                for (int s = 0; s < SPLIT; s++) top = fmaxf(top, bars->ml[s * LANES + r].x);
+                for (int s = 0; s < SPLIT; s++) top = fmaxf(top, s_ml[s * LANES + r].x);
 #pragma unroll
                 for (int s = 0; s < SPLIT; s++) {
-                    const float2 x = bars->ml[s * LANES + r];
+                    const float2 x = s_ml[s * LANES + r];
                     if (x.x != -INFINITY) l += x.y * tt_exp2(x.x - top);
                 }
-                const float own = top2 == -INFINITY ? 0.f : tt_exp2(top2 - top);
+                const float own = ref == -INFINITY ? 0.f : tt_exp2(ref - top);
                 const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
                 if (r < rows && part == 0 && !it.whole) a.ml[piece] = make_float2(top, l);
 #pragma unroll 1
@@ -717,7 +581,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, NB == 1 && HD <= 128 ? 2 : 1)
     if (tid == 0) tree_record(a, run, it, any);
     if (warp == 0) {
         tc_fence_after();
-        tmem_dealloc(tmem, TMEM);
+        tmem_dealloc(tmem, Z::TMEM);
     }
 }
 
@@ -735,19 +599,39 @@ static PFN_cuTensorMapEncodeTiled_v12000 tt_encode_fn() {
     return fn;
 }
 
-// The cache as [n_pages * K * page rows][D], boxes of one page (64 rows at most) by
-// 64 elements; columns past D read zeros.
-static int tt_map(CUtensorMap* map, const void* base, const TreeArgs& a, bool bf) {
+// The cache's rows in groups of 8 (a page holds whole groups): [groups][D / 64][8][64],
+// or with a ragged D [groups][1][8][D], whose columns past D read zeros; boxes of one
+// page, 64 rows at most.
+int tt_map(CUtensorMap* map, const void* base, const TreeArgs& a, bool bf) {
     auto enc = tt_encode_fn();
     CW_CHECK(enc, CW_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    cuuint64_t dims[2] = {(cuuint64_t)a.D, (cuuint64_t)a.n_pages * a.K * a.page};
-    cuuint64_t strides[1] = {(cuuint64_t)a.D * 2};
-    cuuint32_t box[2] = {64, (cuuint32_t)std::min(a.page, TR_TILE)};
-    cuuint32_t estr[2] = {1, 1};
-    CUresult r = enc(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+    const bool wide = a.D % 64 == 0;
+    cuuint64_t dims[4] = {(cuuint64_t)(wide ? 64 : a.D), 8, (cuuint64_t)(wide ? a.D / 64 : 1),
+                          (cuuint64_t)a.n_pages * a.K * a.page / 8};
+    cuuint64_t strides[3] = {(cuuint64_t)a.D * 2, 128, (cuuint64_t)a.D * 16};
+    cuuint32_t box[4] = {64, 8, (cuuint32_t)dims[2], (cuuint32_t)std::min(a.page, TR_TILE) / 8};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                      const_cast<void*>(base), dims, strides, box, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    CW_CHECK(r == CUDA_SUCCESS, CW_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return CW_OK;
+}
+
+// The query rows [n_rows][H][D], boxes of a request's nodes by a kv head's G heads.
+int tt_map_q(CUtensorMap* map, const TreeArgs& a, bool bf) {
+    auto enc = tt_encode_fn();
+    CW_CHECK(enc, CW_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.H, (cuuint64_t)a.n_rows};
+    cuuint64_t strides[2] = {(cuuint64_t)a.D * 2,
+                             (cuuint64_t)std::max(a.q_stride, (long long)a.H * a.D) * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)a.G, (cuuint32_t)a.max_nodes};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                     const_cast<void*>(a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     CW_CHECK(r == CUDA_SUCCESS, CW_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return CW_OK;
 }
@@ -761,7 +645,11 @@ bool tree_tc_takes(const cw_tree_attn_args& p, const void* q, const void* k, con
 }
 // Two row blocks to a CTA where a request can have more than 128 rows, so that its
 // keys are still read once (their TMEM, 2 x (128 + 256) columns, does not fit at 256).
-int tree_tc_rows(const TreeArgs& a) { return a.max_nodes * a.G > 128 && a.D <= 128 ? 256 : 128; }
+int tree_tc_rows(const TreeArgs& a) {
+    const int most = a.max_nodes * a.G;
+    if (tt_few_takes(a)) return most <= 16 ? 16 : most <= 32 ? 32 : 64;
+    return most > 128 && a.D <= 128 ? 256 : 128;
+}
 static int tt_per_sm(const TreeArgs& a) { return a.bm == 128 && a.D <= 128 ? 2 : 1; }
 int tree_tc_grid(cw_ctx* ctx, const TreeArgs& a) { return ctx->sm_count * tt_per_sm(a); }
 
@@ -772,9 +660,10 @@ static int tt_go(cw_ctx* ctx, const TreeArgs& a, const CUtensorMap& mk, const CU
     // the ring takes what the queries leave of the SM's shared memory (two CTAs of
     // 113 KB or one of 227 KB); without a split, products read rows past q_rows as
     // whatever follows
+    typedef TtShape<HD, NB, SPLIT> Z;
     const int q_rows = SPLIT > 1 ? 128 : std::min(128, (a.max_nodes * a.G + 7) / 8 * 8);
-    const size_t q = (size_t)NB * (HD / 64) * q_rows * 128, stage = (HD / 64) * TR_TILE * 128;
-    const size_t cap = tt_per_sm(a) == 2 ? 115712 : 232448, fixed = sizeof(TtBars);
+    const size_t q = (size_t)NB * Z::COLS * q_rows * 128, stage = Z::STAGE;
+    const size_t cap = Z::PER_SM == 2 ? 115712 : 232448, fixed = sizeof(TtBars) + (HD > 64 ? 0 : 128 * 8);
     const int stages = (int)std::min<size_t>((cap - fixed - q) / stage, TT_STAGES);
     const size_t smem = fixed + q + stages * stage;
     static bool set[64] = {};
@@ -808,6 +697,7 @@ int tree_tc_launch(cw_ctx* ctx, const TreeArgs& a, uint32_t type, int grid) {
     CUtensorMap mk, mv;
     CW_TRY(tt_map(&mk, a.k, a, bf));
     CW_TRY(tt_map(&mv, a.v, a, bf));
+    if (tt_few_takes(a)) return tt_few_launch(ctx, a, mk, mv, bf, grid);
     return bf ? tt_dims<true>(ctx, a, mk, mv, grid) : tt_dims<false>(ctx, a, mk, mv, grid);
 }
 
