@@ -99,6 +99,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
     __shared__ TreeShared s_run;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int wm = warp % WM, wk = warp / WM, g = lane >> 2, t4 = lane & 3;
+    pdl_wait();
     pdl_trigger();
     TreeRun run = tree_run<TR_THREADS>(a, &s_run);
     TreeItem it;
@@ -455,51 +456,61 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
     if (tid == 0) tree_record(a, run, it, any);
 }
 
-// Joins the pieces of the items that a run's end cut: out = sum_i w_i o_i / sum_i
-// w_i l_i, w_i = 2^(m_i - max m), in key order.  A warp per row, 8 rows a block.
+// Joins the pieces of the items that a run's end cut: out = sum_i w_i o_i / sum_i w_i
+// l_i, w_i = 2^(m_i - max m), in key order.  A warp per row and 128 dims, 8 warps a
+// block; bound by the latency of three dependent reads, so a lane has the four dims of
+// eight pieces in flight.
 constexpr int TJ_WARPS = 8;
 template <typename T>
-__global__ void __launch_bounds__(TJ_WARPS * 32) k_tree_join(TreeArgs a) {
+__global__ void __launch_bounds__(TJ_WARPS * 32) k_tree_join(const __grid_constant__ TreeArgs a) {
+    pdl_trigger();  // the next call may set itself up; it waits for this one before it reads
     pdl_wait();
     const TreePiece p = a.pieces[blockIdx.x];
-    const int lane = threadIdx.x & 31;
-    if (p.count <= 1) return;
-    for (int m = blockIdx.y * TJ_WARPS + (threadIdx.x >> 5); m < p.rows;
-         m += gridDim.y * TJ_WARPS) {
-        auto piece = [&](int i) {
-            return ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? p.slot : 0)) * a.bm + m;
-        };
-        float top = -INFINITY;
-        for (int i = lane; i < p.count; i += 32) top = fmaxf(top, a.ml[piece(i)].x);
-        top = warp_max(top);
-        float l = 0.f, acc[8] = {};
-        for (int i0 = 0; i0 < p.count; i0 += 32) {
-            const int i = i0 + lane;
-            float w = 0.f;
-            if (i < p.count) {
-                const float2 x = a.ml[piece(i)];
-                if (x.x != -INFINITY) w = exp2f(x.x - top);
-                l += w == 0.f ? 0.f : w * x.y;
-            }
-            const int n = min(32, p.count - i0);
-#pragma unroll 4
-            for (int j = 0; j < n; j++) {
-                const float wj = __shfl_sync(FULL, w, j);
-                if (wj == 0.f) continue;  // a piece in which the row saw nothing
-                const float* o = a.part + piece(i0 + j) * a.dp;
+    const int lane = threadIdx.x & 31, m = blockIdx.y * TJ_WARPS + (threadIdx.x >> 5);
+    const int d = blockIdx.z * 128 + 4 * lane;
+    if (p.count <= 1 || m >= p.rows) return;
+    auto piece = [&](int i) {
+        return ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? p.slot : 0)) * a.bm + m;
+    };
+    float top = -INFINITY;
+    for (int i = lane; i < p.count; i += 32) top = fmaxf(top, __ldcg(&a.ml[piece(i)]).x);
+    top = warp_max(top);
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < p.count; i0 += 32) {
+        float w = 0.f;
+        if (i0 + lane < p.count) {
+            const float2 x = __ldcg(&a.ml[piece(i0 + lane)]);
+            if (x.x != -INFINITY) w = exp2f(x.x - top);
+            if (w != 0.f) l += w * x.y;
+        }
+        const int n = min(32, p.count - i0);
+        for (int j0 = 0; j0 < n; j0 += 8) {
+            float4 x[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (lane + 32 * e < a.D) acc[e] = fmaf(wj, __ldcg(o + lane + 32 * e), acc[e]);
+            for (int j = 0; j < 8; j++)
+                x[j] = j0 + j < n && d < a.D
+                           ? __ldcg((const float4*)(a.part + piece(i0 + j0 + j) * a.dp + d))
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float wj = __shfl_sync(FULL, w, (j0 + j) & 31);
+                if (j0 + j >= n || wj == 0.f) continue;  // 0: a piece where the row saw nothing
+                acc.x = fmaf(wj, x[j].x, acc.x);
+                acc.y = fmaf(wj, x[j].y, acc.y);
+                acc.z = fmaf(wj, x[j].z, acc.z);
+                acc.w = fmaf(wj, x[j].w, acc.w);
             }
         }
-        l = warp_sum(l);
-        const int r = p.block * a.bm + m, node = r / a.G, gi = r - node * a.G;
-        T* out = (T*)a.out + ((long long)(p.row0 + node) * a.H + p.head * a.G + gi) * a.D;
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (lane + 32 * e < a.D)
-                out[lane + 32 * e] = tree_to<T>(l > 0.f || l != l ? acc[e] / l : 0.f);
     }
+    l = warp_sum(l);
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    const int r = p.block * a.bm + m, node = r / a.G, gi = r - node * a.G;
+    T* out = (T*)a.out + ((long long)(p.row0 + node) * a.H + p.head * a.G + gi) * a.D + d;
+    const float y[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (d + e < a.D) out[e] = tree_to<T>(inv == 0.f ? 0.f : y[e] * inv);
 }
 
 template <typename T, int DP, int WM, bool VEC>
@@ -508,7 +519,7 @@ static int tree_go(cw_ctx* ctx, const TreeArgs& a, int grid) {
     static_assert(smem <= TR_SMEM_CAP, "shared memory");
     auto kern = k_tree<T, DP, WM, VEC>;
     CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    return launch_pdl(ctx, false, kern, dim3(grid), dim3(TR_THREADS), smem, a);
+    return launch_pdl(ctx, true, kern, dim3(grid), dim3(TR_THREADS), smem, a);
 }
 template <typename T, int DP, bool VEC>
 static int tree_rows(cw_ctx* ctx, const TreeArgs& a, int grid) {
@@ -635,7 +646,8 @@ extern "C" int cw_tree_attention(cw_ctx* ctx, const cw_tree_attn_args* p) {
         else if (p->type == CW_GGUF_F16) CW_TRY(tree_type<__half>(ctx, a, vec, grid));
         else CW_TRY(tree_type<__nv_bfloat16>(ctx, a, vec, grid));
     }
-    const dim3 join(grid, (unsigned)((std::min<long long>(most, a.bm) + TJ_WARPS - 1) / TJ_WARPS));
+    const dim3 join(grid, (unsigned)((std::min<long long>(most, a.bm) + TJ_WARPS - 1) / TJ_WARPS),
+                    (unsigned)((a.D + 127) / 128));
     auto jk = p->type == CW_GGUF_F32   ? k_tree_join<float>
               : p->type == CW_GGUF_F16 ? k_tree_join<__half>
                                        : k_tree_join<__nv_bfloat16>;

@@ -126,7 +126,6 @@ __global__ void __launch_bounds__(320, 1)
     uint8_t* s_p = ring + stages * STAGE;      // [PB][128 keys][64 rows] of weights
     TfBars<N>* bars = (TfBars<N>*)(s_p + PB * 16384);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    pdl_trigger();
     // the swizzle counts from 1024-byte boundaries; no static shared memory precedes
     if (smem_addr(sm) & 1023) {
         if (tid == 0) tree_bad(a);
@@ -149,6 +148,8 @@ __global__ void __launch_bounds__(320, 1)
         bars->failed = 0;
         fence_mbar_init();
     }
+    pdl_wait();  // the setup above overlaps the launch before
+    pdl_trigger();
     TreeRun run = tree_run<320>(a, &bars->run);
     tc_fence_before();
     __syncthreads();
@@ -567,7 +568,7 @@ static int tf_go(cw_ctx* ctx, const TreeArgs& a, const CUtensorMap& mk, const CU
     }
     CUtensorMap mq;
     CW_TRY(tt_map_q(&mq, a, BF));
-    return launch_pdl(ctx, false, kern, dim3(grid), dim3(320), fixed + stages * Z::STAGE, mk, mv,
+    return launch_pdl(ctx, true, kern, dim3(grid), dim3(320), fixed + stages * Z::STAGE, mk, mv,
                       mq, a, stages);
 }
 template <bool BF, int HD>

@@ -95,7 +95,6 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
     // reference and sum of each lane's part of a row, when the queries are done with
     float2* s_ml = HD > 64 ? (float2*)(s_q + 128 * 128) : (float2*)(bars + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    pdl_trigger();
     // the swizzle counts from 1024-byte boundaries; no static shared memory precedes
     if (smem_addr(sm) & 1023) {
         if (tid == 0) tree_bad(a);
@@ -119,6 +118,8 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
         bars->failed = 0;
         fence_mbar_init();
     }
+    pdl_wait();  // the setup above overlaps the launch before
+    pdl_trigger();
     TreeRun run = tree_run<Z::THREADS>(a, &bars->run);
     tc_fence_before();
     __syncthreads();
@@ -671,7 +672,7 @@ static int tt_go(cw_ctx* ctx, const TreeArgs& a, const CUtensorMap& mk, const CU
         CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)cap));
         set[ctx->device & 63] = true;
     }
-    return launch_pdl(ctx, false, kern, dim3(grid), dim3(NB * 128 + 64), smem, mk, mv, a, stages,
+    return launch_pdl(ctx, true, kern, dim3(grid), dim3(NB * 128 + 64), smem, mk, mv, a, stages,
                       q_rows);
 }
 template <bool BF, int HD>
