@@ -20,18 +20,21 @@ namespace cw {
 // between CTAs.  Rows whose page existed read the table below `have`, rows on
 // fresh pages read the free list itself: no CTA reads what another writes.
 constexpr int PP_THREADS = 512;
-constexpr int PP_MAX_REQ = 16384;  // 2 * 4 bytes each: 128 KB of shared memory
+constexpr int PP_MAX_REQ = 16384;  // 3 * 4 bytes each: 192 KB of shared memory
 
 struct PagePlanArgs {
     const int *lens, *news, *free_pages, *depths;
     int *table, *starts, *positions, *slots, *owners, *used;
-    int n_req, page, max_pages, n_free, max_tokens;
+    int n_req, page, shift, max_pages, n_free, max_tokens;  // shift: page = 1 << shift, or -1
 };
 
-__device__ __forceinline__ int pp_pages(long long tokens, int page, int max_pages) {
-    const long long p = tokens < INT_MAX - page ? ((int)tokens + page - 1) / page
-                                                : (tokens + page - 1) / page;
-    return (int)min(p, (long long)max_pages);
+__device__ __forceinline__ int pp_div(const PagePlanArgs& a, int x) {
+    return a.shift >= 0 ? x >> a.shift : x / a.page;
+}
+__device__ __forceinline__ int pp_pages(const PagePlanArgs& a, long long tokens) {
+    const long long p = tokens < INT_MAX - a.page ? pp_div(a, (int)tokens + a.page - 1)
+                                                  : (tokens + a.page - 1) / a.page;
+    return (int)min(p, (long long)a.max_pages);
 }
 
 // The last i in [0, n) with a[i] <= x (a ascending, a[0] = 0 <= x).
@@ -49,16 +52,18 @@ __global__ void __launch_bounds__(PP_THREADS) k_page_plan(PagePlanArgs a) {
     extern __shared__ int pp_sm[];
     int* s_start = pp_sm;              // [n_req] tokens before the request
     int* s_first = pp_sm + a.n_req;    // [n_req] fresh pages before it
+    int* s_len = s_first + a.n_req;    // [n_req] cached tokens
     __shared__ long long w_tok[PP_THREADS / 32];
     __shared__ int w_pg[PP_THREADS / 32];
     __shared__ long long s_tokens;
     __shared__ int s_pages;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = a.n_req;
+    pdl_wait();
     for (int r = tid; r < R; r += PP_THREADS) {
         const int c = max(a.lens[r], 0), n = max(a.news[r], 0);
         s_start[r] = n;
-        s_first[r] = pp_pages((long long)c + n, a.page, a.max_pages) -
-                     pp_pages(c, a.page, a.max_pages);
+        s_first[r] = pp_pages(a, (long long)c + n) - pp_pages(a, c);
+        s_len[r] = c;
     }
     __syncthreads();
     // each thread sums a run of requests, then the runs are scanned
@@ -88,10 +93,12 @@ __global__ void __launch_bounds__(PP_THREADS) k_page_plan(PagePlanArgs a) {
     __syncthreads();
     long long btok = itok - tok;
     int bpg = ipg - pg;
-    for (int w = 0; w < warp; w++) {
-        btok += w_tok[w];
-        bpg += w_pg[w];
-    }
+#pragma unroll
+    for (int w = 0; w < PP_THREADS / 32; w++)
+        if (w < warp) {
+            btok += w_tok[w];
+            bpg += w_pg[w];
+        }
     for (int r = r0; r < r1; r++) {
         const int n = s_start[r], f = s_first[r];
         s_start[r] = (int)min(btok, (long long)INT_MAX);
@@ -116,7 +123,7 @@ __global__ void __launch_bounds__(PP_THREADS) k_page_plan(PagePlanArgs a) {
     // fresh pages into the table
     for (int u = g0; u < min(pages, a.n_free); u += step) {
         const int r = pp_find(s_first, R, u);  // the last request starting at or before u
-        const int have = pp_pages(max(a.lens[r], 0), a.page, a.max_pages);
+        const int have = pp_pages(a, s_len[r]);
         a.table[(size_t)r * a.max_pages + have + (u - s_first[r])] = a.free_pages[u];
     }
     // token rows, four to a thread (16-byte stores)
@@ -137,13 +144,13 @@ __global__ void __launch_bounds__(PP_THREADS) k_page_plan(PagePlanArgs a) {
                 while (r + 1 < R && s_start[r + 1] <= t) r++;
                 begin = s_start[r];
                 end = r + 1 < R ? s_start[r + 1] : tokens;
-                c = max(a.lens[r], 0);
-                have = pp_pages(c, a.page, a.max_pages);
+                c = s_len[r];
+                have = pp_pages(a, c);
                 first = s_first[r];
                 page_at = -1;
             }
             const long long at = (long long)c + (t - begin);
-            const int ap = at < INT_MAX ? (int)at / a.page : INT_MAX;
+            const int ap = at < INT_MAX ? pp_div(a, (int)at) : INT_MAX;
             if (ap != page_at) {
                 page_at = ap;
                 page_id = -1;
@@ -156,7 +163,7 @@ __global__ void __launch_bounds__(PP_THREADS) k_page_plan(PagePlanArgs a) {
             }
             pos[i] = a.depths ? c + a.depths[t] : (int)at;
             own[i] = r;
-            if (page_id >= 0) slot[i] = page_id * a.page + (int)at % a.page;
+            if (page_id >= 0) slot[i] = page_id * a.page + ((int)at - ap * a.page);
         }
         if (t0 + 4 <= a.max_tokens) {
             ((int4*)a.positions)[g] = make_int4(pos[0], pos[1], pos[2], pos[3]);
@@ -211,10 +218,10 @@ __device__ __forceinline__ void rp_set(__half* d, float x) { *d = __float2half_r
 __device__ __forceinline__ void rp_set(__nv_bfloat16* d, float x) { *d = __float2bfloat16_rn(x); }
 
 constexpr int RP_THREADS = 256;
-constexpr int RP_UNROLL = 4;  // heads whose loads are in flight together
+constexpr int RP_UNROLL = 2;  // heads whose loads are in flight while two others are turned
 
 template <typename T, int VEC, bool HALF>
-__global__ void __launch_bounds__(RP_THREADS) k_rope_append(RopeArgs a) {
+__global__ void __launch_bounds__(RP_THREADS, 3) k_rope_append(RopeArgs a) {
     typedef typename VecOf<VEC * sizeof(T)>::type V;
     union Row {
         V v[2];
@@ -235,18 +242,9 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope_append(RopeArgs a) {
     const int e0 = turn ? (HALF ? c * VEC : 2 * c * VEC) : a.rot + 2 * (c - rot_chunks) * VEC;
     const int e1 = turn && HALF ? e0 + a.rot / 2 : e0 + VEC;
     const bool two = e1 < a.D;
-    float cs[VEC], sn[VEC];
-    if (turn) {
-        const long long p = a.positions[t];
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const long long ph = (long long)((unsigned long long)p * a.steps[c * VEC + i]);
-            sincospif((float)ph * 0x1p-63f, &sn[i], &cs[i]);
-            sn[i] *= a.amp;
-            cs[i] *= a.amp;
-        }
-    }
     const int heads = a.H + 2 * a.K;
+    pdl_wait();
+    const long long pos = a.positions[t];
     long long slot = -1, dst0 = 0;
     if (a.K) {
         slot = a.slots[t];
@@ -259,44 +257,62 @@ __global__ void __launch_bounds__(RP_THREADS) k_rope_append(RopeArgs a) {
             dst0 = (pg * a.K * a.page + (slot - pg * a.page)) * a.D;
         }
     }
+    const T* q = (const T*)a.q + t * a.q_stride;
+    const T* k = (const T*)a.k + t * a.k_stride;
+    const T* v = (const T*)a.v + t * a.v_stride;
+    auto load = [&](int i, Row& w) {  // the thread's i-th head
+        const int h = g + i * a.groups;
+        if (i >= a.per || h >= heads) return;
+        const T* src = h < a.H         ? q + h * a.D
+                       : h < a.H + a.K ? k + (h - a.H) * a.D
+                                       : v + (h - a.H - a.K) * a.D;
+        w.v[0] = *(const V*)(src + e0);
+        if (two) w.v[1] = *(const V*)(src + e1);
+    };
+    Row w[RP_UNROLL];
+#pragma unroll
+    for (int u = 0; u < RP_UNROLL; u++) load(u, w[u]);
+    float cs[VEC], sn[VEC];
+    if (turn) {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+            const long long ph =
+                (long long)((unsigned long long)pos * a.steps[c * VEC + i]);
+            // 16-bit values: within half a turn the fast functions are off by 2^-21
+            if (sizeof(T) == 2) __sincosf((float)ph * 0x1.921fb6p-62f, &sn[i], &cs[i]);
+            else sincospif((float)ph * 0x1p-63f, &sn[i], &cs[i]);
+            sn[i] *= a.amp;
+            cs[i] *= a.amp;
+        }
+    }
     for (int i0 = 0; i0 < a.per; i0 += RP_UNROLL) {
-        Row w[RP_UNROLL];
-        T* dst[RP_UNROLL];
 #pragma unroll
         for (int u = 0; u < RP_UNROLL; u++) {
             const int h = g + (i0 + u) * a.groups;
-            dst[u] = nullptr;
+            Row y = w[u];
+            load(i0 + RP_UNROLL + u, w[u]);  // in flight while this head is turned
             if (i0 + u >= a.per || h >= heads) continue;
-            const T* src;
+            T* dst;
             if (h < a.H) {
-                src = (const T*)a.q + t * a.q_stride + (long long)h * a.D;
-                dst[u] = (T*)a.q_out + ((long long)t * a.H + h) * a.D;
+                dst = (T*)a.q_out + ((long long)t * a.H + h) * a.D;
             } else {
                 if (slot < 0) continue;
-                const int kh = h - a.H, vh = kh - a.K;
-                const long long at = dst0 + (long long)(vh < 0 ? kh : vh) * a.page * a.D;
-                src = vh < 0 ? (const T*)a.k + t * a.k_stride + (long long)kh * a.D
-                             : (const T*)a.v + t * a.v_stride + (long long)vh * a.D;
-                dst[u] = (T*)(vh < 0 ? a.k_cache : a.v_cache) + at;
+                dst = h < a.H + a.K ? (T*)a.k_cache + dst0 + (long long)(h - a.H) * a.page * a.D
+                                    : (T*)a.v_cache + dst0 +
+                                          (long long)(h - a.H - a.K) * a.page * a.D;
             }
-            w[u].v[0] = *(const V*)(src + e0);
-            if (two) w[u].v[1] = *(const V*)(src + e1);
-        }
-#pragma unroll
-        for (int u = 0; u < RP_UNROLL; u++) {
-            if (!dst[u]) continue;
-            if (turn && g + (i0 + u) * a.groups < a.H + a.K) {
+            if (turn && h < a.H + a.K) {
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
-                    T* p0 = HALF ? &w[u].e[i] : &w[u].e[2 * i];
-                    T* p1 = HALF ? &w[u].e[VEC + i] : &w[u].e[2 * i + 1];
+                    T* p0 = HALF ? &y.e[i] : &y.e[2 * i];
+                    T* p1 = HALF ? &y.e[VEC + i] : &y.e[2 * i + 1];
                     const float x0 = rp_f32(*p0), x1 = rp_f32(*p1);
                     rp_set(p0, x0 * cs[i] - x1 * sn[i]);
                     rp_set(p1, x1 * cs[i] + x0 * sn[i]);
                 }
             }
-            *(V*)(dst[u] + e0) = w[u].v[0];
-            if (two) *(V*)(dst[u] + e1) = w[u].v[1];
+            *(V*)(dst + e0) = y.v[0];
+            if (two) *(V*)(dst + e1) = y.v[1];
         }
     }
 }
@@ -308,14 +324,14 @@ static int rope_launch(cw_ctx* ctx, RopeArgs a, bool half) {
     // as many heads to a thread as still leave one full wave of threads
     const long long all = (long long)a.n_tokens * a.chunks * heads;
     const long long wave = (long long)ctx->sm_count * 2048;
-    a.per = (int)std::max<long long>(1, std::min<long long>({all / wave, 8, heads}));
+    a.per = (int)std::max<long long>(1, std::min<long long>(all / wave, heads));
     if (a.per >= RP_UNROLL) a.per = a.per / RP_UNROLL * RP_UNROLL;
     a.groups = (heads + a.per - 1) / a.per;
     const unsigned long long n = (unsigned long long)a.n_tokens * a.chunks * a.groups;
     const unsigned long long blocks = (n + RP_THREADS - 1) / RP_THREADS;
     CW_CHECK(blocks < (1ull << 31), CW_ERR_UNSUPPORTED, "cw_rope_append: too many rows");
-    if (half) k_rope_append<T, VEC, true><<<(unsigned)blocks, RP_THREADS, 0, ctx->stream>>>(a);
-    else k_rope_append<T, VEC, false><<<(unsigned)blocks, RP_THREADS, 0, ctx->stream>>>(a);
+    CW_TRY(launch_pdl(ctx, true, half ? k_rope_append<T, VEC, true> : k_rope_append<T, VEC, false>,
+                      dim3((unsigned)blocks), dim3(RP_THREADS), 0, a));
     return check_launch("rope_append");
 }
 
@@ -367,16 +383,17 @@ int cw_page_plan(cw_ctx* ctx, const cw_page_plan_args* p) {
     a.max_pages = (int)p->max_pages;
     a.n_free = (int)p->n_free;
     a.max_tokens = (int)T;
-    const size_t smem = 8 * R;
+    a.shift = (p->page_size & (p->page_size - 1)) == 0 ? __builtin_ctz(p->page_size) : -1;
+    const size_t smem = 12 * R;
     if (smem > 48 * 1024)
         CW_CUDA(cudaFuncSetAttribute(k_page_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     8 * PP_MAX_REQ));
+                                     12 * PP_MAX_REQ));
     // one group of four rows to a thread until two CTAs per SM are busy
     const long long items = std::max<long long>((long long)(T + 3) / 4, 1);
     const int grid = (int)std::min<long long>((items + PP_THREADS - 1) / PP_THREADS,
                                               2ll * ctx->sm_count);
     OpScope scope(ctx, "page_plan");
-    k_page_plan<<<grid, PP_THREADS, smem, ctx->stream>>>(a);
+    CW_TRY(launch_pdl(ctx, true, k_page_plan, dim3(grid), dim3(PP_THREADS), smem, a));
     return check_launch("page_plan");
 }
 
