@@ -61,20 +61,15 @@ __device__ __forceinline__ bool tt_any(bool x, int blocks) {
 // are KEYS consecutive ones, so SPLIT lanes share a row.
 template <int HD, int NB, int SPLIT> struct TtShape {
     static constexpr int COLS = HD / 64;                // 64-element column blocks
-    static constexpr int TILE = HD <= 128 ? 128 : 64;   // keys of a tile
-    static constexpr int SK = HD <= 64 ? 128 : 64;      // keys of a ring stage
-    static constexpr int HALVES = TILE / SK;            // stages of a K or V tile
-    static constexpr int STAGE = COLS * SK * 128;
-    // TMEM of a row block: SB buffers of scores, then O.  Two fit beside 256 dims (one
-    // CTA per SM, which has to overlap its own steps); below, 128-key tiles with one
-    // buffer halve the hand-overs per key, and the SM's other CTA or row block fills
-    // the gaps.
-    static constexpr int SB = HD <= 128 ? 1 : 2;
-    static constexpr int TCOLS = SB * TILE + HD;
+    static constexpr int STAGE = COLS * TR_TILE * 128;  // a tile of 64 keys
+    // TMEM of a row block: two buffers of scores, then O.  (128-key tiles with one buffer,
+    // half the hand-overs per key, were slower: the scores of the next tile then wait for
+    // the product of this one; 32 x 32 nodes at 8192: 209 us against 176.)
+    static constexpr int TCOLS = 2 * TR_TILE + HD;
     static constexpr uint32_t TMEM = NB * TCOLS <= 256 ? 256 : 512;
     static constexpr int THREADS = NB * 128 + 64;
     static constexpr int PER_SM = NB == 1 && HD <= 128 ? 2 : 1;
-    static constexpr int KEYS = TILE / SPLIT;
+    static constexpr int KEYS = TR_TILE / SPLIT;
     static constexpr int LANES = 128 / SPLIT;           // rows of a row block
 };
 
@@ -83,10 +78,9 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
     k_tree_tc(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
               const __grid_constant__ TreeArgs a, int stages, int q_rows) {
     typedef TtShape<HD, NB, SPLIT> Z;
-    constexpr int COLS = Z::COLS, TILE = Z::TILE, SK = Z::SK, HALVES = Z::HALVES, SB = Z::SB;
+    constexpr int COLS = Z::COLS, TILE = TR_TILE, SB = 2;
     constexpr int STAGE = Z::STAGE, TCOLS = Z::TCOLS, KEYS = Z::KEYS, LANES = Z::LANES;
     static_assert(NB == 1 || SPLIT == 1, "a split row block is the only one");
-    static_assert(SB == 1 || HALVES == 1, "the ring's order");
     extern __shared__ __align__(1024) uint8_t sm[];
     const int q_block = q_rows * 128;         // bytes of a column block of the queries
     uint8_t* s_q = sm;                        // [NB][COLS][q_rows][128]
@@ -131,51 +125,33 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
     auto all = [&](uint64_t* bar, uint32_t parity) {  // the same answer for the warp
         return __all_sync(FULL, wait(bar, parity)) != 0;
     };
-    // barrier and phase of tile n of a row block, where its scores' buffer is reused
-    auto buf = [](uint32_t n) { return SB == 2 ? n & 1 : 0u; };
-    auto turn = [](uint32_t n) { return SB == 2 ? n >> 1 : n; };
     TreeItem it;
     bool any = false, ok = true;
     const bool wide = a.D % 64 == 0;
-    const TtTile tile = wide ? TtTile{COLS * 1024, 1024} : TtTile{1024, SK * 128};
+    const TtTile tile = wide ? TtTile{COLS * 1024, 1024} : TtTile{1024, TILE * 128};
     TtPlace at = {0, 0};
 
     if (warp == NB * 4) {  // ---- TMA: all lanes, a box each
-        TtFeed<COLS, SK> feed(a, ring, bars->full, bars->empty, stages, tile);
+        TtFeed<COLS, TILE> feed(a, ring, bars->full, bars->empty, stages, tile);
         if (lane == 0) {
             tma_prefetch_desc(&map_k);
             tma_prefetch_desc(&map_v);
         }
-        auto load = [&](const CUtensorMap* map, int group) {
-            ok = ok && feed.load(map, group, all);
-        };
         while (run.left > 0 && ok) {
             it = tree_next(a, run);
             feed.begin(it);
-            const int tiles = (it.tiles * TR_TILE + TILE - 1) / TILE;
-            int now[HALVES];
-#pragma unroll
-            for (int h = 0; h < HALVES; h++) now[h] = feed.place(h);
-#pragma unroll
-            for (int h = 0; h < HALVES; h++) load(&map_k, now[h]);
-            for (int i = 0; i < tiles && ok; i++) {
-                int next[HALVES];
-#pragma unroll
-                for (int h = 0; h < HALVES; h++) next[h] = feed.place((i + 1) * HALVES + h);
-                if (SB == 2 && i + 1 < tiles) load(&map_k, next[0]);
-#pragma unroll
-                for (int h = 0; h < HALVES; h++) load(&map_v, now[h]);
-                if (SB == 1 && i + 1 < tiles) {
-#pragma unroll
-                    for (int h = 0; h < HALVES; h++) load(&map_k, next[h]);
-                }
-#pragma unroll
-                for (int h = 0; h < HALVES; h++) now[h] = next[h];
+            int now = feed.place(0);
+            ok = feed.load(&map_k, now, all);
+            for (int i = 0; i < it.tiles && ok; i++) {
+                const int next = feed.place(i + 1);
+                if (i + 1 < it.tiles) ok = feed.load(&map_k, next, all);
+                ok = ok && feed.load(&map_v, now, all);
+                now = next;
             }
         }
         if (!ok) feed.drain();
     } else if (warp == NB * 4 + 1) {  // ---- MMA: the warp waits, one lane issues
-        constexpr uint32_t id_s = tt_idesc<BF>(SK, false, false);
+        constexpr uint32_t id_s = tt_idesc<BF>(TILE, false, false);
         constexpr uint32_t id_o = tt_idesc<BF>(HD, false, true);
         const uint64_t q0 = umma_desc_sw128(smem_addr(s_q)), kv0 = tt_desc(smem_addr(ring), tile);
         const int steps = (a.D + 15) / 16;
@@ -184,79 +160,68 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
         while (run.left > 0 && ok) {
             it = tree_next(a, run);
             const int blocks = it.rows > 128 ? NB : 1;
-            const int tiles = (it.tiles * TR_TILE + TILE - 1) / TILE;
             for (int b = 0; b < blocks && ok; b++) ok = all(&bars->q_full[b], items[b]++);
-            // S = Q K^T of tile i for row block b; K's stages from place k
-            auto scores = [&](int i, int b, TtPlace k) {
-                const uint32_t m = n[b] + i;
-                // this buffer's weights went into the product of tile i - SB
-                if (i >= SB) ok = ok && all(&bars->pv[b][(m - SB) & 1], (m - SB) >> 1);
+            // S = Q K^T of tile i, of each row block
+            auto scores = [&](int i) {
+                const int s = at.stage;
+                ok = ok && all(&bars->full[s], at.phase);
+                at.next(stages);
 #pragma unroll
-                for (int h = 0; h < HALVES; h++, k.next(stages)) {
-                    if (b == 0) ok = ok && all(&bars->full[k.stage], k.phase);
+                for (int b = 0; b < NB; b++) {
+                    if (b >= blocks) break;
+                    const uint32_t m = n[b] + i;
+                    // this buffer's weights went into the product of tile i - 2
+                    if (i >= 2) ok = ok && all(&bars->pv[b][m & 1], (m - 2) >> 1);
                     tc_fence_after();
                     if (one && ok) {
-                        const uint32_t d = tmem + b * TCOLS + buf(m) * TILE + h * SK;
+                        const uint32_t d = tmem + b * TCOLS + (m & 1) * TILE;
                         const uint64_t dq = q0 + ((b * COLS * q_block) >> 4),
-                                       dk = kv0 + ((k.stage * STAGE) >> 4);
+                                       dk = kv0 + ((s * STAGE) >> 4);
 #pragma unroll
                         for (int x = 0; x < HD / 16; x++)
                             if (x < steps)
                                 umma_f16(d, dq + (((x >> 2) * q_block + (x & 3) * 32) >> 4),
                                          dk + (((x >> 2) * tile.col + (x & 3) * 32) >> 4), id_s,
                                          x > 0);
-                        if (b + 1 == blocks) tc_commit(&bars->empty[k.stage]);
-                        if (h + 1 == HALVES) tc_commit(&bars->s_full[b][buf(m)]);
+                        tc_commit(&bars->s_full[b][m & 1]);
+                        if (b + 1 == blocks) tc_commit(&bars->empty[s]);
                     }
                     __syncwarp();
                 }
             };
-            // O += P V; V's stages from place v
-            auto values = [&](int i, int b, TtPlace v) {
-                const uint32_t m = n[b] + i;
-                ok = ok && all(&bars->p_full[b][buf(m)], turn(m));
+            scores(0);
+            for (int i = 0; i < it.tiles && ok; i++) {
+                if (i + 1 < it.tiles) scores(i + 1);
+                // O += P V of tile i
+                const int s = at.stage;
+                ok = ok && all(&bars->full[s], at.phase);
+                at.next(stages);
 #pragma unroll
-                for (int h = 0; h < HALVES; h++, v.next(stages)) {
-                    if (b == 0) ok = ok && all(&bars->full[v.stage], v.phase);
+                for (int b = 0; b < NB; b++) {
+                    if (b >= blocks) break;
+                    const uint32_t m = n[b] + i;
+                    ok = ok && all(&bars->p_full[b][m & 1], m >> 1);
                     tc_fence_after();
                     if (one && ok) {
-                        const uint32_t p = tmem + b * TCOLS + buf(m) * TILE + h * (SK / 2);
-                        const uint64_t dv = kv0 + ((v.stage * STAGE) >> 4);
+                        const uint32_t p = tmem + b * TCOLS + (m & 1) * TILE;
+                        const uint64_t dv = kv0 + ((s * STAGE) >> 4);
                         // 16 keys go to the lanes that weigh them
 #pragma unroll
-                        for (int x = 0; x < SK / 16; x++) {
+                        for (int x = 0; x < TILE / 16; x++) {
                             auto off = [&](int quad) {
-                                return (h * SK + x * 16) / KEYS == quad * 32 / LANES ? 0u : ~0u;
+                                return x * 16 / KEYS == quad * 32 / LANES ? 0u : ~0u;
                             };
                             tt_mma_ts(tmem + b * TCOLS + SB * TILE, p + 8 * x,
                                       dv + ((x * 2 * tile.group) >> 4), id_o, off(0), off(1),
                                       off(2), off(3));
                         }
-                        if (b + 1 == blocks) tc_commit(&bars->empty[v.stage]);
-                        if (h + 1 == HALVES) tc_commit(&bars->pv[b][m & 1]);
+                        tc_commit(&bars->pv[b][m & 1]);
+                        if (b + 1 == blocks) tc_commit(&bars->empty[s]);
                     }
                     __syncwarp();
                 }
-            };
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-                if (b < blocks) scores(0, b, at);
-            at.skip(HALVES, stages);
-            for (int i = 0; i < tiles && ok; i++) {
-                TtPlace k = at, v = at;
-                const bool more = i + 1 < tiles;
-                if (SB == 2 && more) v.skip(1, stages);  // K(i+1) lies before V(i)
-                if (SB == 1) k.skip(HALVES, stages);
-#pragma unroll
-                for (int b = 0; b < NB; b++)
-                    if (b < blocks) {
-                        if (SB == 2 && more) scores(i + 1, b, k);
-                        values(i, b, v);
-                        if (SB == 1 && more) scores(i + 1, b, k);
-                    }
-                at.skip(more ? 2 * HALVES : HALVES, stages);
             }
-            for (int b = 0; b < blocks; b++) n[b] += tiles;
+            for (int b = 0; b < blocks; b++) n[b] += it.tiles;
         }
         // every product issued has ended before the block frees its TMEM
         if (one) tc_commit(&bars->done);
@@ -283,10 +248,10 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
             it = tree_next(a, run);
             any = true;
             const int blocks = it.rows > 128 ? NB : 1;
-            const int tiles = (it.tiles * TR_TILE + TILE - 1) / TILE;
+            const int tiles = it.tiles;
             TtPlace at_v = at;  // of the item's first V tile
-            at_v.skip(SB == 2 && tiles > 1 ? 2 : HALVES, stages);
-            at.skip(2 * HALVES * tiles % (2 * stages), stages);
+            at_v.skip(tiles > 1 ? 2 : 1, stages);
+            at.skip(2 * tiles % (2 * stages), stages);
             if (b >= blocks) continue;
             const int m0 = it.block * a.bm + b * 128;       // row 0 of the request's rows
             const int rows = min(it.rows - b * 128, 128);
@@ -333,44 +298,36 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
             for (int i = 0; i < tiles; i++, n++) {
                 const int kt = key0 + i * TILE;
                 const bool mixed = kt + TILE > end || kt + TILE > it.q.len || kt < edge_max;
-                uint64_t sees[2] = {~0ull, ~0ull};  // this row's, of all the tile's keys
-                if (mixed) {
-#pragma unroll
-                    for (int h = 0; h < TILE / 64; h++) {
-                        const int k = kt + h * 64;
-                        if (k < edge || k + 64 > it.q.len || k + 64 > end)
-                            sees[h] = r < rows && k < end ? tree_sees(a, it.q, m0 + r, k) : 0;
-                    }
-                }
-                const uint64_t mine = (part * KEYS < 64 ? sees[0] : sees[1]) >> (part * KEYS % 64);
-                wait(&bars->s_full[b][buf(n)], turn(n));
+                uint64_t sees = ~0ull;  // this row's, of the tile's keys
+                if (mixed && (kt < edge || kt + TILE > it.q.len || kt + TILE > end))
+                    sees = r < rows ? tree_sees(a, it.q, m0 + r, kt) : 0;
+                const uint64_t mine = sees >> (part * KEYS);
+                wait(&bars->s_full[b][n & 1], n >> 1);
                 __syncwarp();
                 tc_fence_after();
-                const uint32_t t_s = lanes + buf(n) * TILE;
+                const uint32_t t_s = lanes + (n & 1) * TILE;
                 if (work) {
-                    constexpr int CH = KEYS < 64 ? KEYS : 64;  // scores held at a time
-                    float s[CH];
+                    float s[KEYS];
+                    tt_load<KEYS>(t_s + part * KEYS, (uint32_t*)s);
+                    if (cap) {
+#pragma unroll
+                        for (int j = 0; j < KEYS; j++) s[j] = capped(s[j]);
+                    }
+                    if (mixed) {
+#pragma unroll
+                        for (int j = 0; j < KEYS; j++)
+                            if (!(mine >> j & 1)) s[j] = -INFINITY;
+                    }
                     float t0 = top, t1 = top, t2 = top, t3 = top;
-                    uint64_t seen = mine;
-#pragma unroll 1
-                    for (int h = 0; h < KEYS / CH; h++) {
-                        tt_load<CH>(t_s + part * KEYS + h * CH, (uint32_t*)s);
-                        if (KEYS > 64) seen = h ? sees[1] : sees[0];
-                        if (mixed) {
 #pragma unroll
-                            for (int j = 0; j < CH; j++)
-                                if (!(seen >> j & 1)) s[j] = -INFINITY;
-                        }
-#pragma unroll
-                        for (int j = 0; j < CH; j += 4) {
-                            t0 = fmaxf(t0, s[j]);
-                            t1 = fmaxf(t1, s[j + 1]);
-                            t2 = fmaxf(t2, s[j + 2]);
-                            t3 = fmaxf(t3, s[j + 3]);
-                        }
+                    for (int j = 0; j < KEYS; j += 4) {
+                        t0 = fmaxf(t0, s[j]);
+                        t1 = fmaxf(t1, s[j + 1]);
+                        t2 = fmaxf(t2, s[j + 2]);
+                        t3 = fmaxf(t3, s[j + 3]);
                     }
                     top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
-                    const float want = top == -INFINITY ? -INFINITY : (cap ? capped(top) : top) * c2;
+                    const float want = top == -INFINITY ? -INFINITY : top * c2;
                     if (i == 0) {
                         ref = want;
                     } else if (__any_sync(FULL, r < rows && want - ref > 8.f)) {
@@ -383,8 +340,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
 #pragma unroll 1
                         for (int c = 0; c < HD; c += 32) {
                             uint32_t o[32];
-                            tt_ld32(t_o + c, o);
-                            tt_wait_ld32(o);
+                            tt_load<32>(t_o + c, o);
 #pragma unroll
                             for (int j = 0; j < 32; j++)
                                 o[j] = __float_as_uint(__uint_as_float(o[j]) * fix);
@@ -393,48 +349,23 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
                     }
                     const float from = ref == -INFINITY ? 0.f : ref;
                     float l0 = 0.f, l1 = 0.f;
-#pragma unroll 1
-                    for (int h = 0; h < KEYS / CH; h++) {
-                        if (KEYS > CH) {
-                            tt_load<CH>(t_s + h * CH, (uint32_t*)s);
-                            seen = h ? sees[1] : sees[0];
-                        }
-                        uint32_t p[CH / 2];
-                        if (cap) {
+                    uint32_t p[KEYS / 2];
 #pragma unroll
-                            for (int j = 0; j < CH; j++) s[j] = capped(s[j]);
-                        }
+                    for (int j = 0; j < KEYS; j++) s[j] = tt_exp2(fmaf(s[j], c2, -from));
 #pragma unroll
-                        for (int j = 0; j < CH; j++) s[j] = tt_exp2(fmaf(s[j], c2, -from));
-                        if (mixed) {
-#pragma unroll
-                            for (int j = 0; j < CH; j++)
-                                if (!(seen >> j & 1)) s[j] = 0.f;
-                        }
-#pragma unroll
-                        for (int j = 0; j < CH / 2; j += 2) {
-                            p[j] = tt_pack<BF>(s[2 * j], s[2 * j + 1], l0);
-                            p[j + 1] = tt_pack<BF>(s[2 * j + 2], s[2 * j + 3], l1);
-                        }
-                        // over scores that this thread has read (weight j of a part lies
-                        // at half the part's column or before it)
-                        tt_st<CH / 2>(t_s + part * (KEYS / 2) + h * (CH / 2), p);
+                    for (int j = 0; j < KEYS / 2; j += 2) {
+                        p[j] = tt_pack<BF>(s[2 * j], s[2 * j + 1], l0);
+                        p[j + 1] = tt_pack<BF>(s[2 * j + 2], s[2 * j + 3], l1);
                     }
                     sum += l0 + l1;
+                    tt_st<KEYS / 2>(t_s + part * (KEYS / 2), p);
                     tt_wait_st();
                 }
                 if (mixed) {  // v rows past the end, and values that are not finite
-                    TtPlace v1 = at_v;
                     wait(&bars->full[at_v.stage], at_v.phase);
-                    if (HALVES == 2) {
-                        v1.next(stages);
-                        wait(&bars->full[v1.stage], v1.phase);
-                    }
                     __syncwarp();
-                    uint8_t* v[2] = {ring + at_v.stage * STAGE, ring + v1.stage * STAGE};
-                    auto chunk = [&](int j, int c) {
-                        return v[HALVES == 2 ? j / SK : 0] + tile.at(j % SK, c);
-                    };
+                    uint8_t* v = ring + at_v.stage * STAGE;
+                    auto chunk = [&](int j, int c) { return v + tile.at(j, c); };
                     const int live = end - kt;
                     bool odd = false;
                     for (int x = b * 128 + m; x < COLS * TILE * 8; x += blocks * 128) {
@@ -462,8 +393,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
                                         asm volatile("tcgen05.wait::ld.sync.aligned;"
                                                      : "+r"(pj), "+r"(oj)::"memory");
                                         float o = __uint_as_float(oj);
-                                        const uint64_t see = j < 64 ? sees[0] : sees[1];
-                                        if ((see >> (j & 63) & 1) && j / KEYS == part)
+                                        if ((sees >> j & 1) && j / KEYS == part)
                                             o = fmaf(tt_value<BF>(j & 1 ? pj >> 16 : pj & 0xffffu),
                                                      tt_value<BF>(bits), o);
                                         __syncwarp();
@@ -485,8 +415,8 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bars->p_full[b][buf(n)]);
-                at_v.skip(SB == 2 ? (i + 2 < tiles ? 2 : 1) : 2 * HALVES, stages);
+                if (lane == 0) mbar_arrive(&bars->p_full[b][n & 1]);
+                at_v.skip(i + 2 < tiles ? 2 : 1, stages);
             }
             // ---- the item's end
             wait(&bars->pv[b][(n - 1) & 1], (n - 1) >> 1);
@@ -680,9 +610,11 @@ static int tt_split(cw_ctx* ctx, const TreeArgs& a, const CUtensorMap& mk, const
                     int grid) {
     if constexpr (HD <= 128)
         if (a.bm == 256) return tt_go<BF, HD, 2, 1>(ctx, a, mk, mv, grid);
-    const int most = a.max_nodes * a.G;
-    if (most <= 32) return tt_go<BF, HD, 1, 4>(ctx, a, mk, mv, grid);
-    if (most <= 64) return tt_go<BF, HD, 1, 2>(ctx, a, mk, mv, grid);
+    [[maybe_unused]] const int most = a.max_nodes * a.G;
+    if constexpr (HD == 256) {  // at fewer dims short row blocks go to cw_tree_few.cu
+        if (most <= 32) return tt_go<BF, HD, 1, 4>(ctx, a, mk, mv, grid);
+        if (most <= 64) return tt_go<BF, HD, 1, 2>(ctx, a, mk, mv, grid);
+    }
     return tt_go<BF, HD, 1, 1>(ctx, a, mk, mv, grid);
 }
 template <bool BF>

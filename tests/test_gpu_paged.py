@@ -304,6 +304,10 @@ TREE = [  # dtype, heads, kv, dim, page, lens, nodes, options
     ("f16", 32, 8, 64, 32, [4500, 40], [16, 12], dict(softcap=10.0)),
     ("f16", 32, 8, 64, 8, [4500], [33], dict(window=1000)),
     ("f16", 8, 4, 256, 64, [6000], [40], {}),
+    ("bf16", 32, 8, 128, 16, [3000, 70], [25, 31], {}),
+    ("f16", 16, 4, 48, 32, [3500], [30], dict(window=700, softcap=15.0)),
+    ("bf16", 16, 8, 200, 8, [2000], [5], {}),
+    ("f16", 8, 4, 256, 16, [900, 3000], [30, 64], dict(empty=True)),
     ("f32", 16, 8, 128, 16, [3000, 700], [9, 30], {}),
 ]
 
