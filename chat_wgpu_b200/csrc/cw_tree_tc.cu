@@ -150,30 +150,30 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
             }
         }
         if (!ok) feed.drain();
-    } else if (warp == NB * 4 + 1) {  // ---- MMA: the warp waits, one lane issues
+    } else if (warp == NB * 4 + 1) {  // ---- MMA: one elected lane
         constexpr uint32_t id_s = tt_idesc<BF>(TILE, false, false);
         constexpr uint32_t id_o = tt_idesc<BF>(HD, false, true);
         const uint64_t q0 = umma_desc_sw128(smem_addr(s_q)), kv0 = tt_desc(smem_addr(ring), tile);
         const int steps = (a.D + 15) / 16;
-        const bool one = tt_elect();
+        if (tt_elect()) {
         uint32_t n[2] = {0, 0}, items[2] = {0, 0};  // tiles and items of each row block
         while (run.left > 0 && ok) {
             it = tree_next(a, run);
             const int blocks = it.rows > 128 ? NB : 1;
-            for (int b = 0; b < blocks && ok; b++) ok = all(&bars->q_full[b], items[b]++);
+            for (int b = 0; b < blocks && ok; b++) ok = wait(&bars->q_full[b], items[b]++);
             // S = Q K^T of tile i, of each row block
             auto scores = [&](int i) {
                 const int s = at.stage;
-                ok = ok && all(&bars->full[s], at.phase);
+                ok = ok && wait(&bars->full[s], at.phase);
                 at.next(stages);
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
                     if (b >= blocks) break;
                     const uint32_t m = n[b] + i;
                     // this buffer's weights went into the product of tile i - 2
-                    if (i >= 2) ok = ok && all(&bars->pv[b][m & 1], (m - 2) >> 1);
+                    if (i >= 2) ok = ok && wait(&bars->pv[b][m & 1], (m - 2) >> 1);
                     tc_fence_after();
-                    if (one && ok) {
+                    if (ok) {
                         const uint32_t d = tmem + b * TCOLS + (m & 1) * TILE;
                         const uint64_t dq = q0 + ((b * COLS * q_block) >> 4),
                                        dk = kv0 + ((s * STAGE) >> 4);
@@ -186,7 +186,6 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
                         tc_commit(&bars->s_full[b][m & 1]);
                         if (b + 1 == blocks) tc_commit(&bars->empty[s]);
                     }
-                    __syncwarp();
                 }
             };
             scores(0);
@@ -194,15 +193,15 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
                 if (i + 1 < it.tiles) scores(i + 1);
                 // O += P V of tile i
                 const int s = at.stage;
-                ok = ok && all(&bars->full[s], at.phase);
+                ok = ok && wait(&bars->full[s], at.phase);
                 at.next(stages);
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
                     if (b >= blocks) break;
                     const uint32_t m = n[b] + i;
-                    ok = ok && all(&bars->p_full[b][m & 1], m >> 1);
+                    ok = ok && wait(&bars->p_full[b][m & 1], m >> 1);
                     tc_fence_after();
-                    if (one && ok) {
+                    if (ok) {
                         const uint32_t p = tmem + b * TCOLS + (m & 1) * TILE;
                         const uint64_t dv = kv0 + ((s * STAGE) >> 4);
                         // 16 keys go to the lanes that weigh them
@@ -218,14 +217,14 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
                         tc_commit(&bars->pv[b][m & 1]);
                         if (b + 1 == blocks) tc_commit(&bars->empty[s]);
                     }
-                    __syncwarp();
                 }
             }
             for (int b = 0; b < blocks; b++) n[b] += it.tiles;
         }
         // every product issued has ended before the block frees its TMEM
-        if (one) tc_commit(&bars->done);
+        tc_commit(&bars->done);
         (void)mbar_wait(&bars->done, 0, TT_WAIT_NS);
+        }
         __syncwarp();
     } else {  // ---- softmax: a thread per row and part of the keys
         // lane m weighs keys [part * KEYS, ..+KEYS) of each tile for row r
