@@ -28,6 +28,7 @@
 namespace cw {
 
 constexpr int TR_THREADS = 256;
+constexpr int TR_ROWS = 2;  // tiles whose row offsets are kept
 constexpr size_t TR_SMEM_CAP = 226 * 1024 + 384;  // dynamic; the kernel also has static
 
 __device__ __forceinline__ void tr_cp16(void* dst, const void* src, bool live) {
@@ -71,13 +72,13 @@ template <int DP> __device__ __forceinline__ int tr_at(int j, int c) {
 
 // Ring buffers (one K or V tile each) that fit beside the queries.
 template <int DP, int BM> constexpr int tr_ring() {
-    const size_t left = TR_SMEM_CAP - (size_t)BM * DP * 4 - BM * 8 - 2048;
+    const size_t left = TR_SMEM_CAP - (size_t)BM * DP * 4 - BM * 8 - TR_ROWS * TR_TILE * 8 - 1024;
     const size_t n = left / ((size_t)TR_TILE * DP * 4);
     return n > 8 ? 8 : (int)n;
 }
 template <int DP, int BM> constexpr size_t tr_smem() {
     return ((size_t)tr_ring<DP, BM>() * TR_TILE + BM) * DP * 4 + (size_t)BM * 8  // sees
-           + 2 * TR_TILE * 8                                                    // row offsets
+           + TR_ROWS * TR_TILE * 8                                              // row offsets
            + 128 * 8;                                                           // warp max, sum
 }
 
@@ -92,8 +93,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
     float* ring = sm;
     float* sq = ring + RING * TR_TILE * DP;
     uint64_t* s_sees = (uint64_t*)(sq + BM * DP);
-    long long* s_row = (long long*)(s_sees + BM);  // [2][64] element offset of a key row, or -1
-    float2* s_ml = (float2*)(s_row + 2 * TR_TILE); // [WK][BM]
+    long long* s_row = (long long*)(s_sees + BM);  // [TR_ROWS][64] offset of a key row, or -1
+    float2* s_ml = (float2*)(s_row + TR_ROWS * TR_TILE); // [WK][BM]
     __shared__ int s_edge;
     __shared__ TreeShared s_run;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
             tr_commit();
         };
         for (int s = 0; s < RING - 1; s++) {
-            if (!(s & 1)) {
+            if (!(s & 1) && s < steps) {
                 __syncthreads();
                 rows_of(s >> 1);
                 __syncthreads();
@@ -416,38 +417,43 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
             const float x = s_ml[wk * BM + m].x;
             own[h] = x == -INFINITY ? 0.f : exp2f(x - top);
         }
-        float* so = ring;  // [BM][DP], the ring is idle
-        for (int w = 0; w < WK; w++) {
-            if (wk == w) {
+        float* so = ring;  // [WK][BM][DP], the ring is idle
+        float2* s_all = (float2*)s_sees;  // each row's maximum and sum
 #pragma unroll
-                for (int b = 0; b < DB; b++)
+        for (int b = 0; b < DB; b++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++)
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            float* d = so + (wm * 16 + g + 8 * h) * DP + b * 32 + t4 * 8 + e;
-                            const float x = o[b][e & 3][(e >> 2) + 2 * h] * own[h];
-                            *d = w == 0 ? x : *d + x;
-                        }
+                for (int i = 0; i < 2; i++) {  // dims b * 32 + t4 * 8 + 4 i ..
+                    const int m = wm * 16 + g + 8 * h;
+                    *(float4*)(so + wk * BM * DP + tr_at<DP>(m, b * 8 + t4 * 2 + i)) =
+                        make_float4(o[b][0][i + 2 * h] * own[h], o[b][1][i + 2 * h] * own[h],
+                                    o[b][2][i + 2 * h] * own[h], o[b][3][i + 2 * h] * own[h]);
+                }
+        if (tid < BM) {
+            float top = -INFINITY, l = 0.f;
+            for (int w = 0; w < WK; w++) top = fmaxf(top, s_ml[w * BM + tid].x);
+            for (int w = 0; w < WK; w++) {
+                const float2 x = s_ml[w * BM + tid];
+                if (x.x != -INFINITY) l += x.y * exp2f(x.x - top);
             }
-            __syncthreads();
+            s_all[tid] = make_float2(top, l);
         }
+        __syncthreads();
         const size_t piece = (size_t)blockIdx.x * 2 + tree_slot(run, it);
         for (int i = tid; i < it.rows * a.D; i += TR_THREADS) {
             const int m = i / a.D, d = i - m * a.D;
-            float top = -INFINITY, l = 0.f;
-            for (int w = 0; w < WK; w++) top = fmaxf(top, s_ml[w * BM + m].x);
-            for (int w = 0; w < WK; w++) {
-                const float2 x = s_ml[w * BM + m];
-                if (x.x != -INFINITY) l += x.y * exp2f(x.x - top);
-            }
+            const float l = s_all[m].y;
+            float x = 0.f;
+#pragma unroll
+            for (int w = 0; w < WK; w++) x += so[w * BM * DP + tr_at<DP>(m, d >> 2) + (d & 3)];
             if (it.whole) {
                 const int node = (m0 + m) / a.G, gi = (m0 + m) - node * a.G;
                 ((T*)a.out)[((long long)(it.q.row0 + node) * a.H + it.head * a.G + gi) * a.D + d] =
-                    tree_to<T>(l > 0.f || l != l ? so[m * DP + d] / l : 0.f);
+                    tree_to<T>(l > 0.f || l != l ? x / l : 0.f);
             } else {
-                a.part[(piece * BM + m) * a.dp + d] = so[m * DP + d];
-                if (d == 0) a.ml[piece * BM + m] = make_float2(top, l);
+                a.part[(piece * BM + m) * a.dp + d] = x;
+                if (d == 0) a.ml[piece * BM + m] = s_all[m];
             }
         }
         __syncthreads();
