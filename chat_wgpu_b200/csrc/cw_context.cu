@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <mutex>
 
 #include "cw_common.h"
 
@@ -193,6 +194,36 @@ const char* cw_last_error(void) { return g_err.c_str(); }
 
 int cw_abi_version(void) { return CW_ABI_VERSION; }
 
+// What a context asks of its device, asked once per device and process: the full
+// property query takes over a millisecond, which a program that makes a context per
+// stream would pay each time.
+struct DeviceFacts {
+    int major = 0, minor = 0, sms = 0, clock_khz = 0, l2 = 0, smem_optin = 0, smem_sm = 0;
+    char name[256] = {};
+};
+static int device_facts(int device, DeviceFacts* out) {
+    static std::mutex lock;
+    static std::map<int, DeviceFacts> known;
+    std::lock_guard<std::mutex> hold(lock);
+    auto it = known.find(device);
+    if (it == known.end()) {
+        cudaDeviceProp prop;
+        CW_CUDA(cudaGetDeviceProperties(&prop, device));
+        DeviceFacts f;
+        f.major = prop.major;
+        f.minor = prop.minor;
+        f.sms = prop.multiProcessorCount;
+        f.l2 = prop.l2CacheSize;
+        f.smem_optin = (int)prop.sharedMemPerBlockOptin;
+        f.smem_sm = (int)prop.sharedMemPerMultiprocessor;
+        snprintf(f.name, sizeof f.name, "%s", prop.name);
+        CW_CUDA(cudaDeviceGetAttribute(&f.clock_khz, cudaDevAttrClockRate, device));
+        it = known.emplace(device, f).first;
+    }
+    *out = it->second;
+    return CW_OK;
+}
+
 static int ctx_create(int device, cudaStream_t stream, bool own, cw_ctx** out) {
     clear_error();
     CW_CHECK(out, CW_ERR_INVALID_ARG, "cw_ctx_create: out is NULL");
@@ -203,8 +234,8 @@ static int ctx_create(int device, cudaStream_t stream, bool own, cw_ctx** out) {
         return set_error(CW_ERR_NO_DEVICE, "no CUDA device: %s", cudaGetErrorString(e));
     CW_CHECK(device >= 0 && device < n, CW_ERR_NO_DEVICE, "device %d out of range (%d devices)",
              device, n);
-    cudaDeviceProp prop;
-    CW_CUDA(cudaGetDeviceProperties(&prop, device));
+    DeviceFacts prop;
+    CW_TRY(device_facts(device, &prop));
     if (prop.major != 10 || prop.minor != 0)
         return set_error(CW_ERR_NO_DEVICE,
                          "device %d is sm_%d%d; libchatcuda.so is built for sm_100a only", device,
@@ -212,12 +243,11 @@ static int ctx_create(int device, cudaStream_t stream, bool own, cw_ctx** out) {
     CW_CUDA(cudaSetDevice(device));
     cw_ctx* c = new cw_ctx();
     c->device = device;
-    c->sm_count = prop.multiProcessorCount;
-    cudaDeviceGetAttribute(&c->clock_khz, cudaDevAttrClockRate, c->device);
-    if (c->clock_khz <= 0) c->clock_khz = 1;
-    c->l2_bytes = prop.l2CacheSize;
-    c->max_smem_optin = (int)prop.sharedMemPerBlockOptin;
-    c->smem_per_sm = (int)prop.sharedMemPerMultiprocessor;
+    c->sm_count = prop.sms;
+    c->clock_khz = std::max(prop.clock_khz, 1);
+    c->l2_bytes = prop.l2;
+    c->max_smem_optin = prop.smem_optin;
+    c->smem_per_sm = prop.smem_sm;
     char b[320];
     snprintf(b, sizeof b, "CUDA sm_%d%da (%s)", prop.major, prop.minor, prop.name);
     c->backend = b;
@@ -263,7 +293,7 @@ int cw_ctx_destroy(cw_ctx* ctx) {
     if (ctx->d_status) cudaFree(ctx->d_status);
     if (ctx->d_counters) cudaFree(ctx->d_counters);
     if (ctx->gemm_scratch) cudaFree(ctx->gemm_scratch);
-    if (ctx->tree_scratch) cudaFree(ctx->tree_scratch);
+    if (ctx->tree_scratch) cudaFreeAsync(ctx->tree_scratch, ctx->stream);
     if (ctx->stream && ctx->own_stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
     return CW_OK;

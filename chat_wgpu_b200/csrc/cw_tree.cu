@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <mutex>
 
 #include "cw_tree.cuh"
 
@@ -518,6 +519,42 @@ __global__ void __launch_bounds__(TJ_WARPS * 32) k_tree_join(const __grid_consta
         if (d + e < a.D) out[e] = tree_to<T>(inv == 0.f ? 0.f : y[e] * inv);
 }
 
+// The context's scratch of at least `need` bytes, in stream order (no wait).  It comes
+// from a pool of the process, which keeps what a context gives back: the partial states
+// of a grid are up to 39 MB, and a plain allocation of that takes longer than the call.
+static int tree_scratch(cw_ctx* ctx, size_t need) {
+    if (need <= ctx->tree_scratch_bytes) return CW_OK;
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    CW_CUDA(cudaStreamIsCapturing(ctx->stream, &cs));
+    CW_CHECK(cs == cudaStreamCaptureStatusNone, CW_ERR_UNSUPPORTED,
+             "cw_tree_attention: call once with these sizes before a stream capture");
+    static std::mutex lock;
+    static cudaMemPool_t pools[64] = {};
+    CW_CHECK(ctx->device < 64, CW_ERR_UNSUPPORTED, "cw_tree_attention: device %d", ctx->device);
+    cudaMemPool_t pool;
+    {
+        std::lock_guard<std::mutex> hold(lock);
+        if (!pools[ctx->device]) {
+            cudaMemPoolProps props = {};
+            props.allocType = cudaMemAllocationTypePinned;
+            props.location.type = cudaMemLocationTypeDevice;
+            props.location.id = ctx->device;
+            cudaMemPool_t made;
+            CW_CUDA(cudaMemPoolCreate(&made, &props));
+            uint64_t keep = ~0ull;
+            CW_CUDA(cudaMemPoolSetAttribute(made, cudaMemPoolAttrReleaseThreshold, &keep));
+            pools[ctx->device] = made;
+        }
+        pool = pools[ctx->device];
+    }
+    void* p = nullptr;
+    CW_CUDA(cudaMallocFromPoolAsync(&p, need, pool, ctx->stream));
+    if (ctx->tree_scratch) cudaFreeAsync(ctx->tree_scratch, ctx->stream);
+    ctx->tree_scratch = p;
+    ctx->tree_scratch_bytes = need;
+    return CW_OK;
+}
+
 template <typename T, int DP, int WM, bool VEC>
 static int tree_go(cw_ctx* ctx, const TreeArgs& a, int grid) {
     constexpr size_t smem = tr_smem<DP, 16 * WM>();
@@ -630,14 +667,7 @@ extern "C" int cw_tree_attention(cw_ctx* ctx, const cw_tree_attn_args* p) {
     a.dp = (a.D + 3) / 4 * 4;
     const size_t part = (size_t)grid * 2 * a.bm * a.dp * 4, ml = (size_t)grid * 2 * a.bm * 8;
     const size_t need = part + ml + (size_t)grid * sizeof(TreePiece);
-    if (need > ctx->tree_scratch_bytes) {
-        CW_CUDA(cudaStreamSynchronize(ctx->stream));
-        if (ctx->tree_scratch) cudaFree(ctx->tree_scratch);
-        ctx->tree_scratch = nullptr;
-        ctx->tree_scratch_bytes = 0;
-        CW_CUDA(cudaMalloc(&ctx->tree_scratch, need));
-        ctx->tree_scratch_bytes = need;
-    }
+    CW_TRY(tree_scratch(ctx, need));
     a.part = (float*)ctx->tree_scratch;
     a.ml = (float2*)((char*)ctx->tree_scratch + part);
     a.pieces = (TreePiece*)((char*)ctx->tree_scratch + part + ml);

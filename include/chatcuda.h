@@ -389,8 +389,8 @@ typedef struct {
  * multiple of 8 and page_size 8, 16, 32 or a multiple of 64 run on the tcgen05
  * tensor cores (there the softmax weights are rounded to the type before the
  * product with v), everything else on warp-level tensor-core products at f32
- * accuracy.  Uses a context-owned scratch that grows on demand, which
- * synchronises. */
+ * accuracy.  Uses a context-owned scratch that grows on demand, in
+ * stream order: call once with a call's sizes before capturing it. */
 int cw_tree_attention(cw_ctx* ctx, const cw_tree_attn_args* args);
 
 /* ---- model: src/model/{mod,qwen3,layers,cache}.rs --------------------------------------------- */
