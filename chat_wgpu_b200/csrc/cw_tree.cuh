@@ -7,7 +7,9 @@
 // All units of the call, in request, kv head, row block, key order, are dealt to
 // the CTAs in equal runs, so ragged requests, few requests and long contexts all
 // fill the GPU alike.  The lengths are device data: every CTA sums the units of
-// all requests (a few loads per thread) and finds its own run.  An item cut by a
+// all requests (a few loads per thread) and finds its own run.  An item's start and end
+// cost about as much as a few tiles and count as such: with tiles alone the CTAs with
+// many short items ended a fifth later than the others.  An item cut by a
 // run's end leaves one f32 partial state (maximum, sum, weighted values) per piece;
 // a second launch joins the pieces in key order, so results do not depend on which
 // CTA ran first.
@@ -39,6 +41,7 @@ struct TreeArgs {
     float scale, softcap;
     int bm;            // rows of an item
     int least;         // least units of a CTA
+    int pad;           // units that an item's start and end count as
     int dp;            // floats of a partial row
     float* part;       // [grid * 2][bm][dp]
     float2* ml;        // [grid * 2][bm] maximum (times log2 e) and sum
@@ -72,17 +75,18 @@ __device__ __forceinline__ TreeReq tree_req(const TreeArgs& a, int r, bool repor
     q.blocks = (q.n * a.G + a.bm - 1) / a.bm;
     return q;
 }
+// Units of the request: its items' tiles, and `pad` more for each item's start and end.
 __device__ __forceinline__ long long tree_units(const TreeArgs& a, const TreeReq& q) {
-    return (long long)a.K * q.blocks * q.tiles;
+    return q.tiles ? (long long)a.K * q.blocks * (q.tiles + a.pad) : 0;
 }
 
-// This CTA's run of units, walked item by item.
+// This CTA's run of units, walked item by item: next is tile `pos` of item `item` of
+// request r, whose lengths are q.
 struct TreeRun {
-    long long per;    // units of a CTA
-    long long u;      // next unit, of all
-    long long off;    // next unit, within request r
-    int r, left;      // units left in the run
-    int seen;         // the request whose lengths q holds, or -1
+    long long per;       // units of a CTA
+    long long u;         // next unit, of all
+    int r, item, pos;
+    int left;            // units left in the run; above 0 there is a next tile
     TreeReq q;
 };
 struct TreeItem {
@@ -90,7 +94,22 @@ struct TreeItem {
     int r, head, block, rows;  // rows of this block
     int tile, tiles;           // tiles [tile, tile + tiles) of the item, from key tile q.tile0
     bool whole;
+    long long first;           // the item's first unit, of all
 };
+
+// Past the end of an item, its padding and requests without tiles.
+__device__ __forceinline__ void tree_advance(const TreeArgs& a, TreeRun& t) {
+    if (t.pos < t.q.tiles) return;
+    const int rest = t.q.tiles + a.pad - t.pos;
+    t.u += rest;
+    t.left -= rest;
+    t.pos = 0;
+    t.item++;
+    while (t.left > 0 && t.item >= (t.q.tiles ? a.K * t.q.blocks : 0)) {
+        t.q = tree_req(a, ++t.r, false);
+        t.item = 0;
+    }
+}
 
 // All threads (NT of them, a multiple of 32); sh is shared memory.
 struct TreeShared {
@@ -158,54 +177,50 @@ __device__ TreeRun tree_run(const TreeArgs& a, TreeShared* sh) {
     }
     __syncthreads();
     t.r = s_r;
-    t.off = s_off;
-    t.seen = -1;
+    t.item = t.pos = 0;
+    if (t.left > 0) {
+        t.q = tree_req(a, t.r, false);
+        t.item = (int)(s_off / (t.q.tiles + a.pad));
+        t.pos = (int)(s_off - (long long)t.item * (t.q.tiles + a.pad));
+        tree_advance(a, t);
+    }
     return t;
 }
 
 // The next item of the run (t.left > 0).
 __device__ __forceinline__ TreeItem tree_next(const TreeArgs& a, TreeRun& t) {
     TreeItem it;
-    while (true) {
-        if (t.seen != t.r) {  // an item of the request before it needs no loads
-            t.q = tree_req(a, t.r, false);
-            t.seen = t.r;
-        }
-        if (t.off < tree_units(a, t.q)) break;
-        t.r++;
-        t.off = 0;
-    }
     it.q = t.q;
-    const int item = (int)(t.off / it.q.tiles);
     it.r = t.r;
-    it.tile = (int)(t.off - (long long)item * it.q.tiles);
-    it.head = item / it.q.blocks;
-    it.block = item - it.head * it.q.blocks;
+    it.tile = t.pos;
+    it.head = t.item / it.q.blocks;
+    it.block = t.item - it.head * it.q.blocks;
     it.rows = min(a.bm, it.q.n * a.G - it.block * a.bm);
     it.tiles = min(it.q.tiles - it.tile, t.left);
     it.whole = it.tiles == it.q.tiles;
-    t.off += it.tiles;
+    it.first = t.u - it.tile;
+    t.pos += it.tiles;
     t.u += it.tiles;
     t.left -= it.tiles;
+    tree_advance(a, t);
     return it;
 }
 
 // Where an item's partial state goes: the run's first item in slot 0, a later one
 // (it can only be the last) in slot 1.
 __device__ __forceinline__ int tree_slot(const TreeRun& t, const TreeItem& it) {
-    return t.u - it.tiles == blockIdx.x * t.per ? 0 : 1;
+    return it.first + it.tile == blockIdx.x * t.per ? 0 : 1;
 }
 // One thread, after the run's last item: what the joining launch finds.
 __device__ __forceinline__ void tree_record(const TreeArgs& a, const TreeRun& t,
                                             const TreeItem& it, bool any) {
     TreePiece p = {};
     if (any && !it.whole && it.tile == 0) {
-        const long long first = t.u - it.tiles;
         p.row0 = it.q.row0;
         p.rows = it.rows;
         p.head = it.head;
         p.block = it.block;
-        p.count = (int)((first + it.q.tiles - 1) / t.per - blockIdx.x) + 1;
+        p.count = (int)((it.first + it.q.tiles - 1) / t.per - blockIdx.x) + 1;
         p.slot = tree_slot(t, it);
     }
     a.pieces[blockIdx.x] = p;

@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(320, 1)
             for (int i = 0; i < tiles; i++, n++) {
                 const int kt = key0 + i * SK;
                 const bool mixed = kt + SK > end || kt + SK > it.q.len || kt < edge;
-                at_v.skip(run.left == 0 && i + 1 == tiles ? 0 : 1, stages);
+                at_v.skip(run.left <= 0 && i + 1 == tiles ? 0 : 1, stages);
                 if (mixed) {
                     (void)tf_any(false, 3);  // the last tile's sets have been read
                     const int r = tid & 63, h = tid >> 6, k = kt + h * 64;
