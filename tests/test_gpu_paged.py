@@ -356,6 +356,41 @@ def test_tree_visible_not_finite(ctx, dtype):
     assert np.isfinite(got[:, :, rest]).all()
 
 
+@pytest.mark.parametrize("dtype,D,page", [("f32", 32, 8), ("bf16", 64, 8), ("f16", 72, 5)])
+def test_tree_many_requests(ctx, dtype, D, page):
+    """More requests than a block has threads, some without tokens or without nodes."""
+    H, K = 2, 1
+    rng = np.random.default_rng(9)
+    lens, nodes = rng.integers(0, 40, 700), rng.integers(0, 3, 700)
+    lens[::50] = 0
+    c = tree_case(rng, lens, nodes, dtype, H, K, D, page)
+    got = tree_run(ctx, c, dtype, H, K, D, page)
+    want, s, v = ref.attention(c["q"], c["kc"], c["vc"], c["table"], c["lens"], c["starts"], page, c["see"],
+                               c["pos"], 0, 0.0, D ** -0.5)
+    assert np.abs(got - want).max() <= tree_tolerance(dtype, s, v)
+    ctx.sync()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_tree_requests_do_not_meet(ctx, dtype):
+    """Queries of one request that are not finite leave the others' rows alone."""
+    H, K, D, page = 8, 2, 128, 16
+    c = tree_case(np.random.default_rng(10), [200, 30, 300], [3, 16, 7], dtype, H, K, D, page)
+    want, s, v = ref.attention(c["q"], c["kc"], c["vc"], c["table"], c["lens"], c["starts"], page, c["see"],
+                               c["pos"], 0, 0.0, D ** -0.5)
+    c["q"][3:19] = np.nan
+    got = tree_run(ctx, c, dtype, H, K, D, page)
+    rest = np.r_[0:3, 19:26]
+    assert np.abs(got[rest] - want[rest]).max() <= tree_tolerance(dtype, s, v)
+
+
+def test_tree_no_rows(ctx):
+    """A step in which no request has nodes writes nothing."""
+    c = tree_case(np.random.default_rng(11), [20, 3], [0, 0], "bf16", 4, 2, 64, 16)
+    assert (tree_run(ctx, c, "bf16", 4, 2, 64, 16) == 7.0).all()
+    ctx.sync()
+
+
 def test_tree_refusals(ctx):
     from chat_wgpu_b200 import CwError
     from chat_wgpu_b200.kernels.tree import TreeAttention
