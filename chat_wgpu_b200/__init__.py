@@ -7,6 +7,7 @@ Layout:
   context.py   GpuContext (the surface of chat-wgpu src/context.rs)
   kernels/     per-op wrappers (the surface of chat-wgpu src/kernels/)
   model.py     Model / Session / generate (chat-wgpu src/model/)
+  treedecode.py  greedy decode with drafted token trees over a paged cache
   gguf.py      GGUF writer/reader and seeded random-init checkpoints
 """
 from . import _lib  # noqa: F401

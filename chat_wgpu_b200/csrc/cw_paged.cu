@@ -18,7 +18,9 @@ namespace cw {
 // memory (8 bytes per request, read from L2) and then fills its own share of the
 // rows and of the fresh pages, so the plan is one launch with no word passed
 // between CTAs.  Rows whose page existed read the table below `have`, rows on
-// fresh pages read the free list itself: no CTA reads what another writes.
+// fresh pages read the free list itself: no CTA reads what another writes.  8 requests
+// take 5 us (launch and dependent reads), 1500 requests with a million tokens 10 us,
+// whose 13 MB alone would take 2.
 constexpr int PP_THREADS = 512;
 constexpr int PP_MAX_REQ = 16384;  // 3 * 4 bytes each: 192 KB of shared memory
 
@@ -190,7 +192,9 @@ __global__ void __launch_bounds__(PP_THREADS) k_page_plan(PagePlanArgs a) {
 // Memory bound: every row is read and written once.  A thread owns VEC pairs (two
 // 16-byte vectors) of one token and walks a share of the token's q, k and v
 // heads, so one set of sines serves all of them; neighbouring threads take
-// neighbouring vectors, then neighbouring heads.
+// neighbouring vectors, then neighbouring heads.  32768 bf16 rows of 32 + 8 + 8 heads
+// take 138 us (805 MB, 5.8 TB/s; 8 heads to a thread took 166, 2 took 294), 4096 f32
+// rows of 16 + 8 + 8 heads 27 us (4.9 TB/s).
 struct RopeArgs {
     const unsigned long long* steps;
     const int *positions, *slots;

@@ -12,7 +12,8 @@
 // many short items ended a fifth later than the others.  An item cut by a
 // run's end leaves one f32 partial state (maximum, sum, weighted values) per piece;
 // a second launch joins the pieces in key order, so results do not depend on which
-// CTA ran first.
+// CTA ran first.  (Joined by the last CTA to arrive instead, 150 us became 166: code
+// that runs once comes from memory, and it took registers from the main loops.)
 #pragma once
 
 #include <cuda_bf16.h>
@@ -292,7 +293,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 tree_to(float x) {
     return __float2bfloat16_rn(x);
 }
 
-// Host side: the tcgen05 kernel of 16-bit caches (cw_tree_tc.cu).  tree_tc_takes
+// Host side: the tcgen05 kernels of 16-bit caches.  tree_tc_takes
 // says whether the call's shape is one of its own; a.bm, a.dp and the grid follow.
 bool tree_tc_takes(const cw_tree_attn_args& p, const void* q, const void* k, const void* v);
 int tree_tc_rows(const TreeArgs& a);

@@ -11,9 +11,11 @@
 //
 // so the tensor work is proportional to the rows, a thread (one key of the tile) forms
 // N weights instead of padding rows, and K and V are read from shared memory once
-// each.  Bound by the cache's bytes: a tile at D = 128 is 64 KB, 1.5 us of an SM's
-// share of the memory bandwidth, against about 0.3 us of products and 0.1 to 0.5 us
-// of weights.
+// each.  Bound by the cache's bytes in the tiles: 64 KB at D = 128 is 1.5 us of an SM's
+// share of the memory bandwidth, against about 0.3 us of products and 0.5 to 1 us of
+// weights.  An item's start and end add 2 to 5 us, which deeper rings do not hide: 32
+// requests x 16 nodes at 8192 take 135 us where the bytes alone take 108, 256 x 1 of
+// 64 dims at 3001 200 us for 149, five of 256 dims with a window 24 us for 11.
 //
 // No maximum over keys is formed per tile: each row has a reference in shared memory,
 // and only when some weight would pass 2^8 (always at a row's first tile) the maxima
@@ -23,8 +25,9 @@
 //
 // Scores have two TMEM buffers and weights two in shared memory, so the products of
 // neighbouring tiles overlap the weights.  Warps: 2 groups of 4 for the weights, half
-// the rows each; 1 for TMA; 1 whose elected lane issues the products.  Keys that not every row sees, v rows past
-// the end and values that are not finite are treated as in cw_tree_tc.cu.
+// the rows each (one group: 180 us for 135); 1 for TMA; 1 whose elected lane issues the
+// products.  Keys that not every row sees, v rows past the end and values that are not
+// finite are treated as in cw_tree_tc.cu.
 #include <algorithm>
 
 #include "cw_tree_tc.cuh"

@@ -1,5 +1,6 @@
 // cw_tree_tc.cu -- cw_tree_attention over 16-bit caches on the 5th-generation
-// tensor cores (tcgen05, operands staged by TMA, accumulators in TMEM).
+// tensor cores (tcgen05, operands staged by TMA, accumulators in TMEM), for more rows
+// than cw_tree_few.cu takes.
 //
 // Per 64-key tile and 128 query rows (one TMEM lane a row):
 //
@@ -8,14 +9,16 @@
 //   O [128 x D]  += P V     P from TMEM, V as it lies in memory (keys x dims)
 //
 // The cache is read once: all G query heads of a kv head and all nodes of the
-// request share a tile (up to 128 rows, or 256 with two row blocks per CTA).  A
-// tile of 64 keys at D = 128 is 32 KB and takes an SM's share of the memory
-// bandwidth 0.75 us; its two products with all 128 rows take about 0.15 us of
-// tensor time and its exponentials 0.3 us, so the kernel is bound by memory up to
-// those rows and padding short row blocks costs nothing.
+// request share a tile (up to 128 rows, or 256 with two row blocks per CTA; at 256
+// dims 128, whose second block reads the tile through L2).  A tile of 64 keys at
+// D = 128 is 32 KB, 0.75 us of an SM's share of the memory bandwidth.  128 rows take
+// about as long (two CTAs per SM: 32 x 32 nodes at 8192 in 161 us, memory alone 109).
+// 256 rows are bound by their exponentials and the issue slots around them: 1.4 us a
+// tile, of which 0.6 us are the special-function unit's alone (2 x 64 nodes at 131000
+// in 316 us, memory alone 151).
 //
 // Warps: 4 (or 2 x 4) softmax warps, a thread per row, so row maxima and sums need
-// no exchange; one TMA warp; one MMA thread.  S has two TMEM buffers: the scores of
+// no exchange; one TMA warp; one elected MMA lane.  S has two TMEM buffers: the scores of
 // tile i + 1 are formed while the weights of tile i are.  O is rescaled only when a
 // row's maximum has grown by 2^8 since its last reference (weights then stay below
 // 256, far inside both types); the final division makes the reference drop out.

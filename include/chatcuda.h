@@ -385,11 +385,11 @@ typedef struct {
  * included.  mask_words is ceil(max_nodes / 32); a request has at most max_nodes
  * (<= 1024) nodes.  Query head h reads kv head h / (n_heads / n_kv); head_dim <=
  * 256.  Rows of out past starts[n_req] keep their contents.  q, cache and out are
- * of one type; sums and the softmax are f32.  16-bit types with head_dim a
- * multiple of 8 and page_size 8, 16, 32 or a multiple of 64 run on the tcgen05
- * tensor cores (there the softmax weights are rounded to the type before the
- * product with v), everything else on warp-level tensor-core products at f32
- * accuracy.  Uses a context-owned scratch that grows on demand, in
+ * of one type; sums and the softmax are f32.  16-bit types with head_dim,
+ * q_off and q_stride multiples of 8 and page_size 8, 16, 32 or a multiple of 64
+ * run on the tcgen05 tensor cores (there the softmax weights are rounded to the
+ * type before the product with v), everything else on warp-level tensor-core
+ * products at f32 accuracy.  Uses a context-owned scratch that grows on demand, in
  * stream order: call once with a call's sizes before capturing it. */
 int cw_tree_attention(cw_ctx* ctx, const cw_tree_attn_args* args);
 
