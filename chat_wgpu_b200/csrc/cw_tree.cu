@@ -7,7 +7,7 @@
 //
 // f32 accuracy on the warp-level tensor cores: every f32 operand x is the sum of
 // two TF32 values, x = h + l to within 2^-21 |x|, and a product is h h' + h l' + l h'
-// with f32 sums (the dropped l l' is below 2^-20 of the product).
+// with f32 sums (the dropped l l' is below 2^-21 of the product).
 // 16-bit operands are exact in one TF32 value, so their l terms are left out.
 //
 // Block: 8 warps, WM groups of 16 rows by WK = 8 / WM groups of 64 / WK keys; each
@@ -56,12 +56,22 @@ template <int N> __device__ __forceinline__ void tr_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 // x = h + l: h cut to TF32's 10 bits, l = x - h (exact) rounded to them, so h + l is
-// within 2^-21 of x either way.  Whole-number operations: the conversion instruction
-// runs at a fraction of their rate and bounded the kernel (f32, 8 x 24 nodes at 4500:
-// 232 us with it).  Infinities keep l = 0, NaN keeps h.
+// within 2^-21 of x.  Whole-number operations: the conversion instruction runs at a
+// fraction of their rate (8 x 24 f32 nodes at 4500: 232 us with it throughout, 205
+// without).  Infinities keep l = 0, NaN keeps h.
+__device__ __forceinline__ uint32_t tr_low(float x, uint32_t h) {
+    return (__float_as_uint(x - __uint_as_float(h)) + 0x1000u) & 0xffffe000u;
+}
 __device__ __forceinline__ void tr_split(float x, uint32_t& h, uint32_t& l) {
     h = __float_as_uint(x) & 0xffffe000u;
-    l = (__float_as_uint(x - __uint_as_float(h)) + 0x1000u) & 0xffffe000u;
+    l = tr_low(x, h);
+}
+// The same with h rounded, so that l is as often below zero as above.  One operand of a
+// product is split this way: cut on both sides, the dropped l l' would all have the
+// product's sign and scale the scores by about 1 - 2^-22.
+__device__ __forceinline__ void tr_split_even(float x, uint32_t& h, uint32_t& l) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(h) : "f"(x));
+    l = tr_low(x, h);
 }
 __device__ __forceinline__ void tr_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                        uint32_t b1) {
@@ -211,7 +221,12 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
             __syncthreads();
             rows_of((RING - 1) >> 1);
         }
+        // mx: running maximum of the scores; rf: what the weights so far refer to, in powers
+        // of two (-inf before any).  rf is kept, not formed again from mx: its rounding,
+        // 2^-24 of some 20, has to be the same in the weights and in their rescale (8 x 24
+        // nodes at 4500: error 4e-7 against 64 bits, 1.5e-6 with it formed again).
         float o[DB][4][4], mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+        float rf[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int b = 0; b < DB; b++)
 #pragma unroll
@@ -249,7 +264,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
                             for (int i = 0; i < 2; i++) {
                                 const float x = qa[h][2 * k + i];
                                 if (EXACT) ah[k][h + 2 * i] = __float_as_uint(x);
-                                else tr_split(x, ah[k][h + 2 * i], al[k][h + 2 * i]);
+                                else tr_split_even(x, ah[k][h + 2 * i], al[k][h + 2 * i]);
                             }
 #pragma unroll
                     for (int n = 0; n < NB; n++) {
@@ -299,8 +314,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
                         }
                     top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
-                    const float ref = top == -INFINITY ? 0.f : top * c2;
-                    const float fix = mx[h] == -INFINITY ? 0.f : exp2f(mx[h] * c2 - ref);
+                    const float ref = top == -INFINITY ? 0.f : __fmul_rn(top, c2);
+                    const float fix = rf[h] == -INFINITY ? 0.f : exp2f(rf[h] - ref);
                     float add = 0.f;
 #pragma unroll
                     for (int n = 0; n < NB; n++)
@@ -312,6 +327,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
                         }
                     sum[h] = sum[h] * fix + add;
                     mx[h] = top;
+                    rf[h] = top == -INFINITY ? -INFINITY : ref;
                     if (fix != 1.f) {
 #pragma unroll
                         for (int b = 0; b < DB; b++)
@@ -337,10 +353,10 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
 #pragma unroll
                     for (int n = 0; n < NB; n++) {
                         // operand order: row g key 2t, row g+8 key 2t, then key 2t+1
-                        tr_split(p[n][0], ph[n][0], pl[n][0]);
-                        tr_split(p[n][2], ph[n][1], pl[n][1]);
-                        tr_split(p[n][1], ph[n][2], pl[n][2]);
-                        tr_split(p[n][3], ph[n][3], pl[n][3]);
+                        tr_split_even(p[n][0], ph[n][0], pl[n][0]);
+                        tr_split_even(p[n][2], ph[n][1], pl[n][1]);
+                        tr_split_even(p[n][1], ph[n][2], pl[n][2]);
+                        tr_split_even(p[n][3], ph[n][3], pl[n][3]);
                     }
 #pragma unroll
                     for (int b = 0; b < DB; b++) {
@@ -411,7 +427,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
             sum[h] += __shfl_xor_sync(FULL, sum[h], 2);
             if (t4 == 0)
                 s_ml[wk * BM + wm * 16 + g + 8 * h] =
-                    make_float2(mx[h] == -INFINITY ? -INFINITY : mx[h] * c2, sum[h]);
+                    make_float2(rf[h], sum[h]);
         }
         __syncthreads();
         float own[2];
