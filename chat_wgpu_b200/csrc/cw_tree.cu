@@ -674,7 +674,6 @@ extern "C" int cw_tree_attention(cw_ctx* ctx, const cw_tree_attn_args* p) {
     a.scale = p->scale > 0.f ? p->scale : powf((float)D, -0.5f);
     a.softcap = p->softcap;
     a.status = ctx->d_status;
-    a.least = 1;
     const long long most = (long long)p->max_nodes * a.G;  // rows of a request's kv head
     const bool tc = tree_tc_takes(*p, a.q, a.k, a.v);
     int grid;

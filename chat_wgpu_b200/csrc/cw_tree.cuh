@@ -41,7 +41,6 @@ struct TreeArgs {
     int n_req, n_rows, max_nodes, words, H, K, G, D, page, n_pages, max_pages, window;
     float scale, softcap;
     int bm;            // rows of an item
-    int least;         // least units of a CTA
     int pad;           // units that an item's start and end count as
     int dp;            // floats of a partial row
     float* part;       // [grid * 2][bm][dp]
@@ -142,7 +141,7 @@ __device__ TreeRun tree_run(const TreeArgs& a, TreeShared* sh) {
         total += s_w[w];
     }
     TreeRun t;
-    t.per = max((total + gridDim.x - 1) / gridDim.x, (long long)a.least);
+    t.per = max((total + gridDim.x - 1) / gridDim.x, 1ll);
     t.u = blockIdx.x * t.per;
     t.left = (int)max(0ll, min(t.per, total - t.u));
     if (t.left > 0) {

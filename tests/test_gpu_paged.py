@@ -297,6 +297,8 @@ TREE = [  # dtype, heads, kv, dim, page, lens, nodes, options
     ("bf16", 16, 2, 64, 256, [1000], [200], {}),
     ("bf16", 24, 8, 80, 32, [333], [12], {}),
     ("bf16", 1, 1, 8, 8, [9, 0, 2], [1, 0, 3], {}),
+    ("bf16", 8, 4, 64, 192, [1000, 100], [4, 30], {}),
+    ("f16", 16, 2, 128, 320, [1500], [12], {}),
     # several tiles to a block's run, for each way a tile's keys are dealt to the lanes
     ("bf16", 8, 8, 128, 64, [6000], [1], {}),
     ("bf16", 32, 8, 128, 16, [4000, 900], [8, 3], {}),
@@ -382,6 +384,43 @@ def test_tree_requests_do_not_meet(ctx, dtype):
     got = tree_run(ctx, c, dtype, H, K, D, page)
     rest = np.r_[0:3, 19:26]
     assert np.abs(got[rest] - want[rest]).max() <= tree_tolerance(dtype, s, v)
+
+
+@pytest.mark.parametrize("dtype,pages", [("bf16", 70000), ("f32", 36000)])
+def test_far_pages(ctx, dtype, pages):
+    """Pages whose elements lie past 32 bits (bf16: 4.6e9 elements, f32: 2.4e9) hold and
+    give back the same as pages at the start."""
+    torch = pytest.importorskip("torch")
+    from chat_wgpu_b200 import GpuContext
+    from chat_wgpu_b200.kernels import rope, tree
+    H, K, D, page, T, n = 8, 8, 128, 64, 150, 3
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").to(dt)  # noqa: E731
+    i = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    q, k, v = rnd(T, H * D), rnd(T, K * D), rnd(T, K * D)
+    kc, vc = (torch.empty(pages, K, page, D, dtype=dt, device="cuda") for _ in range(2))
+    c = GpuContext(0, stream=torch.cuda.current_stream().cuda_stream)
+    plan = rope.rope_plan(c, D, 1e4)
+    kw, vw, pos, outs = c.wrap(kc), c.wrap(vc), c.wrap(i(range(T))), []
+    for first in (0, pages - n):
+        slots = c.wrap(i([first * page + t for t in range(T)]))
+        rot = torch.empty_like(q)
+        rope.RopeAppend(c, plan=plan, positions=pos, dtype=dtype, n_tokens=T, n_heads=H, n_kv=K, head_dim=D,
+                        q=c.wrap(q), q_out=c.wrap(rot), k=c.wrap(k), v=c.wrap(v), slots=slots, k_cache=kw,
+                        v_cache=vw, page_size=page, n_pages=pages)()
+        out = torch.empty(5, H * D, dtype=dt, device="cuda")
+        tree.TreeAttention(c, q=c.wrap(rot[:5]), k_cache=kw, v_cache=vw, table=c.wrap(i([[first, first + 1, first + 2]])),
+                           lens=c.wrap(i([T - 5])), starts=c.wrap(i([0, 5])), out=c.wrap(out), dtype=dtype, n_req=1,
+                           n_rows=5, max_nodes=5, n_heads=H, n_kv=K, head_dim=D, page_size=page, n_pages=pages,
+                           max_pages=n)()
+        c.sync()
+        assert torch.equal(vc[first + 1].transpose(0, 1).reshape(page, -1), v[page:2 * page])
+        outs.append(out)
+    assert torch.equal(outs[0], outs[1]) and bool(outs[0].isfinite().all())
+    c.close()
+    del kc, vc
+    torch.cuda.empty_cache()
 
 
 def test_tree_no_rows(ctx):
