@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(320, 1)
     TreeItem it;
     bool any = false, ok = true;
     const TtTile tile =
-        a.D % 64 == 0 ? TtTile{COLS * 1024, 1024} : TtTile{1024, SK * 128};
+        tt_wide(a.D) ? TtTile{COLS * 1024, 1024} : TtTile{1024, SK * 128};
 
     // The tiles of all items run through the products as one sequence t = 0, 1, ..: the
     // scores of tile t + 1 are formed before the values of tile t, so the ring holds
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(320, 1)
 // 64 rows, or 32 of 256 dims (the ring needs three tiles beside the queries); a tile's
 // copies have to fit one warp's lanes.
 bool tt_few_takes(const TreeArgs& a) {
-    const int cols = a.D % 64 == 0 ? 1 : a.D <= 64 ? 1 : a.D <= 128 ? 2 : 4;
+    const int cols = tt_wide(a.D) || a.D <= 64 ? 1 : a.D <= 128 ? 2 : 4;
     return a.max_nodes * a.G <= (a.D <= 128 ? 64 : 32) && 128 / std::min(a.page, 64) * cols <= 32;
 }
 

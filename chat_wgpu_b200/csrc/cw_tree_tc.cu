@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
     };
     TreeItem it;
     bool any = false, ok = true;
-    const bool wide = a.D % 64 == 0;
+    const bool wide = tt_wide(a.D);
     const TtTile tile = wide ? TtTile{COLS * 1024, 1024} : TtTile{1024, TILE * 128};
     TtPlace at = {0, 0};
 
@@ -538,7 +538,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 tt_encode_fn() {
 int tt_map(CUtensorMap* map, const void* base, const TreeArgs& a, bool bf) {
     auto enc = tt_encode_fn();
     CW_CHECK(enc, CW_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    const bool wide = a.D % 64 == 0;
+    const bool wide = tt_wide(a.D);
     cuuint64_t dims[4] = {(cuuint64_t)(wide ? 64 : a.D), 8, (cuuint64_t)(wide ? a.D / 64 : 1),
                           (cuuint64_t)a.n_pages * a.K * a.page / 8};
     cuuint64_t strides[3] = {(cuuint64_t)a.D * 2, 128, (cuuint64_t)a.D * 16};

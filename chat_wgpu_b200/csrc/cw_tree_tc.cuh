@@ -128,9 +128,10 @@ __device__ __forceinline__ void tt_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
 }
 // How a K or V tile lies in shared memory: 1024-byte atoms of 8 keys x 64 dims
 // (128-byte swizzled), `group` bytes from 8 keys to the next and `col` bytes from 64
-// dims to the next.  Where D is a multiple of 64 one copy brings all of a page's
-// rows and dims, atoms of 8 keys side by side; else a copy per 64 dims, whose last
-// one reads zeros past D.
+// dims to the next.  Where D fills the instance's columns (tt_wide) one copy brings all
+// of a page's rows and dims, atoms of 8 keys side by side; else a copy per 64 dims, and
+// those past D read zeros.
+__host__ __device__ constexpr bool tt_wide(int D) { return D == 64 || D == 128 || D == 256; }
 struct TtTile {
     uint32_t group, col;
     __device__ __forceinline__ uint32_t at(int key, int chunk) const {  // 16-byte chunk
@@ -251,7 +252,7 @@ template <int COLS, int SK> struct TtFeed {
                       int stages_, const TtTile& t)
         : a(a_), ring(ring_), full(full_), empty(empty_), stages(stages_),
           lane(threadIdx.x & 31) {
-        const bool wide = a.D % 64 == 0;
+        const bool wide = tt_wide(a.D);
         box = min(a.page, 64);
         const int per = SK / box;
         boxes = wide ? per : per * COLS;

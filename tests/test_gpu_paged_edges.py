@@ -1,0 +1,89 @@
+"""Edges of the paged operators: shapes between the common ones, values that are not
+finite, pages that are missing, captured steps, wrapped tensors."""
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+import paged_ref as ref
+from conftest import ROOT
+from test_gpu_paged import get, i32, tree_case, tree_run, tree_tolerance
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(c, page, softcap=0.0, scale=None, gone=None, window=0):
+    """The plain form over the keys a row sees, without those in gone[r] (bool per key)."""
+    T, H, D = c["q"].shape
+    K = c["kc"].shape[1]
+    scale = D ** -0.5 if scale is None else scale
+    out = np.zeros((T, H, D))
+    big_s = big_v = 0.0
+    for r in range(len(c["lens"])):
+        a, b, n0 = int(c["starts"][r]), int(c["starts"][r + 1]), int(c["lens"][r])
+        at = np.arange(n0 + b - a)
+        pages = c["table"][r, at // page]
+        where = np.concatenate([at[:n0], c["pos"][a:b]])
+        for t in range(a, b):
+            vis = np.concatenate([np.ones(n0, bool), c["see"][r][t - a]])
+            if window:
+                vis &= c["pos"][t] - where < window
+            if gone is not None:
+                vis &= ~gone[r]
+            j = np.flatnonzero(vis)
+            if not len(j):
+                continue
+            for h in range(H):
+                k, v = (x[pages[j], h // (H // K), j % page] for x in (c["kc"], c["vc"]))
+                with np.errstate(invalid="ignore"):
+                    s = k @ c["q"][t, h] * scale
+                fine = np.isfinite(s)
+                if fine.any():
+                    big_s = max(big_s, float((np.abs(k[fine]) @ np.abs(c["q"][t, h])).max()) * scale)
+                big_v = max(big_v, float(np.abs(v[np.isfinite(v)]).max()))
+                if softcap:
+                    s = softcap * np.tanh(s / softcap)
+                top = s.max()
+                if top == -np.inf:
+                    continue
+                with np.errstate(invalid="ignore"):
+                    w = np.exp(s - top)
+                    out[t, h] = w @ v / w.sum()
+    return out, big_s, big_v
+
+
+# every kernel: f32; 16 bit with few rows; many rows; two row blocks; 256 dims in parts
+KINDS = [  # dtype, heads, kv, dim, page, nodes
+    ("f32", 4, 2, 64, 16, 5), ("f32", 16, 2, 128, 16, 9), ("bf16", 8, 2, 64, 16, 3), ("f16", 16, 4, 128, 16, 9),
+    ("bf16", 16, 2, 128, 32, 12), ("f16", 16, 2, 64, 16, 30), ("bf16", 8, 4, 256, 8, 3), ("f16", 8, 4, 256, 16, 30),
+]
+kinds = pytest.mark.parametrize("kind", KINDS, ids=lambda k: "-".join(map(str, k)))
+
+
+# ---------------------------------------------------------------- head dims
+@pytest.mark.parametrize("case", [
+    ("bf16", 16, 8, 16, [700, 130, 1], [8, 5, 1], {}), ("f16", 8, 4, 64, [3000], [40], {}),
+    ("bf16", 8, 4, 8, [900, 40], [3, 9], {}), ("f16", 8, 4, 32, [1000], [30], dict(window=300, softcap=20.0)),
+    ("bf16", 16, 8, 128, [5000], [1], {}), ("f16", 32, 8, 192, [500], [64], dict(empty=True)),
+    ("bf16", 8, 4, 256, [777, 2], [100, 7], {})], ids=lambda c: f"{c[0]}-p{c[3]}-{max(c[4])}x{max(c[5])}")
+def test_192_dims(ctx, case):
+    dtype, H, K, page, lens, nodes, opt = case
+    opt = dict(opt)
+    c = tree_case(np.random.default_rng(sum(lens)), lens, nodes, dtype, H, K, 192, page, empty=opt.pop("empty", False))
+    got = tree_run(ctx, c, dtype, H, K, 192, page, pad=8, off=8, **opt)
+    want, s, v = attend(c, page, softcap=opt.get("softcap", 0.0), window=opt.get("window", 0))
+    assert np.abs(got - want).max() <= tree_tolerance(dtype, s, v)
+    ctx.sync()
+
+
+@pytest.mark.parametrize("nodes", [3, 70])
+def test_every_multiple_of_8(ctx, nodes):
+    """All head dims that the tensor-core kernels take, of few rows and of many."""
+    for D in range(8, 257, 8):
+        dtype = "bf16" if D % 16 else "f16"
+        c = tree_case(np.random.default_rng(D), [150, 20], [nodes, 2], dtype, 4, 2, D, 16)
+        got = tree_run(ctx, c, dtype, 4, 2, D, 16)
+        want, s, v = attend(c, 16)
+        assert np.abs(got - want).max() <= tree_tolerance(dtype, s, v), D
+        ctx.sync()
