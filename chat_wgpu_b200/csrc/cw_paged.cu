@@ -389,7 +389,8 @@ int cw_page_plan(cw_ctx* ctx, const cw_page_plan_args* p) {
     a.max_tokens = (int)T;
     a.shift = (p->page_size & (p->page_size - 1)) == 0 ? __builtin_ctz(p->page_size) : -1;
     const size_t smem = 12 * R;
-    if (smem > 48 * 1024)
+    // 48 KB without it, the kernel's own 208 bytes of static shared memory included
+    if (smem > 47 * 1024)
         CW_CUDA(cudaFuncSetAttribute(k_page_plan, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      12 * PP_MAX_REQ));
     // one group of four rows to a thread until two CTAs per SM are busy

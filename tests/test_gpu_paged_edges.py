@@ -87,3 +87,28 @@ def test_every_multiple_of_8(ctx, nodes):
         want, s, v = attend(c, 16)
         assert np.abs(got - want).max() <= tree_tolerance(dtype, s, v), D
         ctx.sync()
+
+
+# ---------------------------------------------------------------- page plan
+@pytest.mark.parametrize("n", [4079, 4080, 4096, 4097])
+def test_plan_is_the_first_call(n):
+    """Request counts around 48 KB of shared memory, each in a process of its own: no
+    earlier call has raised the kernel's limit."""
+    code = f"""
+import sys
+sys.path.insert(0, {ROOT!r})
+import numpy as np
+from chat_wgpu_b200 import GpuContext
+from chat_wgpu_b200.kernels.pages import PagePlan
+n = {n}
+with GpuContext(0) as c:
+    i = lambda a: c.storage_u32(np.ascontiguousarray(a, np.int32).view(np.uint32))
+    out = dict(starts=i(np.zeros(n + 1)), positions=i(np.zeros(n)), slots=i(np.zeros(n)), owners=i(np.zeros(n)),
+               used=i([0]))
+    PagePlan(c, lens=i(np.full(n, 3)), news=i(np.ones(n)), free_pages=None, table=i(np.arange(n)), n_req=n,
+             page_size=4, max_pages=1, n_free=0, max_tokens=n, **out)()
+    assert np.array_equal(c.read_u32(out["slots"], n), np.arange(n) * 4 + 3)
+    assert np.array_equal(c.read_u32(out["starts"], n + 1), np.arange(n + 1))
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
