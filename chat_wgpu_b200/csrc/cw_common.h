@@ -117,9 +117,11 @@ struct cw_ctx {
     void* gemm_scratch = nullptr;
     size_t gemm_scratch_bytes = 0;
 
-    // grow-only scratch of the tree attention (partial states of split keys)
+    // grow-only scratch of the tree attention (partial states of split keys): the
+    // largest block, and the outgrown ones, which captured graphs may still name
     void* tree_scratch = nullptr;
     size_t tree_scratch_bytes = 0;
+    std::vector<void*> tree_outgrown;
 };
 
 namespace cw {

@@ -294,6 +294,7 @@ int cw_ctx_destroy(cw_ctx* ctx) {
     if (ctx->d_counters) cudaFree(ctx->d_counters);
     if (ctx->gemm_scratch) cudaFree(ctx->gemm_scratch);
     if (ctx->tree_scratch) cudaFreeAsync(ctx->tree_scratch, ctx->stream);
+    for (void* p : ctx->tree_outgrown) cudaFreeAsync(p, ctx->stream);
     if (ctx->stream && ctx->own_stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
     return CW_OK;

@@ -543,6 +543,8 @@ __global__ void __launch_bounds__(TJ_WARPS * 32) k_tree_join(const __grid_consta
 // The context's scratch of at least `need` bytes, in stream order (no wait).  It comes
 // from a pool of the process, which keeps what a context gives back: the partial states
 // of a grid are up to 39 MB, and a plain allocation of that takes longer than the call.
+// An outgrown block stays until the context goes, since a graph captured before may still
+// write there; a new block is twice the old one at least, so they add up to less than it.
 static int tree_scratch(cw_ctx* ctx, size_t need) {
     if (need <= ctx->tree_scratch_bytes) return CW_OK;
     cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
@@ -568,9 +570,15 @@ static int tree_scratch(cw_ctx* ctx, size_t need) {
         }
         pool = pools[ctx->device];
     }
+    need = std::max(need, 2 * ctx->tree_scratch_bytes);
+    try {
+        ctx->tree_outgrown.reserve(ctx->tree_outgrown.size() + 1);
+    } catch (...) {
+        return set_error(CW_ERR_OOM, "cw_tree_attention: out of host memory");
+    }
     void* p = nullptr;
     CW_CUDA(cudaMallocFromPoolAsync(&p, need, pool, ctx->stream));
-    if (ctx->tree_scratch) cudaFreeAsync(ctx->tree_scratch, ctx->stream);
+    if (ctx->tree_scratch) ctx->tree_outgrown.push_back(ctx->tree_scratch);
     ctx->tree_scratch = p;
     ctx->tree_scratch_bytes = need;
     return CW_OK;

@@ -390,7 +390,9 @@ typedef struct {
  * run on the tcgen05 tensor cores (there the softmax weights are rounded to the
  * type before the product with v), everything else on warp-level tensor-core
  * products at f32 accuracy.  Uses a context-owned scratch that grows on demand, in
- * stream order: call once with a call's sizes before capturing it. */
+ * stream order: call once with a call's sizes before capturing it.  A captured call
+ * keeps its scratch whatever the context runs later; replay it before the context is
+ * destroyed, and in order with the context's other tree attention calls. */
 int cw_tree_attention(cw_ctx* ctx, const cw_tree_attn_args* args);
 
 /* ---- model: src/model/{mod,qwen3,layers,cache}.rs --------------------------------------------- */

@@ -112,3 +112,75 @@ with GpuContext(0) as c:
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# ---------------------------------------------------------------- captured steps
+def test_captured_step_outlives_larger_calls():
+    """Plan, rotary and attention captured in a graph keep their results when the context
+    later runs calls that need more scratch and another context takes scratch of its own
+    and works beside the graph."""
+    torch = pytest.importorskip("torch")
+    from chat_wgpu_b200 import GpuContext
+    from chat_wgpu_b200.kernels import pages, rope, tree
+    side, beside = torch.cuda.Stream(), torch.cuda.Stream()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").to(torch.bfloat16)  # noqa: E731
+    i = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    H, K, page = 8, 2, 16
+
+    def step(c, lens, n, D):
+        """A request of `lens` tokens and n nodes: its calls and their result."""
+        P = -(-(lens + n) // page)
+        t = dict(lens=i([lens]), news=i([n]), free=i(list(range(P))), table=i([list(range(P))]),
+                 starts=i([0, 0]), pos=i([0] * n), slots=i([0] * n), own=i([0] * n), used=i([0]), q=rnd(n, H * D),
+                 k=rnd(n, K * D), v=rnd(n, K * D), kc=rnd(2 * P, K, page, D), vc=rnd(2 * P, K, page, D),
+                 rot=torch.zeros(n, H * D, dtype=torch.bfloat16, device="cuda"),
+                 out=torch.zeros(n, H * D, dtype=torch.bfloat16, device="cuda"))
+        t["free"] += P
+        w = {k: c.wrap(x) for k, x in t.items()}
+        plan = rope.rope_plan(c, D, 1e4)
+        return [pages.PagePlan(c, lens=w["lens"], news=w["news"], free_pages=w["free"], table=w["table"],
+                               starts=w["starts"], positions=w["pos"], slots=w["slots"], owners=w["own"],
+                               used=w["used"], n_req=1, page_size=page, max_pages=P, n_free=P, max_tokens=n),
+                rope.RopeAppend(c, plan=plan, positions=w["pos"], dtype="bf16", n_tokens=n, n_heads=H, n_kv=K,
+                                head_dim=D, q=w["q"], q_out=w["rot"], k=w["k"], v=w["v"], slots=w["slots"],
+                                k_cache=w["kc"], v_cache=w["vc"], page_size=page, n_pages=2 * P),
+                tree.TreeAttention(c, q=w["rot"], k_cache=w["kc"], v_cache=w["vc"], table=w["table"], lens=w["lens"],
+                                   starts=w["starts"], out=w["out"], dtype="bf16", n_req=1, n_rows=n, max_nodes=n,
+                                   n_heads=H, n_kv=K, head_dim=D, page_size=page, n_pages=2 * P, max_pages=P)], t["out"]
+
+    c, other = GpuContext(0, stream=side.cuda_stream), GpuContext(0, stream=beside.cuda_stream)
+    small, out = step(c, 5000, 3, 64)
+    big, big_out = step(c, 9000, 60, 256)
+    theirs, their_out = step(other, 9000, 3, 64)
+    torch.cuda.synchronize()
+    for f in small:
+        f()
+    side.synchronize()
+    first = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        for f in small:
+            f()
+    for f in big + theirs:
+        f()
+    torch.cuda.synchronize()
+    kept, many = (big_out.clone(), their_out.clone()), []
+    for _ in range(40):
+        with torch.cuda.stream(side):
+            out.zero_()
+            graph.replay()
+            many.append((out.clone(), first))
+        with torch.cuda.stream(beside):
+            theirs[2]()
+            many.append((their_out.clone(), kept[1]))
+    for f in big:
+        f()
+    torch.cuda.synchronize()
+    assert torch.equal(big_out, kept[0]) and bool((first != 0).any())
+    assert all(torch.equal(a, b) for a, b in many)
+    c.sync()
+    other.sync()
+    del graph
+    c.close()
+    other.close()
