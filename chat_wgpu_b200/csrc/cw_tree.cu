@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
             for (int w = 0; w < WK; w++) top = fmaxf(top, s_ml[w * BM + tid].x);
             for (int w = 0; w < WK; w++) {
                 const float2 x = s_ml[w * BM + tid];
-                if (x.x != -INFINITY) l += x.y * exp2f(x.x - top);
+                if (x.y != 0.f) l += x.y * exp2f(x.x - top);  // 0: saw nothing; NaN stays
             }
             s_all[tid] = make_float2(top, l);
         }
@@ -508,8 +508,10 @@ __global__ void __launch_bounds__(TJ_WARPS * 32) k_tree_join(const __grid_consta
         float w = 0.f;
         if (i0 + lane < p.count) {
             const float2 x = __ldcg(&a.ml[piece(i0 + lane)]);
-            if (x.x != -INFINITY) w = exp2f(x.x - top);
-            if (w != 0.f) l += w * x.y;
+            if (x.y != 0.f) {  // 0: the row saw nothing there; NaN stays
+                w = exp2f(x.x - top);
+                l += w * x.y;
+            }
         }
         const int n = min(32, p.count - i0);
         for (int j0 = 0; j0 < n; j0 += 8) {

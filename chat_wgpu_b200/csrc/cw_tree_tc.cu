@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
 #pragma unroll
                 for (int s = 0; s < SPLIT; s++) {
                     const float2 x = s_ml[s * LANES + r];
-                    if (x.x != -INFINITY) l += x.y * tt_exp2(x.x - top);
+                    if (x.y != 0.f) l += x.y * tt_exp2(x.x - top);  // NaN stays
                 }
                 const float own = ref == -INFINITY ? 0.f : tt_exp2(ref - top);
                 const float inv = l > 0.f || l != l ? 1.f / l : 0.f;

@@ -184,3 +184,20 @@ def test_captured_step_outlives_larger_calls():
     del graph
     c.close()
     other.close()
+
+
+# ---------------------------------------------------------------- values that are not finite
+@kinds
+@pytest.mark.parametrize("lens", [[40, 3], [9000, 3]], ids=["whole", "cut"])
+def test_query_of_nan(ctx, kind, lens):
+    """A row whose scores are NaN is NaN, whether its item is cut or not; the others stay."""
+    dtype, H, K, D, page, n = kind
+    c = tree_case(np.random.default_rng(21), lens, [n, 2], dtype, H, K, D, page, poison=False)
+    want, s, v = attend(c, page)
+    c["q"][1, H - 1, 5] = np.nan
+    got = tree_run(ctx, c, dtype, H, K, D, page)
+    assert np.isnan(got[1, H - 1]).all()
+    rest = np.ones(got.shape[:2], bool)
+    rest[1, H - 1] = False
+    assert np.abs(got - want)[rest].max() <= tree_tolerance(dtype, s, v)
+    ctx.sync()
