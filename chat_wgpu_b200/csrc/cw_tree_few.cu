@@ -46,6 +46,7 @@ template <int HD, int N> struct TfShape {
 };
 
 constexpr int TF_STAGES = 12;
+constexpr float TF_NONE = 3.402823466e38f;
 template <int N> struct TfBars {
     uint64_t full[TF_STAGES], empty[TF_STAGES];
     uint64_t q_full[2], q_empty[2];                      // [item % QB]
@@ -53,8 +54,8 @@ template <int N> struct TfBars {
     uint32_t tmem, failed, keep;
     TreeShared run;
     uint64_t sees[2][N];  // [64 keys][row]
-    // what is added to a row's scores: -reference, +inf while it has seen nothing (any
-    // score it sees passes 2^8), -inf past the rows
+    // what is added to a row's scores: -reference, TF_NONE while it has seen nothing above
+    // -inf (any such score passes 2^8, and -inf still weighs 0), -inf past the rows
     alignas(16) float neg[N];
     alignas(16) float fix[N];  // a rescale's factors, or at the item's end 1 / sum
     float sums[4][N];          // each warp's
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(320, 1)
                 edge = __reduce_max_sync(FULL, edge);
             }
             if (m < C) {
-                neg[m] = c0 + m < rows ? INFINITY : -INFINITY;
+                neg[m] = c0 + m < rows ? TF_NONE : -INFINITY;
                 fix[m] = __int_as_float(tf_order(-INFINITY));
             }
             if (tid == 0) bars->keep = 0;
@@ -363,7 +364,7 @@ __global__ void __launch_bounds__(320, 1)
                         if (m < C) {
                             const float was = -neg[m];
                             const float now = fmaxf(tf_float(__float_as_int(fix[m])), was);
-                            fix[m] = was == -INFINITY ? 0.f : tt_exp2(was - now);
+                            fix[m] = tt_exp2(was - now);
                             if (c0 + m < rows) neg[m] = -now;
                         }
                         (void)tf_any(false, id);
@@ -410,11 +411,6 @@ __global__ void __launch_bounds__(320, 1)
                 uint8_t* p = s_p + (n % PB) * 16384;
 #pragma unroll
                 for (int c = 0; c < C; c++) s[c] = tt_exp2(s[c]);
-                if (mixed) {  // -inf + inf of a row that has seen nothing
-#pragma unroll
-                    for (int c = 0; c < C; c++)
-                        if (!(sees[c] >> (m & 63) & 1)) s[c] = 0.f;
-                }
 #pragma unroll
                 for (int c = 0; c < C; c += 8) {
                     uint32_t w[4];

@@ -201,3 +201,22 @@ def test_query_of_nan(ctx, kind, lens):
     rest[1, H - 1] = False
     assert np.abs(got - want)[rest].max() <= tree_tolerance(dtype, s, v)
     ctx.sync()
+
+
+@pytest.mark.parametrize("kind", [k for k in KINDS if k[0] != "f32"], ids=lambda k: "-".join(map(str, k)))
+@pytest.mark.parametrize("lens", [[400, 3], [9000, 3]], ids=["whole", "cut"])
+def test_scores_of_minus_infinity(ctx, kind, lens):
+    """Keys that score -inf weigh nothing, first tiles full of them included; a row with
+    no other key gives zeros."""
+    dtype, H, K, D, page, n = kind
+    c = tree_case(np.random.default_rng(22), lens, [n, 2], dtype, H, K, D, page, poison=False)
+    c["q"][:, :, 2] = 1.0
+    at = np.arange(320)
+    c["kc"][c["table"][0, at // page], :, at % page, 2] = -np.inf
+    every = np.arange(5)  # all keys of the second request
+    c["kc"][c["table"][1, every // page], :, every % page, 2] = -np.inf
+    got = tree_run(ctx, c, dtype, H, K, D, page)
+    want, s, v = attend(c, page)
+    assert (got[n:] == 0).all()
+    assert np.abs(got - want).max() <= tree_tolerance(dtype, s, v)
+    ctx.sync()
