@@ -343,7 +343,11 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
                 // would reach rows that do not see the key, so a tile that rows see
                 // differently is looked over first (keys past the end were zero-filled).
                 bool odd = false;
+                uint64_t see0 = 0, see1 = 0;
                 if (part) {
+                    // read before the vote: after it the next tile's sets may be written
+                    see0 = s_sees[wm * 16 + g] >> (wk * KW);
+                    see1 = s_sees[wm * 16 + g + 8] >> (wk * KW);
                     for (int i = tid; i < TR_TILE * DP; i += TR_THREADS)
                         odd |= !(fabsf(tile[i]) <= 3.402823466e38f);
                     odd = __syncthreads_or(odd);
@@ -390,8 +394,6 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
                             for (int e = 0; e < 4; e++) o[b][i][e] += hh[i][e] + lo[i][e];
                     }
                 } else {
-                    const uint64_t see0 = s_sees[wm * 16 + g] >> (wk * KW);
-                    const uint64_t see1 = s_sees[wm * 16 + g + 8] >> (wk * KW);
 #pragma unroll
                     for (int n = 0; n < NB; n++)
 #pragma unroll

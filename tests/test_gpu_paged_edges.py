@@ -220,3 +220,24 @@ def test_scores_of_minus_infinity(ctx, kind, lens):
     assert (got[n:] == 0).all()
     assert np.abs(got - want).max() <= tree_tolerance(dtype, s, v)
     ctx.sync()
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (16, 2, 128), (8, 4, 256)])
+def test_many_tiles_of_values_that_are_not_finite(ctx, heads, kv, dim):
+    """f32, one tile after another holding values that no row sees and that are not finite: every
+    tile's rows use that tile's own sets."""
+    c = tree_case(np.random.default_rng(24), [30, 0], [400, 3], "f32", heads, kv, dim, 16, poison=False)
+    m = 400
+    for j in range(0, m, 3):  # node j: seen by nobody
+        c["see"][0][:, j] = False
+        c["vc"][c["table"][0, (30 + j) // 16], :, (30 + j) % 16] = np.nan if j % 2 else np.inf
+    words = c["mask"].shape[1]
+    bits = np.zeros((c["T"], words * 32), np.uint8)
+    bits[:m, :m] = c["see"][0]
+    bits[m:, :3] = c["see"][1]
+    c["mask"] = np.packbits(bits, axis=1, bitorder="little").view(np.uint32)
+    want, s, v = attend(c, 16)
+    for _ in range(5):
+        got = tree_run(ctx, c, "f32", heads, kv, dim, 16)
+        assert np.abs(got - want).max() <= tree_tolerance("f32", s, v)
+    ctx.sync()
