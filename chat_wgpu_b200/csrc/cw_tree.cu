@@ -86,6 +86,15 @@ template <int DP> __device__ __forceinline__ int tr_at(int j, int c) {
     return j * DP + ((c & ~7) | ((c ^ j) & 7)) * 4;
 }
 
+// One score from f32 products.
+template <int DP> __device__ __noinline__ float tr_dot(const float* sq, const float* tile, int m, int j) {
+    float x = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < DP; d++)
+        x = fmaf(sq[tr_at<DP>(m, d >> 2) + (d & 3)], tile[tr_at<DP>(j, d >> 2) + (d & 3)], x);
+    return x;
+}
+
 // Ring buffers (one K or V tile each) that fit beside the queries.
 template <int DP, int BM> constexpr int tr_ring() {
     const size_t left = TR_SMEM_CAP - (size_t)BM * DP * 4 - BM * 8 - TR_ROWS * TR_TILE * 8 - 1024;
@@ -119,9 +128,9 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
     pdl_trigger();
     TreeRun run = tree_run<TR_THREADS>(a, &s_run);
     TreeItem it;
-    bool any = false;
-    while (run.left > 0) {
-        it = tree_next(a, run);
+    bool any = false, again = false;
+    while (again || run.left > 0) {
+        if (!again) it = tree_next(a, run);
         any = true;
         const T* kb = (const T*)a.k;
         const T* vb = (const T*)a.v;
@@ -237,7 +246,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
         float p[NB][4];
         for (int s = 0; s < steps; s++) {
             const int kt = key0 + (s >> 1) * TR_TILE;
-            const bool part = tree_partial(it.q, s_edge, kt);
+            const bool part = again || tree_partial(it.q, s_edge, kt);
             if (!(s & 1) && part && tid < BM) s_sees[tid] = tree_sees(a, it.q, m0 + tid, kt);
             tr_wait<RING - 2>();
             __syncthreads();  // tile s is here, and everyone is done with tile s - 1
@@ -297,6 +306,15 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
                     }
                 }
                 // ---- weights; accumulator element e: row g + 8 (e / 2), key 2 t4 + e % 2
+                if (again) {
+#pragma unroll
+                    for (int n = 0; n < NB; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (p[n][e] != p[n][e])
+                                p[n][e] = tr_dot<DP>(sq, tile, wm * 16 + g + 8 * (e >> 1),
+                                                     wk * KW + n * 8 + 2 * t4 + (e & 1));
+                }
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const uint64_t sees =
@@ -421,7 +439,24 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
             if (!((s + RING) & 1)) rows_of((s + RING) >> 1);
         }
         tr_wait<0>();
-        __syncthreads();
+        // A part of a pair times an infinity can be NaN where the whole product is not (0 or
+        // the other sign in its low part).  Sums of NaN send the item through once more,
+        // with such scores formed again and every tile's values looked over.
+        bool nan = false;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if (wm * 16 + g + 8 * h >= it.rows) continue;
+            nan |= sum[h] != sum[h];
+#pragma unroll
+            for (int b = 0; b < DB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    nan |= o[b][i][2 * h] != o[b][i][2 * h] ||
+                           o[b][i][2 * h + 1] != o[b][i][2 * h + 1];
+        }
+        nan = __syncthreads_or(nan);
+        again = nan && !again;
+        if (again) continue;
         // ---- join the WK key groups: weights from the maxima, then the sums in turn
 #pragma unroll
         for (int h = 0; h < 2; h++) {

@@ -380,9 +380,10 @@ typedef struct {
 } cw_tree_attn_args;
 /* out = softmax(cap(scale * q . k) over the keys a row sees) v.  A row sees every
  * cached token of its request and the nodes of its mask; with a window only keys
- * whose position is less than `window` before its own.  A row that sees nothing
- * gives zeros; what a row does not see does not reach it, non-finite values
- * included.  mask_words is ceil(max_nodes / 32); a request has at most max_nodes
+ * whose position is less than `window` before its own.  A row that sees nothing,
+ * or whose scores are all -inf, gives zeros; what a row does not see does not reach
+ * it, non-finite values included.  A NaN score makes its row NaN, and a weight that
+ * rounds to 0 times an infinite value is NaN.  mask_words is ceil(max_nodes / 32); a request has at most max_nodes
  * (<= 1024) nodes.  Query head h reads kv head h / (n_heads / n_kv); head_dim <=
  * 256.  Rows of out past starts[n_req] keep their contents.  q, cache and out are
  * of one type; sums and the softmax are f32.  16-bit types with head_dim,

@@ -241,3 +241,34 @@ def test_many_tiles_of_values_that_are_not_finite(ctx, heads, kv, dim):
         got = tree_run(ctx, c, "f32", heads, kv, dim, 16)
         assert np.abs(got - want).max() <= tree_tolerance("f32", s, v)
     ctx.sync()
+
+
+@pytest.mark.parametrize("kind", [k for k in KINDS if k[0] == "f32"], ids=lambda k: "-".join(map(str, k)))
+@pytest.mark.parametrize("lens", [[400, 3], [9000, 3]], ids=["whole", "cut"])
+def test_f32_scores_of_minus_infinity(ctx, kind, lens):
+    test_scores_of_minus_infinity(ctx, kind, lens)
+
+
+@kinds
+def test_values_of_infinity_in_the_prefix(ctx, kind):
+    """An infinite value that every row sees comes out infinite in its dim, and a score of
+    +inf makes its row NaN; other dims and rows stay."""
+    dtype, H, K, D, page, n = kind
+    c = tree_case(np.random.default_rng(23), [700], [n], dtype, H, K, D, page, poison=False)
+    c["vc"][c["table"][0, 100 // page], :, 100 % page, 4] = np.inf
+    c["vc"][c["table"][0, 130 // page], :, 130 % page, 7] = -np.inf
+    got = tree_run(ctx, c, dtype, H, K, D, page, scale=0.01)
+    want, s, v = attend(c, page, scale=0.01)
+    assert (got[:, :, 4] == np.inf).all() and (got[:, :, 7] == -np.inf).all()
+    rest = np.ones(D, bool)
+    rest[[4, 7]] = False
+    assert np.abs(got[:, :, rest] - want[:, :, rest]).max() <= tree_tolerance(dtype, s, v)
+    c["kc"][c["table"][0, 300 // page], :, 300 % page, 2] = np.inf
+    c["q"][:, :, 2] = -1.0
+    c["q"][0, :, 2] = 1.0    # +inf for row 0, -inf for the others
+    got = tree_run(ctx, c, dtype, H, K, D, page, scale=0.01)
+    want, s, v = attend(c, page, scale=0.01)
+    assert np.isnan(got[0]).all()
+    assert (got[1:, :, 4] == np.inf).all() and (got[1:, :, 7] == -np.inf).all()
+    assert np.abs(got[1:, :, rest] - want[1:, :, rest]).max() <= tree_tolerance(dtype, s, v)
+    ctx.sync()
