@@ -35,6 +35,7 @@ namespace cw {
 
 constexpr int TR_THREADS = 256;
 constexpr int TR_ROWS = 2;  // tiles whose row offsets are kept
+constexpr int TR_HAVE = 8;  // tiles whose sets of keys with a page are kept (the ring's 4 and more)
 constexpr size_t TR_SMEM_CAP = 226 * 1024 + 384;  // dynamic; the kernel also has static
 
 __device__ __forceinline__ void tr_cp16(void* dst, const void* src, bool live) {
@@ -120,6 +121,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
     uint64_t* s_sees = (uint64_t*)(sq + BM * DP);
     long long* s_row = (long long*)(s_sees + BM);  // [TR_ROWS][64] offset of a key row, or -1
     float2* s_ml = (float2*)(s_row + TR_ROWS * TR_TILE); // [WK][BM]
+    __shared__ uint64_t s_have[TR_HAVE];  // [tile % TR_HAVE] keys whose page is in the cache
     __shared__ int s_edge;
     __shared__ TreeShared s_run;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -177,10 +179,12 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
                 const int id = a.table[(size_t)it.r * a.max_pages + pi];
                 if (id >= 0 && id < a.n_pages)
                     at = (((long long)id * a.K + it.head) * a.page + (j - pi * a.page)) * a.D;
-                else
+                else if (j >= tree_first(a, it.q))
                     tree_bad(a);
             }
             s_row[(tile & 1) * TR_TILE + tid] = at;
+            const uint32_t have = __ballot_sync(FULL, at >= 0);
+            if (lane == 0) ((uint32_t*)&s_have[tile & (TR_HAVE - 1)])[warp] = have;
         };
         auto load = [&](int s) {
             if (s < steps) {
@@ -242,6 +246,10 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[b][i][e] = 0.f;
+        // this warp's keys of a tile's set, the first in bit 0
+        auto own_bits = [&](const uint64_t* set) {
+            return ((const uint32_t*)set)[wk * KW >> 5] >> (wk * KW & 31);
+        };
         const float c2 = a.softcap > 0.f ? 1.44269504088896341f : a.scale * 1.44269504088896341f;
         float p[NB][4];
         for (int s = 0; s < steps; s++) {
@@ -317,8 +325,8 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
                 }
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const uint64_t sees =
-                        part ? s_sees[wm * 16 + g + 8 * h] >> (wk * KW) : ~0ull;
+                    uint32_t sees = own_bits(&s_have[(s >> 1) & (TR_HAVE - 1)]);
+                    if (part) sees &= own_bits(&s_sees[wm * 16 + g + 8 * h]);
                     float top = mx[h];
 #pragma unroll
                     for (int n = 0; n < NB; n++)
@@ -361,11 +369,11 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
                 // would reach rows that do not see the key, so a tile that rows see
                 // differently is looked over first (keys past the end were zero-filled).
                 bool odd = false;
-                uint64_t see0 = 0, see1 = 0;
+                uint32_t see0 = 0, see1 = 0;
                 if (part) {
                     // read before the vote: after it the next tile's sets may be written
-                    see0 = s_sees[wm * 16 + g] >> (wk * KW);
-                    see1 = s_sees[wm * 16 + g + 8] >> (wk * KW);
+                    see0 = own_bits(&s_sees[wm * 16 + g]);
+                    see1 = own_bits(&s_sees[wm * 16 + g + 8]);
                     for (int i = tid; i < TR_TILE * DP; i += TR_THREADS)
                         odd |= !(fabsf(tile[i]) <= 3.402823466e38f);
                     odd = __syncthreads_or(odd);

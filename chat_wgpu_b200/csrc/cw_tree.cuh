@@ -57,6 +57,10 @@ __device__ __forceinline__ void tree_bad(const TreeArgs& a) {
     atomicCAS(a.status, DEV_OK, DEV_BAD_INPUT);
 }
 
+// First key that some row may see; pages before it need not be there.
+__device__ __forceinline__ int tree_first(const TreeArgs& a, const TreeReq& q) {
+    return a.window > 0 ? max(0, q.len - a.window + 1) : 0;
+}
 // Request r, every length clamped to the buffers; `report` notes a clamp.
 __device__ __forceinline__ TreeReq tree_req(const TreeArgs& a, int r, bool report) {
     TreeReq q;
@@ -69,11 +73,14 @@ __device__ __forceinline__ TreeReq tree_req(const TreeArgs& a, int r, bool repor
     if (report && (s0 != q.row0 || s1 - s0 != q.n || l != q.len || q.keys != q.len + q.n))
         tree_bad(a);
     // a node's position is at least len: nothing before len - window + 1 is seen
-    const int j0 = a.window > 0 ? max(0, q.len - a.window + 1) : 0;
-    q.tile0 = min(j0, max(q.keys - 1, 0)) / TR_TILE;
+    q.tile0 = min(tree_first(a, q), max(q.keys - 1, 0)) / TR_TILE;
     q.tiles = q.n > 0 ? (q.keys + TR_TILE - 1) / TR_TILE - q.tile0 : 0;
     q.blocks = (q.n * a.G + a.bm - 1) / a.bm;
     return q;
+}
+// Whether the page of the request's key j is in the cache.
+__device__ __forceinline__ bool tree_has(const TreeArgs& a, int r, int j) {
+    return (uint32_t)a.table[(size_t)r * a.max_pages + j / a.page] < (uint32_t)a.n_pages;
 }
 // Units of the request: its items' tiles, and `pad` more for each item's start and end.
 __device__ __forceinline__ long long tree_units(const TreeArgs& a, const TreeReq& q) {

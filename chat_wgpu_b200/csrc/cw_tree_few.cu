@@ -52,6 +52,7 @@ template <int N> struct TfBars {
     uint64_t q_full[2], q_empty[2];                      // [item % QB]
     uint64_t s_full[2], p_full[2], pv[2], done;          // [tile % 2]
     uint32_t tmem, failed, keep;
+    uint32_t lost;  // some key has no page
     TreeShared run;
     uint64_t sees[2][N];  // [64 keys][row]
     // what is added to a row's scores: -reference, TF_NONE while it has seen nothing above
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(320, 1)
             mbar_init(&bars->p_full[i], 8);
             mbar_init(&bars->pv[i], 1);
         }
-        bars->failed = 0;
+        bars->failed = bars->lost = 0;
         fence_mbar_init();
     }
     pdl_wait();  // the setup above overlaps the launch before
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(320, 1)
     // scores of tile t + 1 are formed before the values of tile t, so the ring holds
     // K0, then K(t+1), V(t) in turn.
     if (warp == 8) {  // ---- TMA
-        TtFeed<COLS, SK> feed(a, ring, bars->full, bars->empty, stages, tile);
+        TtFeed<COLS, SK> feed(a, ring, bars->full, bars->empty, &bars->lost, stages, tile);
         if (lane == 0) {
             tma_prefetch_desc(&map_k);
             tma_prefetch_desc(&map_v);
@@ -332,6 +333,8 @@ __global__ void __launch_bounds__(320, 1)
                 wait(&bars->s_full[n & 1], n >> 1);
                 __syncwarp();
                 tc_fence_after();
+                // set before the tile's keys were, if one of them has no page
+                const bool lost = *(volatile uint32_t*)&bars->lost;
                 float s[C];
                 // pass 1: the weights' exponents; were some to pass 8 (0, and at once at
                 // an item's first tile): new references; 2: the exponents again
@@ -352,6 +355,10 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
                         for (int c = 0; c < C; c++)
                             if (!(sees[c] >> (m & 63) & 1)) s[c] = -INFINITY;
+                    }
+                    if (lost && kt + m < end && !tree_has(a, it.r, kt + m)) {
+#pragma unroll
+                        for (int c = 0; c < C; c++) s[c] = -INFINITY;
                     }
                     if (pass == 0) {
                         // maxima over the 128 keys: in fix, as ordered whole numbers

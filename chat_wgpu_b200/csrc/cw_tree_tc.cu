@@ -43,7 +43,7 @@ namespace cw {
 struct TtBars {
     uint64_t full[TT_STAGES], empty[TT_STAGES];
     uint64_t q_full[2], s_full[2][2], p_full[2][2], pv[2][2], done;  // [row block][tile % 2]
-    uint32_t tmem, failed;
+    uint32_t tmem, failed, lost;  // lost: some key has no page
     TreeShared run;
 };
 
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
             }
         }
         mbar_init(&bars->done, 1);
-        bars->failed = 0;
+        bars->failed = bars->lost = 0;
         fence_mbar_init();
     }
     pdl_wait();  // the setup above overlaps the launch before
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
     TtPlace at = {0, 0};
 
     if (warp == NB * 4) {  // ---- TMA: all lanes, a box each
-        TtFeed<COLS, TILE> feed(a, ring, bars->full, bars->empty, stages, tile);
+        TtFeed<COLS, TILE> feed(a, ring, bars->full, bars->empty, &bars->lost, stages, tile);
         if (lane == 0) {
             tma_prefetch_desc(&map_k);
             tma_prefetch_desc(&map_v);
@@ -303,10 +303,11 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
                 uint64_t sees = ~0ull;  // this row's, of the tile's keys
                 if (mixed && (kt < edge || kt + TILE > it.q.len || kt + TILE > end))
                     sees = r < rows ? tree_sees(a, it.q, m0 + r, kt) : 0;
-                const uint64_t mine = sees >> (part * KEYS);
                 wait(&bars->s_full[b][n & 1], n >> 1);
                 __syncwarp();
                 tc_fence_after();
+                // set before the tile's keys were, if one of them has no page
+                const bool lost = *(volatile uint32_t*)&bars->lost;
                 const uint32_t t_s = lanes + (n & 1) * TILE;
                 if (work) {
                     float s[KEYS];
@@ -315,7 +316,13 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
 #pragma unroll
                         for (int j = 0; j < KEYS; j++) s[j] = capped(s[j]);
                     }
-                    if (mixed) {
+                    if (mixed || lost) {
+                        uint64_t mine = sees >> (part * KEYS);
+                        if (lost)
+#pragma unroll 1
+                            for (int j = 0; j < KEYS && kt + part * KEYS + j < end; j++)
+                                if (!tree_has(a, it.r, kt + part * KEYS + j))
+                                    mine &= ~(1ull << j);
 #pragma unroll
                         for (int j = 0; j < KEYS; j++)
                             if (!(mine >> j & 1)) s[j] = -INFINITY;

@@ -237,6 +237,7 @@ template <int COLS, int SK> struct TtFeed {
     const TreeArgs& a;
     uint8_t* ring;
     uint64_t *full, *empty;
+    uint32_t* lost;
     const int stages, lane;
     TtPlace at = {0, 0};
     bool filled = false;  // every stage has been filled once
@@ -247,10 +248,11 @@ template <int COLS, int SK> struct TtFeed {
     // the item: its pages from page0's first key on, 32 ids to a read and a read ahead
     const int* ids;
     int in0, last, pages, head, have, now_ids, next_ids;
+    int first;            // key of the item, counted like `last`, that rows may see first
 
     __device__ TtFeed(const TreeArgs& a_, uint8_t* ring_, uint64_t* full_, uint64_t* empty_,
-                      int stages_, const TtTile& t)
-        : a(a_), ring(ring_), full(full_), empty(empty_), stages(stages_),
+                      uint32_t* lost_, int stages_, const TtTile& t)
+        : a(a_), ring(ring_), full(full_), empty(empty_), lost(lost_), stages(stages_),
           lane(threadIdx.x & 31) {
         const bool wide = tt_wide(a.D);
         box = min(a.page, 64);
@@ -267,6 +269,7 @@ template <int COLS, int SK> struct TtFeed {
         const int key0 = (it.q.tile0 + it.tile) * TR_TILE, page0 = key0 / a.page;
         in0 = key0 - page0 * a.page;
         last = min(it.q.keys - key0, it.tiles * TR_TILE);  // keys of this piece
+        first = tree_first(a, it.q) - key0;
         pages = (in0 + last + a.page - 1) / a.page;
         ids = a.table + (size_t)it.r * a.max_pages + page0;
         head = it.head;
@@ -274,7 +277,8 @@ template <int COLS, int SK> struct TtFeed {
         now_ids = read(0);
         next_ids = read(32);
     }
-    // The lane's copy of the item's keys [j * SK, ..+SK) as the cache's 8-row group, or -1.
+    // The lane's copy of the item's keys [j * SK, ..+SK) as the cache's 8-row group; -1:
+    // none, -2: keys without a page, -3: and a row may see some of them.
     __device__ int place(int j) {
         const int off = in0 + j * SK + pi * box;
         const int p = shift >= 0 ? off >> shift : off / a.page;
@@ -287,19 +291,28 @@ template <int COLS, int SK> struct TtFeed {
         const int y = __shfl_sync(FULL, next_ids, p & 31);
         if (lane >= boxes || j * SK + pi * box >= last) return -1;
         const int id = p - have < 32 ? x : y;
-        if (id < 0 || id >= a.n_pages) {
-            tree_bad(a);
-            return -1;
-        }
+        if (id < 0 || id >= a.n_pages) return j * SK + (pi + 1) * box > first ? -3 : -2;
         return ((id * a.K + head) * a.page + (off - p * a.page)) >> 3;
+    }
+    // Keys without a page: zeros in place of an old tile.
+    static __device__ __noinline__ void lack(uint8_t* to, uint32_t bytes, uint32_t* lost,
+                                             int* status) {
+        for (uint32_t i = 0; i < bytes; i += 16) *(uint4*)(to + i) = make_uint4(0, 0, 0, 0);
+        tt_fence_async();
+        if (!lost) return;
+        *(volatile uint32_t*)lost = 1;  // the weight warps look at ids from here on
+        atomicCAS(status, DEV_OK, DEV_BAD_INPUT);
     }
     // Into the next stage once it is free; all(bar, parity) waits, the warp together.
     template <typename All> __device__ bool load(const CUtensorMap* map, int group, All all) {
         const int s = at.stage;
         if (filled && !all(&empty[s], at.phase ^ 1)) return false;
         const uint32_t live = __popc(__ballot_sync(FULL, group >= 0));
-        if (lane == 0) mbar_expect_tx(&full[s], live * box_bytes);
+        if (group < -1)  // rare, and a call: code in its place made this loop 34 ns a stage slower
+            lack(ring + s * STAGE + dst, box_bytes, group == -3 ? lost : nullptr, a.status);
         __syncwarp();
+        // copies may count before these bytes are announced: the phase lacks lane 0's arrival
+        if (lane == 0) mbar_expect_tx(&full[s], live * box_bytes);
         if (group >= 0) tt_copy(ring + s * STAGE + dst, map, col * 64, group, &full[s]);
         at.next(stages);
         filled |= at.stage == 0;

@@ -383,9 +383,11 @@ typedef struct {
  * whose position is less than `window` before its own.  A row that sees nothing,
  * or whose scores are all -inf, gives zeros; what a row does not see does not reach
  * it, non-finite values included.  A NaN score makes its row NaN, and a weight that
- * rounds to 0 times an infinite value is NaN.  mask_words is ceil(max_nodes / 32); a request has at most max_nodes
- * (<= 1024) nodes.  Query head h reads kv head h / (n_heads / n_kv); head_dim <=
- * 256.  Rows of out past starts[n_req] keep their contents.  q, cache and out are
+ * rounds to 0 times an infinite value is NaN.  Keys whose page id is outside the cache
+ * are not seen and are reported; pages that end before the window of a row at position
+ * lens are not asked for.  mask_words is ceil(max_nodes / 32); a request has at most
+ * max_nodes (<= 1024) nodes.  Query head h reads kv head h / (n_heads / n_kv); head_dim
+ * <= 256.  Rows of out past starts[n_req] keep their contents.  q, cache and out are
  * of one type; sums and the softmax are f32.  16-bit types with head_dim,
  * q_off and q_stride multiples of 8 and page_size 8, 16, 32 or a multiple of 64
  * run on the tcgen05 tensor cores (there the softmax weights are rounded to the

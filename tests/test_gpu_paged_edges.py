@@ -272,3 +272,82 @@ def test_values_of_infinity_in_the_prefix(ctx, kind):
     assert (got[1:, :, 4] == np.inf).all() and (got[1:, :, 7] == -np.inf).all()
     assert np.abs(got[1:, :, rest] - want[1:, :, rest]).max() <= tree_tolerance(dtype, s, v)
     ctx.sync()
+
+
+# ---------------------------------------------------------------- pages that are missing
+def tree_reported(ctx, c, dtype, *shape, **opt):
+    """tree_run of a call that reports its input: the rows, and the report."""
+    from chat_wgpu_b200 import CwError
+    seen, read = [], ref.read
+
+    def after(ctx_, buf, dtype_, size):
+        with pytest.raises(CwError) as e:
+            ctx_.sync()
+        seen.append(e.value.status)
+        return read(ctx_, buf, dtype_, size)
+
+    ref.read = after
+    try:
+        return tree_run(ctx, c, dtype, *shape, **opt), seen[0]
+    finally:
+        ref.read = read
+
+
+@kinds
+@pytest.mark.parametrize("ctx_len", [330, 9000])
+def test_unusable_pages(ctx, kind, ctx_len):
+    """Keys of a page id outside the cache weigh nothing and are reported; other requests'
+    rows are as ever."""
+    dtype, H, K, D, page, n = kind
+    c = tree_case(np.random.default_rng(31), [ctx_len, 50, 300], [n, 2, n], dtype, H, K, D, page, poison=False)
+    good, s0, v0 = attend(c, page)
+    gone = [np.zeros(ctx_len + n, bool), np.zeros(52, bool), np.zeros(300 + n, bool)]
+    lost = [(0, 3, -1), (0, 4, c["n_pages"]), (2, 0, 2 ** 31 - 1), (2, 300 // page, -7)]
+    sent = dict(c, table=c["table"].copy())
+    for r, p, bad in lost:
+        sent["table"][r, p] = bad
+        gone[r][p * page:(p + 1) * page] = True
+    got, status = tree_reported(ctx, sent, dtype, H, K, D, page)
+    assert status == 1
+    ctx.sync()
+    want, s, v = attend(c, page, gone=gone)
+    tol = tree_tolerance(dtype, max(s, s0), max(v, v0))
+    assert np.abs(got - want).max() <= tol
+    assert np.abs(got - good)[n:n + 2].max() <= tol
+
+
+@pytest.mark.parametrize("case", [("f32", 8, 2, 64, 8, 70), ("bf16", 8, 2, 64, 8, 70), ("f16", 8, 1, 128, 128, 40),
+                                  ("bf16", 8, 4, 256, 32, 100), ("bf16", 4, 2, 72, 16, 9)],
+                         ids=lambda c: "-".join(map(str, c)))
+def test_one_page_in_three(ctx, case):
+    """Many missing pages over many tiles, some tiles without any page; no key at all."""
+    dtype, H, K, D, page, n = case
+    rng = np.random.default_rng(33)
+    c = tree_case(rng, [3000, 1500, 70], [n, 1, 2], dtype, H, K, D, page)
+    gone, sent = [], dict(c, table=c["table"].copy())
+    for r in range(3):
+        lost = rng.random(c["max_pages"]) < (1.0 if r == 2 else 0.33)
+        lost[512 // page:1024 // page] |= r == 0
+        sent["table"][r, lost] = -1
+        gone.append(np.repeat(lost, page)[:c["lens"][r] + c["starts"][r + 1] - c["starts"][r]])
+    got, status = tree_reported(ctx, sent, dtype, H, K, D, page, softcap=9.0)
+    assert status == 1
+    want, s, v = attend(c, page, gone=gone, softcap=9.0)
+    assert (got[-2:] == 0).all()
+    assert np.abs(got - want).max() <= tree_tolerance(dtype, s, v)
+
+
+@kinds
+def test_pages_given_up_before_the_window(ctx, kind):
+    """Pages whose keys no row can see need not be there, nor are they reported, where the
+    window's edge lies inside a tile."""
+    dtype, H, K, D, page, n = kind
+    window = 64 + page + 3
+    lens = 1024 + 2 * page + 5 + window  # the first key that a row sees: 1024 + 2 * page + 6
+    c = tree_case(np.random.default_rng(32), [lens], [n], dtype, H, K, D, page, poison=False)
+    want, s, v = attend(c, page, window=window)
+    sent = dict(c, table=c["table"].copy())
+    sent["table"][0, :(lens - window + 1) // page] = -1
+    got = tree_run(ctx, sent, dtype, H, K, D, page, window=window)
+    ctx.sync()
+    assert np.abs(got - want).max() <= tree_tolerance(dtype, s, v)
