@@ -18,9 +18,9 @@
 // 64 dims at 3001 200 us for 149, five of 256 dims with a window 24 us for 11.
 //
 // No maximum over keys is formed per tile: each row has a reference in shared memory,
-// and only when some weight would pass 2^8 (always at a row's first tile) the maxima
-// over the 128 lanes are reduced, references raised and O^T rescaled.  Weights stay
-// below 256; the division by their sum makes the reference drop out.  A thread sums
+// and only when some weight would pass 2^8 (2^15 in f16; always at a row's first tile)
+// the maxima over the 128 lanes are reduced, references raised and O^T rescaled.  The
+// division by the weights' sum makes the reference drop out.  A thread sums
 // its own key's rounded weights, over lanes once at the item's end.
 //
 // Scores have two TMEM buffers and weights two in shared memory, so the products of
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(320, 1)
                 // set before the tile's keys were, if one of them has no page
                 const bool lost = *(volatile uint32_t*)&bars->lost;
                 float s[C];
-                // pass 1: the weights' exponents; were some to pass 8 (0, and at once at
+                // pass 1: the weights' exponents; were some to pass 8 (f16: 15; then 0, and at once at
                 // an item's first tile): new references; 2: the exponents again
 #pragma unroll 1
                 for (int pass = i == 0 ? 0 : 1;;) {
@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(320, 1)
                         (void)tf_any(false, id);
                         if (m < C) {
                             const float was = -neg[m];
-                            const float now = fmaxf(tf_float(__float_as_int(fix[m])), was);
+                            const float now =
+                                fmaxf(tf_float(__float_as_int(fix[m])) - TT_LIFT<BF>, was);
                             fix[m] = tt_exp2(was - now);
                             if (c0 + m < rows) neg[m] = -now;
                         }
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(320, 1)
                         s[c + 3] = fmaf(s[c + 3], c2, f.w);
                         most = fmaxf(most, fmaxf(fmaxf(s[c], s[c + 1]), fmaxf(s[c + 2], s[c + 3])));
                     }
-                    if (pass == 2 || !tf_any(most > 8.f, id)) break;
+                    if (pass == 2 || !tf_any(most > 8.f + TT_LIFT<BF>, id)) break;
                     pass = 0;
                 }
                 // The product that read this weight buffer: with two, that of tile n - 2,

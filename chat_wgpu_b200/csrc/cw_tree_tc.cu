@@ -20,8 +20,8 @@
 // Warps: 4 (or 2 x 4) softmax warps, a thread per row, so row maxima and sums need
 // no exchange; one TMA warp; one elected MMA lane.  S has two TMEM buffers: the scores of
 // tile i + 1 are formed while the weights of tile i are.  O is rescaled only when a
-// row's maximum has grown by 2^8 since its last reference (weights then stay below
-// 256, far inside both types); the final division makes the reference drop out.
+// row's maximum has grown by 2^8 since its last reference (weights then stay below 2^8,
+// in f16 2^15, inside both types); the final division makes the reference drop out.
 // Weights are rounded to the cache's type for the second product; the row's sum is
 // taken over the rounded weights, so a constant v comes out exact.
 //
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
                         t3 = fmaxf(t3, s[j + 3]);
                     }
                     top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
-                    const float want = top == -INFINITY ? -INFINITY : top * c2;
+                    const float want = top == -INFINITY ? -INFINITY : top * c2 - TT_LIFT<BF>;
                     if (i == 0) {
                         ref = want;
                     } else if (__any_sync(FULL, r < rows && want - ref > 8.f)) {

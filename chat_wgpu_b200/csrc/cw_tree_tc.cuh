@@ -13,6 +13,11 @@ namespace cw {
 
 constexpr int TT_STAGES = 16;  // most stages of the ring (one K or V tile each)
 constexpr uint64_t TT_WAIT_NS = 2000000000ull;
+// Weights are powers of two over a reference, rounded to the cache's type.  In f16 the
+// reference is 2^7 below the scores it was taken from: the largest weight is then 2^7 to
+// 2^15 and those down to 2^-31 of it are kept (2^-24 before; 30000 keys e^-17.5 of one
+// other lost their joint share, 7.5e-4 of the result).
+template <bool BF> constexpr float TT_LIFT = BF ? 0.f : 7.f;
 
 __device__ __forceinline__ void tt_ld32(uint32_t addr, uint32_t* r) {
     asm volatile(

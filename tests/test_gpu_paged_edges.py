@@ -351,3 +351,30 @@ def test_pages_given_up_before_the_window(ctx, kind):
     got = tree_run(ctx, sent, dtype, H, K, D, page, window=window)
     ctx.sync()
     assert np.abs(got - want).max() <= tree_tolerance(dtype, s, v)
+
+
+# ---------------------------------------------------------------- weights in 16 bits
+@pytest.mark.parametrize("kind", [k for k in KINDS if k[0] == "f16"], ids=lambda k: "-".join(map(str, k)))
+def test_a_dominating_key(ctx, kind):
+    """A first key e^17.5 above the other 30000, whose joint share is 7.5e-4: the value is 0
+    at that key and 1 elsewhere, so the share is the result.  All requests' tables name the
+    same three pages; there are enough requests that items are whole."""
+    dtype, H, K, D, page, n = kind
+    lens, req = 30000, 160
+    pages = -(-(lens + n) // page)
+    kc, vc = np.zeros((3, K, page, D)), np.ones((3, K, page, D))
+    kc[1, :, 0, 0], vc[1, :, 0] = 17.5, 0.0
+    table = np.zeros((req, pages), np.int32)
+    table[:, 0] = 1
+    q = np.zeros((req * n, H, D))
+    q[:, :, 0] = 1.0
+    c = dict(lens=np.full(req, lens), starts=np.arange(req + 1) * n, T=req * n, N=n, table=table, kc=kc, vc=vc,
+             pos=np.zeros(req * n, np.int32), q=q, max_pages=pages, n_pages=3)
+    got = tree_run(ctx, c, dtype, H, K, D, page, scale=1.0, mask=False)
+    share = (lens + np.arange(n)) * np.exp(-17.5)  # node i sees nodes 0..i; one of the prefix is the large one
+    want = np.tile(share / (1 + share), req)[:, None, None]
+    # the largest weight is 2^7 at least, so f16's fixed step of 2^-24 below 2^-14 moves a
+    # weight by at most 2^-25 / 2^7 of it; the sum takes the same rounded weights.  Then
+    # f32 arithmetic and one rounding of the result.
+    assert np.abs(got - want).max() <= (lens + n) * 2.0 ** -32 + (ref.UNIT["f16"] + 1e-5) * want.max()
+    ctx.sync()
