@@ -122,11 +122,13 @@ __global__ void __launch_bounds__(PP_THREADS) k_page_plan(PagePlanArgs a) {
         }
     }
     const int step = gridDim.x * PP_THREADS, g0 = blockIdx.x * PP_THREADS + tid;
-    // fresh pages into the table
-    for (int u = g0; u < min(pages, a.n_free); u += step) {
+    // fresh pages into the table, -1 for those that lack: what an earlier step left there
+    // may be another request's page by now
+    for (int u = g0; u < pages; u += step) {
         const int r = pp_find(s_first, R, u);  // the last request starting at or before u
         const int have = pp_pages(a, s_len[r]);
-        a.table[(size_t)r * a.max_pages + have + (u - s_first[r])] = a.free_pages[u];
+        a.table[(size_t)r * a.max_pages + have + (u - s_first[r])] =
+            u < a.n_free ? a.free_pages[u] : -1;
     }
     // token rows, four to a thread (16-byte stores)
     const int groups = (a.max_tokens + 3) / 4;

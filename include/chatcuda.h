@@ -316,10 +316,10 @@ typedef struct {
 } cw_page_plan_args;
 /* Block tables and slots of one step from the request lengths, on the device.
  * Request r needs pages ceil(lens/page_size) .. ceil((lens+news)/page_size);
- * these are given out in request order and written to its table row.  Rows past
- * the last token get position 0, slot -1, owner -1.  A token without a page
- * (the free list ran out, the table row is full, the table holds a negative id)
- * gets slot -1 and is no error: compare used with n_free.  n_req <= 16384. */
+ * these are given out in request order and written to its table row, -1 for those
+ * that the free list lacks.  Rows past the last token get position 0, slot -1, owner
+ * -1.  A token without a page (the free list ran out, the table row is full, the
+ * table holds a negative id) gets slot -1 and is no error: compare used with n_free.  n_req <= 16384. */
 int cw_page_plan(cw_ctx* ctx, const cw_page_plan_args* args);
 
 /* Rotary frequencies of rot_dim / 2 pairs with base theta, stretched for

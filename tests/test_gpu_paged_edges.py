@@ -114,6 +114,26 @@ with GpuContext(0) as c:
     assert r.returncode == 0, r.stderr[-2000:]
 
 
+@pytest.mark.parametrize("page", [4, 5])
+def test_plan_marks_pages_that_lack(ctx, page):
+    """Where the free list runs out, ids that an earlier step left in the table do not stay
+    as if they were the request's: they become -1."""
+    from chat_wgpu_b200.kernels.pages import PagePlan
+    table = i32(ctx, [[7, 1, 2, 3], [4, 5, 6, 8], [9, 9, 9, 9]])
+    out = {k: i32(ctx, np.full(s, -77)) for k, s in dict(starts=4, positions=20, slots=20, owners=20, used=1).items()}
+    call = PagePlan(ctx, lens=i32(ctx, [3, 0, 1]), news=i32(ctx, [page, 2 * page + 1, 2]),
+                    free_pages=i32(ctx, [11, 12]), table=table, n_req=3, page_size=page, max_pages=4, n_free=2,
+                    max_tokens=20, **out)
+    for _ in range(2):
+        call()
+        assert int(get(ctx, out["used"], 1)[0]) == 4
+        assert get(ctx, table, 12).reshape(3, 4).tolist() == [[7, 11, 2, 3], [12, -1, -1, 8], [9, 9, 9, 9]]
+        slots = get(ctx, out["slots"], 20)
+        assert (slots[page:2 * page] == 12 * page + np.arange(page)).all()
+        assert (slots[2 * page:3 * page + 1] == -1).all()
+        assert (slots[3 * page + 1:3 * page + 3] == 9 * page + 1 + np.arange(2)).all()
+
+
 # ---------------------------------------------------------------- captured steps
 def test_captured_step_outlives_larger_calls():
     """Plan, rotary and attention captured in a graph keep their results when the context
