@@ -167,7 +167,9 @@ __global__ void __launch_bounds__(PP_THREADS) k_page_plan(PagePlanArgs a) {
             }
             pos[i] = a.depths ? c + a.depths[t] : (int)at;
             own[i] = r;
-            if (page_id >= 0) slot[i] = page_id * a.page + ((int)at - ap * a.page);
+            if (page_id >= 0)  // past 31 bits: a slot that no cache has
+                slot[i] = (int)min((long long)page_id * a.page + ((int)at - ap * a.page),
+                                   (long long)INT_MAX);
         }
         if (t0 + 4 <= a.max_tokens) {
             ((int4*)a.positions)[g] = make_int4(pos[0], pos[1], pos[2], pos[3]);

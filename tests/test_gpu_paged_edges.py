@@ -134,6 +134,20 @@ def test_plan_marks_pages_that_lack(ctx, page):
         assert (slots[3 * page + 1:3 * page + 3] == 9 * page + 1 + np.arange(2)).all()
 
 
+@pytest.mark.parametrize("page", [4, 5])
+def test_slots_past_31_bits(ctx, page):
+    """A page id whose slots do not fit gets a slot that no cache has, so that the rows are
+    reported where they are written, not stored elsewhere."""
+    from chat_wgpu_b200.kernels.pages import PagePlan
+    big = 2 ** 32 // page // 4 + 1  # times page: past 31 bits, and a small number in 32
+    ids = [2 ** 30, 2 ** 31 - 1, big, 2 ** 31 // page]
+    out = {k: i32(ctx, np.full(s, -77)) for k, s in dict(starts=5, positions=8, slots=8, owners=8, used=1).items()}
+    PagePlan(ctx, lens=i32(ctx, [1, 1, 1, 1]), news=i32(ctx, [2, 2, 2, 2]), free_pages=None,
+             table=i32(ctx, ids), n_req=4, page_size=page, max_pages=1, n_free=0, max_tokens=8, **out)()
+    want = [min(p * page + 1 + j, 2 ** 31 - 1) for p in ids for j in range(2)]
+    assert get(ctx, out["slots"], 8).tolist() == want
+
+
 # ---------------------------------------------------------------- captured steps
 def test_captured_step_outlives_larger_calls():
     """Plan, rotary and attention captured in a graph keep their results when the context
