@@ -14,15 +14,43 @@ def op(ctx, fn: str, *args) -> Buffer:
 TYPES = {"f32": 0, "f16": 1, "bf16": 30}
 
 
+DTYPES = {"f32": ("float32",), "f16": ("float16",), "bf16": ("bfloat16",)}
+
+
+def check_tensor(name: str, t, types, row_stride: int | None) -> None:
+    """ValueError unless the wrapped tensor's type is one of `types` and it is contiguous,
+    or, where rows may be apart, has contiguous rows `row_stride` elements apart."""
+    have = str(getattr(t, "dtype", types[0])).rsplit(".", 1)[-1]
+    if have not in types:
+        raise ValueError(f"{name}: a tensor of {have}, not {' or '.join(types)}")
+    shape, strides = [int(d) for d in t.shape], [int(s) for s in t.stride()]
+
+    def dense(shape, strides):
+        step = 1
+        for d, s in zip(reversed(shape), reversed(strides)):
+            if d != 1 and s != step:
+                return False
+            step *= d
+        return True
+
+    if dense(shape, strides):
+        return
+    if row_stride is None or not dense(shape[1:], strides[1:]) or strides[0] != row_stride:
+        raise ValueError(f"{name}: strides {strides} of shape {shape}"
+                         + ("" if row_stride is None else f" with rows {row_stride} apart"))
+
+
 class Prepared:
     """A call whose argument struct is filled once and used every step: calling
     the object enqueues the operator on the context's stream.  It holds its
-    buffers; their contents are read when the operator runs."""
+    buffers; their contents are read when the operator runs.  A wrapped tensor
+    (GpuContext.wrap) must be of the operator's type and lie as it reads it."""
 
     _fn = ""
     _struct = None
+    _rows: dict = {}  # buffers of the call's dtype, and the field of their row stride (or None)
 
-    def __init__(self, ctx, **fields):
+    def __init__(self, ctx, dtype: str | None = None, **fields):
         self.ctx = ctx
         self.args = self._struct()
         self._keep = []
@@ -30,6 +58,9 @@ class Prepared:
             if value is None:
                 continue
             if isinstance(value, Buffer):
+                if value.owner is not None:
+                    want = DTYPES[dtype] if name in self._rows else ("int32", "uint32")
+                    check_tensor(name, value.owner, want, fields.get(self._rows.get(name)))
                 self._keep.append(value)
                 value = value.handle
             setattr(self.args, name, value)

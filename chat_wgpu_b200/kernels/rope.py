@@ -35,6 +35,7 @@ class RopeAppend(Prepared):
 
     _fn = "cw_rope_append"
     _struct = _lib.RopeAppendArgs
+    _rows = dict(q="q_stride", k="k_stride", v="v_stride", q_out=None, k_cache=None, v_cache=None)
 
     def __init__(self, ctx, plan: Buffer, positions: Buffer, dtype: str, n_tokens: int,
                  head_dim: int, layout: str = "half", n_heads: int = 0, n_kv: int = 0,
@@ -47,7 +48,7 @@ class RopeAppend(Prepared):
             raise ValueError(f"layout {layout!r}: one of {sorted(LAYOUTS)}")
         kv = n_kv * head_dim
         super().__init__(
-            ctx, plan=plan, positions=positions, q=q, k=k, v=v, slots=slots, q_out=q_out,
+            ctx, dtype, plan=plan, positions=positions, q=q, k=k, v=v, slots=slots, q_out=q_out,
             k_cache=k_cache, v_cache=v_cache, q_off=q_off, k_off=k_off, v_off=v_off,
             q_stride=q_stride or n_heads * head_dim, k_stride=k_stride or kv,
             v_stride=v_stride or kv, type=type_code(dtype), layout=LAYOUTS[layout],

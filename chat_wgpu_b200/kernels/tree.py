@@ -12,6 +12,7 @@ class TreeAttention(Prepared):
 
     _fn = "cw_tree_attention"
     _struct = _lib.TreeAttnArgs
+    _rows = dict(q="q_stride", k_cache=None, v_cache=None, out=None)
 
     def __init__(self, ctx, q: Buffer, k_cache: Buffer, v_cache: Buffer, table: Buffer,
                  lens: Buffer, starts: Buffer, out: Buffer, dtype: str, n_req: int, n_rows: int,
@@ -20,7 +21,7 @@ class TreeAttention(Prepared):
                  positions: Buffer | None = None, window: int = 0, softcap: float = 0.0,
                  scale: float = 0.0, q_off: int = 0, q_stride: int = 0):
         super().__init__(
-            ctx, q=q, k_cache=k_cache, v_cache=v_cache, table=table, lens=lens, starts=starts,
+            ctx, dtype, q=q, k_cache=k_cache, v_cache=v_cache, table=table, lens=lens, starts=starts,
             mask=mask, positions=positions, out=out, q_off=q_off,
             q_stride=q_stride or n_heads * head_dim, type=type_code(dtype), n_req=n_req,
             n_rows=n_rows, max_nodes=max_nodes, n_heads=n_heads, n_kv=n_kv, head_dim=head_dim,
