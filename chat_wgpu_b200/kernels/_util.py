@@ -1,4 +1,5 @@
 import ctypes as C
+from numbers import Integral
 
 from .. import _lib
 from ..context import Buffer
@@ -54,6 +55,7 @@ class Prepared:
         self.ctx = ctx
         self.args = self._struct()
         self._keep = []
+        types = dict(self._struct._fields_)
         for name, value in fields.items():
             if value is None:
                 continue
@@ -63,6 +65,11 @@ class Prepared:
                     check_tensor(name, value.owner, want, fields.get(self._rows.get(name)))
                 self._keep.append(value)
                 value = value.handle
+            kind = types[name]
+            if kind is not C.c_float:
+                if not (isinstance(value, Integral) and 0 <= value < 1 << 8 * C.sizeof(kind)):
+                    raise ValueError(f"{name}: {value!r} does not fit its field")
+                value = int(value)
             setattr(self.args, name, value)
         self._call = getattr(_lib.load(), self._fn)
         self._ref = C.byref(self.args)

@@ -61,3 +61,15 @@ def test_tensors_that_lie_otherwise_are_refused():
             tree_call(**{name: wrapped(t)})
     with pytest.raises(ValueError, match="k: strides"):
         rope_call(k_stride=64)
+
+
+def test_numbers_outside_their_fields_are_refused():
+    """A struct field keeps the low bits of a number that does not fit: a call of 2^32 + 5
+    rows would be one of 5."""
+    for bad in (dict(n_rows=2 ** 32 + 5), dict(n_req=-1), dict(window=-2 ** 32), dict(q_off=-8),
+                dict(q_off=2 ** 64), dict(max_pages=2.5)):
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            tree_call(**bad)
+    with pytest.raises(ValueError, match="n_tokens"):
+        rope_call(n_tokens=2 ** 32 + 6)
+    assert tree_call(window=2 ** 32 - 1).args.window == 2 ** 32 - 1  # fits: the library refuses it
