@@ -57,6 +57,8 @@ class TreeDecoder:
                  chunk: int = 64, draft=lookup_draft):
         if not prompts or any(len(p) == 0 for p in prompts):
             raise ValueError("every session needs a prompt")
+        if not 1 <= chunk <= 1024:
+            raise ValueError(f"chunk {chunk}: rows of a session in a step, 1..1024")
         self.m, self.ctx, self.page, self.chunk, self.draft = model, model.ctx, page_size, chunk, draft
         self.sessions = [Session(p) for p in prompts]
         self.max_seq = max_seq
