@@ -87,15 +87,6 @@ template <int DP> __device__ __forceinline__ int tr_at(int j, int c) {
     return j * DP + ((c & ~7) | ((c ^ j) & 7)) * 4;
 }
 
-// One score from f32 products.
-template <int DP> __device__ __noinline__ float tr_dot(const float* sq, const float* tile, int m, int j) {
-    float x = 0.f;
-#pragma unroll 1
-    for (int d = 0; d < DP; d++)
-        x = fmaf(sq[tr_at<DP>(m, d >> 2) + (d & 3)], tile[tr_at<DP>(j, d >> 2) + (d & 3)], x);
-    return x;
-}
-
 // Ring buffers (one K or V tile each) that fit beside the queries.
 template <int DP, int BM> constexpr int tr_ring() {
     const size_t left = TR_SMEM_CAP - (size_t)BM * DP * 4 - BM * 8 - TR_ROWS * TR_TILE * 8 - 1024;
@@ -108,6 +99,80 @@ template <int DP, int BM> constexpr size_t tr_smem() {
            + 128 * 8;                                                           // warp max, sum
 }
 
+// An item once more, from f32 products: what the pairs cannot say.  A part of a pair times
+// an infinity can be NaN where the whole product is not (0 or the other sign in its low
+// part), so an item whose sums are NaN ends here, whichever way they came about.  Leaves
+// the weighted values in key group 0 of `so` (zeros in the others) and each row's
+// reference and sum in s_sees.  All threads; out of line, its registers are its own.
+template <typename T, int DP, int BM>
+__device__ __noinline__ void tr_careful(const TreeArgs& a, TreeItem it, float* so, const float* sq,
+                                        uint64_t* s_sees) {
+    float* sx = so + 128 * DP;  // [BM][64] scores, then weights
+    float* s_fix = sx + BM * TR_TILE;
+    const int tid = threadIdx.x;
+    const float c2 = a.softcap > 0.f ? 1.44269504088896341f : a.scale * 1.44269504088896341f;
+    float top = -INFINITY, rf = -INFINITY, sum = 0.f;  // thread m: of row m, as in k_tree
+    for (int i = tid; i < 128 * DP; i += TR_THREADS) so[i] = 0.f;
+#pragma unroll 1
+    for (int t = 0; t < it.tiles; t++) {
+        const int kt = (it.q.tile0 + it.tile + t) * TR_TILE;
+        auto at = [&](int j) {  // a seen key's row in the cache
+            const int pi = (kt + j) / a.page;
+            return (((long long)a.table[(size_t)it.r * a.max_pages + pi] * a.K + it.head) * a.page +
+                    (kt + j - pi * a.page)) * a.D;
+        };
+        if (tid < it.rows) {
+            uint64_t see = tree_sees(a, it.q, it.block * BM + tid, kt);
+            for (uint64_t left = see; left; left &= left - 1) {
+                const int j = __ffsll((long long)left) - 1;
+                if (!tree_has(a, it.r, kt + j)) see &= ~(1ull << j);
+            }
+            s_sees[tid] = see;
+        }
+        __syncthreads();
+        for (int i = tid; i < it.rows * TR_TILE; i += TR_THREADS) {
+            const int m = i / TR_TILE, j = i % TR_TILE;
+            float x = -INFINITY;
+            if (s_sees[m] >> j & 1) {
+                const T* k = (const T*)a.k + at(j);
+                x = 0.f;
+                for (int d = 0; d < a.D; d++)
+                    x = fmaf(sq[tr_at<DP>(m, d >> 2) + (d & 3)], tree_f32<T>(k[d]), x);
+                if (a.softcap > 0.f) x = a.softcap * tanhf(x * a.scale / a.softcap);
+            }
+            sx[i] = x;
+        }
+        __syncthreads();
+        if (tid < it.rows) {
+            float* x = sx + tid * TR_TILE;
+            for (int j = 0; j < TR_TILE; j++) top = fmaxf(top, x[j]);
+            const float ref = top == -INFINITY ? 0.f : __fmul_rn(top, c2);
+            const float fix = rf == -INFINITY ? 0.f : exp2f(rf - ref);
+            sum *= fix;
+            for (int j = 0; j < TR_TILE; j++) {
+                x[j] = exp2f(fmaf(x[j], c2, -ref));
+                sum += x[j];
+            }
+            rf = top == -INFINITY ? -INFINITY : ref;
+            s_fix[tid] = fix;
+        }
+        __syncthreads();
+        for (int i = tid; i < it.rows * a.D; i += TR_THREADS) {
+            const int m = i / a.D, d = i - m * a.D;
+            float* o = so + tr_at<DP>(m, d >> 2) + (d & 3);
+            float x = *o * s_fix[m];
+            for (uint64_t left = s_sees[m]; left; left &= left - 1) {
+                const int j = __ffsll((long long)left) - 1;
+                x = fmaf(sx[m * TR_TILE + j], tree_f32<T>(((const T*)a.v)[at(j) + d]), x);
+            }
+            *o = x;
+        }
+        __syncthreads();
+    }
+    if (tid < BM) ((float2*)s_sees)[tid] = make_float2(rf, sum);
+    __syncthreads();
+}
+
 // VEC: rows and offsets allow 4-element vectors.
 template <typename T, int DP, int WM, bool VEC>
 __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ TreeArgs a) {
@@ -115,6 +180,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
     constexpr int RING = tr_ring<DP, BM>();
     constexpr bool EXACT = sizeof(T) == 2;  // operands are TF32 values already
     static_assert(RING >= 3, "the ring holds a tile in use and two in flight");
+    static_assert(RING * TR_TILE * DP >= 128 * DP + BM * TR_TILE + BM, "room for tr_careful");
     extern __shared__ __align__(16) float sm[];
     float* ring = sm;
     float* sq = ring + RING * TR_TILE * DP;
@@ -130,9 +196,9 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
     pdl_trigger();
     TreeRun run = tree_run<TR_THREADS>(a, &s_run);
     TreeItem it;
-    bool any = false, again = false;
-    while (again || run.left > 0) {
-        if (!again) it = tree_next(a, run);
+    bool any = false;
+    while (run.left > 0) {
+        it = tree_next(a, run);
         any = true;
         const T* kb = (const T*)a.k;
         const T* vb = (const T*)a.v;
@@ -254,7 +320,7 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
         float p[NB][4];
         for (int s = 0; s < steps; s++) {
             const int kt = key0 + (s >> 1) * TR_TILE;
-            const bool part = again || tree_partial(it.q, s_edge, kt);
+            const bool part = tree_partial(it.q, s_edge, kt);
             if (!(s & 1) && part && tid < BM) s_sees[tid] = tree_sees(a, it.q, m0 + tid, kt);
             tr_wait<RING - 2>();
             __syncthreads();  // tile s is here, and everyone is done with tile s - 1
@@ -314,15 +380,6 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
                     }
                 }
                 // ---- weights; accumulator element e: row g + 8 (e / 2), key 2 t4 + e % 2
-                if (again) {
-#pragma unroll
-                    for (int n = 0; n < NB; n++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (p[n][e] != p[n][e])
-                                p[n][e] = tr_dot<DP>(sq, tile, wm * 16 + g + 8 * (e >> 1),
-                                                     wk * KW + n * 8 + 2 * t4 + (e & 1));
-                }
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     uint32_t sees = own_bits(&s_have[(s >> 1) & (TR_HAVE - 1)]);
@@ -447,66 +504,72 @@ __global__ void __launch_bounds__(TR_THREADS, 1) k_tree(const __grid_constant__ 
             if (!((s + RING) & 1)) rows_of((s + RING) >> 1);
         }
         tr_wait<0>();
-        // A part of a pair times an infinity can be NaN where the whole product is not (0 or
-        // the other sign in its low part).  Sums of NaN send the item through once more,
-        // with such scores formed again and every tile's values looked over.
-        bool nan = false;
+        // sums of NaN: the item once more, but not for rows whose query holds a NaN
+        uint32_t nan = 0;  // bit h: of row g + 8 h
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            if (wm * 16 + g + 8 * h >= it.rows) continue;
-            nan |= sum[h] != sum[h];
+            bool odd = sum[h] != sum[h];
 #pragma unroll
             for (int b = 0; b < DB; b++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    nan |= o[b][i][2 * h] != o[b][i][2 * h] ||
+                    odd |= o[b][i][2 * h] != o[b][i][2 * h] ||
                            o[b][i][2 * h + 1] != o[b][i][2 * h + 1];
+            if (odd && wm * 16 + g + 8 * h < it.rows) nan |= 1u << h;
         }
-        nan = __syncthreads_or(nan);
-        again = nan && !again;
-        if (again) continue;
-        // ---- join the WK key groups: weights from the maxima, then the sums in turn
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            sum[h] += __shfl_xor_sync(FULL, sum[h], 1);
-            sum[h] += __shfl_xor_sync(FULL, sum[h], 2);
-            if (t4 == 0)
-                s_ml[wk * BM + wm * 16 + g + 8 * h] =
-                    make_float2(rf[h], sum[h]);
-        }
-        __syncthreads();
-        float own[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int m = wm * 16 + g + 8 * h;
-            float top = -INFINITY;
-            for (int w = 0; w < WK; w++) top = fmaxf(top, s_ml[w * BM + m].x);
-            const float x = s_ml[wk * BM + m].x;
-            own[h] = x == -INFINITY ? 0.f : exp2f(x - top);
+        bool careful = __syncthreads_or(nan);
+        if (careful) {
+            for (int h = 0; h < 2; h++)
+                for (int d = 0; d < DP && (nan >> h & 1); d++) {
+                    const float x = sq[tr_at<DP>(wm * 16 + g + 8 * h, d >> 2) + (d & 3)];
+                    if (x != x) nan &= ~(1u << h);
+                }
+            careful = __syncthreads_or(nan);
         }
         float* so = ring;  // [WK][BM][DP], the ring is idle
         float2* s_all = (float2*)s_sees;  // each row's maximum and sum
+        if (careful) {
+            tr_careful<T, DP, BM>(a, it, so, sq, s_sees);
+        } else {
+            // ---- join the WK key groups: weights from the maxima, then the sums in turn
 #pragma unroll
-        for (int b = 0; b < DB; b++)
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int i = 0; i < 2; i++) {  // dims b * 32 + t4 * 8 + 4 i ..
-                    const int m = wm * 16 + g + 8 * h;
-                    *(float4*)(so + wk * BM * DP + tr_at<DP>(m, b * 8 + t4 * 2 + i)) =
-                        make_float4(o[b][0][i + 2 * h] * own[h], o[b][1][i + 2 * h] * own[h],
-                                    o[b][2][i + 2 * h] * own[h], o[b][3][i + 2 * h] * own[h]);
-                }
-        if (tid < BM) {
-            float top = -INFINITY, l = 0.f;
-            for (int w = 0; w < WK; w++) top = fmaxf(top, s_ml[w * BM + tid].x);
-            for (int w = 0; w < WK; w++) {
-                const float2 x = s_ml[w * BM + tid];
-                if (x.y != 0.f) l += x.y * exp2f(x.x - top);  // 0: saw nothing; NaN stays
+            for (int h = 0; h < 2; h++) {
+                sum[h] += __shfl_xor_sync(FULL, sum[h], 1);
+                sum[h] += __shfl_xor_sync(FULL, sum[h], 2);
+                if (t4 == 0) s_ml[wk * BM + wm * 16 + g + 8 * h] = make_float2(rf[h], sum[h]);
             }
-            s_all[tid] = make_float2(top, l);
+            __syncthreads();
+            float own[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int m = wm * 16 + g + 8 * h;
+                float top = -INFINITY;
+                for (int w = 0; w < WK; w++) top = fmaxf(top, s_ml[w * BM + m].x);
+                const float x = s_ml[wk * BM + m].x;
+                own[h] = x == -INFINITY ? 0.f : exp2f(x - top);
+            }
+#pragma unroll
+            for (int b = 0; b < DB; b++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {  // dims b * 32 + t4 * 8 + 4 i ..
+                        const int m = wm * 16 + g + 8 * h;
+                        *(float4*)(so + wk * BM * DP + tr_at<DP>(m, b * 8 + t4 * 2 + i)) =
+                            make_float4(o[b][0][i + 2 * h] * own[h], o[b][1][i + 2 * h] * own[h],
+                                        o[b][2][i + 2 * h] * own[h], o[b][3][i + 2 * h] * own[h]);
+                    }
+            if (tid < BM) {
+                float top = -INFINITY, l = 0.f;
+                for (int w = 0; w < WK; w++) top = fmaxf(top, s_ml[w * BM + tid].x);
+                for (int w = 0; w < WK; w++) {
+                    const float2 x = s_ml[w * BM + tid];
+                    if (x.y != 0.f) l += x.y * exp2f(x.x - top);  // 0: saw nothing; NaN stays
+                }
+                s_all[tid] = make_float2(top, l);
+            }
+            __syncthreads();
         }
-        __syncthreads();
         const size_t piece = (size_t)blockIdx.x * 2 + tree_slot(run, it);
         for (int i = tid; i < it.rows * a.D; i += TR_THREADS) {
             const int m = i / a.D, d = i - m * a.D;
