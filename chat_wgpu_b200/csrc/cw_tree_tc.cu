@@ -60,6 +60,14 @@ __device__ __forceinline__ bool tt_any(bool x, int blocks) {
     return r != 0;
 }
 
+// Which of the keys [j0, j1) have a page (out of line: 16 x 100 nodes of 64 dims at 4500
+// take 100.6 us, 103.5 with the loop in its place).
+__device__ __noinline__ uint64_t tt_have(const TreeArgs& a, int r, int j0, int j1) {
+    uint64_t have = 0;
+    for (int j = j0; j < j1; j++) have |= (uint64_t)tree_has(a, r, j) << (j - j0);
+    return have;
+}
+
 // The shapes of one instance.  HD: head dims rounded up; a thread's keys of a tile
 // are KEYS consecutive ones, so SPLIT lanes share a row.
 template <int HD, int NB, int SPLIT> struct TtShape {
@@ -318,11 +326,10 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
                     }
                     if (mixed || lost) {
                         uint64_t mine = sees >> (part * KEYS);
-                        if (lost)
-#pragma unroll 1
-                            for (int j = 0; j < KEYS && kt + part * KEYS + j < end; j++)
-                                if (!tree_has(a, it.r, kt + part * KEYS + j))
-                                    mine &= ~(1ull << j);
+                        if (lost) {
+                            const int j0 = kt + part * KEYS;
+                            mine &= tt_have(a, it.r, j0, min(end, j0 + KEYS));
+                        }
 #pragma unroll
                         for (int j = 0; j < KEYS; j++)
                             if (!(mine >> j & 1)) s[j] = -INFINITY;
