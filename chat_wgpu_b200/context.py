@@ -132,7 +132,9 @@ class GpuContext:
         object with data_ptr(), element_size(), shape and stride() (a torch
         tensor on the context's device).  The buffer reaches from the tensor's
         first element to its last, whatever its strides, and keeps the tensor
-        alive; its address must be 16-byte aligned.  The prepared calls
+        alive; its address must be 16-byte aligned.  Ops run on the context's
+        stream: where that is not the tensor's own, the caller orders the two
+        and keeps the tensor until they have run.  The prepared calls
         (kernels.pages, rope, tree) refuse a tensor of another type or whose
         strides are not what they read; other ops see f32 elements."""
         n = 0

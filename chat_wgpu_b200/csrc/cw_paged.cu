@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(PP_THREADS) k_page_plan(PagePlanArgs a) {
 // 16-byte vectors) of one token and walks a share of the token's q, k and v
 // heads, so one set of sines serves all of them; neighbouring threads take
 // neighbouring vectors, then neighbouring heads.  32768 bf16 rows of 32 + 8 + 8 heads
-// take 138 us (805 MB, 5.8 TB/s; 8 heads to a thread took 166, 2 took 294), 4096 f32
+// take 142 us (805 MB, 5.7 TB/s; 8 heads to a thread took 166, 2 took 294), 4096 f32
 // rows of 16 + 8 + 8 heads 27 us (4.9 TB/s).
 struct RopeArgs {
     const unsigned long long* steps;

@@ -14,8 +14,10 @@
 // each.  Bound by the cache's bytes in the tiles: 64 KB at D = 128 is 1.5 us of an SM's
 // share of the memory bandwidth, against about 0.3 us of products and 0.5 to 1 us of
 // weights.  An item's start and end add 2 to 5 us, which deeper rings do not hide: 32
-// requests x 16 nodes at 8192 take 135 us where the bytes alone take 108, 256 x 1 of
-// 64 dims at 3001 200 us for 149, five of 256 dims with a window 24 us for 11.
+// requests x 16 nodes at 8192 take 142 us where the bytes alone take 108, 256 x 1 of
+// 64 dims at 3001 206 us for 149, five of 256 dims with a window 28 us for 11, 250 x 8
+// at 400 110 us for 44.  64 rows want more than the 168 registers that 320 threads leave
+// (they are charged as 12 warps): 104 bytes a thread are spilled at 128 dims.
 //
 // No maximum over keys is formed per tile: each row has a reference in shared memory,
 // and only when some weight would pass 2^8 (2^15 in f16; always at a row's first tile)
@@ -25,9 +27,10 @@
 //
 // Scores have two TMEM buffers and weights two in shared memory, so the products of
 // neighbouring tiles overlap the weights.  Warps: 2 groups of 4 for the weights, half
-// the rows each (one group: 180 us for 135); 1 for TMA; 1 whose elected lane issues the
-// products.  Keys that not every row sees, v rows past the end and values that are not
-// finite are treated as in cw_tree_tc.cu.
+// the rows each (one group: 180 us for 135, 32 x 16 at 8192 when it was tried); 1 for TMA;
+// 1 whose elected lane issues the products.  Keys that not every row sees, v rows past
+// the end, keys without a page and values that are not finite are treated as in
+// cw_tree_tc.cu.
 #include <algorithm>
 
 #include "cw_tree_tc.cuh"
@@ -336,8 +339,8 @@ __global__ void __launch_bounds__(320, 1)
                 // set before the tile's keys were, if one of them has no page
                 const bool lost = *(volatile uint32_t*)&bars->lost;
                 float s[C];
-                // pass 1: the weights' exponents; were some to pass 8 (f16: 15; then 0, and at once at
-                // an item's first tile): new references; 2: the exponents again
+                // pass 1: the weights' exponents; were some to pass 8, or 15 in f16 (0, and
+                // at once at an item's first tile): new references; 2: the exponents again
 #pragma unroll 1
                 for (int pass = i == 0 ? 0 : 1;;) {
                     tt_load<C>(lanes + (n & 1) * N, (uint32_t*)s);

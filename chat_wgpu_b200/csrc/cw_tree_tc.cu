@@ -12,10 +12,10 @@
 // request share a tile (up to 128 rows, or 256 with two row blocks per CTA; at 256
 // dims 128, whose second block reads the tile through L2).  A tile of 64 keys at
 // D = 128 is 32 KB, 0.75 us of an SM's share of the memory bandwidth.  128 rows take
-// about as long (two CTAs per SM: 32 x 32 nodes at 8192 in 161 us, memory alone 109).
+// about as long (two CTAs per SM: 32 x 32 nodes at 8192 in 162 us, memory alone 109).
 // 256 rows are bound by their exponentials and the issue slots around them: 1.4 us a
 // tile, of which 0.6 us are the special-function unit's alone (2 x 64 nodes at 131000
-// in 316 us, memory alone 151).
+// in 360 us, 309 in a short run; memory alone 151).
 //
 // Warps: 4 (or 2 x 4) softmax warps, a thread per row, so row maxima and sums need
 // no exchange; one TMA warp; one elected MMA lane.  S has two TMEM buffers: the scores of
@@ -29,7 +29,8 @@
 // with a window, those at its edge.  There each thread forms its row's 64-bit set
 // of seen keys, v rows past the end are zeroed, and a tile whose v holds values
 // that are not finite is mended: those values are taken out of the product and
-// added to the rows that see them.
+// added to the rows that see them.  Keys without a page (an id outside the cache) are
+// zeros in shared memory, and once there is one the threads look ids up and mask them.
 #include <algorithm>
 #include <mutex>
 
