@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(TJ_WARPS * 32) k_tree_join(const __grid_consta
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float wj = __shfl_sync(FULL, w, (j0 + j) & 31);
-                if (j0 + j >= n || wj == 0.f) continue;  // 0: a piece where the row saw nothing
+                if (j0 + j >= n) continue;  // 0 times a NaN stays: keys of no weight, not finite
                 acc.x = fmaf(wj, x[j].x, acc.x);
                 acc.y = fmaf(wj, x[j].y, acc.y);
                 acc.z = fmaf(wj, x[j].z, acc.z);

@@ -496,10 +496,8 @@ __global__ void __launch_bounds__(NB * 128 + 64, TtShape<HD, NB, SPLIT>::PER_SM)
 #pragma unroll
                         for (int j = 0; j < 8; j++)
                             *(float4*)(q_sm + m * 128 + ((j ^ (m & 7)) << 4)) =
-                                make_float4(own == 0.f ? 0.f : o[4 * j] * own,
-                                            own == 0.f ? 0.f : o[4 * j + 1] * own,
-                                            own == 0.f ? 0.f : o[4 * j + 2] * own,
-                                            own == 0.f ? 0.f : o[4 * j + 3] * own);
+                                make_float4(o[4 * j] * own, o[4 * j + 1] * own, o[4 * j + 2] * own,
+                                            o[4 * j + 3] * own);
                     }
                     (void)tt_any(false, 1);
                     if (r < rows) {  // this thread: 32 / SPLIT of the columns

@@ -412,3 +412,22 @@ def test_a_dominating_key(ctx, kind):
     # f32 arithmetic and one rounding of the result.
     assert np.abs(got - want).max() <= (lens + n) * 2.0 ** -32 + (ref.UNIT["f16"] + 1e-5) * want.max()
     ctx.sync()
+
+
+@kinds
+@pytest.mark.parametrize("lens", [[400, 3], [9000, 3]], ids=["whole", "cut"])
+def test_no_weight_times_infinity(ctx, kind, lens):
+    """A key that scores -inf weighs 0, and 0 times an infinite value is NaN, wherever the
+    key's tile was dealt to; other dims stay."""
+    dtype, H, K, D, page, n = kind
+    c = tree_case(np.random.default_rng(25), lens, [n, 2], dtype, H, K, D, page, poison=False)
+    c["q"][:, :, 2] = 1.0
+    at = np.arange(320)
+    c["kc"][c["table"][0, at // page], :, at % page, 2] = -np.inf
+    c["vc"][c["table"][0, 100 // page], :, 100 % page, 4] = np.inf
+    got = tree_run(ctx, c, dtype, H, K, D, page)
+    want, s, v = attend(c, page)
+    assert np.isnan(want[:n, :, 4]).all() and np.isnan(got[:n, :, 4]).all()
+    fine = np.isfinite(want)
+    assert np.abs(got[fine] - want[fine]).max() <= tree_tolerance(dtype, s, v)
+    ctx.sync()
