@@ -74,6 +74,29 @@ class TreeAttnArgs(C.Structure):
                [("scale", C.c_float), ("softcap", C.c_float)]
 
 
+class NormRopeArgs(C.Structure):
+    _fields_ = [(n, _u64) for n in ("plan", "positions", "q", "k", "v", "q_norm", "k_norm", "slots",
+                                    "q_out", "k_out", "k_cache", "v_cache", "q_off", "k_off",
+                                    "v_off", "q_stride", "k_stride", "v_stride")] + \
+               [(n, _u32) for n in ("type", "layout", "n_tokens", "n_heads", "n_kv", "head_dim",
+                                    "page_size", "n_pages", "norm_kind")] + [("eps", C.c_float)]
+
+
+class PromptAttnArgs(C.Structure):
+    _fields_ = [(n, _u64) for n in ("q", "k", "v", "starts", "key_starts", "out", "q_off", "k_off",
+                                    "v_off", "q_stride", "k_stride", "v_stride")] + \
+               [(n, _u32) for n in ("type", "n_req", "n_rows", "n_keys", "n_heads", "n_kv",
+                                    "head_dim", "window")] + \
+               [("scale", C.c_float), ("softcap", C.c_float)]
+
+
+class AdjustLogitsArgs(C.Structure):
+    _fields_ = [(n, _u64) for n in ("logits", "penalties", "tokens", "starts", "prompts",
+                                    "bias_tokens", "bias_values", "bias_starts", "masks",
+                                    "mask_rows", "out", "best", "off", "stride")] + \
+               [(n, _u32) for n in ("type", "n_rows", "vocab", "n_tokens", "n_bias", "n_masks")]
+
+
 _vp = C.c_void_p
 _sz = C.c_size_t
 _buf = C.c_uint64
@@ -139,6 +162,9 @@ SIGNATURES = {
     "cw_rope_plan": [_vp, _sz, C.c_double, C.POINTER(RopeScaling), _pbuf],
     "cw_rope_append": [_vp, C.POINTER(RopeAppendArgs)],
     "cw_tree_attention": [_vp, C.POINTER(TreeAttnArgs)],
+    "cw_norm_rope": [_vp, C.POINTER(NormRopeArgs)],
+    "cw_prompt_attention": [_vp, C.POINTER(PromptAttnArgs)],
+    "cw_adjust_logits": [_vp, C.POINTER(AdjustLogitsArgs)],
     "cw_model_load_gguf": [_vp, C.c_char_p, C.POINTER(_vp)],
     "cw_model_free": [_vp],
     "cw_model_get_info": [_vp, C.POINTER(ModelInfo)],

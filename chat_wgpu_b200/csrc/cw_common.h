@@ -133,6 +133,11 @@ int arena_get(cw_ctx* ctx, size_t len_f32, cw_buf* out, BufEntry** entry = nullp
 int check_launch(const char* what);
 int check_device_status(cw_ctx* ctx);
 
+// Whether [a, a + na) and [b, b + nb) share a byte.
+inline bool spans_meet(const void* a, size_t na, const void* b, size_t nb) {
+    return na && nb && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
 // A profiler scope: records a start/stop event pair around the launches made
 // while it is alive, labelled with the op name (context.rs:302-328).
 struct OpScope {

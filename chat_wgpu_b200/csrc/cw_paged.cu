@@ -8,7 +8,7 @@
 #include <vector>
 
 #include "cw_common.h"
-#include "cw_device.cuh"
+#include "cw_rotary.cuh"
 
 namespace cw {
 
@@ -212,19 +212,6 @@ struct RopeArgs {
     int* status;
 };
 
-template <int BYTES> struct VecOf;
-template <> struct VecOf<16> { typedef uint4 type; };
-template <> struct VecOf<8> { typedef uint2 type; };
-template <> struct VecOf<4> { typedef uint32_t type; };
-template <> struct VecOf<2> { typedef uint16_t type; };
-
-__device__ __forceinline__ float rp_f32(float x) { return x; }
-__device__ __forceinline__ float rp_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float rp_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void rp_set(float* d, float x) { *d = x; }
-__device__ __forceinline__ void rp_set(__half* d, float x) { *d = __float2half_rn(x); }
-__device__ __forceinline__ void rp_set(__nv_bfloat16* d, float x) { *d = __float2bfloat16_rn(x); }
-
 constexpr int RP_THREADS = 256;
 constexpr int RP_UNROLL = 2;  // heads whose loads are in flight while two others are turned
 
@@ -281,18 +268,7 @@ __global__ void __launch_bounds__(RP_THREADS, 3) k_rope_append(RopeArgs a) {
 #pragma unroll
     for (int u = 0; u < RP_UNROLL; u++) load(u, w[u]);
     float cs[VEC], sn[VEC];
-    if (turn) {
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const long long ph =
-                (long long)((unsigned long long)pos * a.steps[c * VEC + i]);
-            // 16-bit values: within half a turn the fast functions are off by 2^-21
-            if (sizeof(T) == 2) __sincosf((float)ph * 0x1.921fb6p-62f, &sn[i], &cs[i]);
-            else sincospif((float)ph * 0x1p-63f, &sn[i], &cs[i]);
-            sn[i] *= a.amp;
-            cs[i] *= a.amp;
-        }
-    }
+    if (turn) rotary_sines<T, VEC>(a.steps + c * VEC, pos, a.amp, cs, sn);
     for (int i0 = 0; i0 < a.per; i0 += RP_UNROLL) {
 #pragma unroll
         for (int u = 0; u < RP_UNROLL; u++) {

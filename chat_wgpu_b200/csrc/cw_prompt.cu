@@ -1,0 +1,249 @@
+// cw_prompt.cu -- causal attention of packed prompts (cw_prompt_attention): the entry
+// point, and the kernel for every type, alignment and head size in f32 products.
+//
+//   o_i = sum_j w_ij v_j / sum_j w_ij,   w_ij = exp(cap(scale q_i . k_j) - m_i)
+//
+// Keys come in tiles; a row keeps its running maximum m_i, sum and weighted values, and
+// scales the latter two when the maximum grows.  256 threads hold 64 x 64 scores as 4 x 4
+// blocks and 64 x D sums as 4 rows by D / 16 columns.
+#include <math.h>
+
+#include <algorithm>
+
+#include "cw_prompt.cuh"
+
+namespace cw {
+
+constexpr int PF_ROWS = 64, PF_KEYS = 64, PF_THREADS = 256;
+
+// DP: head_dim rounded up to 64, 128 or 256.
+template <typename T, int DP>
+__global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ PromptArgs a) {
+    constexpr int LD = DP + 4, CN = DP / 16;
+    extern __shared__ __align__(16) float sm[];
+    float* sq = sm;                   // [PF_ROWS][LD]
+    float* skv = sq + PF_ROWS * LD;   // [PF_KEYS][LD]
+    float* sp = skv + PF_KEYS * LD;   // [PF_ROWS][PF_KEYS + 4]
+    constexpr int LP = PF_KEYS + 4;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int head = blockIdx.x % a.K, block = blockIdx.x / a.K;
+    pdl_wait();
+    if (blockIdx.x == 0) prompt_check(a, tid, PF_THREADS);
+    // the last blocks of a request have the most keys: they start first
+    const PromptItem it = prompt_item(a, a.slots - 1 - block / ((a.bt * a.G + PF_ROWS - 1) / PF_ROWS));
+    const int m0 = block % ((a.bt * a.G + PF_ROWS - 1) / PF_ROWS) * PF_ROWS;
+    const int rows = min(PF_ROWS, it.rows * a.G - m0);
+    if (rows <= 0) return;
+    const T* qb = (const T*)a.q + (long long)head * a.G * a.D;
+    const T* kb = (const T*)a.k + (long long)it.key0 * a.k_stride + (long long)head * a.D;
+    const T* vb = (const T*)a.v + (long long)it.key0 * a.v_stride + (long long)head * a.D;
+    for (int i = tid; i < PF_ROWS * DP; i += PF_THREADS) {
+        const int m = i / DP, d = i % DP;
+        float x = 0.f;
+        if (m < rows && d < a.D) {
+            const int t = (m0 + m) / a.G, g = (m0 + m) - t * a.G;
+            x = pr_f32(qb[(long long)(it.row0 + t) * a.q_stride + g * a.D + d]);
+        }
+        sq[m * LD + d] = x;
+    }
+    float o[4][CN], top[4], sum[4];
+    int lim[4], low[4];  // the row sees keys [low, lim]
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        top[i] = -INFINITY;
+        sum[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CN; c++) o[i][c] = 0.f;
+        const int m = m0 + ty * 4 + i, t = m / a.G;
+        lim[i] = ty * 4 + i < rows ? min(it.past + t, it.keys - 1) : -1;
+        low[i] = a.window > 0 ? max(it.past + t - a.window + 1, 0) : 0;
+    }
+    const int last = min(it.past + (m0 + rows - 1) / a.G, it.keys - 1);
+    const int first = it.first / PF_KEYS * PF_KEYS;
+    // keys that every row of the block sees
+    const int all1 = min(it.past + m0 / a.G, it.keys - 1);
+    const int all0 = a.window > 0 ? it.past + (m0 + rows - 1) / a.G - a.window + 1 : 0;
+    for (int kt = first; kt <= last; kt += PF_KEYS) {
+        const bool mixed = kt < all0 || kt + PF_KEYS - 1 > all1;
+        __syncthreads();
+        for (int i = tid; i < PF_KEYS * DP; i += PF_THREADS) {
+            const int j = i / DP, d = i % DP;
+            skv[j * LD + d] =
+                kt + j <= last && d < a.D ? pr_f32(kb[(long long)(kt + j) * a.k_stride + d]) : 0.f;
+        }
+        __syncthreads();
+        float s[4][4] = {};
+        for (int d = 0; d < a.D; d += 4) {
+            float4 x[4], y[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = *(const float4*)&sq[(ty * 4 + i) * LD + d];
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] = *(const float4*)&skv[(tx + 16 * j) * LD + d];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
+                    s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
+                    s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
+                    s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float t = top[i];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float x = s[i][j] * a.scale;
+                if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
+                const int key = kt + tx + 16 * j;
+                if (key < low[i] || key > lim[i]) x = -INFINITY;
+                s[i][j] = x;
+                t = fmaxf(t, x);
+            }
+#pragma unroll
+            for (int w = 8; w; w >>= 1) t = fmaxf(t, __shfl_xor_sync(FULL, t, w));
+            // scores of -inf weigh nothing, whatever the maximum
+            const float from = t == -INFINITY ? 0.f : t;
+            const float fix = top[i] == -INFINITY ? 0.f : expf(top[i] - from);
+            top[i] = t;
+            float l = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float p = expf(s[i][j] - from);
+                l += p;
+                sp[(ty * 4 + i) * LP + tx + 16 * j] = p;
+            }
+#pragma unroll
+            for (int w = 8; w; w >>= 1) l += __shfl_xor_sync(FULL, l, w);
+            sum[i] = sum[i] * fix + l;
+            // (a sum that is not finite stays so: zero is kept as zero)
+#pragma unroll
+            for (int c = 0; c < CN; c++) o[i][c] *= fix;
+        }
+        __syncthreads();
+        bool odd = false;
+        for (int i = tid; i < PF_KEYS * DP; i += PF_THREADS) {
+            const int j = i / DP, d = i % DP;
+            const float x =
+                kt + j <= last && d < a.D ? pr_f32(vb[(long long)(kt + j) * a.v_stride + d]) : 0.f;
+            skv[j * LD + d] = x;
+            odd |= !isfinite(x);
+        }
+        // a value that is not finite counts only where it is seen
+        const bool careful = __syncthreads_or(mixed && odd);
+        for (int j = 0; j < PF_KEYS; j++) {
+            float p[4], y[CN];
+            bool see[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                p[i] = sp[(ty * 4 + i) * LP + j];
+                see[i] = kt + j >= low[i] && kt + j <= lim[i];
+            }
+#pragma unroll
+            for (int c = 0; c < CN; c++) y[c] = skv[j * LD + tx + 16 * c];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int c = 0; c < CN; c++)
+                    if (!careful || see[i]) o[i][c] = fmaf(p[i], y[c], o[i][c]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int m = ty * 4 + i;
+        if (m >= rows) continue;
+        const int t = (m0 + m) / a.G, g = (m0 + m) - t * a.G;
+        const float inv = sum[i] > 0.f || sum[i] != sum[i] ? 1.f / sum[i] : 0.f;
+        T* out = (T*)a.out + ((long long)(it.row0 + t) * a.H + head * a.G + g) * a.D;
+#pragma unroll
+        for (int c = 0; c < CN; c++) {
+            const int d = tx + 16 * c;
+            if (d < a.D) out[d] = pr_to<T>(inv == 0.f ? 0.f : o[i][c] * inv);
+        }
+    }
+}
+
+template <typename T, int DP> static int prompt_go(cw_ctx* ctx, PromptArgs& a) {
+    auto kern = k_prompt<T, DP>;
+    const size_t smem = ((size_t)(PF_ROWS + PF_KEYS) * (DP + 4) + PF_ROWS * (PF_KEYS + 4)) * 4;
+    CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    a.bt = std::max(1, PF_ROWS / a.G);
+    a.slots = a.n_rows / a.bt + a.n_req;
+    const long long grid = (long long)a.slots * ((a.bt * a.G + PF_ROWS - 1) / PF_ROWS) * a.K;
+    CW_CHECK(grid < (1ll << 31), CW_ERR_UNSUPPORTED, "cw_prompt_attention: too many rows");
+    CW_TRY(launch_pdl(ctx, true, kern, dim3((unsigned)grid), dim3(PF_THREADS), smem, a));
+    return check_launch("prompt_attention");
+}
+template <typename T> static int prompt_dims(cw_ctx* ctx, PromptArgs& a) {
+    if (a.D <= 64) return prompt_go<T, 64>(ctx, a);
+    if (a.D <= 128) return prompt_go<T, 128>(ctx, a);
+    return prompt_go<T, 256>(ctx, a);
+}
+
+}  // namespace cw
+
+using namespace cw;
+
+extern "C" int cw_prompt_attention(cw_ctx* ctx, const cw_prompt_attn_args* p) {
+    clear_error();
+    CW_CHECK(ctx && p, CW_ERR_INVALID_ARG, "cw_prompt_attention: bad arguments");
+    CW_CHECK(p->type == CW_GGUF_F32 || p->type == CW_GGUF_F16 || p->type == CW_GGUF_BF16,
+             CW_ERR_UNSUPPORTED, "cw_prompt_attention: type %u (f32, f16 or bf16)", p->type);
+    CW_CHECK(p->n_req > 0 && p->n_req <= (1u << 20) && p->n_rows > 0 && p->n_rows <= (1u << 28) &&
+                 p->n_keys > 0 && p->n_keys <= (1u << 28) && p->n_kv > 0 && p->n_heads <= 4096 &&
+                 p->n_heads >= p->n_kv && p->n_heads % p->n_kv == 0 && p->head_dim > 0 &&
+                 p->head_dim <= 256 && p->window < (1u << 31),
+             CW_ERR_INVALID_ARG, "cw_prompt_attention: bad shape");
+    CW_CHECK(isfinite(p->scale) && p->softcap >= 0.f && isfinite(p->softcap), CW_ERR_INVALID_ARG,
+             "cw_prompt_attention: scale and softcap must be finite, softcap not negative");
+    const uint64_t big = 1ull << 40;  // keeps the byte counts below from overflowing
+    const size_t es = p->type == CW_GGUF_F32 ? 4 : 2, T = p->n_rows, L = p->n_keys,
+                 D = p->head_dim, qw = p->n_heads * D, kw = p->n_kv * D;
+    CW_CHECK(p->q_off < big && p->k_off < big && p->v_off < big && p->q_stride < (1ull << 30) &&
+                 p->k_stride < (1ull << 30) && p->v_stride < (1ull << 30) &&
+                 (p->q_stride >= qw || T == 1) &&
+                 ((p->k_stride >= kw && p->v_stride >= kw) || L == 1),
+             CW_ERR_INVALID_ARG, "cw_prompt_attention: bad offset or stride");
+    BufEntry *q, *k, *v, *st, *ks = nullptr, *out;
+    const size_t nq = ((T - 1) * p->q_stride + qw) * es, nk = ((L - 1) * p->k_stride + kw) * es,
+                 nv = ((L - 1) * p->v_stride + kw) * es, no = T * qw * es,
+                 ns = ((size_t)p->n_req + 1) * 4;
+    CW_TRY(buf_get(ctx, p->q, &q, p->q_off * es + nq, "cw_prompt_attention(q)"));
+    CW_TRY(buf_get(ctx, p->k, &k, p->k_off * es + nk, "cw_prompt_attention(k)"));
+    CW_TRY(buf_get(ctx, p->v, &v, p->v_off * es + nv, "cw_prompt_attention(v)"));
+    CW_TRY(buf_get(ctx, p->starts, &st, ns, "cw_prompt_attention(starts)"));
+    if (p->key_starts)
+        CW_TRY(buf_get(ctx, p->key_starts, &ks, ns, "cw_prompt_attention(key_starts)"));
+    CW_TRY(buf_get(ctx, p->out, &out, no, "cw_prompt_attention(out)"));
+    PromptArgs a{};
+    a.q = (const char*)q->ptr + p->q_off * es;
+    a.k = (const char*)k->ptr + p->k_off * es;
+    a.v = (const char*)v->ptr + p->v_off * es;
+    a.starts = (const int*)st->ptr;
+    a.key_starts = ks ? (const int*)ks->ptr : nullptr;
+    a.out = out->ptr;
+    CW_CHECK(!spans_meet(a.out, no, a.q, nq) && !spans_meet(a.out, no, a.k, nk) &&
+                 !spans_meet(a.out, no, a.v, nv) && !spans_meet(a.out, no, a.starts, ns) &&
+                 !(ks && spans_meet(a.out, no, a.key_starts, ns)),
+             CW_ERR_INVALID_ARG, "cw_prompt_attention: out lies on an input");
+    a.q_stride = (long long)p->q_stride;
+    a.k_stride = (long long)p->k_stride;
+    a.v_stride = (long long)p->v_stride;
+    a.n_req = (int)p->n_req;
+    a.n_rows = (int)T;
+    a.n_keys = (int)L;
+    a.H = (int)p->n_heads;
+    a.K = (int)p->n_kv;
+    a.G = a.H / a.K;
+    a.D = (int)D;
+    a.window = (int)p->window;
+    a.scale = p->scale != 0.f ? p->scale : 1.f / sqrtf((float)D);
+    a.softcap = p->softcap;
+    a.status = ctx->d_status;
+    cudaSetDevice(ctx->device);
+    OpScope scope(ctx, "prompt_attention");
+    if (p->type == CW_GGUF_F32) return prompt_dims<float>(ctx, a);
+    if (p->type == CW_GGUF_F16) return prompt_dims<__half>(ctx, a);
+    return prompt_dims<__nv_bfloat16>(ctx, a);
+}

@@ -1,0 +1,95 @@
+// cw_prompt.cuh -- what the kernels of cw_prompt_attention share.
+//
+// For one kv head a request with n rows is a block of n * G query rows (G query heads per
+// kv head, row = i * G + g).  An ITEM is one kv head and up to BT rows of one request.
+// Which rows those are is device data, so the grid has a SLOT for every block there can
+// be: request r owns slots floor(starts[r] / BT) + r on, which is enough for its
+// ceil(n / BT) blocks and ascends in r, so an item finds its request by a search and no
+// sum over the requests is formed.  Slots without rows end at once.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "cw_common.h"
+#include "cw_device.cuh"
+
+namespace cw {
+
+struct PromptArgs {
+    const void *q, *k, *v;
+    void* out;
+    const int *starts, *key_starts;
+    long long q_stride, k_stride, v_stride;
+    int n_req, n_rows, n_keys, H, K, G, D, window;
+    float scale, softcap;
+    int bt;     // rows of an item
+    int slots;  // blocks there can be
+    int* status;
+};
+
+__device__ __forceinline__ void prompt_bad(const PromptArgs& a) {
+    atomicCAS(a.status, DEV_OK, DEV_BAD_INPUT);
+}
+
+struct PromptItem {
+    int row0, rows;  // its rows of q and out
+    int key0, keys;  // its request's keys
+    int past;        // row i of the item sees keys [.., past + i] of the request
+    int first;       // first key that one of its rows may see
+    int end;         // one past the last key that one of its rows may see
+};
+
+// The rows of slot s, of any kv head; rows = 0: none.
+__device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, int s) {
+    int lo = 0, hi = a.n_req;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        const int m = min(max(a.starts[mid], 0), a.n_rows);
+        if (m / a.bt + mid <= s) lo = mid;
+        else hi = mid;
+    }
+    PromptItem it;
+    const int r0 = min(max(a.starts[lo], 0), a.n_rows);
+    const int r1 = min(max(a.starts[lo + 1], r0), a.n_rows);
+    const int n = r1 - r0, block = s - (r0 / a.bt + lo);
+    it.key0 = r0;
+    it.keys = n;
+    const int* ks = a.key_starts ? a.key_starts : a.starts;
+    it.key0 = min(max(ks[lo], 0), a.n_keys);
+    it.keys = min(max(ks[lo + 1], it.key0), a.n_keys) - it.key0;
+    const int i0 = block * a.bt;
+    it.rows = block < 0 || i0 >= n ? 0 : min(a.bt, n - i0);
+    it.row0 = r0 + i0;
+    it.past = i0 + it.keys - n;
+    it.first = a.window > 0 ? max(0, it.past - a.window + 1) : 0;
+    it.end = max(0, min(it.keys, it.past + it.rows));
+    return it;
+}
+// The CTA that meets slot 0 looks all starts over (any number of threads).
+__device__ __forceinline__ void prompt_check(const PromptArgs& a, int tid, int threads) {
+    bool bad = false;
+    for (int r = tid; r <= a.n_req; r += threads) {
+        const int s = a.starts[r], b = r ? a.starts[r - 1] : 0;
+        bad |= s < b || s > a.n_rows;
+        if (a.key_starts) {
+            const int k = a.key_starts[r], c = r ? a.key_starts[r - 1] : 0;
+            bad |= k < c || k > a.n_keys;
+        } else {
+            bad |= s > a.n_keys;
+        }
+    }
+    if (bad) prompt_bad(a);
+}
+
+template <typename T> __device__ __forceinline__ float pr_f32(T x);
+template <> __device__ __forceinline__ float pr_f32(float x) { return x; }
+template <> __device__ __forceinline__ float pr_f32(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float pr_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T pr_to(float x);
+template <> __device__ __forceinline__ float pr_to(float x) { return x; }
+template <> __device__ __forceinline__ __half pr_to(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 pr_to(float x) { return __float2bfloat16_rn(x); }
+
+}  // namespace cw

@@ -50,6 +50,7 @@ class Prepared:
     _fn = ""
     _struct = None
     _rows: dict = {}  # buffers of the call's dtype, and the field of their row stride (or None)
+    _floats: tuple = ()  # buffers of f32 whatever the call's dtype; all others hold i32
 
     def __init__(self, ctx, dtype: str | None = None, **fields):
         self.ctx = ctx
@@ -61,7 +62,8 @@ class Prepared:
                 continue
             if isinstance(value, Buffer):
                 if value.owner is not None:
-                    want = DTYPES[dtype] if name in self._rows else ("int32", "uint32")
+                    want = (DTYPES[dtype] if name in self._rows else
+                            DTYPES["f32"] if name in self._floats else ("int32", "uint32"))
                     check_tensor(name, value.owner, want, fields.get(self._rows.get(name)))
                 self._keep.append(value)
                 value = value.handle

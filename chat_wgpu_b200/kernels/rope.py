@@ -54,3 +54,38 @@ class RopeAppend(Prepared):
             v_stride=v_stride or kv, type=type_code(dtype), layout=LAYOUTS[layout],
             n_tokens=n_tokens, n_heads=n_heads, n_kv=n_kv, head_dim=head_dim, page_size=page_size,
             n_pages=n_pages)
+
+
+class NormRope(Prepared):
+    """RMS norm of each q and k head, rotation at its row's position and the append to a
+    paged cache in one pass (cw_norm_rope).  unit_shift: the weights are 1 + w.  Without
+    a norm weight that side is only rotated, without slots nothing is cached; k_out takes
+    the k rows for an attention over the prompt itself."""
+
+    _fn = "cw_norm_rope"
+    _struct = _lib.NormRopeArgs
+    _rows = dict(q="q_stride", k="k_stride", v="v_stride", q_out=None, k_out=None, k_cache=None,
+                 v_cache=None)
+    _floats = ("q_norm", "k_norm")
+
+    def __init__(self, ctx, plan: Buffer, positions: Buffer, dtype: str, n_tokens: int,
+                 head_dim: int, eps: float, unit_shift: bool = False, layout: str = "half",
+                 n_heads: int = 0, n_kv: int = 0, q: Buffer | None = None,
+                 q_norm: Buffer | None = None, q_out: Buffer | None = None,
+                 k: Buffer | None = None, k_norm: Buffer | None = None,
+                 k_out: Buffer | None = None, v: Buffer | None = None,
+                 slots: Buffer | None = None, k_cache: Buffer | None = None,
+                 v_cache: Buffer | None = None, page_size: int = 0, n_pages: int = 0,
+                 q_off: int = 0, k_off: int = 0, v_off: int = 0, q_stride: int = 0,
+                 k_stride: int = 0, v_stride: int = 0):
+        if layout not in LAYOUTS:
+            raise ValueError(f"layout {layout!r}: one of {sorted(LAYOUTS)}")
+        kv = n_kv * head_dim
+        super().__init__(
+            ctx, dtype, plan=plan, positions=positions, q=q, k=k, v=v, q_norm=q_norm,
+            k_norm=k_norm, slots=slots, q_out=q_out, k_out=k_out, k_cache=k_cache,
+            v_cache=v_cache, q_off=q_off, k_off=k_off, v_off=v_off,
+            q_stride=q_stride or n_heads * head_dim, k_stride=k_stride or kv,
+            v_stride=v_stride or kv, type=type_code(dtype), layout=LAYOUTS[layout],
+            n_tokens=n_tokens, n_heads=n_heads, n_kv=n_kv, head_dim=head_dim,
+            page_size=page_size, n_pages=n_pages, norm_kind=int(bool(unit_shift)), eps=eps)

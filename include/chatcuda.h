@@ -398,6 +398,82 @@ typedef struct {
  * destroyed, and in order with the context's other tree attention calls. */
 int cw_tree_attention(cw_ctx* ctx, const cw_tree_attn_args* args);
 
+/* ---- taking prompts in, and choosing from their logits ----------------------
+ * No counterpart in the reference, whose prompt runs token by token.  A server's
+ * step over whole prompts (or later pieces of them) calls, per layer, cw_norm_rope
+ * after the projections and cw_prompt_attention before the output projection, and
+ * cw_adjust_logits on the rows it picks tokens from.  Structs, offsets, strides,
+ * types and device-side values as in the section above. */
+typedef struct {
+    cw_buf plan, positions;        /* cw_rope_plan; positions [n_tokens]             */
+    cw_buf q, k, v;                /* rows of n_heads / n_kv / n_kv heads            */
+    cw_buf q_norm, k_norm;         /* f32 [head_dim] weights; 0: not normed          */
+    cw_buf slots;                  /* [n_tokens]; -1: the row is not cached          */
+    cw_buf q_out, k_out;           /* [n_tokens][n_heads * head_dim], [..][n_kv * ..] */
+    cw_buf k_cache, v_cache;       /* [n_pages][n_kv][page_size][head_dim]           */
+    uint64_t q_off, k_off, v_off, q_stride, k_stride, v_stride;
+    uint32_t type, layout, n_tokens, n_heads, n_kv, head_dim, page_size, n_pages, norm_kind;
+    float eps;
+} cw_norm_rope_args;
+/* The norm of each q and k head, its rotation and the append in one pass:
+ *   n = x * rsqrt(mean(x^2) + eps) * w   (norm_kind 1: * (1 + w)),   y = R(position) n
+ * in f32, rounded once.  q_out = y of q; k_out (0: none) and the cache rows of the
+ * slots (slots 0: no cache, and v is not read) = y of k; the cache also takes v as it
+ * is.  n_heads = 0 leaves q out, n_kv = 0 k and v.  q_out may be q and k_out may be k
+ * where those rows are contiguous; no other output may overlap an input
+ * (CW_ERR_INVALID_ARG).  Rows whose slots are equal are written in no particular order. */
+int cw_norm_rope(cw_ctx* ctx, const cw_norm_rope_args* args);
+
+typedef struct {
+    cw_buf q;                  /* [n_rows] rows of n_heads * head_dim                  */
+    cw_buf k, v;               /* [n_keys] rows of n_kv * head_dim                     */
+    cw_buf starts;             /* [n_req + 1] first row of each request, ascending     */
+    cw_buf key_starts;         /* [n_req + 1] its first key; 0: starts                 */
+    cw_buf out;                /* [n_rows][n_heads * head_dim]                         */
+    uint64_t q_off, k_off, v_off, q_stride, k_stride, v_stride;
+    uint32_t type, n_req, n_rows, n_keys, n_heads, n_kv, head_dim, window;
+    float scale, softcap;      /* scale 0: head_dim^-0.5; softcap 0: none              */
+} cw_prompt_attn_args;
+/* out = softmax(cap(scale * q . k) over the keys a row sees) v, causal: the last row of
+ * a request sees all of its keys, and row i of n sees key j where j <= i + keys - n and,
+ * with a window, j > i + keys - n - window.  A request with more keys than rows is a
+ * later piece of a prompt; rows before its first key see nothing.  A row that sees
+ * nothing, or whose scores are all -inf, gives zeros; what a row does not see does not
+ * reach it, non-finite values included; a NaN score makes its row NaN.  Query head h
+ * reads kv head h / (n_heads / n_kv); head_dim <= 256.  Rows of out that belong to no
+ * request keep their contents; out may not overlap an input.  Sums and the softmax are
+ * f32.  Starts that descend or pass the buffers are cut to them and reported. */
+int cw_prompt_attention(cw_ctx* ctx, const cw_prompt_attn_args* args);
+
+typedef struct {
+    cw_buf logits;                 /* [n_rows] rows of vocab                           */
+    cw_buf penalties;              /* f32 [n_rows][3] repetition, frequency, presence;
+                                      0: none, and no history is read                  */
+    cw_buf tokens, starts;         /* [n_tokens]; [n_rows + 1]: row r's history is
+                                      tokens[starts[r] .. starts[r + 1])               */
+    cw_buf prompts;                /* [n_rows] leading history tokens that count for the
+                                      repetition penalty only; 0: none                 */
+    cw_buf bias_tokens, bias_values, bias_starts; /* [n_bias], f32 [n_bias], [n_rows + 1];
+                                      bias_starts 0: no biases                         */
+    cw_buf masks;                  /* [n_masks][ceil(vocab / 32)], bit set: allowed; 0: none */
+    cw_buf mask_rows;              /* [n_rows] mask of each row, negative: none; 0: mask r */
+    cw_buf out;                    /* [n_rows][vocab], of the logits' type             */
+    cw_buf best;                   /* u32 [n_rows]; 0: not wanted                      */
+    uint64_t off, stride;
+    uint32_t type, n_rows, vocab, n_tokens, n_bias, n_masks;
+} cw_adjust_logits_args;
+/* Per logit x of token t, each step rounded to f32:
+ *   t in the row's history:       x = x > 0 ? x / repetition : x * repetition
+ *   n > 0 times behind `prompts`: x = (x - frequency * n) - presence
+ *   t in the row's bias list:     x = x + bias (the last entry of t holds)
+ *   t not allowed by the mask:    x = -inf
+ * out = x rounded to the type; best = the lowest index of out's largest value, NaN
+ * left out, 0 where none is above -3.402823e38 (as cw_argmax).  out may be the logits
+ * themselves where their rows are contiguous, and may not overlap anything else.
+ * Tokens outside the vocabulary, starts that descend or pass their buffer and mask rows
+ * past n_masks are skipped and reported (a row with such a mask row has no mask). */
+int cw_adjust_logits(cw_ctx* ctx, const cw_adjust_logits_args* args);
+
 /* ---- model: src/model/{mod,qwen3,layers,cache}.rs --------------------------------------------- */
 typedef struct {
     uint32_t dim, n_layers, n_heads, n_kv, head_dim, hidden, vocab;
