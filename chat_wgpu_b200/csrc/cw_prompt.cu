@@ -243,6 +243,7 @@ extern "C" int cw_prompt_attention(cw_ctx* ctx, const cw_prompt_attn_args* p) {
     a.status = ctx->d_status;
     cudaSetDevice(ctx->device);
     OpScope scope(ctx, "prompt_attention");
+    if (prompt_tc_takes(a, p->type)) return prompt_tc_launch(ctx, a, p->type);
     if (p->type == CW_GGUF_F32) return prompt_dims<float>(ctx, a);
     if (p->type == CW_GGUF_F16) return prompt_dims<__half>(ctx, a);
     return prompt_dims<__nv_bfloat16>(ctx, a);

@@ -92,4 +92,8 @@ template <> __device__ __forceinline__ float pr_to(float x) { return x; }
 template <> __device__ __forceinline__ __half pr_to(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 pr_to(float x) { return __float2bfloat16_rn(x); }
 
+// cw_prompt_tc.cu: 16-bit types on the tcgen05 tensor cores, where the shape allows it.
+bool prompt_tc_takes(const PromptArgs& a, uint32_t type);
+int prompt_tc_launch(cw_ctx* ctx, PromptArgs& a, uint32_t type);
+
 }  // namespace cw

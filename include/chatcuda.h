@@ -442,7 +442,11 @@ typedef struct {
  * reach it, non-finite values included; a NaN score makes its row NaN.  Query head h
  * reads kv head h / (n_heads / n_kv); head_dim <= 256.  Rows of out that belong to no
  * request keep their contents; out may not overlap an input.  Sums and the softmax are
- * f32.  Starts that descend or pass the buffers are cut to them and reported. */
+ * f32.  16-bit types whose head_dim is a multiple of 8 and whose strides and places are
+ * multiples of 16 bytes, with at most 128 query heads per kv head and a positive scale,
+ * run on the tcgen05 tensor cores (there the softmax weights are rounded to the type
+ * before the product with v).  Starts that descend or pass the buffers are cut to them
+ * and reported. */
 int cw_prompt_attention(cw_ctx* ctx, const cw_prompt_attn_args* args);
 
 typedef struct {
