@@ -33,22 +33,74 @@
 namespace cw {
 
 constexpr int PT_KEYS = 128;    // keys of a tile
-constexpr int PT_RING = 2;      // items found ahead
+constexpr int PT_RING = 3;      // items found ahead
 constexpr int PT_LOOKS = 8;     // tiles looked over ahead (the ring holds 5 V tiles at most)
 constexpr int PT_STAGES = 10;   // most stages
 
-struct PtItem {
-    PromptItem it;
-    int head, more;  // more = 0: there are no more items
+// What a row block of an item sees: tiles [lo, hi), all rows the same in [all0, all1).
+struct PtBlock {
+    int lo, hi, all0, all1;
+    __device__ __forceinline__ bool in(int i) const { return i >= lo && i < hi; }
+    __device__ __forceinline__ bool mixed(int i) const { return i < all0 || i >= all1; }
 };
-
-struct PtBars {
+__device__ __forceinline__ PtBlock pt_block(const PromptArgs& a, const PromptItem& it, int b,
+                                            int tpb) {
+    PtBlock x = {0, 0, 0, 0};
+    const int t0 = b * tpb, t1 = min(t0 + tpb, it.rows);
+    if (t0 >= t1) return x;
+    const int first = a.window > 0 ? max(0, it.past + t0 - a.window + 1) : 0;
+    const int end = min(it.keys, it.past + t1);
+    if (end <= first) return x;
+    x.lo = first / PT_KEYS;
+    x.hi = (end + PT_KEYS - 1) / PT_KEYS;
+    const int late = a.window > 0 ? max(0, it.past + t1 - a.window) : 0;  // the last row's first key
+    x.all0 = (late + PT_KEYS - 1) / PT_KEYS;
+    x.all1 = max(0, min(it.past + t0 + 1, it.keys)) / PT_KEYS;  // up to the first row's last key
+    return x;
+}
+// The tiles of an item's row blocks together, [lo, hi), K and V in the order of the ring: K
+// of tile lo, then V of each tile behind K of its own (two row blocks) or of the next one.
+// Tiles outside [all0, all1), which may be mixed for a block, are looked over.
+template <int NB> struct PtTiles {
+    PtBlock b[NB];
+    int lo, hi, all0, all1;
+    __device__ __forceinline__ void set(const PromptArgs& a, const PromptItem& it, int tpb) {
+        lo = all1 = 1 << 30;
+        hi = all0 = 0;
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            b[i] = pt_block(a, it, i, tpb);
+            if (b[i].hi <= b[i].lo) continue;
+            lo = min(lo, b[i].lo);
+            hi = max(hi, b[i].hi);
+            all0 = max(all0, b[i].all0);
+            all1 = min(all1, b[i].all1);
+        }
+        lo = min(lo, hi);
+        all0 = min(max(all0, lo), hi);
+        all1 = min(max(all1, all0), hi);
+    }
+    __device__ __forceinline__ bool look(int i) const { return i < all0 || i >= all1; }
+    // tiles looked over before tile i; K and V tiles in the ring before V of tile i
+    __device__ __forceinline__ int looks(int i) const { return min(i, all0) - lo + max(0, i - all1); }
+    __device__ __forceinline__ int before(int i) const {
+        return 2 * (i - lo) + 1 + (NB == 1 && i + 1 < hi);
+    }
+};
+// What every role reads of an item.  more = 0: there are no more items.
+template <int NB> struct PtItem {
+    PromptItem it;
+    int head, more;
+    PtTiles<NB> t;
+};
+template <int NB> struct PtBars {
     uint64_t full[PT_STAGES], empty[PT_STAGES];
     uint64_t item_full[PT_RING], item_empty[PT_RING];
-    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], pv[2];  // s, p: by buffer of scores
+    uint64_t q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], pv[2];  // s, p: by buffer of scores
     uint64_t ask[PT_LOOKS], look[PT_LOOKS], done;
     uint32_t tmem, failed, odd[PT_LOOKS], skip[2];
-    PtItem item[PT_RING];
+    float meet[2][2][128];  // what the two threads of a row tell each other
+    PtItem<NB> item[PT_RING];
 };
 
 template <int HD> struct PtShape {
@@ -61,55 +113,17 @@ template <int HD> struct PtShape {
     static constexpr int QCOL = 128 * 128;                   // bytes of a column of queries
     static constexpr int QBLOCK = HD / 64 * QCOL;
     static constexpr int TCOLS = SB * PT_KEYS + HD;          // TMEM columns of a row block
-    static constexpr int THREADS = NB * 128 + 128;
-    static constexpr size_t SMEM = (size_t)NB * QBLOCK + STAGES * STAGE + sizeof(PtBars);
+    static constexpr int WARPS = NB * 8;                     // softmax warps
+    static constexpr int THREADS = WARPS * 32 + 128;
+    static constexpr size_t SMEM = (size_t)NB * QBLOCK + STAGES * STAGE + sizeof(PtBars<NB>);
     static_assert(SMEM <= 232448, "shared memory of a block");
     static_assert(STAGES <= PT_STAGES && STAGES / 2 + 1 < PT_LOOKS, "rings");
 };
 
-// What a row block of an item sees: tiles [lo, hi), and the keys that all of its rows see.
-struct PtBlock {
-    int lo, hi, all0, all1;
-    __device__ __forceinline__ bool in(int i) const { return i >= lo && i < hi; }
-    __device__ __forceinline__ bool mixed(int i) const {
-        return i * PT_KEYS < all0 || i * PT_KEYS + PT_KEYS - 1 > all1;
-    }
-};
-__device__ __forceinline__ PtBlock pt_block(const PromptArgs& a, const PromptItem& it, int b,
-                                            int tpb) {
-    PtBlock x = {0, 0, 0, 0};
-    const int t0 = b * tpb, t1 = min(t0 + tpb, it.rows);
-    if (t0 >= t1) return x;
-    const int first = a.window > 0 ? max(0, it.past + t0 - a.window + 1) : 0;
-    const int end = min(it.keys, it.past + t1);
-    if (end <= first) return x;
-    x.lo = first / PT_KEYS;
-    x.hi = (end + PT_KEYS - 1) / PT_KEYS;
-    x.all0 = a.window > 0 ? it.past + t1 - 1 - a.window + 1 : 0;
-    x.all1 = min(it.past + t0, it.keys - 1);
-    return x;
+// The place in the ring after n stages.
+template <int STAGES> __device__ __forceinline__ TtPlace pt_place(uint32_t n) {
+    return {(int)(n % STAGES), n / STAGES & 1};
 }
-// The tiles of an item's row blocks together.
-template <int NB> struct PtTiles {
-    PtBlock b[NB];
-    int lo, hi;
-    __device__ __forceinline__ PtTiles(const PromptArgs& a, const PromptItem& it, int tpb) {
-        lo = 1 << 30;
-        hi = 0;
-#pragma unroll
-        for (int i = 0; i < NB; i++) {
-            b[i] = pt_block(a, it, i, tpb);
-            if (b[i].hi > b[i].lo) lo = min(lo, b[i].lo), hi = max(hi, b[i].hi);
-        }
-        lo = min(lo, hi);
-    }
-    __device__ __forceinline__ bool mixed(int i) const {
-        bool x = false;
-#pragma unroll
-        for (int j = 0; j < NB; j++) x |= b[j].in(i) && b[j].mixed(i);
-        return x;
-    }
-};
 
 __device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
                                           uint32_t accumulate) {
@@ -131,12 +145,68 @@ __device__ __forceinline__ void pt_store32(void* p, const uint32_t* w) {
                  : "memory");
 }
 
-// A tile's product by the threads, a row each: O += the weights of the row's P times the
-// values that it sees, keys [lo, hi] of the tile.  `first`: there is no O before.
+// A wait that was not over at once: bounded, like tt_wait, but out of line and without a look
+// at the clock before many tries, which would delay the wake-up.
+__device__ __noinline__ bool pt_wait_on(uint64_t* bar, uint32_t parity, uint32_t* failed,
+                                        int* status) {
+    for (int i = 0; i < 256; i++)
+        if (mbar_try_wait(bar, parity)) return true;
+    return tt_wait(bar, parity, failed, status);
+}
+__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, uint32_t* failed,
+                                        int* status) {
+    return mbar_try_wait(bar, parity & 1) || pt_wait_on(bar, parity & 1, failed, status);
+}
+// The largest of three, NaN if one is.
+__device__ __forceinline__ float pt_max3(float x, float y, float z) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+// Two weights rounded and packed, first in the low half.
+template <bool BF> __device__ __forceinline__ uint32_t pt_pack(float x, float y) {
+    uint32_t r;
+    if (BF) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+
+// The scores of a row's half of a tile in TMEM, capped: tanh(y) = 1 - 2 / (1 + e^2y), off by 2^-22, times
+// softcap far below one rounding of the weight.  y2: 2 log2(e) scale / softcap.
+__device__ __noinline__ void pt_cap(uint32_t t_s, float softcap, float y2) {
+#pragma unroll 1
+    for (int c = 0; c < PT_KEYS / 2; c += 32) {
+        float s[32];
+        tt_load<32>(t_s + c, (uint32_t*)s);
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            const float y = s[j] * y2;
+            s[j] = softcap - __fdividef(2.f * softcap, 1.f + tt_exp2(y > 120.f ? 120.f : y));
+        }
+        tt_st32(t_s + c, (uint32_t*)s);
+    }
+    tt_wait_st();
+}
+// -inf for the keys of the half outside [lo, hi].
+__device__ __noinline__ void pt_hide(uint32_t t_s, int lo, int hi) {
+#pragma unroll 1
+    for (int c = 0; c < PT_KEYS / 2; c += 32, lo -= 32, hi -= 32) {
+        float s[32];
+        tt_load<32>(t_s + c, (uint32_t*)s);
+#pragma unroll
+        for (int j = 0; j < 32; j++)
+            if (j < lo || j > hi) s[j] = -INFINITY;
+        tt_st32(t_s + c, (uint32_t*)s);
+    }
+    tt_wait_st();
+}
+
+// A tile's product by the threads, two to a row with every other 8 dims each: O += the
+// weights of the row's P times the values that it sees, keys [lo, hi] of the tile.  `first`: there is no O before.
 template <bool BF>
 __device__ __noinline__ void pt_careful(uint32_t t_p, uint32_t t_o, const uint8_t* const* v, int D,
-                                        int lo, int hi, bool first) {
-    for (int d0 = 0; d0 < D; d0 += 8) {
+                                        int half, int lo, int hi, bool first) {
+    for (int d0 = half * 8; d0 < D; d0 += 16) {
         uint32_t o[8];
         tt_ld8(t_o + d0, o);
         float x[8];
@@ -172,11 +242,11 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                 int tpb, int items) {
     typedef PtShape<HD> Z;
     constexpr int NB = Z::NB, SB = Z::SB, HALVES = Z::HALVES, COLS = Z::COLS, STAGE = Z::STAGE;
-    constexpr int STAGES = Z::STAGES, TCOLS = Z::TCOLS;
+    constexpr int STAGES = Z::STAGES, TCOLS = Z::TCOLS, WARPS = Z::WARPS;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t* s_q = sm;  // [NB][HD / 64][128][128]
     uint8_t* ring = sm + NB * Z::QBLOCK;
-    PtBars* bars = (PtBars*)(ring + STAGES * STAGE);
+    PtBars<NB>* bars = (PtBars<NB>*)(ring + STAGES * STAGE);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     // the swizzle counts from 1024-byte boundaries; no static shared memory precedes
     if (smem_addr(sm) & 1023) {
@@ -191,13 +261,14 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
         }
         for (int s = 0; s < PT_RING; s++) {
             mbar_init(&bars->item_full[s], 1);
-            mbar_init(&bars->item_empty[s], 3 + NB * 4);
+            mbar_init(&bars->item_empty[s], 3 + WARPS);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&bars->q_full[b], 1);
             mbar_init(&bars->q_empty[b], 1);
             mbar_init(&bars->s_full[b], 1);
-            mbar_init(&bars->p_full[b], 4);
+            mbar_init(&bars->p_half[b], 8);
+            mbar_init(&bars->p_full[b], 8);
             mbar_init(&bars->pv[b], 1);
             bars->skip[b] = 0;
         }
@@ -216,31 +287,28 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
     pdl_trigger();
     const uint32_t tmem = bars->tmem;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return tt_wait(bar, parity, &bars->failed, a.status);
+        return pt_wait(bar, parity, &bars->failed, a.status);
     };
     auto all = [&](uint64_t* bar, uint32_t parity) {  // the same answer for the warp
         return __all_sync(FULL, wait(bar, parity)) != 0;
     };
-    // the item that every role works on, in the same order; false: no more
+    // the item that every role works on, in the same order, held until `done`; null: no more
     int n_item = 0;
-    PtItem now;
-    auto next = [&]() {
+    auto next = [&]() -> const PtItem<NB>* {
         const int s = n_item % PT_RING;
-        if (!all(&bars->item_full[s], n_item / PT_RING)) return false;
-        now = bars->item[s];
+        if (!all(&bars->item_full[s], n_item / PT_RING)) return nullptr;
+        return bars->item[s].more ? &bars->item[s] : nullptr;
+    };
+    auto done = [&]() {
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->item_empty[s]);
+        if (lane == 0) mbar_arrive(&bars->item_empty[n_item % PT_RING]);
         n_item++;
-        return now.more != 0;
     };
     constexpr TtTile tile = {1024, PT_KEYS * 128};
     TtPlace at = {0, 0};
 
-    // two row blocks: 168 registers a thread at the start, 208 for the softmax warps of 80
-    // left to the others (2 x 128 x 208 + 128 x 80 of 384 x 168)
-    if (warp >= NB * 4) {
-    if constexpr (NB == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-    if (warp == NB * 4) {  // ---- copies
+    if (warp >= WARPS) {
+    if (warp == WARPS) {  // ---- copies
         int q_count[2] = {0, 0};
         int filled = 0, asks = 0;  // stages filled so far, V tiles to be looked over
         bool ok = true;
@@ -250,6 +318,7 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
             tma_prefetch_desc(&map_v);
         }
         __syncwarp();
+        int head = 0, key0 = 0;
         auto load = [&](const CUtensorMap* map, int i) {  // keys of tile i
 #pragma unroll
             for (int h = 0; h < HALVES; h++) {
@@ -260,16 +329,20 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                     const int cols = min(COLS, (a.D - h * 128 + 63) / 64);
                     mbar_expect_tx(&bars->full[s], cols * PT_KEYS * 128);
                     for (int c = 0; c < cols; c++)
-                        pt_copy(ring + s * STAGE + c * PT_KEYS * 128, map, h * 128 + c * 64, now.head,
-                                now.it.key0 + i * PT_KEYS, &bars->full[s]);
+                        pt_copy(ring + s * STAGE + c * PT_KEYS * 128, map, h * 128 + c * 64, head,
+                                key0 + i * PT_KEYS, &bars->full[s]);
                 }
                 __syncwarp();
                 filled += ok;
                 if (ok) at.next(STAGES);
             }
         };
-        while (ok && next()) {
-            const PtTiles<NB> t(a, now.it, tpb);
+        while (const PtItem<NB>* x = ok ? next() : nullptr) {
+            const PtTiles<NB> t = x->t;
+            head = x->head;
+            key0 = x->it.key0;
+            const int row0 = x->it.row0;
+            done();
             if (t.lo >= t.hi) continue;
             load(&map_k, t.lo);
 #pragma unroll
@@ -280,8 +353,8 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                     const int cols = (a.D + 63) / 64;
                     mbar_expect_tx(&bars->q_full[b], cols * tpb * a.G * 128);
                     for (int c = 0; c < cols; c++)
-                        tt_copy_q(s_q + b * Z::QBLOCK + c * Z::QCOL, &map_q, c * 64, now.head * a.G,
-                                  now.it.row0 + b * tpb, &bars->q_full[b]);
+                        tt_copy_q(s_q + b * Z::QBLOCK + c * Z::QCOL, &map_q, c * 64, head * a.G,
+                                  row0 + b * tpb, &bars->q_full[b]);
                 }
                 __syncwarp();
                 q_count[b] += ok;
@@ -289,7 +362,7 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
             for (int i = t.lo; i < t.hi && ok; i++) {
                 if (NB == 1 && i + 1 < t.hi) load(&map_k, i + 1);
                 load(&map_v, i);
-                if (t.mixed(i)) {
+                if (t.look(i)) {
                     if (ok && tt_elect()) mbar_arrive(&bars->ask[asks % PT_LOOKS]);
                     __syncwarp();
                     asks++;
@@ -305,31 +378,36 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
             for (int b = 0; b < NB; b++)
                 if (q_count[b] > 0) (void)mbar_wait(&bars->q_full[b], (q_count[b] - 1) & 1, TT_WAIT_NS);
         }
-    } else if (warp == NB * 4 + 1) {  // ---- products
+    } else if (warp == WARPS + 1) {  // ---- products: one elected lane
         constexpr uint32_t id_s = tt_idesc<BF>(PT_KEYS, false, false);
         const uint64_t q0 = umma_desc_sw128(smem_addr(s_q)), kv0 = tt_desc(smem_addr(ring), tile);
         const int steps = (a.D + 15) / 16, halves = HALVES == 1 || a.D <= 128 ? 1 : HALVES;
+        const uint32_t id_o[2] = {tt_idesc<BF>(min(128, (a.D + 15) & ~15), false, true),
+                                  tt_idesc<BF>(max(16, (a.D - 128 + 15) & ~15), false, true)};
+        if (tt_elect()) {
         int n[2] = {0, 0}, q_count[2] = {0, 0};  // tiles and items of each row block
         bool ok = true;
-        while (ok && next()) {
-            const PtTiles<NB> t(a, now.it, tpb);
-            int done_s[NB];  // tiles of this item whose scores were asked for
-#pragma unroll
-            for (int b = 0; b < NB; b++) done_s[b] = 0;
+        while (ok) {
+            const int slot = n_item % PT_RING;
+            if (!wait(&bars->item_full[slot], n_item / PT_RING)) break;
+            if (!bars->item[slot].more) break;
+            const PtTiles<NB> t = bars->item[slot].t;
+            mbar_arrive(&bars->item_empty[slot]);
+            n_item++;
             // S = Q K^T of row block b, tile i, whose K is at place k
-            auto scores = [&](int b, const TtPlace& k) {
-                const int m = n[b] + done_s[b], sb = NB == 2 ? b : m & 1;
-                if (done_s[b] == 0) ok = ok && all(&bars->q_full[b], q_count[b]++);
+            auto scores = [&](int b, int i, const TtPlace& k) {
+                const int m = n[b] + i - t.b[b].lo, sb = NB == 2 ? b : m & 1;
+                if (i == t.b[b].lo) ok = ok && wait(&bars->q_full[b], q_count[b]++);
+                const uint32_t d = tmem + b * TCOLS + (NB == 2 ? 0 : sb * PT_KEYS);
                 TtPlace x = k;
 #pragma unroll
                 for (int h = 0; h < HALVES; h++) {
                     if (h >= halves) continue;
-                    ok = ok && all(&bars->full[x.stage], x.phase);
+                    ok = ok && wait(&bars->full[x.stage], x.phase);
                     tc_fence_after();
-                    if (ok && tt_elect()) {
-                        const uint32_t d = tmem + b * TCOLS + (NB == 2 ? 0 : sb * PT_KEYS);
-                        const uint64_t dk = kv0 + ((x.stage * STAGE) >> 4);
-                        const uint64_t dq = q0 + ((b * Z::QBLOCK + h * 2 * Z::QCOL) >> 4);
+                    const uint64_t dk = kv0 + ((x.stage * STAGE) >> 4);
+                    const uint64_t dq = q0 + ((b * Z::QBLOCK + h * 2 * Z::QCOL) >> 4);
+                    if (ok) {
 #pragma unroll
                         for (int s = 0; s < COLS * 4; s++)
                             if (h * 8 + s < steps)
@@ -337,58 +415,60 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                                          dk + (((s >> 2) * tile.col + (s & 3) * 32) >> 4), id_s,
                                          h + s > 0);
                     }
-                    __syncwarp();
                     x.next(STAGES);
                 }
-                done_s[b]++;
-                if (ok && tt_elect()) {
-                    tc_commit(&bars->s_full[sb]);
-                    if (done_s[b] == t.b[b].hi - t.b[b].lo) tc_commit(&bars->q_empty[b]);
-                }
-                __syncwarp();
+                if (!ok) return;
+                tc_commit(&bars->s_full[sb]);
+                if (i + 1 == t.b[b].hi) tc_commit(&bars->q_empty[b]);
             };
             // O += P V of row block b, tile i, whose V is at place v
             auto values = [&](int b, int i, const TtPlace& v) {
                 const int m = n[b] + i - t.b[b].lo, sb = NB == 2 ? b : m & 1;
                 TtPlace x = v;
                 for (int h = 0; h < halves; h++, x.next(STAGES))
-                    ok = ok && all(&bars->full[x.stage], x.phase);
-                ok = ok && all(&bars->p_full[sb], NB == 2 ? m : m >> 1);
-                tc_fence_after();
-                const bool skip = *(volatile uint32_t*)&bars->skip[sb];
-                if (ok && tt_elect()) {
-                    const uint32_t p = tmem + b * TCOLS + (NB == 2 ? 0 : sb * PT_KEYS);
-                    x = v;
-                    for (int h = 0; h < halves && !skip; h++, x.next(STAGES)) {
-                        const uint64_t dv = kv0 + ((x.stage * STAGE) >> 4);
-                        const uint32_t id_o =
-                            tt_idesc<BF>(min(128, (a.D - h * 128 + 15) & ~15), false, true);
+                    ok = ok && wait(&bars->full[x.stage], x.phase);
+                const uint32_t p = tmem + b * TCOLS + (NB == 2 ? 0 : sb * PT_KEYS);
+                const uint32_t o = tmem + b * TCOLS + SB * PT_KEYS;
+                const uint32_t before = i > t.b[b].lo;
+                bool skip = false;
 #pragma unroll
-                        for (int s = 0; s < PT_KEYS / 16; s++)
-                            pt_mma_ts(tmem + b * TCOLS + SB * PT_KEYS + h * 128, p + 8 * s,
-                                      dv + ((s * 2 * tile.group) >> 4), id_o, s > 0 || i > t.b[b].lo);
+                for (int part = 0; part < 2; part++) {
+                    ok = ok && wait(part ? &bars->p_full[sb] : &bars->p_half[sb], NB == 2 ? m : m >> 1);
+                    tc_fence_after();
+                    if (part == 0 && t.b[b].mixed(i)) skip = *(volatile uint32_t*)&bars->skip[sb];
+                    if (!ok || skip) continue;
+                    x = v;
+#pragma unroll
+                    for (int h = 0; h < HALVES; h++) {
+                        if (h >= halves) continue;
+                        const uint64_t dv = kv0 + ((x.stage * STAGE) >> 4);
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {  // 32 keys of each half
+                            const int s = (y >> 1) * 4 + (1 - part) * 2 + (y & 1);
+                            pt_mma_ts(o + h * 128, p + 8 * s, dv + ((s * 2 * tile.group) >> 4),
+                                      id_o[h], part + y > 0 ? 1u : before);
+                        }
+                        x.next(STAGES);
                     }
-                    tc_commit(&bars->pv[b]);
                 }
-                __syncwarp();
+                if (ok) tc_commit(&bars->pv[b]);
             };
             auto release = [&](TtPlace& x) {  // a K or V tile, by the products issued so far
-                for (int h = 0; h < halves; h++, x.next(STAGES)) {
-                    if (ok && tt_elect()) tc_commit(&bars->empty[x.stage]);
-                    __syncwarp();
-                }
+                for (int h = 0; h < halves; h++, x.next(STAGES))
+                    if (ok) tc_commit(&bars->empty[x.stage]);
             };
             if (t.lo < t.hi) {
 #pragma unroll
                 for (int b = 0; b < NB; b++)
-                    if (t.b[b].in(t.lo)) scores(b, at);
+                    if (t.b[b].in(t.lo)) scores(b, t.lo, at);
                 release(at);
             }
+#pragma unroll 1
             for (int i = t.lo; i < t.hi && ok; i++) {
                 const bool more = i + 1 < t.hi;
                 if (NB == 1) {
                     if (more) {
-                        scores(0, at);
+                        scores(0, i + 1, at);
                         release(at);
                     }
                     values(0, i, at);
@@ -400,7 +480,7 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                     for (int b = 0; b < NB; b++) {
                         if (t.b[b].in(i)) values(b, i, at);
                         if (b == NB - 1) release(at);
-                        if (more && t.b[b].in(i + 1)) scores(b, k);
+                        if (more && t.b[b].in(i + 1)) scores(b, i + 1, k);
                     }
                     if (more) release(at);
                 }
@@ -409,15 +489,14 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
             for (int b = 0; b < NB; b++) n[b] += t.b[b].hi - t.b[b].lo;
         }
         // every product issued has ended before the block frees its TMEM
-        if (tt_elect()) {
-            tc_commit(&bars->done);
-            (void)mbar_wait(&bars->done, 0, TT_WAIT_NS);
+        tc_commit(&bars->done);
+        (void)mbar_wait(&bars->done, 0, TT_WAIT_NS);
         }
         __syncwarp();
-    } else if (warp == NB * 4 + 2) {  // ---- which item comes next
+    } else if (warp == WARPS + 2) {  // ---- which item comes next
         if (blockIdx.x == 0) prompt_check(a, lane, 32);
         int count = 0;
-        auto give = [&](const PtItem& x) {
+        auto give = [&](const PtItem<NB>& x) {
             const int s = count % PT_RING;
             if (count >= PT_RING && !all(&bars->item_empty[s], count / PT_RING - 1)) return false;
             if (lane == 0) {
@@ -434,136 +513,138 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
             const int c = round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
             const int x = round * gridDim.x + c;
             if (x >= items) continue;
-            PtItem p;
+            PtItem<NB> p;
             p.it = prompt_item(a, a.slots - 1 - x / a.K);
             p.head = x % a.K;
             p.more = 1;
+            p.t.set(a, p.it, tpb);
             if (p.it.rows > 0) ok = give(p);
         }
-        PtItem end = {};
+        PtItem<NB> end = {};
         if (ok) give(end);
     } else {  // ---- values that are not finite, in mixed tiles
+        const int halves = HALVES == 1 || a.D <= 128 ? 1 : HALVES;
         int looks = 0;
+        uint32_t used = 0;  // stages before this item
         bool ok = true;
-        while (ok && next()) {
-            const PtTiles<NB> t(a, now.it, tpb);
-            const int halves = HALVES == 1 || a.D <= 128 ? 1 : HALVES;
-            if (t.lo < t.hi) at.skip(halves, STAGES);
+        while (const PtItem<NB>* item = ok ? next() : nullptr) {
+            const PtTiles<NB> t = item->t;
+            done();
             for (int i = t.lo; i < t.hi && ok; i++) {
-                const bool more = i + 1 < t.hi;
-                if (NB == 1 && more) at.skip(halves, STAGES);
-                if (t.mixed(i)) {
-                    uint32_t bits = 0;
-                    constexpr uint32_t e = BF ? 0x7f807f80u : 0x7c007c00u;
-                    constexpr uint32_t one = BF ? 0x00800080u : 0x04000400u;
-                    TtPlace x = at;
-                    // asked for once the stage's copy before is over: its phase cannot be
-                    // taken for the one before, and the stage is held until P is there
-                    ok = all(&bars->ask[looks % PT_LOOKS], looks / PT_LOOKS);
-                    for (int h = 0; h < halves && ok; h++, x.next(STAGES)) {
-                        ok = all(&bars->full[x.stage], x.phase);
-                        const uint8_t* v = ring + x.stage * STAGE;
-                        const int n = min(COLS, (a.D - h * 128 + 63) / 64) * PT_KEYS * 128;
+                if (i == t.all0 && i < t.all1) i = t.all1;
+                if (i >= t.hi) break;
+                uint32_t bits = 0;
+                constexpr uint32_t e = BF ? 0x7f807f80u : 0x7c007c00u;
+                constexpr uint32_t one = BF ? 0x00800080u : 0x04000400u;
+                TtPlace x = pt_place<STAGES>(used + t.before(i) * halves);
+                // asked for once the stage's copy before is over: its phase cannot be taken
+                // for the one before, and the stage is held until P is there
+                ok = all(&bars->ask[looks % PT_LOOKS], looks / PT_LOOKS);
+                for (int h = 0; h < halves && ok; h++, x.next(STAGES)) {
+                    ok = all(&bars->full[x.stage], x.phase);
+                    const uint8_t* v = ring + x.stage * STAGE;
+                    const int n = min(COLS, (a.D - h * 128 + 63) / 64) * PT_KEYS * 128;
 #pragma unroll 4
-                        for (int o = lane * 16; o < n; o += 512) {
-                            const uint4 w = *(const uint4*)(v + o);
-                            // all exponent bits set: one more carries into the sign's place
-                            bits |= ((w.x & e) + one) | ((w.y & e) + one) | ((w.z & e) + one) |
-                                    ((w.w & e) + one);
-                        }
+                    for (int o = lane * 16; o < n; o += 512) {
+                        const uint4 w = *(const uint4*)(v + o);
+                        // all exponent bits set: one more carries into the sign's place
+                        bits |= ((w.x & e) + one) | ((w.y & e) + one) | ((w.z & e) + one) |
+                                ((w.w & e) + one);
                     }
-                    const bool odd = __any_sync(FULL, (bits & 0x80008000u) != 0);
-                    if (lane == 0) {
-                        bars->odd[looks % PT_LOOKS] = odd;
-                        mbar_arrive(&bars->look[looks % PT_LOOKS]);
-                    }
-                    __syncwarp();
-                    looks++;
                 }
-                at.skip(halves, STAGES);
-                if (NB == 2 && more) at.skip(halves, STAGES);
+                const bool odd = __any_sync(FULL, (bits & 0x80008000u) != 0);
+                if (lane == 0) {
+                    bars->odd[looks % PT_LOOKS] = odd;
+                    mbar_arrive(&bars->look[looks % PT_LOOKS]);
+                }
+                __syncwarp();
+                looks++;
             }
+            used += 2 * (t.hi - t.lo) * halves;
         }
     }
-    } else {  // ---- softmax: a thread per row
-        if constexpr (NB == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int b = warp >> 2, m = tid & 127;
+    } else {  // ---- softmax: two threads to a row, half of a tile's keys each
+        const int b = warp >> 3, half = warp >> 2 & 1, m = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + b * TCOLS + ((uint32_t)(warp & 3) << 21);
         const uint32_t t_o = lanes + SB * PT_KEYS;
         const float log2e = 1.44269504088896341f;
         const bool cap = a.softcap > 0.f;
         const float c2 = cap ? log2e : a.scale * log2e;
         const float y2 = cap ? 2.f * log2e * a.scale / a.softcap : 0.f;
-        // a score with the cap: tanh(y) = 1 - 2 / (1 + e^2y), off by 2^-22, times
-        // softcap far below one rounding of the weight
-        auto capped = [&](float s) {
-            const float y = s * y2;
-            return a.softcap - __fdividef(2.f * a.softcap, 1.f + tt_exp2(y > 120.f ? 120.f : y));
-        };
-        const int tok = b * tpb + m / a.G, g = m - m / a.G * a.G;  // of the item; query head
+        const int tok = b * tpb + m / a.G;  // of the item
         const bool mine = m < tpb * a.G;
+        const int halves = HALVES == 1 || a.D <= 128 ? 1 : HALVES;
+        // a wait that gives up sets `failed`: later ones return at once, and the next item
+        // is the last
+        auto pass = [&](uint64_t* bar, uint32_t parity) {
+            (void)wait(bar, parity);
+            __syncwarp();
+            tc_fence_after();
+        };
+        // the row's two warps meet
+        auto meet = [&]() {
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + b * 4 + (warp & 3)) : "memory");
+        };
         int n = 0, looks = 0;
-        bool ok = true;
-        while (ok && next()) {
-            const PtTiles<NB> t(a, now.it, tpb);
-            const PtBlock& blk = t.b[b];
-            const bool row = mine && tok < now.it.rows;
-            const bool work = __any_sync(FULL, row);
-            const int lim = row ? min(now.it.past + tok, now.it.keys - 1) : -1;
-            const int low = a.window > 0 ? max(0, now.it.past + tok - a.window + 1) : 0;
+        uint32_t used = 0;  // stages before this item
+        while (const PtItem<NB>* x = next()) {
+            const PtBlock blk = x->t.b[b];
+            const bool row = mine && tok < x->it.rows;
+            const bool work = __any_sync(FULL, row);  // the same for the row's two warps
+            // the row sees keys [low, lim]
+            auto lim = [&]() { return row ? min(x->it.past + tok, x->it.keys - 1) : -1; };
+            auto low = [&]() { return a.window > 0 ? max(0, x->it.past + tok - a.window + 1) : 0; };
+            // running maximum of the scores, the weights' reference (in powers of two),
+            // and the sum of this thread's weights
             float top = -INFINITY, ref = -INFINITY, sum = 0.f;
-            const int halves = HALVES == 1 || a.D <= 128 ? 1 : HALVES;
-            TtPlace v = at;  // of tile i's V
-            if (t.lo < t.hi) v.skip(halves, STAGES);
-            for (int i = t.lo; i < t.hi && ok; i++) {
-                const bool more = i + 1 < t.hi, union_mixed = t.mixed(i);
-                if (NB == 1 && more) v.skip(halves, STAGES);
-                const int look = looks;
-                looks += union_mixed;
-                const TtPlace vi = v;
-                v.skip(halves * (NB == 2 && more ? 2 : 1), STAGES);
-                if (!blk.in(i)) continue;
+#pragma unroll 1
+            for (int i = blk.lo; i < blk.hi; i++, n++) {
                 const int sb = NB == 2 ? b : n & 1, kt = i * PT_KEYS;
                 const bool mixed = blk.mixed(i);
-                ok = all(&bars->s_full[sb], NB == 2 ? n : n >> 1);
-                tc_fence_after();
                 const uint32_t t_s = lanes + (NB == 2 ? 0 : sb * PT_KEYS);
+                float s[32], from = 0.f;  // scores of 32 keys
+                const uint32_t t_h = t_s + half * (PT_KEYS / 2);
+                pass(&bars->s_full[sb], NB == 2 ? n : n >> 1);
                 if (work) {
-                    float s[PT_KEYS];
-#pragma unroll
-                    for (int c = 0; c < PT_KEYS; c += 32) tt_ld32(t_s + c, (uint32_t*)s + c);
-#pragma unroll
-                    for (int c = 0; c < PT_KEYS; c += 32) tt_wait_ld32((uint32_t*)s + c);
-                    if (cap) {
-#pragma unroll
-                        for (int j = 0; j < PT_KEYS; j++) s[j] = capped(s[j]);
-                    }
-                    if (mixed) {
-#pragma unroll
-                        for (int j = 0; j < PT_KEYS; j++)
-                            if (j < low - kt || j > lim - kt) s[j] = -INFINITY;
-                    }
+                    // rare work on the scores in place, by calls: the code of every tile is
+                    // then fetched without jumps over it (16384 bf16 tokens: 2.04 ms with it
+                    // in line, 1.88 without it)
+                    if (cap) pt_cap(t_h, a.softcap, y2);
+                    if (mixed) pt_hide(t_h, low() - kt - half * 64, lim() - kt - half * 64);
                     float t0 = top, t1 = top, t2 = top, t3 = top;
+                    auto largest = [&]() {
 #pragma unroll
-                    for (int j = 0; j < PT_KEYS; j += 4) {
-                        t0 = fmaxf(t0, s[j]);
-                        t1 = fmaxf(t1, s[j + 1]);
-                        t2 = fmaxf(t2, s[j + 2]);
-                        t3 = fmaxf(t3, s[j + 3]);
-                    }
-                    top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+                        for (int j = 0; j < 32; j += 8) {
+                            t0 = pt_max3(t0, s[j], s[j + 1]);
+                            t1 = pt_max3(t1, s[j + 2], s[j + 3]);
+                            t2 = pt_max3(t2, s[j + 4], s[j + 5]);
+                            t3 = pt_max3(t3, s[j + 6], s[j + 7]);
+                        }
+                    };
+                    tt_load<32>(t_h, (uint32_t*)s);
+                    largest();
+                    tt_load<32>(t_h + 32, (uint32_t*)s);
+                    largest();
+                    top = pt_max3(pt_max3(t0, t1, t2), t3, t3);
+                    // a buffer of its own for each row block, or for each of two tiles
+                    // running: it is written again when the other thread has read it
+                    float(*at)[128] = bars->meet[sb];
+                    at[half][m] = top;
+                    tc_fence_before();
+                    meet();  // both have read their scores, too: weights may go over them
+                    tc_fence_after();
+                    top = pt_max3(top, at[half ^ 1][m], top);
                     const float want = top == -INFINITY ? -INFINITY : top * c2 - TT_LIFT<BF>;
                     if (i == blk.lo) {
                         ref = want;
-                    } else if (__any_sync(FULL, row && want - ref > 8.f)) {
+                    } else if (__any_sync(FULL, row && !(want - ref <= 8.f) && want != -INFINITY)) {
                         const float fix = ref == -INFINITY ? 0.f : tt_exp2(ref - want);
                         // O holds the tiles so far (two row blocks: since the scores came)
-                        if (NB == 1) ok = ok && all(&bars->pv[b], n - 1);
-                        tc_fence_after();
+                        if (NB == 1) pass(&bars->pv[b], n - 1);
                         sum *= fix;
                         ref = want;
 #pragma unroll 1
-                        for (int c = 0; c < a.D; c += 16) {
+                        for (int c = half * 16; c < a.D; c += 32) {
                             uint32_t o[16];
                             tt_load<16>(t_o + c, o);
 #pragma unroll
@@ -572,70 +653,99 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                             tt_st<16>(t_o + c, o);
                         }
                     }
-                    const float from = ref == -INFINITY ? 0.f : ref;
-                    float l0 = 0.f, l1 = 0.f;
+                    // a reference that is not finite makes every weight NaN
+                    from = ref == -INFINITY ? 0.f : ref + (ref - ref);
+                }
+                float l[4] = {};
+                uint32_t p[16];
+                auto weights = [&]() {  // of 32 keys
 #pragma unroll
-                    for (int c = 0; c < PT_KEYS; c += 64) {
-                        uint32_t p[32];
-#pragma unroll
-                        for (int j = 0; j < 64; j++) s[c + j] = tt_exp2(fmaf(s[c + j], c2, -from));
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            p[j] = tt_pack<BF>(s[c + 2 * j], s[c + 2 * j + 1], l0);
-                            p[j + 1] = tt_pack<BF>(s[c + 2 * j + 2], s[c + 2 * j + 3], l1);
-                        }
-                        tt_st<32>(t_s + c / 2, p);
+                    for (int j = 0; j < 32; j += 2) {
+                        const float y0 = tt_exp2(fmaf(s[j], c2, -from));
+                        const float y1 = tt_exp2(fmaf(s[j + 1], c2, -from));
+                        l[j & 3] += y0;
+                        l[j & 3 | 1] += y1;
+                        p[j >> 1] = pt_pack<BF>(y0, y1);
                     }
-                    sum += l0 + l1;
+                };
+                if (work) {
+                    // the second 32 keys first, whose weights may go over the first ones'
+                    // scores when those have been read again (kept, 96 registers a thread
+                    // were not enough)
+                    weights();
+                    tt_load<32>(t_h, (uint32_t*)s);
+                    tt_st<16>(t_s + half * 32 + 16, p);
                     tt_wait_st();
                 }
                 bool odd = false;
                 if (mixed) {
-                    ok = ok && all(&bars->look[look % PT_LOOKS], look / PT_LOOKS);
-                    odd = *(volatile uint32_t*)&bars->odd[look % PT_LOOKS];
-                    if (odd && ok && work) {
-                        const uint8_t* vt[2];
-                        TtPlace x = vi;
-                        for (int h = 0; h < halves; h++, x.next(STAGES)) {
-                            ok = ok && all(&bars->full[x.stage], x.phase);
-                            vt[h] = ring + x.stage * STAGE;
-                        }
-                        if (i > blk.lo) ok = ok && all(&bars->pv[b], n - 1);
-                        tc_fence_after();
-                        if (ok)
-                            pt_careful<BF>(t_s, t_o, vt, a.D, low - kt, lim - kt, i == blk.lo);
-                    }
+                    const int y = looks + x->t.looks(i);
+                    pass(&bars->look[y % PT_LOOKS], y / PT_LOOKS);
+                    odd = *(volatile uint32_t*)&bars->odd[y % PT_LOOKS];
+                    if ((warp & 7) == 0 && lane == 0) bars->skip[sb] = odd;
                 }
-                if ((warp & 3) == 0 && lane == 0) bars->skip[sb] = odd;
+                // the product starts when half of the weights are there
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->p_half[sb]);
+                if (work) {
+                    weights();
+                    tt_st<16>(t_s + half * 32, p);
+                    tt_wait_st();
+                    sum += (l[0] + l[1]) + (l[2] + l[3]);
+                }
+                if (odd) {
+                    const uint8_t* vt[2];
+                    TtPlace at = pt_place<STAGES>(used + x->t.before(i) * halves);
+                    for (int h = 0; h < halves; h++, at.next(STAGES)) {
+                        pass(&bars->full[at.stage], at.phase);
+                        vt[h] = ring + at.stage * STAGE;
+                    }
+                    if (i > blk.lo) pass(&bars->pv[b], n - 1);
+                    tc_fence_before();
+                    meet();  // the weights of both halves are there
+                    tc_fence_after();
+                    if (work)
+                        pt_careful<BF>(t_s, t_o, vt, a.D, half, low() - kt, lim() - kt,
+                                       i == blk.lo);
+                }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars->p_full[sb]);
-                n++;
             }
-            at = v;
+            looks += x->t.looks(x->t.hi);
+            used += 2 * (x->t.hi - x->t.lo) * halves;
             // ---- the item's end
             const bool none = blk.lo >= blk.hi;
             if (!none) {
-                ok = ok && all(&bars->pv[b], n - 1);
-                tc_fence_after();
+                pass(&bars->pv[b], n - 1);
+                if (work) {
+                    float(*at)[128] = bars->meet[NB == 2 ? b : 0];
+                    at[half][m] = sum;
+                    meet();
+                    sum += at[half ^ 1][m];
+                    meet();  // read before the next item's first tile
+                }
             }
-            if (!work || !ok) continue;
+            const int row0 = x->it.row0, head = x->head;
+            done();
+            if (!work) continue;
+            const int g = m - m / a.G * a.G;  // query head of the kv head
             const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
             uint16_t* out = (uint16_t*)a.out +
-                            ((long long)(now.it.row0 + tok) * a.H + now.head * a.G + g) * a.D;
+                            ((long long)(row0 + tok) * a.H + head * a.G + g) * a.D;
             const bool wide = ((uintptr_t)out & 31) == 0 && (a.D & 15) == 0;
 #pragma unroll 1
-            for (int c = 0; c < a.D; c += 16) {
+            for (int c = half * 16; c < a.D; c += 32) {
                 uint32_t o[16], w[8];
                 __syncwarp();
                 if (!none) tt_load<16>(t_o + c, o);
-                float unused = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; j++)
                     w[j] = none || inv == 0.f
                                ? 0u
-                               : tt_pack<BF>(__uint_as_float(o[2 * j]) * inv,
-                                             __uint_as_float(o[2 * j + 1]) * inv, unused);
+                               : pt_pack<BF>(__uint_as_float(o[2 * j]) * inv,
+                                             __uint_as_float(o[2 * j + 1]) * inv);
                 if (!row) continue;
                 if (wide) {
                     pt_store32(out + c, w);
