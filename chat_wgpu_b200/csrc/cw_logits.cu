@@ -3,15 +3,19 @@
 //
 //   x -> x / rep or x rep (seen)  -> (x - freq n) - pres (n > 0)  -> + bias  -> -inf (masked)
 //
-// Memory bound: a row is read and written once.  A cluster of CTAs takes a row, each a
-// slice of the vocabulary.  A CTA first goes through the row's whole history and counts
-// the tokens of its own slice in shared memory (whole-number atomics, so their order does
-// not matter; the history is short and comes from L2 after the first CTA), and notes the
-// last bias entry of each.  Then it streams its slice.  The argmax is joined over the
-// cluster through distributed shared memory: no word outside the row's own outputs is
-// written, so calls and graph replays share nothing.
+// Memory bound: a row is read and written once, but for logits in 16 bytes of which no
+// token is allowed, which are not read.  A cluster of CTAs takes a row, each a slice of the
+// vocabulary.  A CTA asks for its first logits, then goes through the row's whole lists and
+// counts the tokens of its own slice in shared memory (whole-number atomics, so their order
+// does not matter; the lists are short and come from L2 after the first CTA).  A bit for each
+// listed token says where to look, and the number of bits before it where its count and its
+// last bias entry are: memory goes by the lists' length, not by the vocabulary's.  Then it
+// streams its slice, 8 or 4 logits to a look at the bits.  The argmax is joined over the cluster through distributed
+// shared memory: no word outside the row's own outputs is written, so calls and graph
+// replays share nothing.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
+#include <limits.h>
 
 #include <algorithm>
 
@@ -30,11 +34,13 @@ struct LogitArgs {
     uint32_t* best;
     long long stride;
     int n_rows, vocab, n_tokens, n_bias, n_masks, words;
-    int slice;  // vocabulary entries of a CTA's slice, a multiple of 16
+    int slice;  // vocabulary entries of a CTA's slice, a multiple of 32
     int* status;
 };
 
 constexpr int LG_THREADS = 512;
+constexpr int LG_DEEP = 3;  // 16-byte vectors of a thread in flight
+constexpr int LG_TOKENS = 4096;  // distinct tokens of a row's lists in a slice that there is room for
 constexpr uint32_t LG_LED = 1u << 31;  // in the history's prompt part; the low bits count the rest
 
 __device__ __forceinline__ void lg_bad(const LogitArgs& a) {
@@ -55,6 +61,7 @@ __device__ __forceinline__ void lg_list(const LogitArgs& a, const int* starts, i
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(LG_THREADS) k_adjust_logits(const __grid_constant__ LogitArgs a) {
     constexpr int VEC = WIDE ? 16 / sizeof(T) : 1;
+    constexpr uint32_t EVERY = (1u << VEC) - 1;
     typedef typename VecOf<VEC * sizeof(T)>::type V;
     union Pack {
         V v;
@@ -62,16 +69,55 @@ __global__ void __launch_bounds__(LG_THREADS) k_adjust_logits(const __grid_const
     };
     extern __shared__ __align__(16) uint32_t sm[];
     __shared__ unsigned long long s_key[LG_THREADS / 32], s_all[16];
+    __shared__ int s_sum[LG_THREADS / 32];
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     if (a.best) cluster.barrier_arrive();  // waited for before a CTA writes to another's memory
     const int tid = threadIdx.x, r = blockIdx.y, cta = blockIdx.x, ctas = gridDim.x;
-    uint32_t* s_count = sm;            // [slice]
-    uint32_t* s_bias = sm + a.slice;   // [slice] last entry of the token, counted from 1
+    const int words = a.slice / 32;
+    uint32_t* s_bits = sm;                // [words] the token is in one of the lists
+    uint32_t* s_rank = s_bits + words;    // [words] bits set before the word
+    uint32_t* s_count = s_rank + words;   // [LG_TOKENS] of the listed tokens, in order
+    uint32_t* s_last = s_count + LG_TOKENS;  // and their last bias entry, counted from 1
     pdl_wait();
+    pdl_trigger();
     const T* in = (const T*)a.logits + r * a.stride;
     T* out = (T*)a.out + (long long)r * a.vocab;
     const int shift = WIDE ? (int)(((uintptr_t)in & 15) / sizeof(T)) : 0;
+    const int end = a.vocab + shift;
+    const uint32_t* mask = nullptr;
+    if (a.masks) {
+        const int m = a.mask_rows ? a.mask_rows[r] : r;
+        if (m >= a.n_masks) {
+            if (cta == 0 && tid == 0) lg_bad(a);
+        } else if (m >= 0) {
+            mask = a.masks + (size_t)m * a.words;
+        }
+    }
+    // which of the VEC tokens from position u (all in the vocabulary) are allowed
+    auto allowed = [&](int u) -> uint32_t {
+        if (!mask) return EVERY;
+        const int v = u - shift, w = v >> 5, x = v & 31;
+        uint32_t bits = mask[w] >> x;
+        if (x + VEC > 32) bits |= mask[w + 1] << (32 - x);
+        return bits & EVERY;
+    };
+    auto whole = [&](int u) { return u >= shift && u + VEC <= end; };
+    // a thread's next LG_DEEP vectors; one without an allowed token is not read
+    Pack p[LG_DEEP];
+    uint32_t on[LG_DEEP];
+    auto load = [&](int u, int u1) {
+#pragma unroll
+        for (int i = 0; i < LG_DEEP; i++) {
+            const int x = u + i * LG_THREADS * VEC;
+            on[i] = x < u1 && whole(x) ? allowed(x) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < LG_DEEP; i++)
+            if (on[i]) p[i].v = *(const V*)(in + (u + i * LG_THREADS * VEC - shift));
+    };
+    const int first = cta * a.slice;
+    load(first + tid * VEC, min(first + a.slice, end));  // in flight while the lists are read
     float rep = 1.f, freq = 0.f, pres = 0.f;
     int h0 = 0, h1 = 0, lead = 0, b0 = 0, b1 = 0;
     if (a.penalties) {
@@ -83,93 +129,164 @@ __global__ void __launch_bounds__(LG_THREADS) k_adjust_logits(const __grid_const
         if (rep == 1.f && freq == 0.f && pres == 0.f) h1 = h0;
     }
     if (a.bias_starts) lg_list(a, a.bias_starts, r, a.n_bias, b0, b1, cta == 0 && tid == 0);
-    const uint32_t* mask = nullptr;
-    if (a.masks) {
-        const int m = a.mask_rows ? a.mask_rows[r] : r;
-        if (m >= a.n_masks) {
-            if (cta == 0 && tid == 0) lg_bad(a);
-        } else if (m >= 0) {
-            mask = a.masks + (size_t)m * a.words;
-        }
-    }
     const bool hist = h1 > h0, bias = b1 > b0;
     float top = -3.402823e38f;
     unsigned at = 0;
-    for (long long base = (long long)cta * a.slice; base < (long long)a.vocab + shift;
-         base += (long long)ctas * a.slice) {
-        const int u0 = (int)base, u1 = (int)min(base + a.slice, (long long)a.vocab + shift);
+    // f(place in [u0, u1), entry) for the tokens [x, y) of a list that lie there
+    int u0 = 0, u1 = 0;
+    auto each = [&](const int* tokens, int x, int y, auto f) {
+        for (int i = x + tid; i < y; i += 4 * LG_THREADS) {
+            int t[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                t[k] = i + k * LG_THREADS < y ? tokens[i + k * LG_THREADS] : INT_MAX;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (i + k * LG_THREADS >= y) break;
+                if (t[k] < 0 || t[k] >= a.vocab) {
+                    if (cta == 0) lg_bad(a);
+                } else if (t[k] + shift >= u0 && t[k] + shift < u1) {
+                    f(t[k] + shift - u0, i + k * LG_THREADS);
+                }
+            }
+        }
+    };
+    auto rank = [&](int j) {  // which of the listed tokens the one at place j is
+        return s_rank[j >> 5] + __popc(s_bits[j >> 5] & ((1u << (j & 31)) - 1));
+    };
+    int step = a.slice;  // entries at a time
+    bool loaded = true;  // the first vectors are there
+    for (long long base = first; base < end;) {
+        u0 = (int)base;
+        u1 = (int)min(base / a.slice * a.slice + a.slice, (long long)end);  // of the slice
+        u1 = min(u1, u0 + step);
         if (hist || bias) {
-            __syncthreads();  // the slice before has been read
-            for (int i = tid; i < a.slice / 4; i += LG_THREADS) {
-                if (hist) ((uint4*)s_count)[i] = make_uint4(0, 0, 0, 0);
-                if (bias) ((uint4*)s_bias)[i] = make_uint4(0, 0, 0, 0);
+            __syncthreads();  // what went before has been read
+            for (int i = tid; i < words; i += LG_THREADS) s_bits[i] = 0;
+            __syncthreads();
+            auto mark = [&](int j, int) {
+                const uint32_t bit = 1u << (j & 31);
+                if (!(*(volatile uint32_t*)&s_bits[j >> 5] & bit)) atomicOr(&s_bits[j >> 5], bit);
+            };
+            each(a.tokens, h0, h1, mark);
+            each(a.bias_tokens, b0, b1, mark);
+            __syncthreads();
+            // ranks: a thread's words, then its place among the threads
+            const int per = (words + LG_THREADS - 1) / LG_THREADS;
+            int mine = 0;
+            for (int i = tid * per; i < min(words, tid * per + per); i++) mine += __popc(s_bits[i]);
+            int incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(FULL, incl, o);
+                if ((tid & 31) >= o) incl += x;
+            }
+            if ((tid & 31) == 31) s_sum[tid >> 5] = incl;
+            __syncthreads();
+            int before = 0, total = 0;
+            for (int w = 0; w < LG_THREADS / 32; w++) {
+                if (w == tid >> 5) before = total;
+                total += s_sum[w];
+            }
+            if (total > LG_TOKENS) {  // more listed tokens than there is room for: in pieces
+                step = LG_TOKENS;
+                loaded = false;
+                continue;
+            }
+            before += incl - mine;
+            for (int i = tid * per; i < min(words, tid * per + per); i++) {
+                s_rank[i] = before;
+                before += __popc(s_bits[i]);
+            }
+            for (int i = tid; i < total; i += LG_THREADS) {
+                s_count[i] = 0;
+                if (a.bias_starts) s_last[i] = 0;
             }
             __syncthreads();
-            for (int i = h0 + tid; i < h1; i += LG_THREADS) {
-                const int t = a.tokens[i];
-                if (t < 0 || t >= a.vocab) {
-                    if (cta == 0) lg_bad(a);
-                    continue;
-                }
-                const int u = t + shift;
-                if (u < u0 || u >= u1) continue;
-                if (i - h0 < lead) atomicOr(&s_count[u - u0], LG_LED);
-                else atomicAdd(&s_count[u - u0], 1u);
-            }
-            for (int i = b0 + tid; i < b1; i += LG_THREADS) {
-                const int t = a.bias_tokens[i];
-                if (t < 0 || t >= a.vocab) {
-                    if (cta == 0) lg_bad(a);
-                    continue;
-                }
-                const int u = t + shift;
-                if (u >= u0 && u < u1) atomicMax(&s_bias[u - u0], (unsigned)(i - b0) + 1u);
-            }
+            each(a.tokens, h0, h1, [&](int j, int i) {
+                if (i - h0 < lead) atomicOr(&s_count[rank(j)], LG_LED);
+                else atomicAdd(&s_count[rank(j)], 1u);
+            });
+            each(a.bias_tokens, b0, b1,
+                 [&](int j, int i) { atomicMax(&s_last[rank(j)], (unsigned)(i - b0) + 1u); });
             __syncthreads();
         }
+        auto listed = [&](int u) -> uint32_t {  // of the VEC tokens from position u
+            if (!hist && !bias) return 0;
+            return s_bits[(u - u0) >> 5] >> ((u - u0) & 31) & EVERY;
+        };
         // one logit; each step is rounded by itself, as the definition says
-        auto adjust = [&](T x, int u) {
+        auto adjust = [&](T x, int u, bool in_list, bool is_on) {
             float y = rp_f32(x);
-            if (hist) {
-                const uint32_t c = s_count[u - u0];
+            if (in_list) {
+                const int k = rank(u - u0);
+                const uint32_t c = hist ? s_count[k] : 0, e = bias ? s_last[k] : 0;
                 if (c) {
                     y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
                     const uint32_t n = c & ~LG_LED;
                     if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, (float)n)), pres);
                 }
-            }
-            if (bias) {
-                const uint32_t i = s_bias[u - u0];
-                if (i) y = __fadd_rn(y, a.bias_values[b0 + (int)i - 1]);
-            }
-            if (mask) {
-                const int v = u - shift;
-                if (!(mask[v >> 5] >> (v & 31) & 1)) y = -INFINITY;
+                if (e) y = __fadd_rn(y, a.bias_values[b0 + (int)e - 1]);
             }
             T z;
-            rp_set(&z, y);
-            y = rp_f32(z);
-            if (y > top) {  // positions ascend in a thread: the lowest of equals stays
+            rp_set(&z, is_on ? y : -INFINITY);
+            return z;
+        };
+        auto better = [&](float y, int u) {  // positions ascend in a thread: the lowest of equals
+            if (y > top) {
                 top = y;
                 at = (unsigned)(u - shift);
             }
-            return z;
         };
-        for (int u = u0 + tid * VEC; u < u1; u += LG_THREADS * VEC) {
-            if (u >= shift && u + VEC <= a.vocab + shift) {
-                Pack p;
-                p.v = *(const V*)(in + (u - shift));
+        for (int u = u0 + tid * VEC; u < u1; u += LG_DEEP * LG_THREADS * VEC) {
+            if (!loaded) load(u, u1);
+            loaded = false;
 #pragma unroll
-                for (int i = 0; i < VEC; i++) p.e[i] = adjust(p.e[i], u + i);
-                *(V*)(out + (u - shift)) = p.v;
-            } else {
-                for (int i = 0; i < VEC; i++)
-                    if (u + i >= shift && u + i < a.vocab + shift)
-                        out[u + i - shift] = adjust(in[u + i - shift], u + i);
+            for (int i = 0; i < LG_DEEP; i++) {
+                const int x = u + i * LG_THREADS * VEC;
+                if (x >= u1) break;
+                if (!whole(x)) {  // the row's ends
+                    for (int j = x; j < x + VEC; j++) {
+                        if (j < shift || j >= end) continue;
+                        const int v = j - shift;
+                        const bool is_on = !mask || (mask[v >> 5] >> (v & 31) & 1);
+                        const bool in_list = (hist || bias) && (s_bits[(j - u0) >> 5] >> ((j - u0) & 31) & 1);
+                        const T z = adjust(in[v], j, in_list, is_on);
+                        better(rp_f32(z), j);
+                        out[v] = z;
+                    }
+                    continue;
+                }
+                const uint32_t list = listed(x);
+                bool changed = a.out != a.logits;
+                if (!on[i]) {
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) rp_set(&p[i].e[j], -INFINITY);
+                    changed = true;
+                } else {
+                    if (list || on[i] != EVERY) {
+                        changed = true;
+#pragma unroll
+                        for (int j = 0; j < VEC; j++)
+                            p[i].e[j] = adjust(p[i].e[j], x + j, list >> j & 1, on[i] >> j & 1);
+                    }
+                    if (a.best) {
+                        float m = rp_f32(p[i].e[0]);
+#pragma unroll
+                        for (int j = 1; j < VEC; j++) m = fmaxf(m, rp_f32(p[i].e[j]));
+                        if (m > top) {
+#pragma unroll
+                            for (int j = 0; j < VEC; j++) better(rp_f32(p[i].e[j]), x + j);
+                        }
+                    }
+                }
+                if (changed) *(V*)(out + (x - shift)) = p[i].v;
             }
         }
+        loaded = false;
+        // the next piece of the slice, or the CTA's next slice
+        base = u1 < end && u1 % a.slice ? u1 : base / a.slice * a.slice + (long long)ctas * a.slice;
     }
-    pdl_trigger();
     if (!a.best) return;
     unsigned long long key = argmax_key_init();
     if (top > -3.402823e38f) key = argmax_key(top, at);
@@ -193,12 +310,15 @@ __global__ void __launch_bounds__(LG_THREADS) k_adjust_logits(const __grid_const
 
 template <typename T> static int adjust_launch(cw_ctx* ctx, LogitArgs& a, bool wide) {
     auto kern = wide ? k_adjust_logits<T, true> : k_adjust_logits<T, false>;
-    // up to 16 CTAs to a row (one cluster), no slice shorter than a pass of the threads
-    const int span = a.vocab + 16, ctas = std::max(1, std::min(16, span / (LG_THREADS * 4)));
-    const int most = a.bias_starts ? 24 * 1024 : 48 * 1024;  // 192 KB of shared memory
-    a.slice = std::min(most, ((span + ctas - 1) / ctas + 15) / 16 * 16);
-    const size_t smem = (size_t)a.slice * 4 * (a.bias_starts ? 2 : a.penalties ? 1 : 0);
-    CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 192 * 1024));
+    // up to 16 CTAs to a row (one cluster), no slice shorter than a pass of the threads; with
+    // many rows fewer, so that a row's lists are gone through less often (two rounds of the
+    // four CTAs that fit an SM)
+    const int span = a.vocab + 16, many = std::max(1, 8 * ctx->sm_count / a.n_rows);
+    const int ctas = std::max(1, std::min({16, many, span / (LG_THREADS * 4)}));
+    a.slice = std::min(128 * 1024, ((span + ctas - 1) / ctas + 31) / 32 * 32);
+    const bool lists = a.penalties || a.bias_starts;
+    const size_t smem = lists ? a.slice / 4 + (size_t)LG_TOKENS * 4 * (a.bias_starts ? 2 : 1) : 0;
+    CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
     CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, a.n_rows);

@@ -32,10 +32,16 @@ struct NormRopeArgs {
 };
 
 constexpr int NR_THREADS = 256;
-constexpr int NR_UNROLL = 2;  // heads whose loads are in flight while two others are worked on
+// A head's loads are in flight while the one before is worked on, three blocks to an SM and
+// at most 12 heads to a lane: 32768 bf16 rows of 32 + 8 + 8 heads in 168 us (872 MB, 5.2
+// TB/s).  Two heads at a time took 175 us, four blocks an SM (64 registers) 191, 64 heads to
+// a lane 189.
+constexpr int NR_PER = 12;
 
-template <typename T, int VEC, int C, bool HALF>
-__global__ void __launch_bounds__(NR_THREADS) k_norm_rope(const __grid_constant__ NormRopeArgs a) {
+// ALL: every lane's chunks are whole (L * C chunks of 2 * VEC elements make a head row).
+template <typename T, int VEC, int C, bool HALF, bool ALL>
+__global__ void __launch_bounds__(NR_THREADS, C == 1 ? 3 : 1)
+    k_norm_rope(const __grid_constant__ NormRopeArgs a) {
     typedef typename VecOf<VEC * sizeof(T)>::type V;
     union Row {
         V v[2 * C];
@@ -60,6 +66,7 @@ __global__ void __launch_bounds__(NR_THREADS) k_norm_rope(const __grid_constant_
         e1[i] = turn[i] && HALF ? e0[i] + a.rot / 2 : e0[i] + VEC;
     }
     pdl_wait();
+    pdl_trigger();
     const long long pos = a.positions[t];
     long long slot = -1, dst0 = 0;
     if (a.slots) {
@@ -84,100 +91,95 @@ __global__ void __launch_bounds__(NR_THREADS) k_norm_rope(const __grid_constant_
                                        : v + (h - a.H - a.K) * a.D;
 #pragma unroll
         for (int j = 0; j < C; j++) {
-            if (e0[j] < a.D) w.v[2 * j] = *(const V*)(src + e0[j]);
-            if (e1[j] < a.D) w.v[2 * j + 1] = *(const V*)(src + e1[j]);
+            if (ALL || e0[j] < a.D) w.v[2 * j] = *(const V*)(src + e0[j]);
+            if (ALL || e1[j] < a.D) w.v[2 * j + 1] = *(const V*)(src + e1[j]);
         }
     };
-    Row w[NR_UNROLL];
+    Row w;
 #pragma unroll
-    for (int u = 0; u < NR_UNROLL; u++) {
-#pragma unroll
-        for (int i = 0; i < 2 * VEC * C; i++) rp_set(&w[u].e[i], 0.f);
-        load(u, w[u]);
-    }
+    for (int i = 0; i < 2 * VEC * C; i++) rp_set(&w.e[i], 0.f);
+    load(0, w);
     float cs[C * VEC], sn[C * VEC];
 #pragma unroll
     for (int j = 0; j < C; j++)
         if (turn[j]) rotary_sines<T, VEC>(a.steps + (sub + j * L) * VEC, pos, a.amp, cs + j * VEC, sn + j * VEC);
     float gain[2 * VEC * C];
-    const float* held = nullptr;  // the weights in `gain`
-    for (int i0 = 0; i0 < a.per; i0 += NR_UNROLL) {
+    const float* held = nullptr;  // the weights in `gain`; without any, ones
+    const float unit = a.unit ? 1.f : 0.f;
 #pragma unroll
-        for (int u = 0; u < NR_UNROLL; u++) {
-            const int h = g + (i0 + u) * a.groups;
-            Row y = w[u];
-            load(i0 + NR_UNROLL + u, w[u]);  // in flight while this head is worked on
-            // the same for all lanes of a group: every lane of the warp meets the shuffles
-            const bool on = i0 + u < a.per && h < a.heads;
-            const bool norm = on && h < a.H + a.K && (h < a.H ? a.q_norm : a.k_norm);
-            float r = 1.f;
-            if (__any_sync(FULL, norm)) {
-                float s = 0.f;
+    for (int i = 0; i < 2 * VEC * C; i++) gain[i] = 1.f;
+    for (int i = 0; i < a.per; i++) {
+        const int h = g + i * a.groups;
+        Row y = w;
+        load(i + 1, w);  // in flight while this head is worked on
+        // the same for all lanes of a group: every lane of the warp meets the shuffles
+        const bool on = h < a.heads;
+        const bool norm = on && h < a.H + a.K && (h < a.H ? a.q_norm : a.k_norm);
+        float r = 1.f;
+        if (__any_sync(FULL, norm)) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < C; j++)
+#pragma unroll
+                for (int i = 0; i < 2 * VEC; i++) {
+                    const float x = rp_f32(y.e[2 * VEC * j + i]);
+                    if (ALL || (i < VEC ? e0[j] : e1[j]) < a.D) s = fmaf(x, x, s);
+                }
+            for (int o = L >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(FULL, s, o);
+            // (16-bit values: the fast root is off by 2^-22)
+            if (norm) r = sizeof(T) == 2 ? rsqrtf(s / (float)a.D + a.eps)
+                                         : 1.f / sqrtf(s / (float)a.D + a.eps);
+        }
+        if (!on || !live) continue;
+        if (h < a.H + a.K) {
+            const float* want = h < a.H ? a.q_norm : a.k_norm;
+            if (want != held) {
+                held = want;
 #pragma unroll
                 for (int j = 0; j < C; j++)
 #pragma unroll
                     for (int i = 0; i < 2 * VEC; i++) {
-                        const float x = rp_f32(y.e[2 * VEC * j + i]);
-                        if ((i < VEC ? e0[j] : e1[j]) < a.D) s = fmaf(x, x, s);
+                        const int e = i < VEC ? e0[j] + i : e1[j] + i - VEC;
+                        gain[2 * VEC * j + i] = want && (ALL || e < a.D) ? want[e] + unit : 1.f;
                     }
-                for (int o = L >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(FULL, s, o);
-                if (norm) r = 1.f / sqrtf(s / (float)a.D + a.eps);
             }
-            if (!on || !live) continue;
-            if (h < a.H + a.K) {
-                const float* want = h < a.H ? a.q_norm : a.k_norm;
-                if (norm && want != held) {
 #pragma unroll
-                    for (int j = 0; j < C; j++)
+            for (int j = 0; j < C; j++) {
+                float x[2 * VEC];
 #pragma unroll
-                        for (int i = 0; i < 2 * VEC; i++) {
-                            const int e = i < VEC ? e0[j] + i : e1[j] + i - VEC;
-                            gain[2 * VEC * j + i] =
-                                e < a.D ? (a.unit ? 1.f + want[e] : want[e]) : 0.f;
-                        }
-                    held = want;
-                }
+                for (int i = 0; i < 2 * VEC; i++)
+                    x[i] = rp_f32(y.e[2 * VEC * j + i]) * r * gain[2 * VEC * j + i];
+                if (turn[j]) {
 #pragma unroll
-                for (int j = 0; j < C; j++) {
-                    float x[2 * VEC];
-#pragma unroll
-                    for (int i = 0; i < 2 * VEC; i++) {
-                        x[i] = rp_f32(y.e[2 * VEC * j + i]);
-                        if (norm) x[i] = x[i] * r * gain[2 * VEC * j + i];
+                    for (int i = 0; i < VEC; i++) {
+                        const int p0 = HALF ? i : 2 * i, p1 = HALF ? VEC + i : 2 * i + 1;
+                        const float c = cs[j * VEC + i], s = sn[j * VEC + i];
+                        const float x0 = x[p0], x1 = x[p1];
+                        x[p0] = x0 * c - x1 * s;
+                        x[p1] = x1 * c + x0 * s;
                     }
-                    if (turn[j]) {
-#pragma unroll
-                        for (int i = 0; i < VEC; i++) {
-                            const int p0 = HALF ? i : 2 * i, p1 = HALF ? VEC + i : 2 * i + 1;
-                            const float c = cs[j * VEC + i], s = sn[j * VEC + i];
-                            const float x0 = x[p0], x1 = x[p1];
-                            x[p0] = x0 * c - x1 * s;
-                            x[p1] = x1 * c + x0 * s;
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 2 * VEC; i++) rp_set(&y.e[2 * VEC * j + i], x[i]);
                 }
-            }
-            auto put = [&](T* dst) {
 #pragma unroll
-                for (int j = 0; j < C; j++) {
-                    if (e0[j] < a.D) *(V*)(dst + e0[j]) = y.v[2 * j];
-                    if (e1[j] < a.D) *(V*)(dst + e1[j]) = y.v[2 * j + 1];
-                }
-            };
-            if (h < a.H) {
-                put((T*)a.q_out + ((long long)t * a.H + h) * a.D);
-            } else if (h < a.H + a.K) {
-                if (a.k_out) put((T*)a.k_out + ((long long)t * a.K + h - a.H) * a.D);
-                if (slot >= 0)
-                    put((T*)a.k_cache + dst0 + (long long)(h - a.H) * a.page * a.D);
-            } else if (slot >= 0) {
-                put((T*)a.v_cache + dst0 + (long long)(h - a.H - a.K) * a.page * a.D);
+                for (int i = 0; i < 2 * VEC; i++) rp_set(&y.e[2 * VEC * j + i], x[i]);
             }
         }
+        auto put = [&](T* dst) {
+#pragma unroll
+            for (int j = 0; j < C; j++) {
+                if (ALL || e0[j] < a.D) *(V*)(dst + e0[j]) = y.v[2 * j];
+                if (ALL || e1[j] < a.D) *(V*)(dst + e1[j]) = y.v[2 * j + 1];
+            }
+        };
+        if (h < a.H) {
+            put((T*)a.q_out + ((long long)t * a.H + h) * a.D);
+        } else if (h < a.H + a.K) {
+            if (a.k_out) put((T*)a.k_out + ((long long)t * a.K + h - a.H) * a.D);
+            if (slot >= 0)
+                put((T*)a.k_cache + dst0 + (long long)(h - a.H) * a.page * a.D);
+        } else if (slot >= 0) {
+            put((T*)a.v_cache + dst0 + (long long)(h - a.H - a.K) * a.page * a.D);
+        }
     }
-    pdl_trigger();
 }
 
 template <typename T, int VEC, int C>
@@ -187,15 +189,17 @@ static int norm_rope_go(cw_ctx* ctx, NormRopeArgs& a, bool half, int chunks) {
     // as many heads to a lane as still leave one full wave of threads
     const long long all = (long long)a.n_tokens * a.lanes * a.heads;
     const long long wave = (long long)ctx->sm_count * 2048;
-    a.per = (int)std::max<long long>(1, std::min<long long>(all / wave, a.heads));
-    if (a.per >= NR_UNROLL) a.per = a.per / NR_UNROLL * NR_UNROLL;
+    a.per = (int)std::max<long long>(1, std::min<long long>(all / wave, std::min(a.heads, NR_PER)));
     a.groups = (a.heads + a.per - 1) / a.per;
     const unsigned long long n = (unsigned long long)a.n_tokens * a.lanes * a.groups;
     const unsigned long long blocks = (n + NR_THREADS - 1) / NR_THREADS;
     CW_CHECK(blocks < (1ull << 31), CW_ERR_UNSUPPORTED, "cw_norm_rope: too many rows");
-    CW_TRY(launch_pdl(ctx, true,
-                      half ? k_norm_rope<T, VEC, C, true> : k_norm_rope<T, VEC, C, false>,
-                      dim3((unsigned)blocks), dim3(NR_THREADS), 0, a));
+    // (vectors narrower than 16 bytes, and several chunks to a lane, are rare: checked only)
+    constexpr bool CAN = C == 1 && VEC * sizeof(T) == 16;
+    auto kern = half ? k_norm_rope<T, VEC, C, true, false> : k_norm_rope<T, VEC, C, false, false>;
+    if (CAN && a.D == a.lanes * C * 2 * VEC && a.rot % (2 * VEC) == 0)
+        kern = half ? k_norm_rope<T, VEC, C, true, CAN> : k_norm_rope<T, VEC, C, false, CAN>;
+    CW_TRY(launch_pdl(ctx, true, kern, dim3((unsigned)blocks), dim3(NR_THREADS), 0, a));
     return check_launch("norm_rope");
 }
 // A head row in 32 lanes or fewer: one chunk each, or for long rows of narrow vectors several.
