@@ -59,7 +59,7 @@ __device__ __forceinline__ void lg_list(const LogitArgs& a, const int* starts, i
 // Positions u count from the 16-byte boundary at or before the row's first logit: logit
 // v is at u = v + shift, and slices and vectors start at multiples of VEC.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(LG_THREADS) k_adjust_logits(const __grid_constant__ LogitArgs a) {
+__global__ void __launch_bounds__(LG_THREADS, 2) k_adjust_logits(const __grid_constant__ LogitArgs a) {
     constexpr int VEC = WIDE ? 16 / sizeof(T) : 1;
     constexpr uint32_t EVERY = (1u << VEC) - 1;
     typedef typename VecOf<VEC * sizeof(T)>::type V;
@@ -78,7 +78,8 @@ __global__ void __launch_bounds__(LG_THREADS) k_adjust_logits(const __grid_const
     uint32_t* s_bits = sm;                // [words] the token is in one of the lists
     uint32_t* s_rank = s_bits + words;    // [words] bits set before the word
     uint32_t* s_count = s_rank + words;   // [LG_TOKENS] of the listed tokens, in order
-    uint32_t* s_last = s_count + LG_TOKENS;  // and their last bias entry, counted from 1
+    int* s_place = (int*)s_count + LG_TOKENS;  // where they are in the slice
+    uint32_t* s_last = s_count + 2 * LG_TOKENS;  // and their last bias entry, counted from 1
     pdl_wait();
     pdl_trigger();
     const T* in = (const T*)a.logits + r * a.stride;
@@ -156,10 +157,11 @@ __global__ void __launch_bounds__(LG_THREADS) k_adjust_logits(const __grid_const
     };
     int step = a.slice;  // entries at a time
     bool loaded = true;  // the first vectors are there
-    for (long long base = first; base < end;) {
-        u0 = (int)base;
-        u1 = (int)min(base / a.slice * a.slice + a.slice, (long long)end);  // of the slice
-        u1 = min(u1, u0 + step);
+    // pieces of the CTA's slices (positions stay below 2^30 + 16, sums of two below 2^31)
+    for (int slice0 = first, base = first; base < end;) {
+        u0 = base;
+        u1 = min(min(slice0 + a.slice, end), u0 + step);
+        int n_listed = 0;
         if (hist || bias) {
             __syncthreads();  // what went before has been read
             for (int i = tid; i < words; i += LG_THREADS) s_bits[i] = 0;
@@ -204,40 +206,33 @@ __global__ void __launch_bounds__(LG_THREADS) k_adjust_logits(const __grid_const
             }
             __syncthreads();
             each(a.tokens, h0, h1, [&](int j, int i) {
-                if (i - h0 < lead) atomicOr(&s_count[rank(j)], LG_LED);
-                else atomicAdd(&s_count[rank(j)], 1u);
+                const int k = rank(j);
+                s_place[k] = j;
+                if (i - h0 < lead) atomicOr(&s_count[k], LG_LED);
+                else atomicAdd(&s_count[k], 1u);
             });
-            each(a.bias_tokens, b0, b1,
-                 [&](int j, int i) { atomicMax(&s_last[rank(j)], (unsigned)(i - b0) + 1u); });
+            each(a.bias_tokens, b0, b1, [&](int j, int i) {
+                const int k = rank(j);
+                s_place[k] = j;
+                atomicMax(&s_last[k], (unsigned)(i - b0) + 1u);
+            });
+            n_listed = total;
             __syncthreads();
         }
         auto listed = [&](int u) -> uint32_t {  // of the VEC tokens from position u
             if (!hist && !bias) return 0;
             return s_bits[(u - u0) >> 5] >> ((u - u0) & 31) & EVERY;
         };
-        // one logit; each step is rounded by itself, as the definition says
-        auto adjust = [&](T x, int u, bool in_list, bool is_on) {
-            float y = rp_f32(x);
-            if (in_list) {
-                const int k = rank(u - u0);
-                const uint32_t c = hist ? s_count[k] : 0, e = bias ? s_last[k] : 0;
-                if (c) {
-                    y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-                    const uint32_t n = c & ~LG_LED;
-                    if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, (float)n)), pres);
-                }
-                if (e) y = __fadd_rn(y, a.bias_values[b0 + (int)e - 1]);
-            }
-            T z;
-            rp_set(&z, is_on ? y : -INFINITY);
-            return z;
-        };
-        auto better = [&](float y, int u) {  // positions ascend in a thread: the lowest of equals
-            if (y > top) {
+        auto is_on = [&](int v) { return !mask || (mask[v >> 5] >> (v & 31) & 1); };
+        auto better = [&](float y, int v) {  // the lowest index of equals
+            if (y > top || (y == top && (unsigned)v < at)) {
                 top = y;
-                at = (unsigned)(u - shift);
+                at = (unsigned)v;
             }
         };
+        // ---- all tokens as if none was listed; the listed ones are left out of the argmax
+        float most = -INFINITY;  // of the thread's vectors
+        int where = -1;
         for (int u = u0 + tid * VEC; u < u1; u += LG_DEEP * LG_THREADS * VEC) {
             if (!loaded) load(u, u1);
             loaded = false;
@@ -246,50 +241,71 @@ __global__ void __launch_bounds__(LG_THREADS) k_adjust_logits(const __grid_const
                 const int x = u + i * LG_THREADS * VEC;
                 if (x >= u1) break;
                 if (!whole(x)) {  // the row's ends
-                    for (int j = x; j < x + VEC; j++) {
-                        if (j < shift || j >= end) continue;
+                    for (int j = max(x, shift); j < min(x + VEC, end); j++) {
                         const int v = j - shift;
-                        const bool is_on = !mask || (mask[v >> 5] >> (v & 31) & 1);
-                        const bool in_list = (hist || bias) && (s_bits[(j - u0) >> 5] >> ((j - u0) & 31) & 1);
-                        const T z = adjust(in[v], j, in_list, is_on);
-                        better(rp_f32(z), j);
+                        T z = in[v];
+                        if (!is_on(v)) rp_set(&z, -INFINITY);
+                        else if (!((hist || bias) && (s_bits[(j - u0) >> 5] >> ((j - u0) & 31) & 1)))
+                            better(rp_f32(z), v);
                         out[v] = z;
                     }
                     continue;
                 }
-                const uint32_t list = listed(x);
-                bool changed = a.out != a.logits;
-                if (!on[i]) {
+                if (on[i] != EVERY) {
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) rp_set(&p[i].e[j], -INFINITY);
-                    changed = true;
-                } else {
-                    if (list || on[i] != EVERY) {
-                        changed = true;
-#pragma unroll
-                        for (int j = 0; j < VEC; j++)
-                            p[i].e[j] = adjust(p[i].e[j], x + j, list >> j & 1, on[i] >> j & 1);
-                    }
-                    if (a.best) {
-                        float m = rp_f32(p[i].e[0]);
-#pragma unroll
-                        for (int j = 1; j < VEC; j++) m = fmaxf(m, rp_f32(p[i].e[j]));
-                        if (m > top) {
-#pragma unroll
-                            for (int j = 0; j < VEC; j++) better(rp_f32(p[i].e[j]), x + j);
-                        }
-                    }
+                    for (int j = 0; j < VEC; j++)
+                        if (!(on[i] >> j & 1)) rp_set(&p[i].e[j], -INFINITY);
                 }
-                if (changed) *(V*)(out + (x - shift)) = p[i].v;
+                if (on[i] != EVERY || a.out != a.logits) *(V*)(out + (x - shift)) = p[i].v;
+                if (!a.best) continue;
+                const uint32_t list = listed(x);
+                if (list) {
+#pragma unroll
+                    for (int j = 0; j < VEC; j++)
+                        if (list >> j & 1) rp_set(&p[i].e[j], -INFINITY);
+                }
+                float m = rp_f32(p[i].e[0]);
+#pragma unroll
+                for (int j = 1; j < VEC; j++) m = fmaxf(m, rp_f32(p[i].e[j]));
+                if (m > most) {  // positions ascend: the first of equal vectors
+                    most = m;
+                    where = x;
+                }
             }
         }
+        if (where >= 0) {  // which of its tokens it was
+            Pack q;
+            q.v = *(const V*)(out + (where - shift));
+            const uint32_t list = listed(where);
+#pragma unroll
+            for (int j = VEC - 1; j >= 0; j--)
+                if (!(list >> j & 1) && rp_f32(q.e[j]) == most) better(most, where + j - shift);
+        }
+        // ---- the listed ones; each step is rounded by itself, as the definition says
+        if (n_listed) __syncthreads();
+        for (int k = tid; k < n_listed; k += LG_THREADS) {
+            const int v = s_place[k] + u0 - shift;
+            if (!is_on(v)) continue;
+            float y = rp_f32(in[v]);
+            const uint32_t c = hist ? s_count[k] : 0, e = bias ? s_last[k] : 0;
+            if (c) {
+                y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+                const uint32_t n = c & ~LG_LED;
+                if (n) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, (float)n)), pres);
+            }
+            if (e) y = __fadd_rn(y, a.bias_values[b0 + (int)e - 1]);
+            T z;
+            rp_set(&z, y);
+            better(rp_f32(z), v);
+            out[v] = z;
+        }
         loaded = false;
-        // the next piece of the slice, or the CTA's next slice
-        base = u1 < end && u1 % a.slice ? u1 : base / a.slice * a.slice + (long long)ctas * a.slice;
+        base = u1;
+        if (u1 == slice0 + a.slice) base = slice0 += ctas * a.slice;
     }
     if (!a.best) return;
     unsigned long long key = argmax_key_init();
-    if (top > -3.402823e38f) key = argmax_key(top, at);
+    if (top > -3.402823e38f) key = argmax_key(top, at);  // else index 0
     for (int o = 16; o; o >>= 1) {
         const unsigned long long x = __shfl_xor_sync(FULL, key, o);
         key = x > key ? x : key;
@@ -311,14 +327,14 @@ __global__ void __launch_bounds__(LG_THREADS) k_adjust_logits(const __grid_const
 template <typename T> static int adjust_launch(cw_ctx* ctx, LogitArgs& a, bool wide) {
     auto kern = wide ? k_adjust_logits<T, true> : k_adjust_logits<T, false>;
     // up to 16 CTAs to a row (one cluster), no slice shorter than a pass of the threads; with
-    // many rows fewer, so that a row's lists are gone through less often (two rounds of the
-    // four CTAs that fit an SM)
-    const int span = a.vocab + 16, many = std::max(1, 8 * ctx->sm_count / a.n_rows);
+    // many rows fewer, so that a row's lists are gone through less often (256 rows of 151936: 56
+    // us with two CTAs to a row, 68 with four, 63 with one)
+    const int span = a.vocab + 16, many = std::max(1, 4 * ctx->sm_count / a.n_rows);
     const int ctas = std::max(1, std::min({16, many, span / (LG_THREADS * 4)}));
     a.slice = std::min(128 * 1024, ((span + ctas - 1) / ctas + 31) / 32 * 32);
     const bool lists = a.penalties || a.bias_starts;
-    const size_t smem = lists ? a.slice / 4 + (size_t)LG_TOKENS * 4 * (a.bias_starts ? 2 : 1) : 0;
-    CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
+    const size_t smem = lists ? a.slice / 4 + (size_t)LG_TOKENS * 4 * (a.bias_starts ? 3 : 2) : 0;
+    CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024));
     CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, a.n_rows);
