@@ -117,11 +117,14 @@ struct cw_ctx {
     void* gemm_scratch = nullptr;
     size_t gemm_scratch_bytes = 0;
 
-    // grow-only scratch of the tree attention (partial states of split keys): the
-    // largest block, and the outgrown ones, which captured graphs may still name
+    // grow-only scratch of the tree attention (partial states of split keys) and of the
+    // prompt attention (operands as pairs): the largest blocks, and the outgrown ones, which
+    // captured graphs may still name
     void* tree_scratch = nullptr;
     size_t tree_scratch_bytes = 0;
-    std::vector<void*> tree_outgrown;
+    void* prompt_scratch = nullptr;
+    size_t prompt_scratch_bytes = 0;
+    std::vector<void*> outgrown;
 };
 
 namespace cw {
@@ -130,6 +133,12 @@ namespace cw {
 int buf_get(cw_ctx* ctx, cw_buf b, BufEntry** out, size_t min_bytes, const char* what);
 int buf_new(cw_ctx* ctx, size_t nbytes, int kind, cw_buf* out, BufEntry** entry = nullptr);
 int arena_get(cw_ctx* ctx, size_t len_f32, cw_buf* out, BufEntry** entry = nullptr);
+// A scratch block of the context of at least `need` bytes, in stream order (no wait).  It
+// comes from a pool of the process, which keeps what a context gives back: a plain
+// allocation of tens of MB takes longer than the calls.  An outgrown block stays until the
+// context goes, since a graph captured before may still write there; a new block is twice the
+// old one at least, so they add up to less than it.
+int stream_scratch(cw_ctx* ctx, void** block, size_t* bytes, size_t need, const char* what);
 int check_launch(const char* what);
 int check_device_status(cw_ctx* ctx);
 

@@ -32,6 +32,45 @@ void clear_error() {
     (void)cudaGetLastError();
 }
 
+int stream_scratch(cw_ctx* ctx, void** block, size_t* bytes, size_t need, const char* what) {
+    if (need <= *bytes) return CW_OK;
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    CW_CUDA(cudaStreamIsCapturing(ctx->stream, &cs));
+    CW_CHECK(cs == cudaStreamCaptureStatusNone, CW_ERR_UNSUPPORTED,
+             "%s: call once with these sizes before a stream capture", what);
+    static std::mutex lock;
+    static cudaMemPool_t pools[64] = {};
+    CW_CHECK(ctx->device < 64, CW_ERR_UNSUPPORTED, "%s: device %d", what, ctx->device);
+    cudaMemPool_t pool;
+    {
+        std::lock_guard<std::mutex> hold(lock);
+        if (!pools[ctx->device]) {
+            cudaMemPoolProps props = {};
+            props.allocType = cudaMemAllocationTypePinned;
+            props.location.type = cudaMemLocationTypeDevice;
+            props.location.id = ctx->device;
+            cudaMemPool_t made;
+            CW_CUDA(cudaMemPoolCreate(&made, &props));
+            uint64_t keep = ~0ull;
+            CW_CUDA(cudaMemPoolSetAttribute(made, cudaMemPoolAttrReleaseThreshold, &keep));
+            pools[ctx->device] = made;
+        }
+        pool = pools[ctx->device];
+    }
+    need = std::max(need, 2 * *bytes);
+    try {
+        ctx->outgrown.reserve(ctx->outgrown.size() + 1);
+    } catch (...) {
+        return set_error(CW_ERR_OOM, "%s: out of host memory", what);
+    }
+    void* p = nullptr;
+    CW_CUDA(cudaMallocFromPoolAsync(&p, need, pool, ctx->stream));
+    if (*block) ctx->outgrown.push_back(*block);
+    *block = p;
+    *bytes = need;
+    return CW_OK;
+}
+
 int check_launch(const char* what) {
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess)
@@ -294,7 +333,8 @@ int cw_ctx_destroy(cw_ctx* ctx) {
     if (ctx->d_counters) cudaFree(ctx->d_counters);
     if (ctx->gemm_scratch) cudaFree(ctx->gemm_scratch);
     if (ctx->tree_scratch) cudaFreeAsync(ctx->tree_scratch, ctx->stream);
-    for (void* p : ctx->tree_outgrown) cudaFreeAsync(p, ctx->stream);
+    if (ctx->prompt_scratch) cudaFreeAsync(ctx->prompt_scratch, ctx->stream);
+    for (void* p : ctx->outgrown) cudaFreeAsync(p, ctx->stream);
     if (ctx->stream && ctx->own_stream) cudaStreamDestroy(ctx->stream);
     delete ctx;
     return CW_OK;

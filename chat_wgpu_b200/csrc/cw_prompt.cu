@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
     const PromptItem it = prompt_item(a, a.slots - 1 - block / ((a.bt * a.G + PF_ROWS - 1) / PF_ROWS));
     const int m0 = block % ((a.bt * a.G + PF_ROWS - 1) / PF_ROWS) * PF_ROWS;
     const int rows = min(PF_ROWS, it.rows * a.G - m0);
-    if (rows <= 0) return;
+    if (rows <= 0 || (a.amax && !pr_odd(a, it.req, head))) return;
     const T* qb = (const T*)a.q + (long long)head * a.G * a.D;
     const T* kb = (const T*)a.k + (long long)it.key0 * a.k_stride + (long long)head * a.D;
     const T* vb = (const T*)a.v + (long long)it.key0 * a.v_stride + (long long)head * a.D;
@@ -243,7 +243,10 @@ extern "C" int cw_prompt_attention(cw_ctx* ctx, const cw_prompt_attn_args* p) {
     a.status = ctx->d_status;
     cudaSetDevice(ctx->device);
     OpScope scope(ctx, "prompt_attention");
-    if (prompt_tc_takes(a, p->type)) return prompt_tc_launch(ctx, a, p->type);
+    if (prompt_tc_takes(a, p->type)) {
+        CW_TRY(prompt_tc_launch(ctx, a, p->type));
+        if (p->type != CW_GGUF_F32) return CW_OK;  // else what the tensor cores left
+    }
     if (p->type == CW_GGUF_F32) return prompt_dims<float>(ctx, a);
     if (p->type == CW_GGUF_F16) return prompt_dims<__half>(ctx, a);
     return prompt_dims<__nv_bfloat16>(ctx, a);

@@ -24,6 +24,10 @@ struct PromptArgs {
     long long q_stride, k_stride, v_stride;
     int n_req, n_rows, n_keys, H, K, G, D, window;
     float scale, softcap;
+    // f32 on the tensor cores: magnitudes of each request's kv heads, [n_req][K][3] (k, v, q:
+    // f32 bits, of q only what is too large), and what the q rows were divided by, [n_rows][H]
+    uint32_t* amax;
+    float* q_back;
     int bt;     // rows of an item
     int slots;  // blocks there can be
     int* status;
@@ -34,6 +38,7 @@ __device__ __forceinline__ void prompt_bad(const PromptArgs& a) {
 }
 
 struct PromptItem {
+    int req;
     int row0, rows;  // its rows of q and out
     int key0, keys;  // its request's keys
     int past;        // row i of the item sees keys [.., past + i] of the request
@@ -54,8 +59,7 @@ __device__ __forceinline__ PromptItem prompt_item(const PromptArgs& a, int s) {
     const int r0 = min(max(a.starts[lo], 0), a.n_rows);
     const int r1 = min(max(a.starts[lo + 1], r0), a.n_rows);
     const int n = r1 - r0, block = s - (r0 / a.bt + lo);
-    it.key0 = r0;
-    it.keys = n;
+    it.req = lo;
     const int* ks = a.key_starts ? a.key_starts : a.starts;
     it.key0 = min(max(ks[lo], 0), a.n_keys);
     it.keys = min(max(ks[lo + 1], it.key0), a.n_keys) - it.key0;
@@ -83,6 +87,18 @@ __device__ __forceinline__ void prompt_check(const PromptArgs& a, int tid, int t
     if (bad) prompt_bad(a);
 }
 
+// Operands as pairs: values are multiplied by 2^s so that the largest, `bits`, lies in
+// [2^14, 2^15).  What is not finite, or so large that products could leave f32's range, is
+// left to the f32 kernel.
+constexpr uint32_t PR_ODD = (127u + 60) << 23;
+__device__ __forceinline__ int pr_shift(uint32_t bits) {
+    return bits ? min(14 - ((int)(bits >> 23) - 127), 100) : 0;
+}
+__device__ __forceinline__ bool pr_odd(const PromptArgs& a, int req, int head) {
+    const uint32_t* m = a.amax + ((size_t)req * a.K + head) * 3;
+    return m[0] >= PR_ODD || m[1] >= PR_ODD || m[2] >= PR_ODD;
+}
+
 template <typename T> __device__ __forceinline__ float pr_f32(T x);
 template <> __device__ __forceinline__ float pr_f32(float x) { return x; }
 template <> __device__ __forceinline__ float pr_f32(__half x) { return __half2float(x); }
@@ -92,7 +108,8 @@ template <> __device__ __forceinline__ float pr_to(float x) { return x; }
 template <> __device__ __forceinline__ __half pr_to(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 pr_to(float x) { return __float2bfloat16_rn(x); }
 
-// cw_prompt_tc.cu: 16-bit types on the tcgen05 tensor cores, where the shape allows it.
+// cw_prompt_tc.cu: on the tcgen05 tensor cores, where the shape allows it.  For f32 the
+// items that pr_odd leaves out are the caller's (a.amax and a.q_back are set).
 bool prompt_tc_takes(const PromptArgs& a, uint32_t type);
 int prompt_tc_launch(cw_ctx* ctx, PromptArgs& a, uint32_t type);
 

@@ -26,6 +26,7 @@
 // product themselves, from what each row sees.
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "cw_prompt.cuh"
 #include "cw_tree_tc.cuh"
@@ -91,6 +92,7 @@ template <int NB> struct PtTiles {
 template <int NB> struct PtItem {
     PromptItem it;
     int head, more;
+    float k_back, v_back;  // pairs: what k and v were divided by
     PtTiles<NB> t;
 };
 template <int NB> struct PtBars {
@@ -103,15 +105,18 @@ template <int NB> struct PtBars {
     PtItem<NB> item[PT_RING];
 };
 
-template <int HD> struct PtShape {
-    static constexpr int NB = HD <= 128 ? 2 : 1;             // row blocks
+// HD: head_dim rounded up to 64, 128 or 256.  PAIR: f32 operands as pairs of f16 (HD <= 128),
+// whose high and low parts are the two halves of a tile.
+template <int HD, bool PAIR> struct PtShape {
+    static constexpr int NB = HD <= 128 && !PAIR ? 2 : 1;    // row blocks
     static constexpr int SB = 3 - NB;                        // buffers of scores of a block
-    static constexpr int HALVES = HD <= 128 ? 1 : HD / 128;  // stages of a K or V tile
-    static constexpr int COLS = HD / 64 / HALVES;            // 64-dim columns of a stage
+    static constexpr int HALVES = PAIR ? 2 : HD <= 128 ? 1 : HD / 128;  // stages of a K or V tile
+    static constexpr int WIDTH = PAIR ? HD : 128;            // dims from half to half in memory
+    static constexpr int COLS = PAIR ? HD / 64 : HD / 64 / HALVES;      // 64-dim columns of a stage
     static constexpr int STAGE = COLS * PT_KEYS * 128;
     static constexpr int STAGES = HD == 64 ? 10 : 5;
     static constexpr int QCOL = 128 * 128;                   // bytes of a column of queries
-    static constexpr int QBLOCK = HD / 64 * QCOL;
+    static constexpr int QBLOCK = HALVES * COLS * QCOL;
     static constexpr int TCOLS = SB * PT_KEYS + HD;          // TMEM columns of a row block
     static constexpr int WARPS = NB * 8;                     // softmax warps
     static constexpr int THREADS = WARPS * 32 + 128;
@@ -119,7 +124,6 @@ template <int HD> struct PtShape {
     static_assert(SMEM <= 232448, "shared memory of a block");
     static_assert(STAGES <= PT_STAGES && STAGES / 2 + 1 < PT_LOOKS, "rings");
 };
-
 // The place in the ring after n stages.
 template <int STAGES> __device__ __forceinline__ TtPlace pt_place(uint32_t n) {
     return {(int)(n % STAGES), n / STAGES & 1};
@@ -132,11 +136,6 @@ __device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
         "r"(idesc), "r"(accumulate)
         : "memory");
-}
-// 64 dims from x of 128 keys of a head.
-__device__ __forceinline__ void pt_copy(void* dst, const CUtensorMap* map, int x, int head, int row,
-                                        uint64_t* bar) {
-    tt_copy_q(dst, map, x, head, row, bar);
 }
 // 32 bytes at a 32-byte boundary.
 __device__ __forceinline__ void pt_store32(void* p, const uint32_t* w) {
@@ -187,6 +186,18 @@ __device__ __noinline__ void pt_cap(uint32_t t_s, float softcap, float y2) {
     }
     tt_wait_st();
 }
+// The same to f32's accuracy; y: scale / softcap.
+__device__ __noinline__ void pt_cap_f32(uint32_t t_s, float softcap, float y) {
+#pragma unroll 1
+    for (int c = 0; c < PT_KEYS / 2; c += 16) {
+        float s[16];
+        tt_load<16>(t_s + c, (uint32_t*)s);
+#pragma unroll
+        for (int j = 0; j < 16; j++) s[j] = softcap * tanhf(s[j] * y);
+        tt_st<16>(t_s + c, (uint32_t*)s);
+    }
+    tt_wait_st();
+}
 // -inf for the keys of the half outside [lo, hi].
 __device__ __noinline__ void pt_hide(uint32_t t_s, int lo, int hi) {
 #pragma unroll 1
@@ -216,7 +227,7 @@ __device__ __noinline__ void pt_careful(uint32_t t_p, uint32_t t_o, const uint8_
         const int chunk = (d0 >> 3) & 7;
 #pragma unroll 1
         for (int j = 0; j < PT_KEYS; j++) {
-            uint32_t p2 = tt_ld1(t_p + (j >> 1));
+            uint32_t p2 = tt_ld1(t_p + (j >> 6) * (PT_KEYS / 2) + ((j & 63) >> 1));
             asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(p2)::"memory");
             const float p = tt_value<BF>(j & 1 ? p2 >> 16 : p2 & 0xffffu);
             const uint4 w = *(const uint4*)(col + j * 128 + ((chunk ^ (j & 7)) << 4));
@@ -235,12 +246,14 @@ __device__ __noinline__ void pt_careful(uint32_t t_p, uint32_t t_o, const uint8_
     }
 }
 
-template <bool BF, int HD>
-__global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
+// T: __half, __nv_bfloat16, or float for pairs.
+template <typename T, int HD>
+__global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
     k_prompt_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PromptArgs a,
                 int tpb, int items) {
-    typedef PtShape<HD> Z;
+    constexpr bool PAIR = sizeof(T) == 4, BF = std::is_same<T, __nv_bfloat16>::value;
+    typedef PtShape<HD, PAIR> Z;
     constexpr int NB = Z::NB, SB = Z::SB, HALVES = Z::HALVES, COLS = Z::COLS, STAGE = Z::STAGE;
     constexpr int STAGES = Z::STAGES, TCOLS = Z::TCOLS, WARPS = Z::WARPS;
     extern __shared__ __align__(1024) uint8_t sm[];
@@ -306,6 +319,9 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
     };
     constexpr TtTile tile = {1024, PT_KEYS * 128};
     TtPlace at = {0, 0};
+    const int halves = PAIR ? 2 : HALVES == 1 || a.D <= 128 ? 1 : HALVES;
+    // columns of 64 dims that half h of a row has
+    auto cols_of = [&](int h) { return PAIR ? (a.D + 63) / 64 : min(COLS, (a.D - h * 128 + 63) / 64); };
 
     if (warp >= WARPS) {
     if (warp == WARPS) {  // ---- copies
@@ -322,15 +338,15 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
         auto load = [&](const CUtensorMap* map, int i) {  // keys of tile i
 #pragma unroll
             for (int h = 0; h < HALVES; h++) {
-                if (h * 128 >= a.D) continue;
+                if (h >= halves) continue;
                 const int s = at.stage;
                 if (filled >= STAGES) ok = ok && all(&bars->empty[s], at.phase ^ 1);
                 if (ok && tt_elect()) {
-                    const int cols = min(COLS, (a.D - h * 128 + 63) / 64);
+                    const int cols = cols_of(h);
                     mbar_expect_tx(&bars->full[s], cols * PT_KEYS * 128);
                     for (int c = 0; c < cols; c++)
-                        pt_copy(ring + s * STAGE + c * PT_KEYS * 128, map, h * 128 + c * 64, head,
-                                key0 + i * PT_KEYS, &bars->full[s]);
+                        tt_copy_q(ring + s * STAGE + c * PT_KEYS * 128, map, h * Z::WIDTH + c * 64,
+                                  head, key0 + i * PT_KEYS, &bars->full[s]);
                 }
                 __syncwarp();
                 filled += ok;
@@ -350,11 +366,14 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                 if (t.b[b].lo >= t.b[b].hi) continue;
                 if (q_count[b] > 0) ok = ok && all(&bars->q_empty[b], q_count[b] - 1);
                 if (ok && tt_elect()) {
-                    const int cols = (a.D + 63) / 64;
+                    int cols = 0;
+                    for (int h = 0; h < halves; h++) cols += cols_of(h);
                     mbar_expect_tx(&bars->q_full[b], cols * tpb * a.G * 128);
-                    for (int c = 0; c < cols; c++)
-                        tt_copy_q(s_q + b * Z::QBLOCK + c * Z::QCOL, &map_q, c * 64, head * a.G,
-                                  row0 + b * tpb, &bars->q_full[b]);
+                    for (int h = 0; h < halves; h++)
+                        for (int c = 0; c < cols_of(h); c++)
+                            tt_copy_q(s_q + b * Z::QBLOCK + (h * COLS + c) * Z::QCOL, &map_q,
+                                      h * Z::WIDTH + c * 64, head * a.G, row0 + b * tpb,
+                                      &bars->q_full[b]);
                 }
                 __syncwarp();
                 q_count[b] += ok;
@@ -362,7 +381,7 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
             for (int i = t.lo; i < t.hi && ok; i++) {
                 if (NB == 1 && i + 1 < t.hi) load(&map_k, i + 1);
                 load(&map_v, i);
-                if (t.look(i)) {
+                if (!PAIR && t.look(i)) {
                     if (ok && tt_elect()) mbar_arrive(&bars->ask[asks % PT_LOOKS]);
                     __syncwarp();
                     asks++;
@@ -381,7 +400,7 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
     } else if (warp == WARPS + 1) {  // ---- products: one elected lane
         constexpr uint32_t id_s = tt_idesc<BF>(PT_KEYS, false, false);
         const uint64_t q0 = umma_desc_sw128(smem_addr(s_q)), kv0 = tt_desc(smem_addr(ring), tile);
-        const int steps = (a.D + 15) / 16, halves = HALVES == 1 || a.D <= 128 ? 1 : HALVES;
+        const int steps = (a.D + 15) / 16;
         const uint32_t id_o[2] = {tt_idesc<BF>(min(128, (a.D + 15) & ~15), false, true),
                                   tt_idesc<BF>(max(16, (a.D - 128 + 15) & ~15), false, true)};
         if (tt_elect()) {
@@ -406,14 +425,19 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                     ok = ok && wait(&bars->full[x.stage], x.phase);
                     tc_fence_after();
                     const uint64_t dk = kv0 + ((x.stage * STAGE) >> 4);
-                    const uint64_t dq = q0 + ((b * Z::QBLOCK + h * 2 * Z::QCOL) >> 4);
+                    // pairs: high and low parts of q times the high ones of k, then the high
+                    // ones of q times the low ones of k
+                    const uint64_t dq = q0 + ((b * Z::QBLOCK + (PAIR ? 0 : h * COLS * Z::QCOL)) >> 4);
                     if (ok) {
 #pragma unroll
-                        for (int s = 0; s < COLS * 4; s++)
-                            if (h * 8 + s < steps)
-                                umma_f16(d, dq + (((s >> 2) * Z::QCOL + (s & 3) * 32) >> 4),
-                                         dk + (((s >> 2) * tile.col + (s & 3) * 32) >> 4), id_s,
-                                         h + s > 0);
+                        for (int s = 0; s < COLS * 4; s++) {
+                            if ((PAIR ? 0 : h * 8) + s >= steps) continue;
+                            const int q_at = (s >> 2) * Z::QCOL + (s & 3) * 32;
+                            const uint64_t ds = dk + (((s >> 2) * tile.col + (s & 3) * 32) >> 4);
+                            umma_f16(d, dq + (q_at >> 4), ds, id_s, h + s > 0);
+                            if (PAIR && h == 0)
+                                umma_f16(d, dq + ((COLS * Z::QCOL + q_at) >> 4), ds, id_s, 1);
+                        }
                     }
                     x.next(STAGES);
                 }
@@ -435,7 +459,7 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                 for (int part = 0; part < 2; part++) {
                     ok = ok && wait(part ? &bars->p_full[sb] : &bars->p_half[sb], NB == 2 ? m : m >> 1);
                     tc_fence_after();
-                    if (part == 0 && t.b[b].mixed(i)) skip = *(volatile uint32_t*)&bars->skip[sb];
+                    if (!PAIR && part == 0 && t.b[b].mixed(i)) skip = *(volatile uint32_t*)&bars->skip[sb];
                     if (!ok || skip) continue;
                     x = v;
 #pragma unroll
@@ -445,8 +469,14 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
 #pragma unroll
                         for (int y = 0; y < 4; y++) {  // 32 keys of each half
                             const int s = (y >> 1) * 4 + (1 - part) * 2 + (y & 1);
-                            pt_mma_ts(o + h * 128, p + 8 * s, dv + ((s * 2 * tile.group) >> 4),
-                                      id_o[h], part + y > 0 ? 1u : before);
+                            const uint64_t ds = dv + ((s * 2 * tile.group) >> 4);
+                            const uint32_t ps = p + (s >> 2) * (PT_KEYS / 2) + (s & 3) * 8;
+                            if (PAIR) {
+                                pt_mma_ts(o, ps, ds, id_o[0], h + part + y > 0 ? 1u : before);
+                                if (h == 0) pt_mma_ts(o, ps + 32, ds, id_o[0], 1);
+                            } else {
+                                pt_mma_ts(o + h * 128, ps, ds, id_o[h], part + y > 0 ? 1u : before);
+                            }
                         }
                         x.next(STAGES);
                     }
@@ -518,19 +548,26 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
             p.head = x % a.K;
             p.more = 1;
             p.t.set(a, p.it, tpb);
+            if (PAIR && p.it.rows > 0) {
+                if (pr_odd(a, p.it.req, p.head)) continue;
+                const uint32_t* m = a.amax + ((size_t)p.it.req * a.K + p.head) * 3;
+                p.k_back = exp2f((float)-pr_shift(m[0]));
+                p.v_back = exp2f((float)-pr_shift(m[1]));
+            }
             if (p.it.rows > 0) ok = give(p);
         }
         PtItem<NB> end = {};
         if (ok) give(end);
     } else {  // ---- values that are not finite, in mixed tiles
-        const int halves = HALVES == 1 || a.D <= 128 ? 1 : HALVES;
         int looks = 0;
         uint32_t used = 0;  // stages before this item
         bool ok = true;
         while (const PtItem<NB>* item = ok ? next() : nullptr) {
             const PtTiles<NB> t = item->t;
             done();
-            for (int i = t.lo; i < t.hi && ok; i++) {
+            // (pairs are finite: what was not is zero)
+            const int last = PAIR ? t.lo : t.hi;
+            for (int i = t.lo; i < last && ok; i++) {
                 if (i == t.all0 && i < t.all1) i = t.all1;
                 if (i >= t.hi) break;
                 uint32_t bits = 0;
@@ -543,7 +580,7 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                 for (int h = 0; h < halves && ok; h++, x.next(STAGES)) {
                     ok = all(&bars->full[x.stage], x.phase);
                     const uint8_t* v = ring + x.stage * STAGE;
-                    const int n = min(COLS, (a.D - h * 128 + 63) / 64) * PT_KEYS * 128;
+                    const int n = cols_of(h) * PT_KEYS * 128;
 #pragma unroll 4
                     for (int o = lane * 16; o < n; o += 512) {
                         const uint4 w = *(const uint4*)(v + o);
@@ -569,11 +606,10 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
         const uint32_t t_o = lanes + SB * PT_KEYS;
         const float log2e = 1.44269504088896341f;
         const bool cap = a.softcap > 0.f;
-        const float c2 = cap ? log2e : a.scale * log2e;
-        const float y2 = cap ? 2.f * log2e * a.scale / a.softcap : 0.f;
+        const float c0 = cap ? log2e : a.scale * log2e;
+        const float y0 = cap ? 2.f * log2e * a.scale / a.softcap : 0.f;
         const int tok = b * tpb + m / a.G;  // of the item
         const bool mine = m < tpb * a.G;
-        const int halves = HALVES == 1 || a.D <= 128 ? 1 : HALVES;
         // a wait that gives up sets `failed`: later ones return at once, and the next item
         // is the last
         auto pass = [&](uint64_t* bar, uint32_t parity) {
@@ -594,6 +630,11 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
             // the row sees keys [low, lim]
             auto lim = [&]() { return row ? min(x->it.past + tok, x->it.keys - 1) : -1; };
             auto low = [&]() { return a.window > 0 ? max(0, x->it.past + tok - a.window + 1) : 0; };
+            float back = 1.f;  // pairs: what the row's scores were divided by
+            if (PAIR && row)
+                back = x->k_back * a.q_back[(long long)(x->it.row0 + tok) * a.H + x->head * a.G +
+                                            m - m / a.G * a.G];
+            const float c2 = PAIR && !cap ? c0 * back : c0;
             // running maximum of the scores, the weights' reference (in powers of two),
             // and the sum of this thread's weights
             float top = -INFINITY, ref = -INFINITY, sum = 0.f;
@@ -609,7 +650,8 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                     // rare work on the scores in place, by calls: the code of every tile is
                     // then fetched without jumps over it (16384 bf16 tokens: 2.04 ms with it
                     // in line, 1.88 without it)
-                    if (cap) pt_cap(t_h, a.softcap, y2);
+                    if (cap && PAIR) pt_cap_f32(t_h, a.softcap, back * a.scale / a.softcap);
+                    else if (cap) pt_cap(t_h, a.softcap, y0);
                     if (mixed) pt_hide(t_h, low() - kt - half * 64, lim() - kt - half * 64);
                     float t0 = top, t1 = top, t2 = top, t3 = top;
                     auto largest = [&]() {
@@ -631,7 +673,7 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                     float(*at)[128] = bars->meet[sb];
                     at[half][m] = top;
                     tc_fence_before();
-                    meet();  // both have read their scores, too: weights may go over them
+                    meet();
                     tc_fence_after();
                     top = pt_max3(top, at[half ^ 1][m], top);
                     const float want = top == -INFINITY ? -INFINITY : top * c2 - TT_LIFT<BF>;
@@ -657,8 +699,8 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                     from = ref == -INFINITY ? 0.f : ref + (ref - ref);
                 }
                 float l[4] = {};
-                uint32_t p[16];
-                auto weights = [&]() {  // of 32 keys
+                auto weights = [&](int c) {  // of keys c .. c + 31 of the half, over its scores
+                    uint32_t p[16], low[16];
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
                         const float y0 = tt_exp2(fmaf(s[j], c2, -from));
@@ -666,19 +708,22 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                         l[j & 3] += y0;
                         l[j & 3 | 1] += y1;
                         p[j >> 1] = pt_pack<BF>(y0, y1);
+                        if constexpr (PAIR) {
+                            const float2 h = __half22float2(*(const __half2*)&p[j >> 1]);
+                            low[j >> 1] = pt_pack<BF>(y0 - h.x, y1 - h.y);
+                        }
                     }
-                };
-                if (work) {
-                    // the second 32 keys first, whose weights may go over the first ones'
+                    // the second 32 keys come first, whose weights may go over the first ones'
                     // scores when those have been read again (kept, 96 registers a thread
                     // were not enough)
-                    weights();
-                    tt_load<32>(t_h, (uint32_t*)s);
-                    tt_st<16>(t_s + half * 32 + 16, p);
+                    if (c > 0) tt_load<32>(t_h, (uint32_t*)s);
+                    tt_st<16>(t_h + c / 2, p);
+                    if constexpr (PAIR) tt_st<16>(t_h + 32 + c / 2, low);
                     tt_wait_st();
-                }
+                };
+                if (work) weights(32);
                 bool odd = false;
-                if (mixed) {
+                if (mixed && !PAIR) {
                     const int y = looks + x->t.looks(i);
                     pass(&bars->look[y % PT_LOOKS], y / PT_LOOKS);
                     odd = *(volatile uint32_t*)&bars->odd[y % PT_LOOKS];
@@ -689,12 +734,10 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars->p_half[sb]);
                 if (work) {
-                    weights();
-                    tt_st<16>(t_s + half * 32, p);
-                    tt_wait_st();
+                    weights(0);
                     sum += (l[0] + l[1]) + (l[2] + l[3]);
                 }
-                if (odd) {
+                if (!PAIR && odd) {
                     const uint8_t* vt[2];
                     TtPlace at = pt_place<STAGES>(used + x->t.before(i) * halves);
                     for (int h = 0; h < halves; h++, at.next(STAGES)) {
@@ -728,30 +771,45 @@ __global__ void __launch_bounds__(PtShape<HD>::THREADS, 1)
                 }
             }
             const int row0 = x->it.row0, head = x->head;
+            const float v_back = PAIR ? x->v_back : 1.f;
             done();
             if (!work) continue;
             const int g = m - m / a.G * a.G;  // query head of the kv head
-            const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-            uint16_t* out = (uint16_t*)a.out +
-                            ((long long)(row0 + tok) * a.H + head * a.G + g) * a.D;
+            const float inv = (sum > 0.f || sum != sum ? 1.f / sum : 0.f) * v_back;
+            T* out = (T*)a.out + ((long long)(row0 + tok) * a.H + head * a.G + g) * a.D;
             const bool wide = ((uintptr_t)out & 31) == 0 && (a.D & 15) == 0;
 #pragma unroll 1
             for (int c = half * 16; c < a.D; c += 32) {
-                uint32_t o[16], w[8];
+                uint32_t o[16];
                 __syncwarp();
                 if (!none) tt_load<16>(t_o + c, o);
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    w[j] = none || inv == 0.f
-                               ? 0u
-                               : pt_pack<BF>(__uint_as_float(o[2 * j]) * inv,
-                                             __uint_as_float(o[2 * j + 1]) * inv);
                 if (!row) continue;
-                if (wide) {
-                    pt_store32(out + c, w);
+                if constexpr (PAIR) {
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        o[j] = none || inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[j]) * inv);
+                    if (wide) {
+                        pt_store32(out + c, o);
+                        pt_store32(out + c + 8, o + 8);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            if (c + j < a.D) out[c + j] = __uint_as_float(o[j]);
+                    }
                 } else {
-                    *(uint4*)(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                    if (c + 8 < a.D) *(uint4*)(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                    uint32_t w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        w[j] = none || inv == 0.f
+                                   ? 0u
+                                   : pt_pack<BF>(__uint_as_float(o[2 * j]) * inv,
+                                                 __uint_as_float(o[2 * j + 1]) * inv);
+                    if (wide) {
+                        pt_store32(out + c, w);
+                    } else {
+                        *(uint4*)(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (c + 8 < a.D) *(uint4*)(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
                 }
             }
             __syncwarp();
@@ -780,15 +838,15 @@ static PFN_cuTensorMapEncodeTiled_v12000 pt_encode_fn() {
     return fn;
 }
 
-// Rows of `heads` heads as [rows][heads][D], boxes of 64 dims (zeros past D) by
+// Rows of `heads` heads as [rows][heads][dims], boxes of 64 dims (zeros past the last) by
 // `box_heads` heads by `box_rows` rows.
-static int pt_map(CUtensorMap* map, const void* base, const PromptArgs& a, bool bf, int heads,
-                  int rows, long long stride, int box_heads, int box_rows) {
+static int pt_map(CUtensorMap* map, const void* base, bool bf, int dims_, int heads, int rows,
+                  long long stride, int box_heads, int box_rows) {
     auto enc = pt_encode_fn();
     CW_CHECK(enc, CW_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    if (rows == 1) stride = (long long)heads * a.D;  // not used, and may be anything
-    cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)heads, (cuuint64_t)rows};
-    cuuint64_t strides[2] = {(cuuint64_t)a.D * 2, (cuuint64_t)stride * 2};
+    if (rows == 1) stride = (long long)heads * dims_;  // not used, and may be anything
+    cuuint64_t dims[3] = {(cuuint64_t)dims_, (cuuint64_t)heads, (cuuint64_t)rows};
+    cuuint64_t strides[2] = {(cuuint64_t)dims_ * 2, (cuuint64_t)stride * 2};
     cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = enc(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
@@ -799,25 +857,151 @@ static int pt_map(CUtensorMap* map, const void* base, const PromptArgs& a, bool 
     return CW_OK;
 }
 
+// ---- f32 operands as pairs ---------------------------------------------------------
+// x 2^s = h + l to 22 bits, h and l f16, s by request and kv head (k, v) or by row and head
+// (q).  With the largest in [2^14, 2^15), what l drops is at most 2^-39 of the largest, or
+// 2^-22 of the value itself.  A warp takes a head row, or for the magnitudes 32 of them.
+constexpr int PS_WARPS = 8;
+
+// The request whose rows [starts[r], starts[r + 1]) hold row t, or -1.
+__device__ __forceinline__ int ps_req(const int* starts, int n_req, int t) {
+    int lo = 0, hi = n_req;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (starts[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    return starts[lo] <= t && t < starts[lo + 1] ? lo : -1;
+}
+__global__ void __launch_bounds__(PS_WARPS * 32) k_prompt_amax(const __grid_constant__ PromptArgs a) {
+    const int lane = threadIdx.x & 31;
+    const long long w = (long long)blockIdx.x * PS_WARPS + (threadIdx.x >> 5);
+    const int heads = 2 * a.K, head = (int)(w % heads), t0 = (int)(w / heads) * 32;
+    pdl_wait();
+    pdl_trigger();
+    if (t0 >= a.n_keys) return;
+    const bool is_v = head >= a.K;
+    const int h = is_v ? head - a.K : head;
+    const float* x = (const float*)(is_v ? a.v : a.k) + (long long)h * a.D;
+    const long long stride = is_v ? a.v_stride : a.k_stride;
+    const int* ks = a.key_starts ? a.key_starts : a.starts;
+    uint32_t most = 0;
+    int mine = -1;
+    auto flush = [&]() {
+        const uint32_t m = __reduce_max_sync(FULL, most);
+        if (lane == 0 && mine >= 0 && m) atomicMax(&a.amax[((size_t)mine * a.K + h) * 3 + is_v], m);
+        most = 0;
+    };
+    for (int t = t0; t < min(t0 + 32, a.n_keys); t++) {
+        if (mine < 0 || t >= ks[mine + 1]) {
+            flush();
+            mine = ps_req(ks, a.n_req, t);
+        }
+        if (mine < 0) continue;
+        for (int d = lane; d < a.D; d += 32)
+            most = max(most, __float_as_uint(fabsf(x[t * stride + d])));
+    }
+    flush();
+}
+// out: q, then k, then v, as [rows][heads][h: W, l: W] f16, zeros past D.
+template <int W>
+__global__ void __launch_bounds__(PS_WARPS * 32)
+    k_prompt_pairs(const __grid_constant__ PromptArgs a, __half* out) {
+    constexpr int N = W / 32;
+    const int lane = threadIdx.x & 31;
+    const long long w = (long long)blockIdx.x * PS_WARPS + (threadIdx.x >> 5);
+    const long long nq = (long long)a.n_rows * a.H, nk = (long long)a.n_keys * a.K;
+    if (w >= nq + 2 * nk) return;
+    pdl_wait();
+    pdl_trigger();
+    const int kind = w < nq ? 0 : w < nq + nk ? 1 : 2;
+    const long long i = kind == 0 ? w : kind == 1 ? w - nq : w - nq - nk;
+    const int heads = kind == 0 ? a.H : a.K, t = (int)(i / heads), h = (int)(i - (long long)t * heads);
+    const float* src = (const float*)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
+                       t * (kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride) +
+                       (long long)h * a.D;
+    const int req = ps_req(kind == 0 || !a.key_starts ? a.starts : a.key_starts, a.n_req, t);
+    float x[N];
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        x[e] = lane * N + e < a.D && req >= 0 ? src[lane * N + e] : 0.f;
+        most = max(most, __float_as_uint(fabsf(x[e])));
+    }
+    uint32_t* m = req >= 0 ? a.amax + ((size_t)req * a.K + (kind == 0 ? h / a.G : h)) * 3 : nullptr;
+    if (kind == 0) {
+        most = __reduce_max_sync(FULL, most);
+        if (lane == 0) {
+            if (most >= PR_ODD && m) atomicMax(&m[2], most);
+            a.q_back[i] = exp2f((float)-pr_shift(most));
+        }
+    } else {
+        most = m ? m[kind - 1] : 0;
+    }
+    const float by = exp2f((float)pr_shift(most));
+    __half hi[N], lo[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        float y = x[e] * by;
+        if (!(fabsf(y) < 65504.f)) y = 0.f;  // not used: the f32 kernel's
+        hi[e] = __float2half_rn(y);
+        lo[e] = __float2half_rn(y - __half2float(hi[e]));
+    }
+    __half* to = out + w * 2 * W + lane * N;
+    if constexpr (N == 4) {
+        *(uint2*)to = *(const uint2*)hi;
+        *(uint2*)(to + W) = *(const uint2*)lo;
+    } else {
+        *(uint32_t*)to = *(const uint32_t*)hi;
+        *(uint32_t*)(to + W) = *(const uint32_t*)lo;
+    }
+}
+
 bool prompt_tc_takes(const PromptArgs& a, uint32_t type) {
+    if (a.G > 128 || !(a.scale > 0.f)) return false;
+    if (type == CW_GGUF_F32)  // any place and stride; the pairs are laid out anew
+        return a.D <= 128 && (long long)a.n_rows >= 256;
     const long long strides = (a.n_rows > 1 ? a.q_stride : 0) |
                               (a.n_keys > 1 ? a.k_stride | a.v_stride : 0);
-    return type != CW_GGUF_F32 && a.D % 8 == 0 && a.G <= 128 && a.scale > 0.f && strides % 8 == 0 &&
+    return a.D % 8 == 0 && strides % 8 == 0 &&
            (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) & 15) == 0;
 }
 
-template <bool BF, int HD> static int pt_go(cw_ctx* ctx, PromptArgs& a) {
-    typedef PtShape<HD> Z;
-    auto kern = k_prompt_tc<BF, HD>;
+template <typename T, int HD> static int pt_go(cw_ctx* ctx, PromptArgs& a) {
+    constexpr bool PAIR = sizeof(T) == 4, BF = std::is_same<T, __nv_bfloat16>::value;
+    typedef PtShape<HD, PAIR> Z;
+    auto kern = k_prompt_tc<T, HD>;
     const int tpb = 128 / a.G;  // tokens of a row block
     a.bt = Z::NB * tpb;
     a.slots = a.n_rows / a.bt + a.n_req;
     const long long items = (long long)a.slots * a.K;
     CW_CHECK(items < (1ll << 30), CW_ERR_UNSUPPORTED, "cw_prompt_attention: too many rows");
     CUtensorMap mq, mk, mv;
-    CW_TRY(pt_map(&mq, a.q, a, BF, a.H, a.n_rows, a.q_stride, a.G, tpb));
-    CW_TRY(pt_map(&mk, a.k, a, BF, a.K, a.n_keys, a.k_stride, 1, PT_KEYS));
-    CW_TRY(pt_map(&mv, a.v, a, BF, a.K, a.n_keys, a.v_stride, 1, PT_KEYS));
+    if constexpr (PAIR) {
+        const size_t nq = (size_t)a.n_rows * a.H, nk = (size_t)a.n_keys * a.K;
+        const size_t pairs = (nq + 2 * nk) * 2 * HD * 2, back = (nq * 4 + 255) / 256 * 256;
+        const size_t most = (size_t)a.n_req * a.K * 3 * 4;
+        CW_TRY(stream_scratch(ctx, &ctx->prompt_scratch, &ctx->prompt_scratch_bytes,
+                              pairs + back + most, "cw_prompt_attention"));
+        __half* out = (__half*)ctx->prompt_scratch;
+        a.q_back = (float*)((char*)out + pairs);
+        a.amax = (uint32_t*)((char*)a.q_back + back);
+        CW_CUDA(cudaMemsetAsync(a.amax, 0, most, ctx->stream));
+        const size_t b0 = ((size_t)(a.n_keys + 31) / 32 * 2 * a.K + PS_WARPS - 1) / PS_WARPS;
+        const size_t b1 = (nq + 2 * nk + PS_WARPS - 1) / PS_WARPS;
+        CW_CHECK(b1 < (1ull << 31), CW_ERR_UNSUPPORTED, "cw_prompt_attention: too many rows");
+        CW_TRY(launch_pdl(ctx, false, k_prompt_amax, dim3((unsigned)b0), dim3(PS_WARPS * 32), 0, a));
+        CW_TRY(launch_pdl(ctx, true, k_prompt_pairs<HD>, dim3((unsigned)b1), dim3(PS_WARPS * 32), 0,
+                          a, out));
+        CW_TRY(pt_map(&mq, out, false, 2 * HD, a.H, a.n_rows, 2ll * HD * a.H, a.G, tpb));
+        CW_TRY(pt_map(&mk, out + nq * 2 * HD, false, 2 * HD, a.K, a.n_keys, 2ll * HD * a.K, 1, PT_KEYS));
+        CW_TRY(pt_map(&mv, out + (nq + nk) * 2 * HD, false, 2 * HD, a.K, a.n_keys, 2ll * HD * a.K, 1,
+                      PT_KEYS));
+    } else {
+        CW_TRY(pt_map(&mq, a.q, BF, a.D, a.H, a.n_rows, a.q_stride, a.G, tpb));
+        CW_TRY(pt_map(&mk, a.k, BF, a.D, a.K, a.n_keys, a.k_stride, 1, PT_KEYS));
+        CW_TRY(pt_map(&mv, a.v, BF, a.D, a.K, a.n_keys, a.v_stride, 1, PT_KEYS));
+    }
     static bool set[64] = {};
     if (!set[ctx->device & 63]) {
         CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -829,13 +1013,15 @@ template <bool BF, int HD> static int pt_go(cw_ctx* ctx, PromptArgs& a) {
                       (int)items));
     return check_launch("prompt_attention");
 }
-template <bool BF> static int pt_dims(cw_ctx* ctx, PromptArgs& a) {
-    if (a.D <= 64) return pt_go<BF, 64>(ctx, a);
-    if (a.D <= 128) return pt_go<BF, 128>(ctx, a);
-    return pt_go<BF, 256>(ctx, a);
+template <typename T> static int pt_dims(cw_ctx* ctx, PromptArgs& a) {
+    if (a.D <= 64) return pt_go<T, 64>(ctx, a);
+    if constexpr (sizeof(T) == 2)
+        if (a.D > 128) return pt_go<T, 256>(ctx, a);
+    return pt_go<T, 128>(ctx, a);
 }
 int prompt_tc_launch(cw_ctx* ctx, PromptArgs& a, uint32_t type) {
-    return type == CW_GGUF_BF16 ? pt_dims<true>(ctx, a) : pt_dims<false>(ctx, a);
+    if (type == CW_GGUF_F32) return pt_dims<float>(ctx, a);
+    return type == CW_GGUF_BF16 ? pt_dims<__nv_bfloat16>(ctx, a) : pt_dims<__half>(ctx, a);
 }
 
 }  // namespace cw
