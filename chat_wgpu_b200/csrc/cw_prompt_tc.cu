@@ -117,7 +117,8 @@ template <int HD, bool PAIR> struct PtShape {
     static constexpr int STAGES = HD == 64 ? 10 : 5;
     static constexpr int QCOL = 128 * 128;                   // bytes of a column of queries
     static constexpr int QBLOCK = HALVES * COLS * QCOL;
-    static constexpr int TCOLS = SB * PT_KEYS + HD;          // TMEM columns of a row block
+    static constexpr int OB = PAIR ? 2 : 1;                  // buffers of sums
+    static constexpr int TCOLS = SB * PT_KEYS + OB * HD;     // TMEM columns of a row block
     static constexpr int WARPS = NB * 8;                     // softmax warps
     static constexpr int THREADS = WARPS * 32 + 128;
     static constexpr size_t SMEM = (size_t)NB * QBLOCK + STAGES * STAGE + sizeof(PtBars<NB>);
@@ -419,28 +420,31 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                 if (i == t.b[b].lo) ok = ok && wait(&bars->q_full[b], q_count[b]++);
                 const uint32_t d = tmem + b * TCOLS + (NB == 2 ? 0 : sb * PT_KEYS);
                 TtPlace x = k;
+                uint32_t more = 0;
+                // q columns from column col of the block, times the stage at place x
+                auto product = [&](int col, const TtPlace& x, int from) {
+                    const uint64_t dk = kv0 + ((x.stage * STAGE) >> 4);
+                    const uint64_t dq = q0 + ((b * Z::QBLOCK + col * Z::QCOL) >> 4);
+#pragma unroll
+                    for (int s = 0; s < COLS * 4; s++) {
+                        if (from + s >= steps) continue;
+                        umma_f16(d, dq + (((s >> 2) * Z::QCOL + (s & 3) * 32) >> 4),
+                                 dk + (((s >> 2) * tile.col + (s & 3) * 32) >> 4), id_s, more);
+                        more = 1;
+                    }
+                };
 #pragma unroll
                 for (int h = 0; h < HALVES; h++) {
                     if (h >= halves) continue;
                     ok = ok && wait(&bars->full[x.stage], x.phase);
                     tc_fence_after();
-                    const uint64_t dk = kv0 + ((x.stage * STAGE) >> 4);
-                    // pairs: high and low parts of q times the high ones of k, then the high
-                    // ones of q times the low ones of k
-                    const uint64_t dq = q0 + ((b * Z::QBLOCK + (PAIR ? 0 : h * COLS * Z::QCOL)) >> 4);
-                    if (ok) {
-#pragma unroll
-                        for (int s = 0; s < COLS * 4; s++) {
-                            if ((PAIR ? 0 : h * 8) + s >= steps) continue;
-                            const int q_at = (s >> 2) * Z::QCOL + (s & 3) * 32;
-                            const uint64_t ds = dk + (((s >> 2) * tile.col + (s & 3) * 32) >> 4);
-                            umma_f16(d, dq + (q_at >> 4), ds, id_s, h + s > 0);
-                            if (PAIR && h == 0)
-                                umma_f16(d, dq + ((COLS * Z::QCOL + q_at) >> 4), ds, id_s, 1);
-                        }
-                    }
+                    // pairs: low parts of q times the high ones of k, high ones of q times the
+                    // low ones of k, and the high ones of both last, since a sum is cut at each
+                    // step by what it has grown to
+                    if (ok) product(PAIR ? (1 - h) * COLS : h * COLS, x, PAIR ? 0 : h * 8);
                     x.next(STAGES);
                 }
+                if (PAIR && ok) product(0, k, 0);
                 if (!ok) return;
                 tc_commit(&bars->s_full[sb]);
                 if (i + 1 == t.b[b].hi) tc_commit(&bars->q_empty[b]);
@@ -452,8 +456,8 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                 for (int h = 0; h < halves; h++, x.next(STAGES))
                     ok = ok && wait(&bars->full[x.stage], x.phase);
                 const uint32_t p = tmem + b * TCOLS + (NB == 2 ? 0 : sb * PT_KEYS);
-                const uint32_t o = tmem + b * TCOLS + SB * PT_KEYS;
-                const uint32_t before = i > t.b[b].lo;
+                const uint32_t o = tmem + b * TCOLS + SB * PT_KEYS + (PAIR ? (m & 1) * HD : 0);
+                const uint32_t before = i > t.b[b].lo;  // (pairs: a tile's sums alone)
                 bool skip = false;
 #pragma unroll
                 for (int part = 0; part < 2; part++) {
@@ -461,27 +465,33 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                     tc_fence_after();
                     if (!PAIR && part == 0 && t.b[b].mixed(i)) skip = *(volatile uint32_t*)&bars->skip[sb];
                     if (!ok || skip) continue;
-                    x = v;
+                    // 16 keys' weights (pairs: their low parts) times half h of the values
+                    auto product = [&](int s, int h, bool low, uint32_t more) {
+                        TtPlace y = v;
+                        if (h) y.next(STAGES);
+                        pt_mma_ts(PAIR ? o : o + h * 128,
+                                  p + (s >> 2) * (PT_KEYS / 2) + (s & 3) * 8 + (low ? 32 : 0),
+                                  kv0 + ((y.stage * STAGE + s * 2 * tile.group) >> 4),
+                                  id_o[PAIR ? 0 : h], more);
+                    };
 #pragma unroll
-                    for (int h = 0; h < HALVES; h++) {
-                        if (h >= halves) continue;
-                        const uint64_t dv = kv0 + ((x.stage * STAGE) >> 4);
+                    for (int y = 0; y < 4; y++) {  // 32 keys of each half of the tile
+                        const int s = (y >> 1) * 4 + (1 - part) * 2 + (y & 1);
+                        if (PAIR) {
+                            product(s, 0, true, part + y > 0);
+                            product(s, 1, false, 1);
+                        } else {
 #pragma unroll
-                        for (int y = 0; y < 4; y++) {  // 32 keys of each half
-                            const int s = (y >> 1) * 4 + (1 - part) * 2 + (y & 1);
-                            const uint64_t ds = dv + ((s * 2 * tile.group) >> 4);
-                            const uint32_t ps = p + (s >> 2) * (PT_KEYS / 2) + (s & 3) * 8;
-                            if (PAIR) {
-                                pt_mma_ts(o, ps, ds, id_o[0], h + part + y > 0 ? 1u : before);
-                                if (h == 0) pt_mma_ts(o, ps + 32, ds, id_o[0], 1);
-                            } else {
-                                pt_mma_ts(o + h * 128, ps, ds, id_o[h], part + y > 0 ? 1u : before);
-                            }
+                            for (int h = 0; h < HALVES; h++)
+                                if (h < halves) product(s, h, false, part + y > 0 ? 1u : before);
                         }
-                        x.next(STAGES);
+                    }
+                    if (PAIR && part) {  // high times high last, as for the scores
+#pragma unroll
+                        for (int s = 0; s < PT_KEYS / 16; s++) product(s, 0, false, 1);
                     }
                 }
-                if (ok) tc_commit(&bars->pv[b]);
+                if (ok) tc_commit(&bars->pv[PAIR ? m & 1 : b]);
             };
             auto release = [&](TtPlace& x) {  // a K or V tile, by the products issued so far
                 for (int h = 0; h < halves; h++, x.next(STAGES))
@@ -638,6 +648,24 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
             // running maximum of the scores, the weights' reference (in powers of two),
             // and the sum of this thread's weights
             float top = -INFINITY, ref = -INFINITY, sum = 0.f;
+            // pairs: half of the row's sums.  The tensor cores cut their f32 sums, which over
+            // many tiles shows (4096 keys: 7e-6), so each tile's are added here
+            [[maybe_unused]] float acc[PAIR ? HD / 2 : 1], late = 1.f;  // late: for the tile not added yet
+            [[maybe_unused]] auto add = [&](int tile_n) {
+                pass(&bars->pv[tile_n & 1], tile_n >> 1);
+#pragma unroll
+                for (int c = 0; c < HD / 2; c += 16) {
+                    uint32_t o[16];
+                    tt_load<16>(t_o + (tile_n & 1) * HD + half * (HD / 2) + c, o);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) acc[c + j] = fmaf(__uint_as_float(o[j]), late, acc[c + j]);
+                }
+                late = 1.f;
+            };
+            if constexpr (PAIR) {
+#pragma unroll
+                for (int c = 0; c < HD / 2; c++) acc[c] = 0.f;
+            }
 #pragma unroll 1
             for (int i = blk.lo; i < blk.hi; i++, n++) {
                 const int sb = NB == 2 ? b : n & 1, kt = i * PT_KEYS;
@@ -682,11 +710,16 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                     } else if (__any_sync(FULL, row && !(want - ref <= 8.f) && want != -INFINITY)) {
                         const float fix = ref == -INFINITY ? 0.f : tt_exp2(ref - want);
                         // O holds the tiles so far (two row blocks: since the scores came)
-                        if (NB == 1) pass(&bars->pv[b], n - 1);
+                        if (NB == 1 && !PAIR) pass(&bars->pv[b], n - 1);
                         sum *= fix;
                         ref = want;
+                        if constexpr (PAIR) {
+                            late = fix;
+#pragma unroll
+                            for (int c = 0; c < HD / 2; c++) acc[c] *= fix;
+                        }
 #pragma unroll 1
-                        for (int c = half * 16; c < a.D; c += 32) {
+                        for (int c = PAIR ? a.D : half * 16; c < a.D; c += 32) {
                             uint32_t o[16];
                             tt_load<16>(t_o + c, o);
 #pragma unroll
@@ -755,13 +788,16 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars->p_full[sb]);
+                if constexpr (PAIR)
+                    if (work && i > blk.lo) add(n - 1);
             }
             looks += x->t.looks(x->t.hi);
             used += 2 * (x->t.hi - x->t.lo) * halves;
             // ---- the item's end
             const bool none = blk.lo >= blk.hi;
             if (!none) {
-                pass(&bars->pv[b], n - 1);
+                if constexpr (PAIR) add(n - 1);
+                else pass(&bars->pv[b], n - 1);
                 if (work) {
                     float(*at)[128] = bars->meet[NB == 2 ? b : 0];
                     at[half][m] = sum;
@@ -778,26 +814,26 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
             const float inv = (sum > 0.f || sum != sum ? 1.f / sum : 0.f) * v_back;
             T* out = (T*)a.out + ((long long)(row0 + tok) * a.H + head * a.G + g) * a.D;
             const bool wide = ((uintptr_t)out & 31) == 0 && (a.D & 15) == 0;
-#pragma unroll 1
-            for (int c = half * 16; c < a.D; c += 32) {
-                uint32_t o[16];
-                __syncwarp();
-                if (!none) tt_load<16>(t_o + c, o);
-                if (!row) continue;
-                if constexpr (PAIR) {
+            if constexpr (PAIR) {
+                if (row) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        o[j] = none || inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[j]) * inv);
-                    if (wide) {
-                        pt_store32(out + c, o);
-                        pt_store32(out + c + 8, o + 8);
-                    } else {
+                    for (int c = 0; c < HD / 2; c += 8) {
+                        const int d = half * (HD / 2) + c;
 #pragma unroll
-                        for (int j = 0; j < 16; j++)
-                            if (c + j < a.D) out[c + j] = __uint_as_float(o[j]);
+                        for (int j = 0; j < 8; j++) acc[c + j] = inv == 0.f ? 0.f : acc[c + j] * inv;
+                        if (wide && d < a.D) pt_store32(out + d, (const uint32_t*)acc + c);
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (!wide && d + j < a.D) out[d + j] = acc[c + j];
                     }
-                } else {
-                    uint32_t w[8];
+                }
+            } else {
+#pragma unroll 1
+                for (int c = half * 16; c < a.D; c += 32) {
+                    uint32_t o[16], w[8];
+                    __syncwarp();
+                    if (!none) tt_load<16>(t_o + c, o);
+                    if (!row) continue;
 #pragma unroll
                     for (int j = 0; j < 8; j++)
                         w[j] = none || inv == 0.f
