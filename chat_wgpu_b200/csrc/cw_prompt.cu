@@ -14,8 +14,30 @@
 
 namespace cw {
 
-constexpr int PF_ROWS = 64, PF_KEYS = 64, PF_THREADS = 256;
+constexpr int PF_ROWS = 64, PF_KEYS = PF_ROWS, PF_THREADS = 256;
 
+// Fills [64][DP + 4] from row(m), zeros where it is null and past D: eight reads in flight (a
+// row of 4000 keys one read at a time took 980 us).  Whether what this thread read is finite.
+template <typename T, int DP, typename F>
+__device__ __forceinline__ bool pf_fill(float* to, int D, F row) {
+    bool odd = false;
+    for (int i0 = threadIdx.x; i0 < PF_ROWS * DP; i0 += 8 * PF_THREADS) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int i = i0 + e * PF_THREADS, d = i % DP;
+            const T* from = row(i / DP);
+            x[e] = from && d < D ? pr_f32(from[d]) : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int i = i0 + e * PF_THREADS;
+            to[i / DP * (DP + 4) + i % DP] = x[e];
+            odd |= !isfinite(x[e]);
+        }
+    }
+    return odd;
+}
 // DP: head_dim rounded up to 64, 128 or 256.
 template <typename T, int DP>
 __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ PromptArgs a) {
@@ -37,15 +59,10 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
     const T* qb = (const T*)a.q + (long long)head * a.G * a.D;
     const T* kb = (const T*)a.k + (long long)it.key0 * a.k_stride + (long long)head * a.D;
     const T* vb = (const T*)a.v + (long long)it.key0 * a.v_stride + (long long)head * a.D;
-    for (int i = tid; i < PF_ROWS * DP; i += PF_THREADS) {
-        const int m = i / DP, d = i % DP;
-        float x = 0.f;
-        if (m < rows && d < a.D) {
-            const int t = (m0 + m) / a.G, g = (m0 + m) - t * a.G;
-            x = pr_f32(qb[(long long)(it.row0 + t) * a.q_stride + g * a.D + d]);
-        }
-        sq[m * LD + d] = x;
-    }
+    (void)pf_fill<T, DP>(sq, a.D, [&](int m) -> const T* {
+        const int t = (m0 + m) / a.G, g = (m0 + m) - t * a.G;
+        return m < rows ? qb + (long long)(it.row0 + t) * a.q_stride + g * a.D : nullptr;
+    });
     float o[4][CN], top[4], sum[4];
     int lim[4], low[4];  // the row sees keys [low, lim]
 #pragma unroll
@@ -66,11 +83,9 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
     for (int kt = first; kt <= last; kt += PF_KEYS) {
         const bool mixed = kt < all0 || kt + PF_KEYS - 1 > all1;
         __syncthreads();
-        for (int i = tid; i < PF_KEYS * DP; i += PF_THREADS) {
-            const int j = i / DP, d = i % DP;
-            skv[j * LD + d] =
-                kt + j <= last && d < a.D ? pr_f32(kb[(long long)(kt + j) * a.k_stride + d]) : 0.f;
-        }
+        (void)pf_fill<T, DP>(skv, a.D, [&](int j) -> const T* {
+            return kt + j <= last ? kb + (long long)(kt + j) * a.k_stride : nullptr;
+        });
         __syncthreads();
         float s[4][4] = {};
         for (int d = 0; d < a.D; d += 4) {
@@ -122,14 +137,9 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
             for (int c = 0; c < CN; c++) o[i][c] *= fix;
         }
         __syncthreads();
-        bool odd = false;
-        for (int i = tid; i < PF_KEYS * DP; i += PF_THREADS) {
-            const int j = i / DP, d = i % DP;
-            const float x =
-                kt + j <= last && d < a.D ? pr_f32(vb[(long long)(kt + j) * a.v_stride + d]) : 0.f;
-            skv[j * LD + d] = x;
-            odd |= !isfinite(x);
-        }
+        const bool odd = pf_fill<T, DP>(skv, a.D, [&](int j) -> const T* {
+            return kt + j <= last ? vb + (long long)(kt + j) * a.v_stride : nullptr;
+        });
         // a value that is not finite counts only where it is seen
         const bool careful = __syncthreads_or(mixed && odd);
         for (int j = 0; j < PF_KEYS; j++) {

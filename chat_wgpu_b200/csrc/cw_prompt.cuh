@@ -17,6 +17,10 @@
 
 namespace cw {
 
+struct PromptPiece {  // an item whose first piece is this CTA's last one
+    int row0, rows, head, count, slot;
+};
+
 struct PromptArgs {
     const void *q, *k, *v;
     void* out;
@@ -28,6 +32,12 @@ struct PromptArgs {
     // f32 bits, of q only what is too large), and what the q rows were divided by, [n_rows][H]
     uint32_t* amax;
     float* q_back;
+    // partial states of items that a CTA's run cuts, two to a CTA: [grid * 2][rows][dp] sums,
+    // [grid * 2][rows] reference and sum of the weights (-1: no tile), and [grid] items
+    float* part;
+    float2* ml;
+    PromptPiece* pieces;
+    int cut, dp;
     int bt;     // rows of an item
     int slots;  // blocks there can be
     int* status;

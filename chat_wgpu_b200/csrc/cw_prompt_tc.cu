@@ -25,6 +25,7 @@
 // the weights are formed, and where it finds such values the threads add that tile's
 // product themselves, from what each row sees.
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <type_traits>
 
@@ -32,11 +33,17 @@
 #include "cw_tree_tc.cuh"
 
 namespace cw {
+#ifndef MINR
+#define MINR 256
+#endif
 
 constexpr int PT_KEYS = 128;    // keys of a tile
 constexpr int PT_RING = 3;      // items found ahead
 constexpr int PT_LOOKS = 8;     // tiles looked over ahead (the ring holds 5 V tiles at most)
 constexpr int PT_STAGES = 10;   // most stages
+constexpr int PT_PAD = 2;       // tiles that an item's start and end count as
+constexpr int PT_CUT = 6;       // items of fewer tiles are not cut
+constexpr int PT_LEAST = 4;     // units of a CTA's run where items are cut
 
 // What a row block of an item sees: tiles [lo, hi), all rows the same in [all0, all1).
 struct PtBlock {
@@ -81,6 +88,18 @@ template <int NB> struct PtTiles {
         all0 = min(max(all0, lo), hi);
         all1 = min(max(all1, all0), hi);
     }
+    // tiles [x, y) of them only
+    __device__ __forceinline__ void clip(int x, int y) {
+        lo = max(lo, x);
+        hi = max(lo, min(hi, y));
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            b[i].lo = max(b[i].lo, x);
+            b[i].hi = max(b[i].lo, min(b[i].hi, y));
+        }
+        all0 = min(max(all0, lo), hi);
+        all1 = min(max(all1, all0), hi);
+    }
     __device__ __forceinline__ bool look(int i) const { return i < all0 || i >= all1; }
     // tiles looked over before tile i; K and V tiles in the ring before V of tile i
     __device__ __forceinline__ int looks(int i) const { return min(i, all0) - lo + max(0, i - all1); }
@@ -92,8 +111,15 @@ template <int NB> struct PtTiles {
 template <int NB> struct PtItem {
     PromptItem it;
     int head, more;
+    int whole, slot;       // all of its tiles; else where its partial state goes
     float k_back, v_back;  // pairs: what k and v were divided by
     PtTiles<NB> t;
+};
+// A CTA's run of the units of all items, in slot, kv head, tile order: it begins `off` units
+// behind the start of slot's first kv head and has `left`.
+struct PtRun {
+    long long w[24], off;
+    int slot;
 };
 template <int NB> struct PtBars {
     uint64_t full[PT_STAGES], empty[PT_STAGES];
@@ -102,6 +128,7 @@ template <int NB> struct PtBars {
     uint64_t ask[PT_LOOKS], look[PT_LOOKS], done;
     uint32_t tmem, failed, odd[PT_LOOKS], skip[2];
     float meet[2][2][128];  // what the two threads of a row tell each other
+    PtRun run;
     PtItem<NB> item[PT_RING];
 };
 
@@ -247,6 +274,63 @@ __device__ __noinline__ void pt_careful(uint32_t t_p, uint32_t t_o, const uint8_
     }
 }
 
+// Units of slot s for one kv head: its tiles, and PT_PAD for its start and end.
+template <int NB> __device__ int pt_units(const PromptArgs& a, int s, int tpb) {
+    const PromptItem it = prompt_item(a, s);
+    if (it.rows <= 0) return 0;
+    PtTiles<NB> t;
+    t.set(a, it, tpb);
+    return t.hi - t.lo + PT_PAD;
+}
+// All threads (NT of them): this CTA's run.  The units of all slots are summed by every CTA,
+// a slot to a thread.
+template <int NB, int NT>
+__device__ void pt_run(const PromptArgs& a, int tpb, PtRun* run, long long& per, long long& left) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // sums of the threads' values before each, and of all
+    auto scan = [&](long long mine, long long& total) {
+        long long incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(FULL, incl, o);
+            if (lane >= o) incl += x;
+        }
+        __syncthreads();
+        if (lane == 31) run->w[warp] = incl;
+        __syncthreads();
+        long long before = 0;
+        total = 0;
+        for (int w = 0; w < NT / 32; w++) {
+            if (w == warp) before = total;
+            total += run->w[w];
+        }
+        return before + incl - mine;
+    };
+    long long mine = 0, total, round;
+    for (int s = tid; s < a.slots; s += NT) mine += pt_units<NB>(a, s, tpb);
+    const long long at = scan(mine, total);
+    per = max((total * a.K + gridDim.x - 1) / gridDim.x, (long long)PT_LEAST);
+    const long long from = blockIdx.x * per;
+    left = max(0ll, min(per, total * a.K - from));
+    auto found = [&](int s, long long before, long long units) {
+        if (units > 0 && before * a.K <= from && from < (before + units) * a.K) {
+            run->slot = s;
+            run->off = from - before * a.K;
+        }
+    };
+    if (a.slots <= NT) {
+        found(tid, at, mine);
+    } else if (left > 0) {  // the same for all threads
+        long long before = 0;
+        for (int s0 = 0; s0 < a.slots; s0 += NT) {
+            const long long u = s0 + tid < a.slots ? pt_units<NB>(a, s0 + tid, tpb) : 0;
+            const long long x = scan(u, round);
+            found(s0 + tid, before + x, u);
+            before += round;
+        }
+    }
+}
+
 // T: __half, __nv_bfloat16, or float for pairs.
 template <typename T, int HD>
 __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
@@ -295,6 +379,8 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
         fence_mbar_init();
     }
     pdl_wait();  // the setup above overlaps the launch before
+    long long per = 0, left = 0;
+    if (a.cut) pt_run<NB, Z::THREADS>(a, tpb, &bars->run, per, left);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -547,24 +633,75 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
             count++;
             return true;
         };
-        // long items first; every second round of the CTAs goes the other way
         bool ok = true;
-        for (int round = 0; ok && round * (int)gridDim.x < items; round++) {
-            const int c = round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
-            const int x = round * gridDim.x + c;
-            if (x >= items) continue;
-            PtItem<NB> p;
-            p.it = prompt_item(a, a.slots - 1 - x / a.K);
-            p.head = x % a.K;
-            p.more = 1;
-            p.t.set(a, p.it, tpb);
-            if (PAIR && p.it.rows > 0) {
-                if (pr_odd(a, p.it.req, p.head)) continue;
-                const uint32_t* m = a.amax + ((size_t)p.it.req * a.K + p.head) * 3;
-                p.k_back = exp2f((float)-pr_shift(m[0]));
-                p.v_back = exp2f((float)-pr_shift(m[1]));
+        PtItem<NB> p;
+        p.more = 1;
+        p.slot = 0;
+        // the item's head, and whether there is work for it here
+        auto ready = [&](int head) {
+            p.head = head;
+            if (!PAIR) return true;
+            const uint32_t* m = a.amax + ((size_t)p.it.req * a.K + head) * 3;
+            p.k_back = exp2f((float)-pr_shift(m[0]));
+            p.v_back = exp2f((float)-pr_shift(m[1]));
+            return !pr_odd(a, p.it.req, head);
+        };
+        if (!a.cut) {  // whole items, long ones first; every second round of the CTAs goes back
+            p.whole = 1;
+            for (int round = 0; ok && round * (int)gridDim.x < items; round++) {
+                const int c = round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+                const int x = round * gridDim.x + c;
+                if (x >= items) continue;
+                p.it = prompt_item(a, a.slots - 1 - x / a.K);
+                if (p.it.rows <= 0 || !ready(x % a.K)) continue;
+                p.t.set(a, p.it, tpb);
+                ok = give(p);
             }
-            if (p.it.rows > 0) ok = give(p);
+        } else {
+            PromptPiece cut = {};
+            int slot = left > 0 ? bars->run.slot : a.slots, u = 0, head = 0, pos = 0;
+            long long at = blockIdx.x * per;  // unit of the item's tile `pos`
+            auto open = [&]() {               // the next slot with rows, from `slot`
+                for (; slot < a.slots; slot++) {
+                    p.it = prompt_item(a, slot);
+                    if (p.it.rows > 0) break;
+                }
+                if (slot >= a.slots) return;
+                p.t.set(a, p.it, tpb);
+                u = p.t.hi - p.t.lo + PT_PAD;
+            };
+            open();
+            if (left > 0 && u > 0) {
+                head = (int)(bars->run.off / u);
+                pos = (int)(bars->run.off - (long long)head * u);
+            }
+            while (ok && left > 0 && slot < a.slots) {
+                const int tiles = u - PT_PAD;
+                const bool cuts = tiles >= PT_CUT;
+                const int n = cuts ? (int)min((long long)(tiles - pos), left) : tiles;
+                // (an item that is not cut is its first unit's CTA's)
+                if (ready(head) && (cuts ? n > 0 : pos == 0)) {
+                    PtItem<NB> x = p;
+                    x.whole = n == tiles;
+                    x.slot = at == blockIdx.x * per ? 0 : 1;
+                    if (!x.whole) {
+                        x.t.clip(p.t.lo + pos, p.t.lo + pos + n);
+                        if (pos == 0)
+                            cut = {p.it.row0, p.it.rows, head,
+                                   (int)((at + tiles - 1) / per - blockIdx.x) + 1, x.slot};
+                    }
+                    ok = give(x);
+                }
+                at += u - pos;
+                left -= u - pos;
+                pos = 0;
+                if (++head == a.K) {
+                    head = 0;
+                    slot++;
+                    open();
+                }
+            }
+            if (lane == 0) a.pieces[blockIdx.x] = cut;
         }
         PtItem<NB> end = {};
         if (ok) give(end);
@@ -807,10 +944,38 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                 }
             }
             const int row0 = x->it.row0, head = x->head;
+            const bool whole = x->whole;
+            const size_t piece = ((size_t)blockIdx.x * 2 + x->slot) * (NB * 128) + b * 128 + m;
             const float v_back = PAIR ? x->v_back : 1.f;
             done();
             if (!work) continue;
             const int g = m - m / a.G * a.G;  // query head of the kv head
+            if (!whole) {  // the partial state
+                if (half == 0) a.ml[piece] = make_float2(ref, none ? -1.f : sum);
+                if (none) continue;
+                float* to = a.part + piece * a.dp;
+                if constexpr (PAIR) {
+#pragma unroll
+                    for (int c = 0; c < HD / 2; c += 8) {
+                        const int d = half * (HD / 2) + c;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) acc[c + j] *= v_back;
+                        if (d < a.dp) pt_store32(to + d, (const uint32_t*)acc + c);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = half * 16; c < a.D; c += 32) {
+                        uint32_t o[16];
+                        __syncwarp();
+                        tt_load<16>(t_o + c, o);
+                        pt_store32(to + c, o);
+                        if (c + 8 < a.D) pt_store32(to + c + 8, o + 8);
+                    }
+                }
+                __syncwarp();
+                tc_fence_before();
+                continue;
+            }
             const float inv = (sum > 0.f || sum != sum ? 1.f / sum : 0.f) * v_back;
             T* out = (T*)a.out + ((long long)(row0 + tok) * a.H + head * a.G + g) * a.D;
             const bool wide = ((uintptr_t)out & 31) == 0 && (a.D & 15) == 0;
@@ -857,6 +1022,70 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
     if (warp == 0) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the pieces of the items that a run's end cut: out = sum_i w_i o_i / sum_i w_i l_i,
+// w_i = 2^(m_i - max m), in key order.  A warp per row: a lane holds a piece's weight, then four
+// dims (eight past 128) of every piece.  Bound by the latency of its dependent reads.
+constexpr int PJ_WARPS = 8;
+template <typename T>
+__global__ void __launch_bounds__(PJ_WARPS * 32)
+    k_prompt_join(const __grid_constant__ PromptArgs a, int tpb, int rows) {
+    pdl_trigger();
+    pdl_wait();
+    const PromptPiece p = a.pieces[blockIdx.x];
+    const int lane = threadIdx.x & 31, m = blockIdx.y * PJ_WARPS + (threadIdx.x >> 5);
+    const int r = m & 127, tok = (m >> 7) * tpb + r / a.G;
+    if (p.count <= 1 || r >= tpb * a.G || tok >= p.rows) return;
+    auto piece = [&](int i) {
+        return ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? p.slot : 0)) * rows + m;
+    };
+    float top = -INFINITY, l = 0.f;
+    for (int i = lane; i < p.count; i += 32) {
+        const float2 x = a.ml[piece(i)];
+        if (!(x.y < 0.f)) top = fmaxf(top, x.x);
+    }
+    top = warp_max(top);
+    float4 o[2] = {};
+    for (int i0 = 0; i0 < p.count; i0 += 32) {
+        float w = 0.f;
+        bool live = false;  // had a tile: a piece without weight keeps the NaN of its values
+        if (i0 + lane < p.count) {
+            const float2 x = a.ml[piece(i0 + lane)];
+            live = !(x.y < 0.f);
+            if (live && x.x != -INFINITY) w = exp2f(x.x - top);
+            if (live && x.y != 0.f) l += x.y * w;
+        }
+        const unsigned on = __ballot_sync(FULL, live);
+        const int n = min(32, p.count - i0);
+#pragma unroll 4
+        for (int i = 0; i < n; i++) {
+            const float wi = __shfl_sync(FULL, w, i);
+            if (!(on >> i & 1)) continue;
+            const float* from = a.part + piece(i0 + i) * a.dp;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int d = h * 128 + lane * 4;
+                if (d >= a.dp) continue;
+                const float4 x = *(const float4*)(from + d);
+                o[h].x = fmaf(wi, x.x, o[h].x);
+                o[h].y = fmaf(wi, x.y, o[h].y);
+                o[h].z = fmaf(wi, x.z, o[h].z);
+                o[h].w = fmaf(wi, x.w, o[h].w);
+            }
+        }
+    }
+    l = warp_sum(l);
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    T* out = (T*)a.out + ((long long)(p.row0 + tok) * a.H + p.head * a.G + r - r / a.G * a.G) * a.D;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const float y[4] = {o[h].x, o[h].y, o[h].z, o[h].w};
+        const int d = h * 128 + lane * 4;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (d + e < a.D) out[d + e] = pr_to<T>(inv == 0.f ? 0.f : y[e] * inv);
     }
 }
 
@@ -996,7 +1225,7 @@ __global__ void __launch_bounds__(PS_WARPS * 32)
 bool prompt_tc_takes(const PromptArgs& a, uint32_t type) {
     if (a.G > 128 || !(a.scale > 0.f)) return false;
     if (type == CW_GGUF_F32)  // any place and stride; the pairs are laid out anew
-        return a.D <= 128 && (long long)a.n_rows >= 256;
+        return a.D <= 128 && (long long)a.n_rows >= MINR;
     const long long strides = (a.n_rows > 1 ? a.q_stride : 0) |
                               (a.n_keys > 1 ? a.k_stride | a.v_stride : 0);
     return a.D % 8 == 0 && strides % 8 == 0 &&
@@ -1012,16 +1241,47 @@ template <typename T, int HD> static int pt_go(cw_ctx* ctx, PromptArgs& a) {
     a.slots = a.n_rows / a.bt + a.n_req;
     const long long items = (long long)a.slots * a.K;
     CW_CHECK(items < (1ll << 30), CW_ERR_UNSUPPORTED, "cw_prompt_attention: too many rows");
+    // Whole items or equal runs, from what the host knows: the longest item, or rounds of the
+    // mean one, against the tiles a CTA would have and 9 tiles' time for the second launch and
+    // the partial states (us, whole and cut: one prompt of 1024 rows 27 and 37, 2048 rows 49
+    // and 70; four pieces of 270 rows after 6000 209 and 158, a row after 16000 209 and 31).
+    const double rows = (double)a.n_rows / a.n_req, keys = (double)a.n_keys / a.n_req;
+    const double work = a.K * (double)a.n_req * std::ceil(rows / a.bt), sms = ctx->sm_count;
+    const double longest = keys / PT_KEYS, mean = std::max(keys - rows / 2, 1.0) / PT_KEYS;
+    a.cut = std::max(longest, std::ceil(work / sms) * mean) > work * (mean + PT_PAD) / sms + 9.0;
+    const int grid = a.cut ? ctx->sm_count : (int)std::min<long long>(items, ctx->sm_count);
+    a.dp = (a.D + 7) / 8 * 8;
+    constexpr int ROWS = Z::NB * 128;
+    size_t need = 0;
+    auto take = [&](size_t n) {  // a part of the scratch, at a multiple of 256
+        const size_t at = need;
+        need += (n + 255) / 256 * 256;
+        return at;
+    };
+    const size_t pieces = a.cut ? (size_t)grid * 2 * ROWS : 0;
+    const size_t at_part = take(pieces * a.dp * 4), at_ml = take(pieces * 8),
+                 at_pieces = take(a.cut ? grid * sizeof(PromptPiece) : 0);
+    char* base = nullptr;
+    auto scratch = [&]() -> int {
+        if (!need) return CW_OK;
+        CW_TRY(stream_scratch(ctx, &ctx->prompt_scratch, &ctx->prompt_scratch_bytes, need,
+                              "cw_prompt_attention"));
+        base = (char*)ctx->prompt_scratch;
+        a.part = (float*)(base + at_part);
+        a.ml = (float2*)(base + at_ml);
+        a.pieces = (PromptPiece*)(base + at_pieces);
+        return CW_OK;
+    };
     CUtensorMap mq, mk, mv;
     if constexpr (PAIR) {
         const size_t nq = (size_t)a.n_rows * a.H, nk = (size_t)a.n_keys * a.K;
-        const size_t pairs = (nq + 2 * nk) * 2 * HD * 2, back = (nq * 4 + 255) / 256 * 256;
         const size_t most = (size_t)a.n_req * a.K * 3 * 4;
-        CW_TRY(stream_scratch(ctx, &ctx->prompt_scratch, &ctx->prompt_scratch_bytes,
-                              pairs + back + most, "cw_prompt_attention"));
-        __half* out = (__half*)ctx->prompt_scratch;
-        a.q_back = (float*)((char*)out + pairs);
-        a.amax = (uint32_t*)((char*)a.q_back + back);
+        const size_t at_pairs = take((nq + 2 * nk) * 2 * HD * 2), at_back = take(nq * 4),
+                     at_most = take(most);
+        CW_TRY(scratch());
+        __half* out = (__half*)(base + at_pairs);
+        a.q_back = (float*)(base + at_back);
+        a.amax = (uint32_t*)(base + at_most);
         CW_CUDA(cudaMemsetAsync(a.amax, 0, most, ctx->stream));
         const size_t b0 = ((size_t)(a.n_keys + 31) / 32 * 2 * a.K + PS_WARPS - 1) / PS_WARPS;
         const size_t b1 = (nq + 2 * nk + PS_WARPS - 1) / PS_WARPS;
@@ -1034,6 +1294,7 @@ template <typename T, int HD> static int pt_go(cw_ctx* ctx, PromptArgs& a) {
         CW_TRY(pt_map(&mv, out + (nq + nk) * 2 * HD, false, 2 * HD, a.K, a.n_keys, 2ll * HD * a.K, 1,
                       PT_KEYS));
     } else {
+        CW_TRY(scratch());
         CW_TRY(pt_map(&mq, a.q, BF, a.D, a.H, a.n_rows, a.q_stride, a.G, tpb));
         CW_TRY(pt_map(&mk, a.k, BF, a.D, a.K, a.n_keys, a.k_stride, 1, PT_KEYS));
         CW_TRY(pt_map(&mv, a.v, BF, a.D, a.K, a.n_keys, a.v_stride, 1, PT_KEYS));
@@ -1044,9 +1305,11 @@ template <typename T, int HD> static int pt_go(cw_ctx* ctx, PromptArgs& a) {
                                      (int)Z::SMEM));
         set[ctx->device & 63] = true;
     }
-    const int grid = (int)std::min<long long>(items, ctx->sm_count);
     CW_TRY(launch_pdl(ctx, true, kern, dim3(grid), dim3(Z::THREADS), Z::SMEM, mq, mk, mv, a, tpb,
                       (int)items));
+    if (a.cut)
+        CW_TRY(launch_pdl(ctx, true, k_prompt_join<T>, dim3(grid, ROWS / PJ_WARPS), dim3(PJ_WARPS * 32), 0,
+                          a, tpb, ROWS));
     return check_launch("prompt_attention");
 }
 template <typename T> static int pt_dims(cw_ctx* ctx, PromptArgs& a) {
