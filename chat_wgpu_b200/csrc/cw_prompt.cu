@@ -47,10 +47,11 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
     float* skv = sq + PF_ROWS * LD;   // [PF_KEYS][LD]
     float* sp = skv + PF_KEYS * LD;   // [PF_ROWS][PF_KEYS + 4]
     constexpr int LP = PF_KEYS + 4;
+    const float log2e = 1.44269504088896341f;  // scores are in powers of two
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int head = blockIdx.x % a.K, block = blockIdx.x / a.K;
     pdl_wait();
-    if (blockIdx.x == 0) prompt_check(a, tid, PF_THREADS);
+    if (blockIdx.x == 0 && blockIdx.y == 0) prompt_check(a, tid, PF_THREADS);
     // the last blocks of a request have the most keys: they start first
     const PromptItem it = prompt_item(a, a.slots - 1 - block / ((a.bt * a.G + PF_ROWS - 1) / PF_ROWS));
     const int m0 = block % ((a.bt * a.G + PF_ROWS - 1) / PF_ROWS) * PF_ROWS;
@@ -75,8 +76,14 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
         lim[i] = ty * 4 + i < rows ? min(it.past + t, it.keys - 1) : -1;
         low[i] = a.window > 0 ? max(it.past + t - a.window + 1, 0) : 0;
     }
-    const int last = min(it.past + (m0 + rows - 1) / a.G, it.keys - 1);
-    const int first = it.first / PF_KEYS * PF_KEYS;
+    int last = min(it.past + (m0 + rows - 1) / a.G, it.keys - 1);
+    int first = it.first / PF_KEYS * PF_KEYS;
+    if (gridDim.y > 1) {  // this block's share of the tiles
+        const int tiles = last >= first ? (last - first) / PF_KEYS + 1 : 0;
+        const int per = (tiles + gridDim.y - 1) / gridDim.y * PF_KEYS;
+        first += blockIdx.y * per;
+        last = min(last, first + per - 1);
+    }
     // keys that every row of the block sees
     const int all1 = min(it.past + m0 / a.G, it.keys - 1);
     const int all0 = a.window > 0 ? it.past + (m0 + rows - 1) / a.G - a.window + 1 : 0;
@@ -109,8 +116,8 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
             float t = top[i];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                float x = s[i][j] * a.scale;
-                if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
+                float x = s[i][j] * (a.softcap > 0.f ? a.scale / a.softcap : a.scale * log2e);
+                if (a.softcap > 0.f) x = a.softcap * log2e * tanhf(x);
                 const int key = kt + tx + 16 * j;
                 if (key < low[i] || key > lim[i]) x = -INFINITY;
                 s[i][j] = x;
@@ -120,19 +127,18 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
             for (int w = 8; w; w >>= 1) t = fmaxf(t, __shfl_xor_sync(FULL, t, w));
             // scores of -inf weigh nothing, whatever the maximum
             const float from = t == -INFINITY ? 0.f : t;
-            const float fix = top[i] == -INFINITY ? 0.f : expf(top[i] - from);
+            const float fix = top[i] == -INFINITY ? 0.f : exp2f(top[i] - from);
             top[i] = t;
             float l = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float p = expf(s[i][j] - from);
+                const float p = exp2f(s[i][j] - from);
                 l += p;
                 sp[(ty * 4 + i) * LP + tx + 16 * j] = p;
             }
 #pragma unroll
             for (int w = 8; w; w >>= 1) l += __shfl_xor_sync(FULL, l, w);
             sum[i] = sum[i] * fix + l;
-            // (a sum that is not finite stays so: zero is kept as zero)
 #pragma unroll
             for (int c = 0; c < CN; c++) o[i][c] *= fix;
         }
@@ -163,6 +169,14 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
     for (int i = 0; i < 4; i++) {
         const int m = ty * 4 + i;
         if (m >= rows) continue;
+        if (gridDim.y > 1) {
+            const size_t at = ((size_t)blockIdx.x * gridDim.y + blockIdx.y) * PF_ROWS + m;
+            if (tx == 0) a.ml[at] = make_float2(top[i], last < first ? -1.f : sum[i]);
+#pragma unroll
+            for (int c = 0; c < CN; c++)
+                if (tx + 16 * c < a.dp) a.part[at * a.dp + tx + 16 * c] = o[i][c];
+            continue;
+        }
         const int t = (m0 + m) / a.G, g = (m0 + m) - t * a.G;
         const float inv = sum[i] > 0.f || sum[i] != sum[i] ? 1.f / sum[i] : 0.f;
         T* out = (T*)a.out + ((long long)(it.row0 + t) * a.H + head * a.G + g) * a.D;
@@ -174,6 +188,23 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
     }
 }
 
+// Joins the shares of each block's rows, a warp per row.
+template <typename T>
+__global__ void __launch_bounds__(PF_THREADS)
+    k_prompt_split_join(const __grid_constant__ PromptArgs a, int splits) {
+    const int m = blockIdx.y * (PF_THREADS / 32) + (threadIdx.x >> 5);
+    const int per = (a.bt * a.G + PF_ROWS - 1) / PF_ROWS;
+    const int head = blockIdx.x % a.K, block = blockIdx.x / a.K;
+    pdl_trigger();
+    pdl_wait();
+    const PromptItem it = prompt_item(a, a.slots - 1 - block / per);
+    const int row = block % per * PF_ROWS + m;
+    if (row >= it.rows * a.G) return;
+    const int t = row / a.G, g = row - t * a.G;
+    prompt_join_row(a, splits, (T*)a.out + ((long long)(it.row0 + t) * a.H + head * a.G + g) * a.D,
+                    [&](int i) { return ((size_t)blockIdx.x * splits + i) * PF_ROWS + m; });
+}
+
 template <typename T, int DP> static int prompt_go(cw_ctx* ctx, PromptArgs& a) {
     auto kern = k_prompt<T, DP>;
     const size_t smem = ((size_t)(PF_ROWS + PF_KEYS) * (DP + 4) + PF_ROWS * (PF_KEYS + 4)) * 4;
@@ -182,7 +213,25 @@ template <typename T, int DP> static int prompt_go(cw_ctx* ctx, PromptArgs& a) {
     a.slots = a.n_rows / a.bt + a.n_req;
     const long long grid = (long long)a.slots * ((a.bt * a.G + PF_ROWS - 1) / PF_ROWS) * a.K;
     CW_CHECK(grid < (1ll << 31), CW_ERR_UNSUPPORTED, "cw_prompt_attention: too many rows");
-    CW_TRY(launch_pdl(ctx, true, kern, dim3((unsigned)grid), dim3(PF_THREADS), smem, a));
+    // few blocks over many keys share them out, four tiles each at least (what is left of a
+    // call on the tensor cores is rare, and whole)
+    int splits = 1;
+    if (!a.amax && grid < ctx->sm_count) {
+        splits = (int)std::min<long long>({2ll * ctx->sm_count / grid, a.n_keys / (4 * PF_KEYS), 64});
+        splits = std::max(splits, 1);
+    }
+    if (splits > 1) {
+        a.dp = (a.D + 7) / 8 * 8;
+        const size_t rows = (size_t)grid * splits * PF_ROWS;
+        CW_TRY(stream_scratch(ctx, &ctx->prompt_scratch, &ctx->prompt_scratch_bytes,
+                              rows * a.dp * 4 + rows * 8, "cw_prompt_attention"));
+        a.part = (float*)ctx->prompt_scratch;
+        a.ml = (float2*)(a.part + rows * a.dp);
+    }
+    CW_TRY(launch_pdl(ctx, true, kern, dim3((unsigned)grid, splits), dim3(PF_THREADS), smem, a));
+    if (splits > 1)
+        CW_TRY(launch_pdl(ctx, true, k_prompt_split_join<T>, dim3((unsigned)grid, PF_ROWS / (PF_THREADS / 32)),
+                          dim3(PF_THREADS), 0, a, splits));
     return check_launch("prompt_attention");
 }
 template <typename T> static int prompt_dims(cw_ctx* ctx, PromptArgs& a) {

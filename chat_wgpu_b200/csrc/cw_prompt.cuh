@@ -118,6 +118,59 @@ template <> __device__ __forceinline__ float pr_to(float x) { return x; }
 template <> __device__ __forceinline__ __half pr_to(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 pr_to(float x) { return __float2bfloat16_rn(x); }
 
+// A row's result from its pieces, by a warp: out = sum_i w_i o_i / sum_i w_i l_i, w_i = 2^(m_i -
+// max m), in key order; place(i) is piece i's row in part and ml.  A lane holds a piece's
+// weight, then four dims (eight past 128) of every piece.  Bound by its dependent reads.
+template <typename T, typename F>
+__device__ __forceinline__ void prompt_join_row(const PromptArgs& a, int count, T* out, F piece) {
+    const int lane = threadIdx.x & 31;
+    float top = -INFINITY, l = 0.f;
+    for (int i = lane; i < count; i += 32) {
+        const float2 x = a.ml[piece(i)];
+        if (!(x.y < 0.f)) top = fmaxf(top, x.x);
+    }
+    top = warp_max(top);
+    float4 o[2] = {};
+    for (int i0 = 0; i0 < count; i0 += 32) {
+        float w = 0.f;
+        bool live = false;  // had a tile: a piece without weight keeps the NaN of its values
+        if (i0 + lane < count) {
+            const float2 x = a.ml[piece(i0 + lane)];
+            live = !(x.y < 0.f);
+            if (live && x.x != -INFINITY) w = exp2f(x.x - top);
+            if (live && x.y != 0.f) l += x.y * w;
+        }
+        const unsigned on = __ballot_sync(FULL, live);
+        const int n = min(32, count - i0);
+#pragma unroll 4
+        for (int i = 0; i < n; i++) {
+            const float wi = __shfl_sync(FULL, w, i);
+            if (!(on >> i & 1)) continue;
+            const float* from = a.part + piece(i0 + i) * a.dp;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int d = h * 128 + lane * 4;
+                if (d >= a.dp) continue;
+                const float4 x = *(const float4*)(from + d);
+                o[h].x = fmaf(wi, x.x, o[h].x);
+                o[h].y = fmaf(wi, x.y, o[h].y);
+                o[h].z = fmaf(wi, x.z, o[h].z);
+                o[h].w = fmaf(wi, x.w, o[h].w);
+            }
+        }
+    }
+    l = warp_sum(l);
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const float y[4] = {o[h].x, o[h].y, o[h].z, o[h].w};
+        const int d = h * 128 + lane * 4;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (d + e < a.D) out[d + e] = pr_to<T>(inv == 0.f ? 0.f : y[e] * inv);
+    }
+}
+
 // cw_prompt_tc.cu: on the tcgen05 tensor cores, where the shape allows it.  For f32 the
 // items that pr_odd leaves out are the caller's (a.amax and a.q_back are set).
 bool prompt_tc_takes(const PromptArgs& a, uint32_t type);

@@ -33,9 +33,6 @@
 #include "cw_tree_tc.cuh"
 
 namespace cw {
-#ifndef MINR
-#define MINR 256
-#endif
 
 constexpr int PT_KEYS = 128;    // keys of a tile
 constexpr int PT_RING = 3;      // items found ahead
@@ -1025,9 +1022,7 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
     }
 }
 
-// Joins the pieces of the items that a run's end cut: out = sum_i w_i o_i / sum_i w_i l_i,
-// w_i = 2^(m_i - max m), in key order.  A warp per row: a lane holds a piece's weight, then four
-// dims (eight past 128) of every piece.  Bound by the latency of its dependent reads.
+// Joins the pieces of the items that a run's end cut, a warp per row.
 constexpr int PJ_WARPS = 8;
 template <typename T>
 __global__ void __launch_bounds__(PJ_WARPS * 32)
@@ -1035,58 +1030,13 @@ __global__ void __launch_bounds__(PJ_WARPS * 32)
     pdl_trigger();
     pdl_wait();
     const PromptPiece p = a.pieces[blockIdx.x];
-    const int lane = threadIdx.x & 31, m = blockIdx.y * PJ_WARPS + (threadIdx.x >> 5);
+    const int m = blockIdx.y * PJ_WARPS + (threadIdx.x >> 5);
     const int r = m & 127, tok = (m >> 7) * tpb + r / a.G;
     if (p.count <= 1 || r >= tpb * a.G || tok >= p.rows) return;
-    auto piece = [&](int i) {
-        return ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? p.slot : 0)) * rows + m;
-    };
-    float top = -INFINITY, l = 0.f;
-    for (int i = lane; i < p.count; i += 32) {
-        const float2 x = a.ml[piece(i)];
-        if (!(x.y < 0.f)) top = fmaxf(top, x.x);
-    }
-    top = warp_max(top);
-    float4 o[2] = {};
-    for (int i0 = 0; i0 < p.count; i0 += 32) {
-        float w = 0.f;
-        bool live = false;  // had a tile: a piece without weight keeps the NaN of its values
-        if (i0 + lane < p.count) {
-            const float2 x = a.ml[piece(i0 + lane)];
-            live = !(x.y < 0.f);
-            if (live && x.x != -INFINITY) w = exp2f(x.x - top);
-            if (live && x.y != 0.f) l += x.y * w;
-        }
-        const unsigned on = __ballot_sync(FULL, live);
-        const int n = min(32, p.count - i0);
-#pragma unroll 4
-        for (int i = 0; i < n; i++) {
-            const float wi = __shfl_sync(FULL, w, i);
-            if (!(on >> i & 1)) continue;
-            const float* from = a.part + piece(i0 + i) * a.dp;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int d = h * 128 + lane * 4;
-                if (d >= a.dp) continue;
-                const float4 x = *(const float4*)(from + d);
-                o[h].x = fmaf(wi, x.x, o[h].x);
-                o[h].y = fmaf(wi, x.y, o[h].y);
-                o[h].z = fmaf(wi, x.z, o[h].z);
-                o[h].w = fmaf(wi, x.w, o[h].w);
-            }
-        }
-    }
-    l = warp_sum(l);
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     T* out = (T*)a.out + ((long long)(p.row0 + tok) * a.H + p.head * a.G + r - r / a.G * a.G) * a.D;
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const float y[4] = {o[h].x, o[h].y, o[h].z, o[h].w};
-        const int d = h * 128 + lane * 4;
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (d + e < a.D) out[d + e] = pr_to<T>(inv == 0.f ? 0.f : y[e] * inv);
-    }
+    prompt_join_row(a, p.count, out, [&](int i) {
+        return ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? p.slot : 0)) * rows + m;
+    });
 }
 
 static PFN_cuTensorMapEncodeTiled_v12000 pt_encode_fn() {
@@ -1225,7 +1175,9 @@ __global__ void __launch_bounds__(PS_WARPS * 32)
 bool prompt_tc_takes(const PromptArgs& a, uint32_t type) {
     if (a.G > 128 || !(a.scale > 0.f)) return false;
     if (type == CW_GGUF_F32)  // any place and stride; the pairs are laid out anew
-        return a.D <= 128 && (long long)a.n_rows >= MINR;
+        // (short prompts take fewer launches on the f32 kernel; us there and here: one of 64
+        // tokens 24 and 34, of 128 39 and 35, of 2048 737 and 104)
+        return a.D <= 128 && (long long)a.n_keys >= 96ll * a.n_req;
     const long long strides = (a.n_rows > 1 ? a.q_stride : 0) |
                               (a.n_keys > 1 ? a.k_stride | a.v_stride : 0);
     return a.D % 8 == 0 && strides % 8 == 0 &&

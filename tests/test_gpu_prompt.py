@@ -90,6 +90,16 @@ CASES = [  # dtype, heads, kv, dim, rows, keys (None: the rows), options
     ("bf16", 64, 1, 64, [40, 5], None, {}),
     ("f16", 130, 1, 64, [7], None, {}),
     ("bf16", 4, 2, 200, [140], [150], dict(window=33)),
+    # few rows over many keys, which are cut and joined
+    ("bf16", 32, 8, 128, [1], [3000], {}),
+    ("bf16", 32, 8, 128, [3, 0, 40, 1], [2100, 5, 1300, 2], {}),
+    ("f16", 8, 4, 256, [5, 70], [2000, 1500], dict(window=700, softcap=20.0)),
+    ("f16", 14, 2, 64, [19], [1700], {}),
+    ("f32", 16, 8, 128, [3], [2500], {}),
+    ("f32", 16, 8, 40, [90, 7], [1200, 1900], dict(softcap=15.0)),
+    ("f32", 8, 4, 256, [2, 9], [1800, 900], {}),
+    ("f32", 2, 2, 130, [4], [1400], dict(window=600, pad=3, off=1)),
+    ("bf16", 3, 1, 128, [40], [1500], dict(pad=3, off=1)),
 ]
 
 
@@ -138,6 +148,25 @@ def test_prompt_not_finite(ctx, dtype, D):
     bad = np.zeros(got.shape, bool)
     bad[198:200, :2] = bad[170:200, 2:, 3] = bad[190:200, 2:, 5] = bad[349, :2, 0] = True
     assert np.abs(got[~bad] - clean[~bad]).max() <= tol
+
+
+@pytest.mark.parametrize("dtype,D", [("f32", 128), ("f32", 200), ("f16", 256), ("bf16", 64)])
+def test_prompt_pieces_not_finite(ctx, dtype, D):
+    """Cut items: what is not finite reaches the rows that see it, whichever piece it is in; a
+    piece whose keys all score -inf keeps the NaN of 0 times an infinite value."""
+    H, K = 2, 1
+    c = make(np.random.default_rng(8), [4], [2600], dtype, H, K, D)
+    c["q"][:, :, 0] = 1.0
+    c["k"][:900, :, 0] = -np.inf
+    want, s, v = prompt_ref.attention(c["q"], c["k"], c["v"], c["starts"], c["ks"], 0, 0.0, D ** -0.5, c["q"])
+    c["v"][300, 0, 5] = np.inf     # weighs nothing: NaN
+    c["v"][1500, 0, 9] = np.inf    # weighs something
+    c["v"][2599, 0, 1] = np.nan    # the last row alone sees it
+    c["k"][2598, 0, 2] = np.nan    # the last two rows see it
+    got = run(ctx, c, dtype)
+    assert np.isnan(got[:, :, 5]).all() and (got[:2, :, 9] == np.inf).all() and np.isnan(got[2:]).all()
+    rest = np.setdiff1d(np.arange(D), [5, 9])
+    assert np.abs(got[:2][:, :, rest] - want[:2][:, :, rest]).max() <= tolerance(dtype, s, v, 2600)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
