@@ -8,13 +8,19 @@ would have produced itself are kept, so the tokens are those of plain greedy dec
 (model.generate_op_by_op) in fewer steps.  Drafts come from the session's own text:
 what followed the last occurrences of its last tokens.
 
-    python -m chat_wgpu_b200.treedecode model.gguf 1 5 9 2 --new 32
+TreeDecoder.prefill takes whole prompts in at once, whatever their lengths: per layer
+cw_norm_rope writes their keys and values and cw_prompt_attention lets each token see its
+own prompt up to itself.  With penalties, biases or a set of allowed tokens
+cw_adjust_logits chooses the step's tokens.
+
+    python -m chat_wgpu_b200.treedecode model.gguf 1 5 9 2 --new 32 --prefill --repetition 1.1
 """
 from __future__ import annotations
 
 import numpy as np
 
-from .kernels import activation, argmax, attention, norm, pages, q4, rope, tree
+from .kernels import (activation, argmax, attention, logits as rules, norm, pages, prompt, q4, rope,
+                      tree)
 from .model import OpByOpQwen3
 
 
@@ -51,10 +57,12 @@ class Session:
 
 
 class TreeDecoder:
-    """Several sessions of one OpByOpQwen3 stepped together."""
+    """Several sessions of one OpByOpQwen3 stepped together.  penalties = (repetition,
+    frequency, presence), biases = {token: value} and allowed = token ids (None: all) apply
+    to every session's logits; the repetition penalty counts the prompt, too."""
 
     def __init__(self, model: OpByOpQwen3, prompts, max_seq: int, page_size: int = 16,
-                 chunk: int = 64, draft=lookup_draft):
+                 chunk: int = 64, draft=lookup_draft, penalties=None, biases=None, allowed=None):
         if not prompts or any(len(p) == 0 for p in prompts):
             raise ValueError("every session needs a prompt")
         if not 1 <= chunk <= 1024:
@@ -73,13 +81,19 @@ class TreeDecoder:
         self.table = self._i32(np.full((n, self.max_pages), -1))
         self.plan = rope.rope_plan(self.ctx, model.head_dim, model.rope_theta)
         self.steps = 0
+        self.penalties, self.biases, self.mask = penalties, dict(biases or {}), None
+        if allowed is not None:
+            bits = np.zeros(-(-model.vocab // 32) * 32, np.uint8)
+            bits[list(allowed)] = 1
+            self.mask = self.ctx.storage_u32(np.packbits(bits, bitorder="little").view(np.uint32))
 
     def close(self) -> None:
         for k, v in self.cache:
             k.release()
             v.release()
-        for b in (self.table, self.plan):
-            b.release()
+        for b in (self.table, self.plan, self.mask):
+            if b is not None:
+                b.release()
         self.cache = []
 
     def _i32(self, a):
@@ -92,10 +106,49 @@ class TreeDecoder:
         held = [rows[i, :-(-s.stored // self.page)] for i, s in enumerate(self.sessions)]
         return np.setdiff1d(np.arange(self.n_pages), np.concatenate(held))
 
+    def _place(self, lens, news, T, depths=None):
+        """Pages, positions and slots of a step's T rows; the buffers, to be released."""
+        ctx, n = self.ctx, len(lens)
+        free = self._free_pages()
+        given = [self._i32(a) for a in (lens, news, free)]
+        deep = None if depths is None else self._i32(depths)
+        out = {k: self._i32(np.zeros(c)) for k, c in dict(starts=n + 1, positions=T, slots=T,
+                                                          owners=T, used=1).items()}
+        pages.PagePlan(ctx, lens=given[0], news=given[1], free_pages=given[2], table=self.table,
+                       depths=deep, n_req=n, page_size=self.page, max_pages=self.max_pages,
+                       n_free=len(free), max_tokens=T, **out)()
+        out.update(lens=given[0], news=given[1], free=given[2])
+        if deep is not None:
+            out["depths"] = deep
+        return out
+
+    def _layers(self, rows, attend):
+        """Hidden rows of the tokens after the layers; attend(q, k, v, layer, cache) gives the
+        attention's rows."""
+        m, ctx, T = self.m, self.ctx, len(rows)
+        dim = m.dim
+        x = ctx.empty(T * dim)
+        for i, t in enumerate(rows):
+            ctx.copy(m.embed_tbl, int(t) * dim, x, i * dim, dim)
+        for l, cache in zip(m.layers, self.cache):
+            a = norm.rmsnorm(ctx, x, l["attn_norm"], T, dim, m.eps)
+            o = attend(self._proj(l["wq"], a, T), self._proj(l["wk"], a, T),
+                       self._proj(l["wv"], a, T), l, cache)
+            x = attention.add(ctx, x, self._proj(l["wo"], o, T), T * dim)
+            a = norm.rmsnorm(ctx, x, l["ffn_norm"], T, dim, m.eps)
+            act = activation.swiglu(ctx, self._proj(l["gate"], a, T), self._proj(l["up"], a, T),
+                                    T * m.hidden)
+            x = attention.add(ctx, x, self._proj(l["down"], act, T), T * dim)
+        return x
+
+    def _proj(self, w, a, T):
+        buf, in_f, out_f = w
+        return q4.q4_0_gemm(self.ctx, a, buf, T, in_f, out_f)
+
     def _forward(self, rows, lens, news, depths, see):
         """Logits [rows, vocab] buffer of the step's nodes."""
         m, ctx, T, n = self.m, self.ctx, len(rows), len(lens)
-        free = self._free_pages()
+        nh, nkv, hd = m.n_heads, m.n_kv_heads, m.head_dim
         most = int(news.max())
         words = -(-most // 32)
         bits = np.zeros((T, words * 32), np.uint8)
@@ -103,51 +156,94 @@ class TreeDecoder:
         for r in range(n):
             bits[start:start + news[r], :news[r]] = see[r]
             start += int(news[r])
-        temp = [self._i32(a) for a in (lens, news, free, depths)]
-        outs = [self._i32(np.zeros(k)) for k in (n + 1, T, T, T, 1)]
+        at = self._place(lens, news, T, depths)
         mask = ctx.storage_u32(np.packbits(bits, axis=1, bitorder="little").view(np.uint32))
-        starts, pos, slots, owners, used = outs
-        pages.PagePlan(ctx, lens=temp[0], news=temp[1], free_pages=temp[2], table=self.table,
-                       depths=temp[3], starts=starts, positions=pos, slots=slots, owners=owners,
-                       used=used, n_req=n, page_size=self.page, max_pages=self.max_pages,
-                       n_free=len(free), max_tokens=T)()
-        nh, nkv, hd, dim = m.n_heads, m.n_kv_heads, m.head_dim, m.dim
-        x = ctx.empty(T * dim)
-        for i, t in enumerate(rows):
-            ctx.copy(m.embed_tbl, int(t) * dim, x, i * dim, dim)
 
-        def proj(w, a):
-            buf, in_f, out_f = w
-            return q4.q4_0_gemm(ctx, a, buf, T, in_f, out_f)
-
-        for l, (kc, vc) in zip(m.layers, self.cache):
-            a = norm.rmsnorm(ctx, x, l["attn_norm"], T, dim, m.eps)
-            q = norm.rmsnorm(ctx, proj(l["wq"], a), l["q_norm"], T * nh, hd, m.eps)
-            k = norm.rmsnorm(ctx, proj(l["wk"], a), l["k_norm"], T * nkv, hd, m.eps)
-            rope.RopeAppend(ctx, plan=self.plan, positions=pos, dtype="f32", n_tokens=T,
-                            n_heads=nh, n_kv=nkv, head_dim=hd, q=q, q_out=q, k=k,
-                            v=proj(l["wv"], a), slots=slots, k_cache=kc, v_cache=vc,
-                            page_size=self.page, n_pages=self.n_pages)()
+        def attend(q, k, v, l, cache):
+            kc, vc = cache
+            q = norm.rmsnorm(ctx, q, l["q_norm"], T * nh, hd, m.eps)
+            k = norm.rmsnorm(ctx, k, l["k_norm"], T * nkv, hd, m.eps)
+            rope.RopeAppend(ctx, plan=self.plan, positions=at["positions"], dtype="f32", n_tokens=T,
+                            n_heads=nh, n_kv=nkv, head_dim=hd, q=q, q_out=q, k=k, v=v,
+                            slots=at["slots"], k_cache=kc, v_cache=vc, page_size=self.page,
+                            n_pages=self.n_pages)()
             o = ctx.empty(T * nh * hd)
-            tree.TreeAttention(ctx, q=q, k_cache=kc, v_cache=vc, table=self.table, lens=temp[0],
-                               starts=starts, mask=mask, out=o, dtype="f32", n_req=n, n_rows=T,
+            tree.TreeAttention(ctx, q=q, k_cache=kc, v_cache=vc, table=self.table, lens=at["lens"],
+                               starts=at["starts"], mask=mask, out=o, dtype="f32", n_req=n, n_rows=T,
                                max_nodes=most, n_heads=nh, n_kv=nkv, head_dim=hd,
                                page_size=self.page, n_pages=self.n_pages,
                                max_pages=self.max_pages)()
-            x = attention.add(ctx, x, proj(l["wo"], o), T * dim)
-            a = norm.rmsnorm(ctx, x, l["ffn_norm"], T, dim, m.eps)
-            act = activation.swiglu(ctx, proj(l["gate"], a), proj(l["up"], a), T * m.hidden)
-            x = attention.add(ctx, x, proj(l["down"], act), T * dim)
-        logits = proj(m.lm_head, norm.rmsnorm(ctx, x, m.final_norm, T, dim, m.eps))
-        for b in temp + outs + [mask]:
+            return o
+
+        x = self._layers(rows, attend)
+        logits = self._proj(m.lm_head, norm.rmsnorm(ctx, x, m.final_norm, T, m.dim, m.eps), T)
+        for b in list(at.values()) + [mask]:
             b.release()
         return logits
+
+    def prefill(self) -> None:
+        """The prompts of the sessions that no step has run yet, but for their last tokens, in
+        one pass: packed rows, each prompt's own length."""
+        m, ctx = self.m, self.ctx
+        nh, nkv, hd = m.n_heads, m.n_kv_heads, m.head_dim
+        news = np.array([0 if s.stored else s.n_prompt - 1 for s in self.sessions])
+        T, n = int(news.sum()), len(news)
+        if T == 0:
+            return
+        ctx.reset_frame()
+        at = self._place(np.array([s.stored for s in self.sessions]), news, T)
+
+        def attend(q, k, v, l, cache):
+            k_rows, o = ctx.empty(T * nkv * hd), ctx.empty(T * nh * hd)
+            rope.NormRope(ctx, plan=self.plan, positions=at["positions"], dtype="f32", n_tokens=T,
+                          head_dim=hd, eps=m.eps, n_heads=nh, n_kv=nkv, q=q, q_norm=l["q_norm"],
+                          q_out=q, k=k, k_norm=l["k_norm"], k_out=k_rows, v=v, slots=at["slots"],
+                          k_cache=cache[0], v_cache=cache[1], page_size=self.page,
+                          n_pages=self.n_pages)()
+            prompt.PromptAttention(ctx, q=q, k=k_rows, v=v, starts=at["starts"], out=o, dtype="f32",
+                                   n_req=n, n_rows=T, n_heads=nh, n_kv=nkv, head_dim=hd)()
+            return o
+
+        self._layers([t for s, c in zip(self.sessions, news) for t in s.tokens[:c]], attend)
+        ctx.sync()
+        for b in at.values():
+            b.release()
+        for s, c in zip(self.sessions, news):
+            s.stored += int(c)
+
+    def _choose(self, logits, histories, leads):
+        """The token of each row of logits, which become the adjusted ones."""
+        ctx, T, vocab = self.ctx, len(histories), self.m.vocab
+        flat = lambda lists: [x for y in lists for x in y]  # noqa: E731
+        begin = lambda lists: np.concatenate([[0], np.cumsum([len(x) for x in lists])])  # noqa: E731
+        temp, more = {}, {}
+        if self.penalties is not None:
+            temp.update(penalties=ctx.storage(np.tile(np.float32(self.penalties), (T, 1))),
+                        tokens=self._i32(flat(histories)), starts=self._i32(begin(histories)),
+                        prompts=self._i32(leads))
+            more["n_tokens"] = sum(map(len, histories))
+        if self.biases:
+            pairs = [list(self.biases)] * T
+            temp.update(bias_tokens=self._i32(flat(pairs)), bias_starts=self._i32(begin(pairs)),
+                        bias_values=ctx.storage(np.tile(np.float32(list(self.biases.values())), T)))
+            more["n_bias"] = len(self.biases) * T
+        if self.mask is not None:
+            temp["mask_rows"] = self._i32(np.zeros(T))
+            more.update(masks=self.mask, n_masks=1)
+        temp["best"] = self._i32(np.zeros(T))
+        rules.AdjustLogits(ctx, logits=logits, out=logits, dtype="f32", n_rows=T, vocab=vocab, **temp,
+                           **more)()
+        best = ctx.read_u32(temp["best"], T).astype(np.int64)
+        for b in temp.values():
+            b.release()
+        return best
 
     def step(self, max_new: int, want_logits: bool = False):
         """One step of every session that still has tokens to produce; with
         want_logits the logits that each newly produced token was chosen from."""
         ctx, vocab = self.ctx, self.m.vocab
         rows, lens, news, depths, see, trees = [], [], [], [], [], []
+        histories, leads = [], []
         for s in self.sessions:
             open_ = s.tokens[s.stored:s.stored + self.chunk]
             done = len(s.produced) >= max_new
@@ -160,13 +256,18 @@ class TreeDecoder:
             c, m = len(open_), len(open_) + len(drafts)
             v = np.zeros((m, m), bool)
             depth = list(range(c))
+            text = []
             for i in range(c):
                 v[i, :i + 1] = True
-            for j, (parent, _) in enumerate(drafts):
+                text.append(s.tokens[:s.stored + i + 1])
+            for j, (parent, token) in enumerate(drafts):
                 up = c - 1 if parent < 0 else c + parent
                 v[c + j] = v[up]
                 v[c + j, c + j] = True
                 depth.append(depth[up] + 1)
+                text.append(text[up] + [token])
+            histories += text
+            leads += [s.n_prompt] * m
             rows += open_ + [t for _, t in drafts]
             lens.append(s.stored)
             news.append(m)
@@ -179,11 +280,14 @@ class TreeDecoder:
         lens, news = np.array(lens), np.array(news)
         logits = self._forward(rows, lens, news, np.array(depths), see)
         self.steps += 1
-        best = np.empty(len(rows), np.int64)
         row = ctx.empty(vocab)
-        for i in range(len(rows)):
-            ctx.copy(logits, i * vocab, row, 0, vocab)
-            best[i] = ctx.read_u32(argmax.argmax(ctx, row, vocab), 1)[0]
+        if self.penalties is not None or self.biases or self.mask is not None:
+            best = self._choose(logits, histories, leads)
+        else:
+            best = np.empty(len(rows), np.int64)
+            for i in range(len(rows)):
+                ctx.copy(logits, i * vocab, row, 0, vocab)
+                best[i] = ctx.read_u32(argmax.argmax(ctx, row, vocab), 1)[0]
         out, first = [], 0
         for s, (c, drafts), m in zip(self.sessions, trees, news):
             base, first = first, first + int(m)
@@ -226,9 +330,17 @@ def main() -> None:
     ap.add_argument("model")
     ap.add_argument("prompt", nargs="+", type=int)
     ap.add_argument("--new", type=int, default=32)
+    ap.add_argument("--prefill", action="store_true", help="take the prompt in as one pass")
+    ap.add_argument("--repetition", type=float, default=1.0)
+    ap.add_argument("--frequency", type=float, default=0.0)
+    ap.add_argument("--presence", type=float, default=0.0)
     a = ap.parse_args()
+    penalties = (a.repetition, a.frequency, a.presence)
     with GpuContext(0) as ctx:
-        d = TreeDecoder(OpByOpQwen3(ctx, a.model), [a.prompt], len(a.prompt) + a.new)
+        d = TreeDecoder(OpByOpQwen3(ctx, a.model), [a.prompt], len(a.prompt) + a.new,
+                        penalties=None if penalties == (1.0, 0.0, 0.0) else penalties)
+        if a.prefill:
+            d.prefill()
         print(*d.generate(a.new)[0])
         print(f"{a.new} tokens in {d.steps} steps")
         d.close()
