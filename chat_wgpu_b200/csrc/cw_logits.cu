@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(LG_THREADS, 2) k_adjust_logits(const __grid_co
     };
     extern __shared__ __align__(16) uint32_t sm[];
     __shared__ unsigned long long s_key[LG_THREADS / 32], s_all[16];
-    __shared__ int s_sum[LG_THREADS / 32];
+    __shared__ int s_sum[LG_THREADS / 32], s_n;
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     if (a.best) cluster.barrier_arrive();  // waited for before a CTA writes to another's memory
@@ -79,7 +79,8 @@ __global__ void __launch_bounds__(LG_THREADS, 2) k_adjust_logits(const __grid_co
     uint32_t* s_rank = s_bits + words;    // [words] bits set before the word
     uint32_t* s_count = s_rank + words;   // [LG_TOKENS] of the listed tokens, in order
     int* s_place = (int*)s_count + LG_TOKENS;  // where they are in the slice
-    uint32_t* s_last = s_count + 2 * LG_TOKENS;  // and their last bias entry, counted from 1
+    uint32_t* s_mine = s_count + 2 * LG_TOKENS;  // the history's tokens that lie here, if few
+    uint32_t* s_last = s_count + 3 * LG_TOKENS;  // and their last bias entry, counted from 1
     pdl_wait();
     pdl_trigger();
     const T* in = (const T*)a.logits + r * a.stride;
@@ -136,13 +137,13 @@ __global__ void __launch_bounds__(LG_THREADS, 2) k_adjust_logits(const __grid_co
     // f(place in [u0, u1), entry) for the tokens [x, y) of a list that lie there
     int u0 = 0, u1 = 0;
     auto each = [&](const int* tokens, int x, int y, auto f) {
-        for (int i = x + tid; i < y; i += 4 * LG_THREADS) {
-            int t[4];
+        for (int i = x + tid; i < y; i += 8 * LG_THREADS) {
+            int t[8];
 #pragma unroll
-            for (int k = 0; k < 4; k++)
+            for (int k = 0; k < 8; k++)
                 t[k] = i + k * LG_THREADS < y ? tokens[i + k * LG_THREADS] : INT_MAX;
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
+            for (int k = 0; k < 8; k++) {
                 if (i + k * LG_THREADS >= y) break;
                 if (t[k] < 0 || t[k] >= a.vocab) {
                     if (cta == 0) lg_bad(a);
@@ -165,12 +166,22 @@ __global__ void __launch_bounds__(LG_THREADS, 2) k_adjust_logits(const __grid_co
         if (hist || bias) {
             __syncthreads();  // what went before has been read
             for (int i = tid; i < words; i += LG_THREADS) s_bits[i] = 0;
+            if (tid == 0) s_n = 0;
             __syncthreads();
             auto mark = [&](int j, int) {
                 const uint32_t bit = 1u << (j & 31);
                 if (!(*(volatile uint32_t*)&s_bits[j >> 5] & bit)) atomicOr(&s_bits[j >> 5], bit);
             };
-            each(a.tokens, h0, h1, mark);
+            each(a.tokens, h0, h1, [&](int j, int i) {
+                mark(j, i);
+                // kept for the count, so that it need not go through the history again
+                const unsigned among = __activemask();
+                const int first = __ffs(among) - 1, mine = __popc(among & ((1u << (tid & 31)) - 1));
+                int k = 0;
+                if ((tid & 31) == first) k = atomicAdd(&s_n, __popc(among));
+                k = __shfl_sync(among, k, first) + mine;
+                if (k < LG_TOKENS) s_mine[k] = (uint32_t)j | (i - h0 < lead ? LG_LED : 0u);
+            });
             each(a.bias_tokens, b0, b1, mark);
             __syncthreads();
             // ranks: a thread's words, then its place among the threads
@@ -205,12 +216,18 @@ __global__ void __launch_bounds__(LG_THREADS, 2) k_adjust_logits(const __grid_co
                 if (a.bias_starts) s_last[i] = 0;
             }
             __syncthreads();
-            each(a.tokens, h0, h1, [&](int j, int i) {
+            auto count = [&](int j, bool led) {
                 const int k = rank(j);
                 s_place[k] = j;
-                if (i - h0 < lead) atomicOr(&s_count[k], LG_LED);
+                if (led) atomicOr(&s_count[k], LG_LED);
                 else atomicAdd(&s_count[k], 1u);
-            });
+            };
+            if (s_n <= LG_TOKENS) {
+                for (int i = tid; i < s_n; i += LG_THREADS)
+                    count((int)(s_mine[i] & ~LG_LED), (s_mine[i] & LG_LED) != 0);
+            } else {
+                each(a.tokens, h0, h1, [&](int j, int i) { count(j, i - h0 < lead); });
+            }
             each(a.bias_tokens, b0, b1, [&](int j, int i) {
                 const int k = rank(j);
                 s_place[k] = j;
@@ -333,8 +350,8 @@ template <typename T> static int adjust_launch(cw_ctx* ctx, LogitArgs& a, bool w
     const int ctas = std::max(1, std::min({16, many, span / (LG_THREADS * 4)}));
     a.slice = std::min(128 * 1024, ((span + ctas - 1) / ctas + 31) / 32 * 32);
     const bool lists = a.penalties || a.bias_starts;
-    const size_t smem = lists ? a.slice / 4 + (size_t)LG_TOKENS * 4 * (a.bias_starts ? 3 : 2) : 0;
-    CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024));
+    const size_t smem = lists ? a.slice / 4 + (size_t)LG_TOKENS * 4 * (a.bias_starts ? 4 : 3) : 0;
+    CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024));
     CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, a.n_rows);

@@ -48,11 +48,12 @@ __global__ void __launch_bounds__(NR_THREADS, C == 1 ? 3 : 1)
         T e[2 * VEC * C];
     };
     const int L = a.lanes, sub = threadIdx.x & (L - 1);
-    const unsigned long long row = ((unsigned long long)blockIdx.x * NR_THREADS + threadIdx.x) / L;
-    const unsigned long long t64 = row / a.groups;
+    // (whole 32-bit numbers: 64-bit divisions took a microsecond of a small call)
+    const unsigned row = blockIdx.x * (unsigned)(NR_THREADS / L) + threadIdx.x / L;
+    const unsigned at = row / (unsigned)a.groups;
     // every lane stays for the shuffles: one past the last token does its work unseen
-    const bool live = t64 < (unsigned long long)a.n_tokens;
-    const int t = live ? (int)t64 : a.n_tokens - 1, g = (int)(row - t64 * a.groups);
+    const bool live = at < (unsigned)a.n_tokens;
+    const int t = live ? (int)at : a.n_tokens - 1, g = (int)(row - at * a.groups);
     const int rot_chunks = a.rot / (2 * VEC);
     // the lane's chunks: vectors at e0 and e1, a pair's elements in different vectors (HALF)
     // or side by side; past the rotated part plain neighbours
@@ -76,8 +77,8 @@ __global__ void __launch_bounds__(NR_THREADS, C == 1 ? 3 : 1)
             slot = -1;
         }
         if (slot >= 0) {
-            const long long pg = slot / a.page;
-            dst0 = (pg * a.K * a.page + (slot - pg * a.page)) * a.D;
+            const int pg = (int)slot / a.page;
+            dst0 = ((long long)pg * a.K * a.page + ((int)slot - pg * a.page)) * a.D;
         }
     }
     const T* q = (const T*)a.q + t * a.q_stride;
@@ -193,7 +194,8 @@ static int norm_rope_go(cw_ctx* ctx, NormRopeArgs& a, bool half, int chunks) {
     a.groups = (a.heads + a.per - 1) / a.per;
     const unsigned long long n = (unsigned long long)a.n_tokens * a.lanes * a.groups;
     const unsigned long long blocks = (n + NR_THREADS - 1) / NR_THREADS;
-    CW_CHECK(blocks < (1ull << 31), CW_ERR_UNSUPPORTED, "cw_norm_rope: too many rows");
+    CW_CHECK(blocks < (1ull << 31) && (unsigned long long)a.n_tokens * a.groups < (1ull << 32) - 512,
+             CW_ERR_UNSUPPORTED, "cw_norm_rope: too many rows");
     // (vectors narrower than 16 bytes, and several chunks to a lane, are rare: checked only)
     constexpr bool CAN = C == 1 && VEC * sizeof(T) == 16;
     auto kern = half ? k_norm_rope<T, VEC, C, true, false> : k_norm_rope<T, VEC, C, false, false>;

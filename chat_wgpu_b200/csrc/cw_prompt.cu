@@ -49,6 +49,7 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
     constexpr int LP = PF_KEYS + 4;
     const float log2e = 1.44269504088896341f;  // scores are in powers of two
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int warp_row = (tid >> 5) * 8;  // the warp's first row
     const int head = blockIdx.x % a.K, block = blockIdx.x / a.K;
     pdl_wait();
     if (blockIdx.x == 0 && blockIdx.y == 0) prompt_check(a, tid, PF_THREADS);
@@ -94,22 +95,27 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
             return kt + j <= last ? kb + (long long)(kt + j) * a.k_stride : nullptr;
         });
         __syncthreads();
+        // of the tile only the keys there are, 16 to a column block, and only warps with rows
+        const int keys = min(PF_KEYS, last - kt + 1);
         float s[4][4] = {};
-        for (int d = 0; d < a.D; d += 4) {
-            float4 x[4], y[4];
+        if (warp_row < rows) {
+            for (int d = 0; d < a.D; d += 4) {
+                float4 x[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = *(const float4*)&sq[(ty * 4 + i) * LD + d];
-#pragma unroll
-            for (int j = 0; j < 4; j++) y[j] = *(const float4*)&skv[(tx + 16 * j) * LD + d];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
+                for (int i = 0; i < 4; i++) x[i] = *(const float4*)&sq[(ty * 4 + i) * LD + d];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    s[i][j] = fmaf(x[i].x, y[j].x, s[i][j]);
-                    s[i][j] = fmaf(x[i].y, y[j].y, s[i][j]);
-                    s[i][j] = fmaf(x[i].z, y[j].z, s[i][j]);
-                    s[i][j] = fmaf(x[i].w, y[j].w, s[i][j]);
+                    if (16 * j >= keys) break;
+                    const float4 y = *(const float4*)&skv[(tx + 16 * j) * LD + d];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        s[i][j] = fmaf(x[i].x, y.x, s[i][j]);
+                        s[i][j] = fmaf(x[i].y, y.y, s[i][j]);
+                        s[i][j] = fmaf(x[i].z, y.z, s[i][j]);
+                        s[i][j] = fmaf(x[i].w, y.w, s[i][j]);
+                    }
                 }
+            }
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
         });
         // a value that is not finite counts only where it is seen
         const bool careful = __syncthreads_or(mixed && odd);
-        for (int j = 0; j < PF_KEYS; j++) {
+        for (int j = 0; j < keys && warp_row < rows; j++) {
             float p[4], y[CN];
             bool see[4];
 #pragma unroll
