@@ -145,11 +145,9 @@ __global__ void __launch_bounds__(LG_THREADS, 2) k_adjust_logits(const __grid_co
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 if (i + k * LG_THREADS >= y) break;
-                if (t[k] < 0 || t[k] >= a.vocab) {
-                    if (cta == 0) lg_bad(a);
-                } else if (t[k] + shift >= u0 && t[k] + shift < u1) {
-                    f(t[k] + shift - u0, i + k * LG_THREADS);
-                }
+                const unsigned j = (unsigned)t[k] + (unsigned)shift - (unsigned)u0;
+                if (j < (unsigned)(u1 - u0) && t[k] >= 0) f((int)j, i + k * LG_THREADS);
+                else if (cta == 0 && (unsigned)t[k] >= (unsigned)a.vocab) lg_bad(a);
             }
         }
     };
