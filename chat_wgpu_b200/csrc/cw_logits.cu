@@ -349,8 +349,12 @@ template <typename T> static int adjust_launch(cw_ctx* ctx, LogitArgs& a, bool w
     a.slice = std::min(128 * 1024, ((span + ctas - 1) / ctas + 31) / 32 * 32);
     const bool lists = a.penalties || a.bias_starts;
     const size_t smem = lists ? a.slice / 4 + (size_t)LG_TOKENS * 4 * (a.bias_starts ? 4 : 3) : 0;
-    CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024));
-    CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    static bool set[2][64] = {};
+    if (!set[wide][ctx->device & 63]) {
+        CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024));
+        CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        set[wide][ctx->device & 63] = true;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, a.n_rows);
     cfg.blockDim = dim3(LG_THREADS);

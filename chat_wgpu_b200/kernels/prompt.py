@@ -19,6 +19,8 @@ class PromptAttention(Prepared):
                  key_starts: Buffer | None = None, n_keys: int | None = None, window: int = 0,
                  softcap: float = 0.0, scale: float = 0.0, q_off: int = 0, k_off: int = 0,
                  v_off: int = 0, q_stride: int = 0, k_stride: int = 0, v_stride: int = 0):
+        if key_starts is not None and n_keys is None:
+            raise ValueError("key_starts: how many key rows there are, n_keys, goes with it")
         kv = n_kv * head_dim
         super().__init__(
             ctx, dtype, q=q, k=k, v=v, starts=starts, key_starts=key_starts, out=out, q_off=q_off,

@@ -445,8 +445,13 @@ typedef struct {
  * f32.  16-bit types whose head_dim is a multiple of 8 and whose strides and places are
  * multiples of 16 bytes, with at most 128 query heads per kv head and a positive scale,
  * run on the tcgen05 tensor cores (there the softmax weights are rounded to the type
- * before the product with v).  Starts that descend or pass the buffers are cut to them
- * and reported. */
+ * before the product with v).  f32 with head_dim <= 128 and 96 keys a request or more runs
+ * there as pairs of f16, at f32 accuracy: what a value loses is below 2^-22 of it or 2^-39
+ * of the largest of its request and head.  Everything else runs in f32 products.  Starts
+ * that descend or pass the buffers are cut to them and reported.  Uses a context-owned
+ * scratch that grows on demand, in stream order: call once with a call's sizes before
+ * capturing it, and replay a captured call before the context is destroyed and in order
+ * with the context's other prompt attention calls. */
 int cw_prompt_attention(cw_ctx* ctx, const cw_prompt_attn_args* args);
 
 typedef struct {

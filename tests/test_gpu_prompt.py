@@ -261,8 +261,8 @@ def test_prompt_refusals(ctx):
                 dict(head_dim=257), dict(window=2 ** 31), dict(softcap=-1.0), dict(softcap=float("inf")),
                 dict(scale=float("nan")), dict(q_off=1), dict(k_off=1), dict(v_off=1), dict(q_stride=31),
                 dict(q_stride=33), dict(k_stride=15), dict(v_stride=17), dict(q=None), dict(k=None), dict(v=None),
-                dict(starts=None), dict(out=None), dict(out=q), dict(q=o), dict(k=o), dict(key_starts=b(2)),
-                dict(key_starts=o)):
+                dict(starts=None), dict(out=None), dict(out=q), dict(q=o), dict(k=o), dict(key_starts=b(2), n_keys=6),
+                dict(key_starts=o, n_keys=6)):
         with pytest.raises(CwError) as e:
             PromptAttention(ctx, **{**good, **bad})()
         assert e.value.status == 1, bad

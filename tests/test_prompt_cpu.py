@@ -55,7 +55,9 @@ def test_wrapped_tensors_of_another_type_or_layout_are_refused():
     rows = torch.zeros(5, 8 * 16, dtype=torch.bfloat16)
     q, k, v = (wrapped(t) for t in rows.split([64, 32, 32], dim=1))
     prompt = dict(q=q, k=k, v=v, starts=i(3), key_starts=i(3), out=x(5, 64), dtype="bf16", n_req=2, n_rows=5,
-                  n_heads=4, n_kv=2, head_dim=16, q_stride=128, k_stride=128, v_stride=128)
+                  n_heads=4, n_kv=2, head_dim=16, n_keys=5, q_stride=128, k_stride=128, v_stride=128)
+    with pytest.raises(ValueError, match="n_keys"):
+        PromptAttention(None, **{**prompt, "n_keys": None})
     heads = dict(plan=i(4), positions=i(5), dtype="bf16", n_tokens=5, head_dim=16, eps=1e-6, n_heads=4, n_kv=2, q=q,
                  k=k, v=v, q_norm=f(16), k_norm=f(16), q_out=x(5, 64), k_out=x(5, 32), slots=i(5),
                  k_cache=x(1, 2, 16, 16), v_cache=x(1, 2, 16, 16), page_size=16, n_pages=1, q_stride=128, k_stride=128,
