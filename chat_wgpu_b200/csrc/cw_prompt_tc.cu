@@ -527,18 +527,16 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                 if (i == t.b[b].lo) ok = ok && wait(&bars->q_full[b], q_count[b]++);
                 const uint32_t d = tmem + b * TCOLS + (NB == 2 ? 0 : sb * PT_KEYS);
                 TtPlace x = k;
-                uint32_t more = 0;
-                // q columns from column col of the block, times the stage at place x
-                auto product = [&](int col, const TtPlace& x, int from) {
+                // half h of q's columns times the stage at place x
+                auto product = [&](int h, const TtPlace& x, uint32_t more) {
                     const uint64_t dk = kv0 + ((x.stage * STAGE) >> 4);
-                    const uint64_t dq = q0 + ((b * Z::QBLOCK + col * Z::QCOL) >> 4);
+                    const uint64_t dq = q0 + ((b * Z::QBLOCK + h * COLS * Z::QCOL) >> 4);
 #pragma unroll
-                    for (int s = 0; s < COLS * 4; s++) {
-                        if (from + s >= steps) continue;
-                        umma_f16(d, dq + (((s >> 2) * Z::QCOL + (s & 3) * 32) >> 4),
-                                 dk + (((s >> 2) * tile.col + (s & 3) * 32) >> 4), id_s, more);
-                        more = 1;
-                    }
+                    for (int s = 0; s < COLS * 4; s++)
+                        if ((PAIR ? 0 : h * 8) + s < steps)
+                            umma_f16(d, dq + (((s >> 2) * Z::QCOL + (s & 3) * 32) >> 4),
+                                     dk + (((s >> 2) * tile.col + (s & 3) * 32) >> 4), id_s,
+                                     s > 0 ? 1u : more);
                 };
 #pragma unroll
                 for (int h = 0; h < HALVES; h++) {
@@ -548,10 +546,10 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                     // pairs: low parts of q times the high ones of k, high ones of q times the
                     // low ones of k, and the high ones of both last, since a sum is cut at each
                     // step by what it has grown to
-                    if (ok) product(PAIR ? (1 - h) * COLS : h * COLS, x, PAIR ? 0 : h * 8);
+                    if (ok) product(PAIR ? 1 - h : h, x, h > 0);
                     x.next(STAGES);
                 }
-                if (PAIR && ok) product(0, k, 0);
+                if (PAIR && ok) product(0, k, 1);
                 if (!ok) return;
                 tc_commit(&bars->s_full[sb]);
                 if (i + 1 == t.b[b].hi) tc_commit(&bars->q_empty[b]);
@@ -564,7 +562,7 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                     ok = ok && wait(&bars->full[x.stage], x.phase);
                 const uint32_t p = tmem + b * TCOLS + (NB == 2 ? 0 : sb * PT_KEYS);
                 const uint32_t o = tmem + b * TCOLS + SB * PT_KEYS + (PAIR ? (m & 1) * HD : 0);
-                const uint32_t before = i > t.b[b].lo;  // (pairs: a tile's sums alone)
+                const uint32_t before = !PAIR && i > t.b[b].lo;  // (pairs: a tile's sums alone)
                 bool skip = false;
 #pragma unroll
                 for (int part = 0; part < 2; part++) {
@@ -572,30 +570,30 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                     tc_fence_after();
                     if (!PAIR && part == 0 && t.b[b].mixed(i)) skip = *(volatile uint32_t*)&bars->skip[sb];
                     if (!ok || skip) continue;
-                    // 16 keys' weights (pairs: their low parts) times half h of the values
-                    auto product = [&](int s, int h, bool low, uint32_t more) {
-                        TtPlace y = v;
-                        if (h) y.next(STAGES);
-                        pt_mma_ts(PAIR ? o : o + h * 128,
-                                  p + (s >> 2) * (PT_KEYS / 2) + (s & 3) * 8 + (low ? 32 : 0),
-                                  kv0 + ((y.stage * STAGE + s * 2 * tile.group) >> 4),
-                                  id_o[PAIR ? 0 : h], more);
-                    };
+                    x = v;
 #pragma unroll
-                    for (int y = 0; y < 4; y++) {  // 32 keys of each half of the tile
-                        const int s = (y >> 1) * 4 + (1 - part) * 2 + (y & 1);
-                        if (PAIR) {
-                            product(s, 0, true, part + y > 0);
-                            product(s, 1, false, 1);
-                        } else {
+                    for (int h = 0; h < HALVES; h++) {
+                        if (h >= halves) continue;
+                        const uint64_t dv = kv0 + ((x.stage * STAGE) >> 4);
 #pragma unroll
-                            for (int h = 0; h < HALVES; h++)
-                                if (h < halves) product(s, h, false, part + y > 0 ? 1u : before);
+                        for (int y = 0; y < 4; y++) {  // 32 keys of each half of the tile
+                            const int s = (y >> 1) * 4 + (1 - part) * 2 + (y & 1);
+                            const uint64_t ds = dv + ((s * 2 * tile.group) >> 4);
+                            // pairs: low weights times high values, high weights times low ones
+                            pt_mma_ts(PAIR ? o : o + h * 128,
+                                      p + (s >> 2) * (PT_KEYS / 2) + (s & 3) * 8 +
+                                          (PAIR && h == 0 ? 32 : 0),
+                                      ds, id_o[PAIR ? 0 : h],
+                                      part + y + (PAIR ? h : 0) > 0 ? 1u : before);
                         }
+                        x.next(STAGES);
                     }
                     if (PAIR && part) {  // high times high last, as for the scores
+                        const uint64_t dv = kv0 + ((v.stage * STAGE) >> 4);
 #pragma unroll
-                        for (int s = 0; s < PT_KEYS / 16; s++) product(s, 0, false, 1);
+                        for (int s = 0; s < PT_KEYS / 16; s++)
+                            pt_mma_ts(o, p + (s >> 2) * (PT_KEYS / 2) + (s & 3) * 8,
+                                      dv + ((s * 2 * tile.group) >> 4), id_o[0], 1);
                     }
                 }
                 if (ok) tc_commit(&bars->pv[PAIR ? m & 1 : b]);
