@@ -24,7 +24,7 @@
 //
 // What bounds it: at 16384 bf16 tokens the products alone, with no softmax between them, take
 // 1.40 ms (1570 TFLOP/s, 0.94 of the measured burst peak), all of it 1.8 to 1.9 ms in short
-// runs and 2.15 ms in long ones, where the power limit lowers the clock.  The tensor pipe is
+// runs and 2.1 to 2.2 ms in long ones, where the power limit lowers the clock.  The tensor pipe is
 // active 55 to 60 % of the time, the special-function unit half of it; the rest is the chain
 // scores -> weights -> product of each row block.  Powers of two by polynomials on the FMA
 // pipe made it slower in every share tried (1/8 of them: 1.83 -> 1.88 ms; 3/8: 2.00 ms), as
@@ -37,7 +37,7 @@
 // to the row's by the threads (error against 64 bits at 4096 keys 7.1e-6 without either,
 // 6.8e-7 with both; a plain f32 form has 1.2e-6).  Bound by shared memory and the tensor
 // pipe: 128 rows take 416 KB of operands a tile through it, 3300 cycles at 128 bytes, for
-// 3072 cycles of products.  What does not fit pairs (infinities, NaN, magnitudes from 2^60)
+// 3100 cycles of products.  What does not fit pairs (infinities, NaN, magnitudes from 2^60)
 // is left to the f32 kernel, by request and kv head.
 //
 // Unseen keys weigh 0, but 0 times a value that is not finite is NaN.  So in the tiles
