@@ -13,6 +13,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cw_prompt.cuh"
 
@@ -54,6 +55,7 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
     const float log2e = 1.44269504088896341f;  // scores are in powers of two
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int warp_row = (tid >> 5) * 8;  // the warp's first row
+    auto col = [&](int c) { return tx * 4 + c / 4 * 64 + c % 4; };  // the thread's dims
     const int head = blockIdx.x % a.K, block = blockIdx.x / a.K;
     pdl_wait();
     if (blockIdx.x == 0 && blockIdx.y == 0) prompt_check(a, tid, PF_THREADS);
@@ -100,16 +102,16 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
         });
         __syncthreads();
         // of the tile only the keys there are, 16 to a column block, and only warps with rows
+        // (asked inside the loop, it made a row block of 256 dims 14 % slower)
         const int keys = min(PF_KEYS, last - kt + 1);
         float s[4][4] = {};
-        if (warp_row < rows) {
+        auto scores = [&](auto n) {
             for (int d = 0; d < a.D; d += 4) {
                 float4 x[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[i] = *(const float4*)&sq[(ty * 4 + i) * LD + d];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (16 * j >= keys) break;
+                for (int j = 0; j < decltype(n)::value; j++) {
                     const float4 y = *(const float4*)&skv[(tx + 16 * j) * LD + d];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -120,6 +122,12 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
                     }
                 }
             }
+        };
+        if (warp_row >= rows) {
+        } else if (keys > 32) {
+            scores(std::integral_constant<int, 4>());
+        } else {
+            scores(std::integral_constant<int, 2>());
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -158,21 +166,34 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
         });
         // a value that is not finite counts only where it is seen
         const bool careful = __syncthreads_or(mixed && odd);
-        for (int j = 0; j < keys && warp_row < rows; j++) {
-            float p[4], y[CN];
-            bool see[4];
+        // four keys at a time: past the last one weights and values are 0
+        auto values = [&](auto strict) {
+            for (int j0 = 0; j0 < keys; j0 += 4) {
+                alignas(16) float p[4][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                p[i] = sp[(ty * 4 + i) * LP + j];
-                see[i] = kt + j >= low[i] && kt + j <= lim[i];
+                for (int i = 0; i < 4; i++)
+                    *(float4*)p[i] = *(const float4*)&sp[(ty * 4 + i) * LP + j0];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    alignas(16) float y[CN];
+#pragma unroll
+                    for (int c = 0; c < CN; c += 4)
+                        *(float4*)&y[c] = *(const float4*)&skv[(j0 + j) * LD + col(c)];
+                    const int key = kt + j0 + j;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (decltype(strict)::value && (key < low[i] || key > lim[i])) continue;
+#pragma unroll
+                        for (int c = 0; c < CN; c++) o[i][c] = fmaf(p[i][j], y[c], o[i][c]);
+                    }
+                }
             }
-#pragma unroll
-            for (int c = 0; c < CN; c++) y[c] = skv[j * LD + tx + 16 * c];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int c = 0; c < CN; c++)
-                    if (!careful || see[i]) o[i][c] = fmaf(p[i], y[c], o[i][c]);
+        };
+        if (warp_row >= rows) {
+        } else if (careful) {
+            values(std::true_type());
+        } else {
+            values(std::false_type());
         }
     }
 #pragma unroll
@@ -184,7 +205,7 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
             if (tx == 0) a.ml[at] = make_float2(top[i], last < first ? -1.f : sum[i]);
 #pragma unroll
             for (int c = 0; c < CN; c++)
-                if (tx + 16 * c < a.dp) a.part[at * a.dp + tx + 16 * c] = o[i][c];
+                if (col(c) < a.dp) a.part[at * a.dp + col(c)] = o[i][c];
             continue;
         }
         const int t = (m0 + m) / a.G, g = (m0 + m) - t * a.G;
@@ -192,7 +213,7 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
         T* out = (T*)a.out + ((long long)(it.row0 + t) * a.H + head * a.G + g) * a.D;
 #pragma unroll
         for (int c = 0; c < CN; c++) {
-            const int d = tx + 16 * c;
+            const int d = col(c);
             if (d < a.D) out[d] = pr_to<T>(inv == 0.f ? 0.f : o[i][c] * inv);
         }
     }
