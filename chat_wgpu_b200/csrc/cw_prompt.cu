@@ -22,26 +22,44 @@ namespace cw {
 constexpr int PF_ROWS = 64, PF_KEYS = PF_ROWS, PF_THREADS = 256;
 
 // Fills [64][DP + 4] from row(m), zeros where it is null and past D: eight reads in flight (a
-// row of 4000 keys one read at a time took 980 us).  Whether what this thread read is finite.
-template <typename T, int DP, typename F>
-__device__ __forceinline__ bool pf_fill(float* to, int D, F row) {
+// row of 4000 keys one read at a time took 980 us), each of four elements where rows allow
+// it (`wide`: D, strides and addresses are multiples).  Whether what this thread read is finite.
+template <typename T, int DP, int N, typename F>
+__device__ __forceinline__ bool pf_fill_by(float* to, int D, F row) {
+    struct alignas(N * sizeof(T)) Vec {
+        T e[N];
+    };
+    constexpr int PER = DP / N, ALL = PF_ROWS * PER, DEEP = ALL / PF_THREADS < 8 ? ALL / PF_THREADS : 8;
     bool odd = false;
-    for (int i0 = threadIdx.x; i0 < PF_ROWS * DP; i0 += 8 * PF_THREADS) {
-        float x[8];
+    for (int i0 = threadIdx.x; i0 < ALL; i0 += DEEP * PF_THREADS) {
+        Vec x[DEEP];
+        bool on[DEEP];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int i = i0 + e * PF_THREADS, d = i % DP;
-            const T* from = row(i / DP);
-            x[e] = from && d < D ? pr_f32(from[d]) : 0.f;
+        for (int e = 0; e < DEEP; e++) {
+            const int i = i0 + e * PF_THREADS, d = i % PER * N;
+            const T* from = row(i / PER);
+            on[e] = from && d < D;
+            if (on[e]) x[e] = *(const Vec*)(from + d);
         }
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int i = i0 + e * PF_THREADS;
-            to[i / DP * (DP + 4) + i % DP] = x[e];
-            odd |= !isfinite(x[e]);
+        for (int e = 0; e < DEEP; e++) {
+            const int i = i0 + e * PF_THREADS, d = i % PER * N;
+            alignas(16) float y[N];
+#pragma unroll
+            for (int n = 0; n < N; n++) {
+                y[n] = on[e] ? pr_f32(x[e].e[n]) : 0.f;
+                odd |= !isfinite(y[n]);
+            }
+            float* at = to + i / PER * (DP + 4) + d;
+            if constexpr (N == 4) *(float4*)at = *(const float4*)y;
+            else *at = y[0];
         }
     }
     return odd;
+}
+template <typename T, int DP, typename F>
+__device__ __forceinline__ bool pf_fill(float* to, int D, bool wide, F row) {
+    return wide ? pf_fill_by<T, DP, 4>(to, D, row) : pf_fill_by<T, DP, 1>(to, D, row);
 }
 // DP: head_dim rounded up to 64, 128 or 256.
 template <typename T, int DP>
@@ -67,7 +85,9 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
     const T* qb = (const T*)a.q + (long long)head * a.G * a.D;
     const T* kb = (const T*)a.k + (long long)it.key0 * a.k_stride + (long long)head * a.D;
     const T* vb = (const T*)a.v + (long long)it.key0 * a.v_stride + (long long)head * a.D;
-    (void)pf_fill<T, DP>(sq, a.D, [&](int m) -> const T* {
+    const bool wide = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v) & (4 * sizeof(T) - 1)) == 0 &&
+                      ((a.q_stride | a.k_stride | a.v_stride | a.D) & 3) == 0;
+    (void)pf_fill<T, DP>(sq, a.D, wide, [&](int m) -> const T* {
         const int t = (m0 + m) / a.G, g = (m0 + m) - t * a.G;
         return m < rows ? qb + (long long)(it.row0 + t) * a.q_stride + g * a.D : nullptr;
     });
@@ -97,7 +117,7 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
     for (int kt = first; kt <= last; kt += PF_KEYS) {
         const bool mixed = kt < all0 || kt + PF_KEYS - 1 > all1;
         __syncthreads();
-        (void)pf_fill<T, DP>(skv, a.D, [&](int j) -> const T* {
+        (void)pf_fill<T, DP>(skv, a.D, wide, [&](int j) -> const T* {
             return kt + j <= last ? kb + (long long)(kt + j) * a.k_stride : nullptr;
         });
         __syncthreads();
@@ -161,7 +181,7 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
             for (int c = 0; c < CN; c++) o[i][c] *= fix;
         }
         __syncthreads();
-        const bool odd = pf_fill<T, DP>(skv, a.D, [&](int j) -> const T* {
+        const bool odd = pf_fill<T, DP>(skv, a.D, wide, [&](int j) -> const T* {
             return kt + j <= last ? vb + (long long)(kt + j) * a.v_stride : nullptr;
         });
         // a value that is not finite counts only where it is seen
