@@ -1207,9 +1207,12 @@ __global__ void __launch_bounds__(PS_WARPS * 32)
 bool prompt_tc_takes(const PromptArgs& a, uint32_t type) {
     if (a.G > 128 || !(a.scale > 0.f)) return false;
     if (type == CW_GGUF_F32)  // any place and stride; the pairs are laid out anew
-        // (short prompts take fewer launches on the f32 kernel; us there and here: one of 64
-        // tokens 24 and 34, of 128 39 and 35, of 2048 737 and 104)
-        return a.D <= 128 && (long long)a.n_keys >= 96ll * a.n_req;
+        // (short prompts, and single rows over many keys, whose pairs are formed for little, are
+        // faster on the f32 kernel; us there and here, 16/8 heads: a prompt of 128 tokens 27 and
+        // 34, 192 tokens 38 and 35, eight of 128 40 and 52; a row after 1000 keys 57 and 46,
+        // after 4000 54 and 62, eight after 2000 93 and 172; 16 rows after 4000 65 and 62)
+        return a.D <= 128 && (long long)a.n_keys >= 160ll * a.n_req &&
+               (a.n_rows >= 8ll * a.n_req || (long long)a.n_keys < 2000ll * a.n_req);
     const long long strides = (a.n_rows > 1 ? a.q_stride : 0) |
                               (a.n_keys > 1 ? a.k_stride | a.v_stride : 0);
     return a.D % 8 == 0 && strides % 8 == 0 &&
