@@ -951,6 +951,9 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                         pt_careful<BF>(t_s, t_o, vt, a.D, half, low() - kt, lim() - kt,
                                        i == blk.lo);
                 }
+                // with two buffers of scores the product before may still run: the item's end
+                // waits for this tile's by parity, which must not take the phase before for it
+                if (NB == 1 && !PAIR && i > blk.lo && i + 1 == blk.hi) pass(&bars->pv[b], n - 1);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars->p_full[sb]);

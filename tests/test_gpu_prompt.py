@@ -96,6 +96,7 @@ CASES = [  # dtype, heads, kv, dim, rows, keys (None: the rows), options
     ("f16", 8, 4, 256, [5, 70], [2000, 1500], dict(window=700, softcap=20.0)),
     ("f16", 14, 2, 64, [19], [1700], {}),
     ("f32", 16, 8, 128, [3], [2500], {}),
+    ("f32", 16, 8, 128, [9], [2500], {}),
     ("f32", 16, 8, 40, [90, 7], [1200, 1900], dict(softcap=15.0)),
     ("f32", 8, 4, 256, [2, 9], [1800, 900], {}),
     ("f32", 2, 2, 130, [4], [1400], dict(window=600, pad=3, off=1)),
