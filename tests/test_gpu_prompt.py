@@ -170,6 +170,15 @@ def test_prompt_pieces_not_finite(ctx, dtype, D):
     assert np.abs(got[:2][:, :, rest] - want[:2][:, :, rest]).max() <= tolerance(dtype, s, v, 2600)
 
 
+@pytest.mark.parametrize("keys", [300, 2600])
+def test_prompt_repeated(ctx, keys):
+    """Calls on the same rows give the same bits: an item's end waits for its last product."""
+    c = make(np.random.default_rng(9), [4, 70], [keys, keys - 40], "f16", 2, 1, 256)
+    first = run(ctx, c, "f16")
+    for _ in range(40):
+        assert np.array_equal(run(ctx, c, "f16"), first)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_prompt_scores_of_minus_infinity(ctx, dtype):
     """Keys that score -inf weigh nothing, in the first tile and in a later one; a row that
