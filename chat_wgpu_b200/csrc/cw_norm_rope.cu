@@ -252,22 +252,23 @@ extern "C" int cw_norm_rope(cw_ctx* ctx, const cw_norm_rope_args* p) {
     CW_CHECK(plan->rope_dim <= D, CW_ERR_INVALID_ARG,
              "cw_norm_rope: the plan rotates %u of %zu elements", plan->rope_dim, D);
     CW_TRY(buf_get(ctx, p->positions, &pos, T * 4, "cw_norm_rope(positions)"));
-    // what is read and what is written: an output may lie on its own input only
+    // what is read and what is written: an output may lie on its own input only, whose heads
+    // the lanes that write them have read; another input at the same place is read by others
     struct Span {
         const char* at;
         size_t n;
         const char* what;
-        const char* may;  // the input that it may be
+        int may;  // which input it may be, or -1
     } in[8], out[4];
     int ins = 0, outs = 0;
-    in[ins++] = {(const char*)plan->ptr, plan->rope_dim / 2 * 8, "plan", nullptr};
-    in[ins++] = {(const char*)pos->ptr, T * 4, "positions", nullptr};
+    in[ins++] = {(const char*)plan->ptr, plan->rope_dim / 2 * 8, "plan", -1};
+    in[ins++] = {(const char*)pos->ptr, T * 4, "positions", -1};
     NormRopeArgs a{};
     auto norm = [&](cw_buf b, const float** to, const char* what) -> int {
         if (!b) return CW_OK;
         CW_TRY(buf_get(ctx, b, &e, D * 4, what));
         *to = (const float*)e->ptr;
-        in[ins++] = {(const char*)e->ptr, D * 4, what, nullptr};
+        in[ins++] = {(const char*)e->ptr, D * 4, what, -1};
         return CW_OK;
     };
     // rows of w elements; contiguous ones may be written in place
@@ -277,32 +278,32 @@ extern "C" int cw_norm_rope(cw_ctx* ctx, const cw_norm_rope_args* p) {
                  (unsigned long long)stride);
         CW_TRY(buf_get(ctx, b, &e, (off + (T - 1) * stride + w) * es, what));
         *to = (const char*)e->ptr + off * es;
-        in[ins++] = {(const char*)*to, ((T - 1) * stride + w) * es, what, nullptr};
+        in[ins++] = {(const char*)*to, ((T - 1) * stride + w) * es, what, -1};
         return CW_OK;
     };
-    auto result = [&](cw_buf b, size_t n, void** to, const char* what, const void* may) -> int {
+    auto result = [&](cw_buf b, size_t n, void** to, const char* what, int may) -> int {
         CW_TRY(buf_get(ctx, b, &e, n, what));
         *to = e->ptr;
-        out[outs++] = {(const char*)e->ptr, n, what, (const char*)may};
+        out[outs++] = {(const char*)e->ptr, n, what, may};
         return CW_OK;
     };
     const bool cache = p->n_kv && p->slots;
     if (p->n_heads) {
         const size_t w = p->n_heads * D;
+        const int own = p->q_stride == w || T == 1 ? ins : -1;
         CW_TRY(rows(p->q, p->q_off, p->q_stride, w, &a.q, "cw_norm_rope(q)"));
         CW_TRY(norm(p->q_norm, &a.q_norm, "cw_norm_rope(q_norm)"));
-        CW_TRY(result(p->q_out, T * w * es, &a.q_out, "cw_norm_rope(q_out)",
-                      p->q_stride == w || T == 1 ? a.q : nullptr));
+        CW_TRY(result(p->q_out, T * w * es, &a.q_out, "cw_norm_rope(q_out)", own));
     }
     if (p->n_kv) {
         const size_t w = p->n_kv * D;
         CW_CHECK(p->k_out || cache, CW_ERR_INVALID_ARG,
                  "cw_norm_rope: k has neither k_out nor a cache to go to");
+        const int own = p->k_stride == w || T == 1 ? ins : -1;
         CW_TRY(rows(p->k, p->k_off, p->k_stride, w, &a.k, "cw_norm_rope(k)"));
         CW_TRY(norm(p->k_norm, &a.k_norm, "cw_norm_rope(k_norm)"));
         if (p->k_out)
-            CW_TRY(result(p->k_out, T * w * es, &a.k_out, "cw_norm_rope(k_out)",
-                          p->k_stride == w || T == 1 ? a.k : nullptr));
+            CW_TRY(result(p->k_out, T * w * es, &a.k_out, "cw_norm_rope(k_out)", own));
         if (cache) {
             CW_CHECK(p->page_size > 0 && p->page_size <= (1u << 20) && p->n_pages > 0 &&
                          (uint64_t)p->n_pages * p->page_size < (1ull << 31),
@@ -310,19 +311,18 @@ extern "C" int cw_norm_rope(cw_ctx* ctx, const cw_norm_rope_args* p) {
             CW_TRY(rows(p->v, p->v_off, p->v_stride, w, &a.v, "cw_norm_rope(v)"));
             CW_TRY(buf_get(ctx, p->slots, &e, T * 4, "cw_norm_rope(slots)"));
             a.slots = (const int*)e->ptr;
-            in[ins++] = {(const char*)e->ptr, T * 4, "slots", nullptr};
+            in[ins++] = {(const char*)e->ptr, T * 4, "slots", -1};
             const size_t n = (size_t)p->n_pages * p->page_size * w * es;
-            CW_TRY(result(p->k_cache, n, &a.k_cache, "cw_norm_rope(k_cache)", nullptr));
-            CW_TRY(result(p->v_cache, n, &a.v_cache, "cw_norm_rope(v_cache)", nullptr));
+            CW_TRY(result(p->k_cache, n, &a.k_cache, "cw_norm_rope(k_cache)", -1));
+            CW_TRY(result(p->v_cache, n, &a.v_cache, "cw_norm_rope(v_cache)", -1));
             a.page = (int)p->page_size;
             a.n_slots = (long long)p->n_pages * p->page_size;
         }
     }
     for (int o = 0; o < outs; o++) {
         for (int i = 0; i < ins; i++)
-            CW_CHECK(out[o].at == out[o].may && out[o].at == in[i].at
-                         ? true
-                         : !spans_meet(out[o].at, out[o].n, in[i].at, in[i].n),
+            CW_CHECK((i == out[o].may && out[o].at == in[i].at) ||
+                         !spans_meet(out[o].at, out[o].n, in[i].at, in[i].n),
                      CW_ERR_INVALID_ARG, "%s lies on %s", out[o].what, in[i].what);
         for (int i = 0; i < o; i++)
             CW_CHECK(!spans_meet(out[o].at, out[o].n, out[i].at, out[i].n), CW_ERR_INVALID_ARG,

@@ -420,7 +420,8 @@ typedef struct {
  * in f32, rounded once.  q_out = y of q; k_out (0: none) and the cache rows of the
  * slots (slots 0: no cache, and v is not read) = y of k; the cache also takes v as it
  * is.  n_heads = 0 leaves q out, n_kv = 0 k and v.  q_out may be q and k_out may be k
- * where those rows are contiguous; no other output may overlap an input
+ * where those rows are contiguous; no other output may overlap an input, nor these two
+ * another input than their own, as v where k and v are the same rows
  * (CW_ERR_INVALID_ARG).  Rows whose slots are equal are written in no particular order. */
 int cw_norm_rope(cw_ctx* ctx, const cw_norm_rope_args* args);
 
