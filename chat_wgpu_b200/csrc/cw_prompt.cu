@@ -351,7 +351,9 @@ extern "C" int cw_prompt_attention(cw_ctx* ctx, const cw_prompt_attn_args* p) {
     a.K = (int)p->n_kv;
     a.G = a.H / a.K;
     a.D = (int)D;
-    a.window = (int)p->window;
+    // a window of all keys hides none; below that, sums with it stay in 32 bits although rows
+    // before a request's first key count from a negative place
+    a.window = p->window < L ? (int)p->window : 0;
     a.scale = p->scale != 0.f ? p->scale : 1.f / sqrtf((float)D);
     a.softcap = p->softcap;
     a.status = ctx->d_status;
