@@ -28,8 +28,8 @@ struct PromptArgs {
     long long q_stride, k_stride, v_stride;
     int n_req, n_rows, n_keys, H, K, G, D, window;
     float scale, softcap;
-    // f32 on the tensor cores: magnitudes of each request's kv heads, [n_req][K][3] (k, v, q:
-    // f32 bits, of q only what is too large), and what the q rows were divided by, [n_rows][H]
+    // f32 on the tensor cores: magnitudes of each request's kv heads, [n_req][K][PR_MAGS] (f32
+    // bits; PrMag), and what the q rows were divided by, [n_rows][H]
     uint32_t* amax;
     float* q_back;
     // partial states of items that a CTA's run cuts, two to a CTA: [grid * 2][rows][dp] sums,
@@ -99,14 +99,26 @@ __device__ __forceinline__ void prompt_check(const PromptArgs& a, int tid, int t
 
 // Operands as pairs: values are multiplied by 2^s so that the largest, `bits`, lies in
 // [2^14, 2^15).  What is not finite, or so large that products could leave f32's range, is
-// left to the f32 kernel.
+// left to the f32 kernel.  So are a request and kv head with rows of k or v (a token's head)
+// whose largest values are more than PR_APART powers of two apart: a pair loses up to 2^-39
+// of the largest in sight or out of it, which is then 2^-27 of any row's own largest, and a
+// weight 2^-38 of the heaviest, which times any row of v is then below 2^-25 of the heaviest
+// key's row.  (Rows of zeros are exact.)
 constexpr uint32_t PR_ODD = (127u + 60) << 23;
+constexpr uint32_t PR_APART = 12;
+// Of k and v the largest value, of q only what does not fit; of the rows of k and v the
+// smallest of their largest values but 0, as its complement (the words start at 0).
+enum PrMag { PR_K, PR_V, PR_Q, PR_K_LEAST, PR_V_LEAST, PR_MAGS };
 __device__ __forceinline__ int pr_shift(uint32_t bits) {
     return bits ? min(14 - ((int)(bits >> 23) - 127), 100) : 0;
 }
 __device__ __forceinline__ bool pr_odd(const PromptArgs& a, int req, int head) {
-    const uint32_t* m = a.amax + ((size_t)req * a.K + head) * 3;
-    return m[0] >= PR_ODD || m[1] >= PR_ODD || m[2] >= PR_ODD;
+    const uint32_t* m = a.amax + ((size_t)req * a.K + head) * PR_MAGS;
+    auto apart = [](uint32_t most, uint32_t least) {  // no row but of zeros: 0 and ~0
+        return most && (most >> 23) - (~least >> 23) > PR_APART;
+    };
+    return m[PR_K] >= PR_ODD || m[PR_V] >= PR_ODD || m[PR_Q] >= PR_ODD ||
+           apart(m[PR_K], m[PR_K_LEAST]) || apart(m[PR_V], m[PR_V_LEAST]);
 }
 
 template <typename T> __device__ __forceinline__ float pr_f32(T x);

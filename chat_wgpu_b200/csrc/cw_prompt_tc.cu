@@ -18,7 +18,8 @@
 // scheduler waited for itself: 16384 bf16 tokens of 32/8 heads 1.88 ms against 1.82); one
 // warp each to copy, to issue products (one lane: 1.87 ms without any softmax when the warp
 // went together, 1.40 ms alone), to find the next item, and to look for values that are not
-// finite.  O is rescaled only when a row's maximum has grown by 2^8 since its last reference.
+// finite.  O is rescaled only when a row's weights have grown by 2^8 (pairs: 2^2) since its last
+// reference.
 // Weights are rounded to the type for the second product, half a step each at most; the
 // row's sum takes them unrounded, which saves two instructions a key.
 //
@@ -37,8 +38,8 @@
 // to the row's by the threads (error against 64 bits at 4096 keys 7.1e-6 without either,
 // 6.8e-7 with both; a plain f32 form has 1.2e-6).  Bound by shared memory and the tensor
 // pipe: 128 rows take 416 KB of operands a tile through it, 3300 cycles at 128 bytes, for
-// 3100 cycles of products.  What does not fit pairs (infinities, NaN, magnitudes from 2^60)
-// is left to the f32 kernel, by request and kv head.
+// 3100 cycles of products.  What does not fit pairs (infinities, NaN, magnitudes from 2^60,
+// rows of very different sizes) is left to the f32 kernel, by request and kv head.
 //
 // Unseen keys weigh 0, but 0 times a value that is not finite is NaN.  So in the tiles
 // that rows see differently (the diagonal, the window's edge) one warp looks V over while
@@ -660,9 +661,9 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
         auto ready = [&](int head) {
             p.head = head;
             if (!PAIR) return true;
-            const uint32_t* m = a.amax + ((size_t)p.it.req * a.K + head) * 3;
-            p.k_back = exp2f((float)-pr_shift(m[0]));
-            p.v_back = exp2f((float)-pr_shift(m[1]));
+            const uint32_t* m = a.amax + ((size_t)p.it.req * a.K + head) * PR_MAGS;
+            p.k_back = exp2f((float)-pr_shift(m[PR_K]));
+            p.v_back = exp2f((float)-pr_shift(m[PR_V]));
             return !pr_odd(a, p.it.req, head);
         };
         if (!a.cut) {  // whole items, long ones first; every second round of the CTAs goes back
@@ -771,6 +772,10 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
         const uint32_t lanes = tmem + b * TCOLS + ((uint32_t)(warp & 3) << 21);
         const uint32_t t_o = lanes + SB * PT_KEYS;
         const float log2e = 1.44269504088896341f;
+        // the reference lies LIFT below the largest score that it was taken from, which may
+        // grow by GROWN before the sums are rescaled: weights stay below 2^15.  Of pairs the
+        // heaviest is 2^13 at least, so that the others lose at most 2^-38 of it
+        constexpr float LIFT = PAIR ? 13.f : TT_LIFT<BF>, GROWN = PAIR ? 2.f : 8.f;
         const bool cap = a.softcap > 0.f;
         const float c0 = cap ? log2e : a.scale * log2e;
         const float y0 = cap ? 2.f * log2e * a.scale / a.softcap : 0.f;
@@ -870,10 +875,10 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                     meet();
                     tc_fence_after();
                     top = pt_max3(top, at[half ^ 1][m], top);
-                    const float want = top == -INFINITY ? -INFINITY : top * c2 - TT_LIFT<BF>;
+                    const float want = top == -INFINITY ? -INFINITY : top * c2 - LIFT;
                     if (i == blk.lo) {
                         ref = want;
-                    } else if (__any_sync(FULL, row && !(want - ref <= 8.f) && want != -INFINITY)) {
+                    } else if (__any_sync(FULL, row && !(want - ref <= GROWN) && want != -INFINITY)) {
                         const float fix = ref == -INFINITY ? 0.f : tt_exp2(ref - want);
                         // O holds the tiles so far (two row blocks: since the scores came)
                         if (NB == 1 && !PAIR) pass(&bars->pv[b], n - 1);
@@ -1110,8 +1115,10 @@ static int pt_map(CUtensorMap* map, const void* base, bool bf, int dims_, int he
 // ---- f32 operands as pairs ---------------------------------------------------------
 // x 2^s = h + l to 22 bits, h and l f16, s by request and kv head (k, v) or by row and head
 // (q).  With the largest in [2^14, 2^15), what l drops is at most 2^-39 of the largest, or
-// 2^-22 of the value itself.  A warp takes a head row, or for the magnitudes 32 of them.
+// 2^-22 of the value itself (what that asks of the values: PR_APART).  A warp takes a head
+// row, or for the magnitudes 32 of them.
 constexpr int PS_WARPS = 8;
+constexpr int PS_ROWS = 8;  // rows of a warp in flight
 
 // The request whose rows [starts[r], starts[r + 1]) hold row t, or -1.
 __device__ __forceinline__ int ps_req(const int* starts, int n_req, int t) {
@@ -1135,21 +1142,38 @@ __global__ void __launch_bounds__(PS_WARPS * 32) k_prompt_amax(const __grid_cons
     const float* x = (const float*)(is_v ? a.v : a.k) + (long long)h * a.D;
     const long long stride = is_v ? a.v_stride : a.k_stride;
     const int* ks = a.key_starts ? a.key_starts : a.starts;
-    uint32_t most = 0;
+    uint32_t most = 0, least = ~0u;
     int mine = -1;
     auto flush = [&]() {
-        const uint32_t m = __reduce_max_sync(FULL, most);
-        if (lane == 0 && mine >= 0 && m) atomicMax(&a.amax[((size_t)mine * a.K + h) * 3 + is_v], m);
-        most = 0;
-    };
-    for (int t = t0; t < min(t0 + 32, a.n_keys); t++) {
-        if (mine < 0 || t >= ks[mine + 1]) {
-            flush();
-            mine = ps_req(ks, a.n_req, t);
+        if (lane == 0 && mine >= 0 && most) {
+            uint32_t* m = a.amax + ((size_t)mine * a.K + h) * PR_MAGS;
+            atomicMax(&m[is_v ? PR_V : PR_K], most);
+            atomicMax(&m[is_v ? PR_V_LEAST : PR_K_LEAST], ~least);
         }
-        if (mine < 0) continue;
-        for (int d = lane; d < a.D; d += 32)
-            most = max(most, __float_as_uint(fabsf(x[t * stride + d])));
+        most = 0;
+        least = ~0u;
+    };
+    // several rows at a time: their reads are in flight together
+    for (int t = t0; t < min(t0 + 32, a.n_keys); t += PS_ROWS) {
+        uint32_t row[PS_ROWS] = {};
+#pragma unroll
+        for (int u = 0; u < PS_ROWS; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (t + u < a.n_keys && e * 32 + lane < a.D)
+                    row[u] = max(row[u], __float_as_uint(fabsf(x[(t + u) * stride + e * 32 + lane])));
+#pragma unroll
+        for (int u = 0; u < PS_ROWS; u++) {
+            if (t + u >= a.n_keys) break;
+            const uint32_t r = __reduce_max_sync(FULL, row[u]);
+            if (mine < 0 || t + u >= ks[mine + 1]) {
+                flush();
+                mine = ps_req(ks, a.n_req, t + u);
+            }
+            if (mine < 0 || r == 0) continue;
+            most = max(most, r);
+            least = min(least, r);
+        }
     }
     flush();
 }
@@ -1178,15 +1202,15 @@ __global__ void __launch_bounds__(PS_WARPS * 32)
         x[e] = lane * N + e < a.D && req >= 0 ? src[lane * N + e] : 0.f;
         most = max(most, __float_as_uint(fabsf(x[e])));
     }
-    uint32_t* m = req >= 0 ? a.amax + ((size_t)req * a.K + (kind == 0 ? h / a.G : h)) * 3 : nullptr;
+    uint32_t* m = req >= 0 ? a.amax + ((size_t)req * a.K + (kind == 0 ? h / a.G : h)) * PR_MAGS : nullptr;
     if (kind == 0) {
         most = __reduce_max_sync(FULL, most);
         if (lane == 0) {
-            if (most >= PR_ODD && m) atomicMax(&m[2], most);
+            if (most >= PR_ODD && m) atomicMax(&m[PR_Q], most);
             a.q_back[i] = exp2f((float)-pr_shift(most));
         }
     } else {
-        most = m ? m[kind - 1] : 0;
+        most = m ? m[kind == 1 ? PR_K : PR_V] : 0;
     }
     const float by = exp2f((float)pr_shift(most));
     __half hi[N], lo[N];
@@ -1265,7 +1289,7 @@ template <typename T, int HD> static int pt_go(cw_ctx* ctx, PromptArgs& a) {
     CUtensorMap mq, mk, mv;
     if constexpr (PAIR) {
         const size_t nq = (size_t)a.n_rows * a.H, nk = (size_t)a.n_keys * a.K;
-        const size_t most = (size_t)a.n_req * a.K * 3 * 4;
+        const size_t most = (size_t)a.n_req * a.K * PR_MAGS * 4;
         const size_t at_pairs = take((nq + 2 * nk) * 2 * HD * 2), at_back = take(nq * 4),
                      at_most = take(most);
         CW_TRY(scratch());

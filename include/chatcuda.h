@@ -446,9 +446,11 @@ typedef struct {
  * f32.  16-bit types whose head_dim is a multiple of 8 and whose strides and places are
  * multiples of 16 bytes, with at most 128 query heads per kv head and a positive scale,
  * run on the tcgen05 tensor cores (there the softmax weights are rounded to the type
- * before the product with v).  f32 with head_dim <= 128 and 96 keys a request or more runs
- * there as pairs of f16, at f32 accuracy: what a value loses is below 2^-22 of it or 2^-39
- * of the largest of its request and head.  Everything else runs in f32 products.  Starts
+ * before the product with v).  f32 with head_dim <= 128 runs there as pairs of f16 where
+ * there are keys enough, at f32 accuracy: a value loses less than 2^-22 of it or 2^-27 of the
+ * largest of its row and head.  Requests and kv heads that pairs cannot hold so (infinities,
+ * NaN, magnitudes from 2^60, rows of k or v whose largest values are more than 2^12
+ * apart) run in f32 products, and so does everything else.  Starts
  * that descend or pass the buffers are cut to them and reported.  Uses a context-owned
  * scratch that grows on demand, in stream order: call once with a call's sizes before
  * capturing it, and replay a captured call before the context is destroyed and in order
