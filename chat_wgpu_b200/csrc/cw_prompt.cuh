@@ -106,18 +106,24 @@ __device__ __forceinline__ void prompt_check(const PromptArgs& a, int tid, int t
 // key's row.  (Rows of zeros are exact.)
 constexpr uint32_t PR_ODD = (127u + 60) << 23;
 constexpr uint32_t PR_APART = 12;
+// 2^s is at most 2^100 (k's and q's are multiplied together), so what is smaller than this is
+// left out as well, but for zeros.
+constexpr uint32_t PR_TINY = (127u - 86) << 23;
 // Of k and v the largest value, of q only what does not fit; of the rows of k and v the
 // smallest of their largest values but 0, as its complement (the words start at 0).
 enum PrMag { PR_K, PR_V, PR_Q, PR_K_LEAST, PR_V_LEAST, PR_MAGS };
 __device__ __forceinline__ int pr_shift(uint32_t bits) {
     return bits ? min(14 - ((int)(bits >> 23) - 127), 100) : 0;
 }
+__device__ __forceinline__ bool pr_misfit(uint32_t bits) {
+    return bits >= PR_ODD || (bits && bits < PR_TINY);
+}
 __device__ __forceinline__ bool pr_odd(const PromptArgs& a, int req, int head) {
     const uint32_t* m = a.amax + ((size_t)req * a.K + head) * PR_MAGS;
     auto apart = [](uint32_t most, uint32_t least) {  // no row but of zeros: 0 and ~0
         return most && (most >> 23) - (~least >> 23) > PR_APART;
     };
-    return m[PR_K] >= PR_ODD || m[PR_V] >= PR_ODD || m[PR_Q] >= PR_ODD ||
+    return pr_misfit(m[PR_K]) || pr_misfit(m[PR_V]) || pr_misfit(m[PR_Q]) ||
            apart(m[PR_K], m[PR_K_LEAST]) || apart(m[PR_V], m[PR_V_LEAST]);
 }
 

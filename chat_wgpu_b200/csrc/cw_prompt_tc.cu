@@ -38,8 +38,8 @@
 // to the row's by the threads (error against 64 bits at 4096 keys 7.1e-6 without either,
 // 6.8e-7 with both; a plain f32 form has 1.2e-6).  Bound by shared memory and the tensor
 // pipe: 128 rows take 416 KB of operands a tile through it, 3300 cycles at 128 bytes, for
-// 3100 cycles of products.  What does not fit pairs (infinities, NaN, magnitudes from 2^60,
-// rows of very different sizes) is left to the f32 kernel, by request and kv head.
+// 3100 cycles of products.  What does not fit pairs (infinities, NaN, magnitudes from 2^60 or
+// below 2^-86, rows of very different sizes) is left to the f32 kernel, by request and kv head.
 //
 // Unseen keys weigh 0, but 0 times a value that is not finite is NaN.  So in the tiles
 // that rows see differently (the diagonal, the window's edge) one warp looks V over while
@@ -815,7 +815,8 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
             if (PAIR && row)
                 back = x->k_back * a.q_back[(long long)(x->it.row0 + tok) * a.H + x->head * a.G +
                                             m - m / a.G * a.G];
-            const float c2 = PAIR && !cap ? c0 * back : c0;
+            // (not 0, however small q and k: scores of -inf stay -inf)
+            const float c2 = PAIR && !cap ? fmaxf(c0 * back, 0x1p-126f) : c0;
             // running maximum of the scores, the weights' reference (in powers of two),
             // and the sum of this thread's weights
             float top = -INFINITY, ref = -INFINITY, sum = 0.f;
@@ -1206,7 +1207,7 @@ __global__ void __launch_bounds__(PS_WARPS * 32)
     if (kind == 0) {
         most = __reduce_max_sync(FULL, most);
         if (lane == 0) {
-            if (most >= PR_ODD && m) atomicMax(&m[PR_Q], most);
+            if (pr_misfit(most) && m) atomicMax(&m[PR_Q], PR_ODD);
             a.q_back[i] = exp2f((float)-pr_shift(most));
         }
     } else {

@@ -449,12 +449,12 @@ typedef struct {
  * before the product with v).  f32 with head_dim <= 128 runs there as pairs of f16 where
  * there are keys enough, at f32 accuracy: a value loses less than 2^-22 of it or 2^-27 of the
  * largest of its row and head.  Requests and kv heads that pairs cannot hold so (infinities,
- * NaN, magnitudes from 2^60, rows of k or v whose largest values are more than 2^12
- * apart) run in f32 products, and so does everything else.  Starts
- * that descend or pass the buffers are cut to them and reported.  Uses a context-owned
- * scratch that grows on demand, in stream order: call once with a call's sizes before
- * capturing it, and replay a captured call before the context is destroyed and in order
- * with the context's other prompt attention calls. */
+ * NaN, magnitudes from 2^60 or below 2^-86, rows of k or v whose largest values are more
+ * than 2^12 apart) run in f32 products, and so does everything else.  Starts that descend
+ * or pass the buffers are cut to them and reported.  Uses a context-owned scratch that grows
+ * on demand, in stream order: call once with a call's sizes before capturing it, and replay a
+ * captured call before the context is destroyed and in order with the context's other prompt
+ * attention calls. */
 int cw_prompt_attention(cw_ctx* ctx, const cw_prompt_attn_args* args);
 
 typedef struct {
