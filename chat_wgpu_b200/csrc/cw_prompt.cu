@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(PF_THREADS) k_prompt(const __grid_constant__ P
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 float x = s[i][j] * (a.softcap > 0.f ? a.scale / a.softcap : a.scale * log2e);
-                if (a.softcap > 0.f) x = a.softcap * log2e * tanhf(x);
+                if (a.softcap > 0.f) x = a.softcap * tanhf(x) * log2e;  // (softcap * log2e may pass f32)
                 const int key = kt + tx + 16 * j;
                 if (key < low[i] || key > lim[i]) x = -INFINITY;
                 s[i][j] = x;

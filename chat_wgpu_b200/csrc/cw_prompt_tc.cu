@@ -219,9 +219,29 @@ template <bool BF> __device__ __forceinline__ uint32_t pt_pack(float x, float y)
     return r;
 }
 
-// The scores of a row's half of a tile in TMEM, capped: tanh(y) = 1 - 2 / (1 + e^2y), off by
-// 2^-22, times softcap far below one rounding of the weight.  y2: 2 log2(e) scale / softcap.
+// The scores of a row's half of a tile in TMEM, capped, to f32's accuracy.  y: scale / softcap.
+__device__ __noinline__ void pt_cap_f32(uint32_t t_s, float softcap, float y) {
+#pragma unroll 1
+    for (int c = 0; c < PT_KEYS / 2; c += 16) {
+        float s[16];
+        tt_load<16>(t_s + c, (uint32_t*)s);
+#pragma unroll
+        for (int j = 0; j < 16; j++) s[j] = softcap * tanhf(s[j] * y);
+        tt_st<16>(t_s + c, (uint32_t*)s);
+    }
+    tt_wait_st();
+}
+// The same for weights in 16 bits: tanh(y) = 1 - 2 / (1 + e^2y), off by 2^-22, which times a
+// softcap of PT_CAP_FAST at most is 2^-14, an eighth of the rounding of an f16 weight.  (Larger
+// caps would lose the score in the difference: scores of 8 are off by 0.1 at 1e6.  They are
+// told here and not where it is called: two calls there made every kernel of 16-bit types
+// 3.5 % slower.)  y2: 2 log2(e) scale / softcap.
+constexpr float PT_CAP_FAST = 256.f;
 __device__ __noinline__ void pt_cap(uint32_t t_s, float softcap, float y2) {
+    if (softcap > PT_CAP_FAST) {
+        pt_cap_f32(t_s, softcap, y2 * 0.346573590279972655f);  // ln(2) / 2
+        return;
+    }
 #pragma unroll 1
     for (int c = 0; c < PT_KEYS / 2; c += 32) {
         float s[32];
@@ -232,18 +252,6 @@ __device__ __noinline__ void pt_cap(uint32_t t_s, float softcap, float y2) {
             s[j] = softcap - __fdividef(2.f * softcap, 1.f + tt_exp2(y > 120.f ? 120.f : y));
         }
         tt_st32(t_s + c, (uint32_t*)s);
-    }
-    tt_wait_st();
-}
-// The same to f32's accuracy; y: scale / softcap.
-__device__ __noinline__ void pt_cap_f32(uint32_t t_s, float softcap, float y) {
-#pragma unroll 1
-    for (int c = 0; c < PT_KEYS / 2; c += 16) {
-        float s[16];
-        tt_load<16>(t_s + c, (uint32_t*)s);
-#pragma unroll
-        for (int j = 0; j < 16; j++) s[j] = softcap * tanhf(s[j] * y);
-        tt_st<16>(t_s + c, (uint32_t*)s);
     }
     tt_wait_st();
 }
