@@ -8,9 +8,9 @@ would have produced itself are kept, so the tokens are those of plain greedy dec
 (model.generate_op_by_op) in fewer steps.  Drafts come from the session's own text:
 what followed the last occurrences of its last tokens.
 
-TreeDecoder.prefill takes whole prompts in at once, whatever their lengths: per layer
-cw_norm_rope writes their keys and values and cw_prompt_attention lets each token see its
-own prompt up to itself.  With penalties, biases or a set of allowed tokens
+TreeDecoder.prefill takes whole prompts in at once, whatever their lengths: per
+layer cw_norm_rope writes their keys and values and cw_prompt_attention lets each token see
+its own prompt up to itself.  With penalties, biases or a set of allowed tokens
 cw_adjust_logits chooses the step's tokens.
 
     python -m chat_wgpu_b200.treedecode model.gguf 1 5 9 2 --new 32 --prefill --repetition 1.1
@@ -122,12 +122,15 @@ class TreeDecoder:
             out["depths"] = deep
         return out
 
-    def _layers(self, rows, attend):
+    def _layers(self, rows, attend, x=None):
         """Hidden rows of the tokens after the layers; attend(q, k, v, layer, cache) gives the
-        attention's rows."""
+        attention's rows.  With x, a buffer of their own for the rows, each layer is a frame:
+        the activations of one are held at a time, not of all."""
         m, ctx, T = self.m, self.ctx, len(rows)
         dim = m.dim
-        x = ctx.empty(T * dim)
+        own = x
+        if own is None:
+            x = ctx.empty(T * dim)
         for i, t in enumerate(rows):
             ctx.copy(m.embed_tbl, int(t) * dim, x, i * dim, dim)
         for l, cache in zip(m.layers, self.cache):
@@ -139,6 +142,10 @@ class TreeDecoder:
             act = activation.swiglu(ctx, self._proj(l["gate"], a, T), self._proj(l["up"], a, T),
                                     T * m.hidden)
             x = attention.add(ctx, x, self._proj(l["down"], act, T), T * dim)
+            if own is not None:
+                ctx.copy(x, 0, own, 0, T * dim)
+                ctx.reset_frame()
+                x = own
         return x
 
     def _proj(self, w, a, T):
@@ -183,7 +190,9 @@ class TreeDecoder:
 
     def prefill(self) -> None:
         """The prompts of the sessions that no step has run yet, but for their last tokens, in
-        one pass: packed rows, each prompt's own length."""
+        one pass: packed rows, each prompt's own length.  It holds one layer's activations of
+        all rows, 4 bytes times 7 dim + 3 hidden + 2 n_heads * head_dim + 3 n_kv_heads * head_dim
+        a token, and the attention's scratch (cw_prompt_attention)."""
         m, ctx = self.m, self.ctx
         nh, nkv, hd = m.n_heads, m.n_kv_heads, m.head_dim
         news = np.array([0 if s.stored else s.n_prompt - 1 for s in self.sessions])
@@ -204,7 +213,8 @@ class TreeDecoder:
                                    n_req=n, n_rows=T, n_heads=nh, n_kv=nkv, head_dim=hd)()
             return o
 
-        self._layers([t for s, c in zip(self.sessions, news) for t in s.tokens[:c]], attend)
+        at["x"] = ctx.empty_persistent(T * m.dim)
+        self._layers([t for s, c in zip(self.sessions, news) for t in s.tokens[:c]], attend, at["x"])
         ctx.sync()
         for b in at.values():
             b.release()
