@@ -8,7 +8,7 @@ would have produced itself are kept, so the tokens are those of plain greedy dec
 (model.generate_op_by_op) in fewer steps.  Drafts come from the session's own text:
 what followed the last occurrences of its last tokens.
 
-TreeDecoder.prefill takes whole prompts in at once, whatever their lengths: per
+TreeDecoder.prefill takes whole prompts in at once, each of its own length up to max_seq: per
 layer cw_norm_rope writes their keys and values and cw_prompt_attention lets each token see
 its own prompt up to itself.  With penalties, biases or a set of allowed tokens
 cw_adjust_logits chooses the step's tokens.
@@ -195,6 +195,8 @@ class TreeDecoder:
         a token, and the attention's scratch (cw_prompt_attention)."""
         m, ctx = self.m, self.ctx
         nh, nkv, hd = m.n_heads, m.n_kv_heads, m.head_dim
+        if any(s.n_prompt > self.max_seq for s in self.sessions):
+            raise ValueError("a prompt exceeds max_seq")
         news = np.array([0 if s.stored else s.n_prompt - 1 for s in self.sessions])
         T, n = int(news.sum()), len(news)
         if T == 0:

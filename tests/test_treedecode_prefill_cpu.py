@@ -101,3 +101,12 @@ def test_activations_of_one_layer_are_held(decoder):
         added.append(d.ctx.most - before)
         assert sum(b.n for b in d.ctx.live.values()) == before
     assert added[0] == added[1] == added[2]
+
+
+def test_prompts_past_max_seq_are_refused(decoder):
+    d = decoder([[1] * 20, [2] * 65])
+    before = dict(d.ctx.live)
+    with pytest.raises(ValueError, match="max_seq"):
+        d.prefill()
+    assert d.ctx.live == before and not d.ctx.slots and [s.stored for s in d.sessions] == [0, 0]
+    decoder([[1] * 64]).prefill()
