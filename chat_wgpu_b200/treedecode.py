@@ -215,11 +215,14 @@ class TreeDecoder:
                                    n_req=n, n_rows=T, n_heads=nh, n_kv=nkv, head_dim=hd)()
             return o
 
-        at["x"] = ctx.empty_persistent(T * m.dim)
-        self._layers([t for s, c in zip(self.sessions, news) for t in s.tokens[:c]], attend, at["x"])
-        ctx.sync()
-        for b in at.values():
-            b.release()
+        try:
+            at["x"] = ctx.empty_persistent(T * m.dim)
+            self._layers([t for s, c in zip(self.sessions, news) for t in s.tokens[:c]], attend,
+                         at["x"])
+            ctx.sync()
+        finally:
+            for b in at.values():
+                b.release()
         for s, c in zip(self.sessions, news):
             s.stored += int(c)
 

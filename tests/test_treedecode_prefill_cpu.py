@@ -110,3 +110,23 @@ def test_prompts_past_max_seq_are_refused(decoder):
         d.prefill()
     assert d.ctx.live == before and not d.ctx.slots and [s.stored for s in d.sessions] == [0, 0]
     decoder([[1] * 64]).prefill()
+
+
+def test_a_failed_launch_leaves_nothing(decoder):
+    d = decoder([[1] * 20, [2] * 7])
+    before = dict(d.ctx.live)
+    place = d._place
+
+    def late(*a):
+        at = place(*a)
+        d.fails.append(1)
+        return at
+
+    d._place = late
+    with pytest.raises(RuntimeError, match="launch"):
+        d.prefill()
+    assert d.ctx.live == before and [s.stored for s in d.sessions] == [0, 0]
+    d.fails.clear()
+    d._place = place
+    d.prefill()
+    assert [s.stored for s in d.sessions] == [19, 6]
