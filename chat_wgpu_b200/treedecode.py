@@ -227,7 +227,8 @@ class TreeDecoder:
             s.stored += int(c)
 
     def _choose(self, logits, histories, leads):
-        """The token of each row of logits, which become the adjusted ones."""
+        """The token of each row of logits, which become the adjusted ones; without penalties
+        the histories are not read."""
         ctx, T, vocab = self.ctx, len(histories), self.m.vocab
         flat = lambda lists: [x for y in lists for x in y]  # noqa: E731
         begin = lambda lists: np.concatenate([[0], np.cumsum([len(x) for x in lists])])  # noqa: E731
@@ -271,16 +272,20 @@ class TreeDecoder:
             c, m = len(open_), len(open_) + len(drafts)
             v = np.zeros((m, m), bool)
             depth = list(range(c))
-            text = []
+            # histories of the rows that tokens are picked from, the last open one and the drafts
+            counted = self.penalties is not None and c > 0 and s.stored + c == len(s.tokens)
+            text = [[] for _ in range(m)]
+            if counted:
+                text[c - 1] = list(s.tokens)
             for i in range(c):
                 v[i, :i + 1] = True
-                text.append(s.tokens[:s.stored + i + 1])
             for j, (parent, token) in enumerate(drafts):
                 up = c - 1 if parent < 0 else c + parent
                 v[c + j] = v[up]
                 v[c + j, c + j] = True
                 depth.append(depth[up] + 1)
-                text.append(text[up] + [token])
+                if counted:
+                    text[c + j] = text[up] + [token]
             histories += text
             leads += [s.n_prompt] * m
             rows += open_ + [t for _, t in drafts]
