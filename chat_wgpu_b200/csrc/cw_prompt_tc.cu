@@ -1242,13 +1242,20 @@ __global__ void __launch_bounds__(PS_WARPS * 32)
 
 bool prompt_tc_takes(const PromptArgs& a, uint32_t type) {
     if (a.G > 128 || !(a.scale > 0.f)) return false;
-    if (type == CW_GGUF_F32)  // any place and stride; the pairs are laid out anew
-        // (short prompts, and single rows over many keys, whose pairs are formed for little, are
-        // faster on the f32 kernel; us there and here, 16/8 heads: a prompt of 128 tokens 27 and
-        // 34, 192 tokens 38 and 35, eight of 128 40 and 52; a row after 1000 keys 57 and 46,
-        // after 4000 54 and 62, eight after 2000 93 and 172; 16 rows after 4000 65 and 62)
+    if (type == CW_GGUF_F32)
+        // Any place and stride; the pairs are laid out anew.  Short requests are faster on the
+        // f32 kernel, and so are few rows over many keys, whose pairs are formed for little (us
+        // there and here, heads of 128: with 16/8 heads a prompt of 128 tokens 28 and 33, of 192
+        // 39 and 35, 32 of 64 47 and 79, 32 of 128 125 and 129; eight rows after 500 keys each 27
+        // and 62, 32 after 300 53 and 119, 128 times four after 1000 650 and 1130, a row after
+        // 1000 57 and 46, after 4000 54 and 64, 16 after 4000 62 and 65; with 32/8 heads 32 prompts
+        // of 128 219 and 191, with 4/2 heads 42 and 54; 128 rows after 1000 645 and 1110 with
+        // either 16/8 or 32/8 heads, 167 and 312 with 4/2).  The lengths are means, all that the
+        // host knows: 4096 tokens beside 30 requests of one token take 2090 there and 300
+        // here.  (Requests told apart on the device ended that, but the launches that then found
+        // nothing made even batches slower: 32 prompts of 64 47 and 68, 128 of 16 48 and 70.)
         return a.D <= 128 && (long long)a.n_keys >= 160ll * a.n_req &&
-               (a.n_rows >= 8ll * a.n_req || (long long)a.n_keys < 2000ll * a.n_req);
+               (a.n_rows >= 8ll * a.n_req || (a.n_req == 1 && a.n_keys < 2000));
     const long long strides = (a.n_rows > 1 ? a.q_stride : 0) |
                               (a.n_keys > 1 ? a.k_stride | a.v_stride : 0);
     return a.D % 8 == 0 && strides % 8 == 0 &&
