@@ -67,6 +67,10 @@ class TreeDecoder:
             raise ValueError("every session needs a prompt")
         if not 1 <= chunk <= 1024:
             raise ValueError(f"chunk {chunk}: rows of a session in a step, 1..1024")
+        if allowed is not None:
+            allowed = np.array(sorted(allowed), np.int64)
+            if allowed.size == 0 or allowed[0] < 0 or allowed[-1] >= model.vocab:
+                raise ValueError(f"allowed: at least one token, each in 0..{model.vocab - 1}")
         self.m, self.ctx, self.page, self.chunk, self.draft = model, model.ctx, page_size, chunk, draft
         self.sessions = [Session(p) for p in prompts]
         self.max_seq = max_seq
@@ -84,7 +88,7 @@ class TreeDecoder:
         self.penalties, self.biases, self.mask = penalties, dict(biases or {}), None
         if allowed is not None:
             bits = np.zeros(-(-model.vocab // 32) * 32, np.uint8)
-            bits[list(allowed)] = 1
+            bits[allowed] = 1
             self.mask = self.ctx.storage_u32(np.packbits(bits, bitorder="little").view(np.uint32))
 
     def close(self) -> None:
