@@ -342,8 +342,8 @@ __global__ void __launch_bounds__(LG_THREADS, 2) k_adjust_logits(const __grid_co
 template <typename T> static int adjust_launch(cw_ctx* ctx, LogitArgs& a, bool wide) {
     auto kern = wide ? k_adjust_logits<T, true> : k_adjust_logits<T, false>;
     // up to 16 CTAs to a row (one cluster), no slice shorter than a pass of the threads; with
-    // many rows fewer, so that a row's lists are gone through less often (256 rows of 151936: 56
-    // us with two CTAs to a row, 68 with four, 63 with one)
+    // many rows fewer, so that a row's lists are gone through less often (256 rows of 151936: 61
+    // us with two CTAs to a row, 74 with four, 65 with one)
     const int span = a.vocab + 16, many = std::max(1, 4 * ctx->sm_count / a.n_rows);
     const int ctas = std::max(1, std::min({16, many, span / (LG_THREADS * 4)}));
     a.slice = std::min(128 * 1024, ((span + ctas - 1) / ctas + 31) / 32 * 32);

@@ -33,10 +33,12 @@ struct NormRopeArgs {
 
 constexpr int NR_THREADS = 256;
 // A head's loads are in flight while the one before is worked on, three blocks to an SM and
-// at most 12 heads to a lane: 32768 bf16 rows of 32 + 8 + 8 heads in 163 us (872 MB, 5.4
-// TB/s; 168 before results were converted two at a time).  Two heads at a time took 175 us,
-// four blocks an SM (64 registers) 191, 24 heads to a lane 166 and 64 189, streaming stores
-// 166, the arithmetic in paired f32 instructions no different.
+// at most 12 heads to a lane: 32768 bf16 rows of 32 + 8 + 8 heads in 168 us (872 MB, 5.2
+// TB/s); 16384 f32 rows of 16 + 8 + 8 heads with k rows besides in 108 us (5.6 TB/s), 4096 in
+// 31, 128 in 4.2.  The choices were made on the bf16 rows where this form took 163 us: 168
+// before results were converted two at a time, 175 with two heads in flight, 191 with four
+// blocks an SM (64 registers), 166 with 24 heads to a lane and 189 with 64, 166 with
+// streaming stores, the arithmetic in paired f32 instructions no different.
 constexpr int NR_PER = 12;
 
 // Two neighbours at once: one conversion instruction for 16-bit types.
@@ -198,7 +200,8 @@ template <typename T, int VEC, int C>
 static int norm_rope_go(cw_ctx* ctx, NormRopeArgs& a, bool half, int chunks) {
     a.lanes = 1;
     while (a.lanes * C < chunks) a.lanes *= 2;
-    // as many heads to a lane as still leave one full wave of threads
+    // as many heads to a lane as leave 2048 threads an SM (768 of them are resident at a time,
+    // so 2.7 waves): 1003 f16 rows of 8 + 4 + 4 heads of 256 run with one head to a lane, 2.3 waves
     const long long all = (long long)a.n_tokens * a.lanes * a.heads;
     const long long wave = (long long)ctx->sm_count * 2048;
     a.per = (int)std::max<long long>(1, std::min<long long>(all / wave, std::min(a.heads, NR_PER)));

@@ -1125,7 +1125,9 @@ static int pt_map(CUtensorMap* map, const void* base, bool bf, int dims_, int he
 // x 2^s = h + l to 22 bits, h and l f16, s by request and kv head (k, v) or by row and head
 // (q).  With the largest in [2^14, 2^15), what l drops is at most 2^-39 of the largest, or
 // 2^-22 of the value itself (what that asks of the values: PR_APART).  A warp takes a head
-// row, or for the magnitudes 32 of them.
+// row, or for the magnitudes 32 of them.  4096 tokens of 16/8 heads of 128: 28 us for the
+// magnitudes and 36 for the pairs of 252 (cold launches; 171 are the attention's, 6.5 the f32
+// kernel's look at what is left to it); both wait for their reads.
 constexpr int PS_WARPS = 8;
 constexpr int PS_ROWS = 8;  // rows of a warp in flight
 

@@ -451,10 +451,13 @@ typedef struct {
  * largest of its row and head.  Requests and kv heads that pairs cannot hold so (infinities,
  * NaN, magnitudes from 2^60 or below 2^-86, rows of k or v whose largest values are more
  * than 2^12 apart) run in f32 products, and so does everything else.  Starts that descend
- * or pass the buffers are cut to them and reported.  Uses a context-owned scratch that grows
- * on demand, in stream order: call once with a call's sizes before capturing it, and replay a
- * captured call before the context is destroyed and in order with the context's other prompt
- * attention calls. */
+ * or pass the buffers are cut to them and reported.  Which kernel a call takes goes by the mean
+ * lengths of its requests, all that the host knows: an f32 call of one long prompt among many
+ * short or empty requests runs in f32 products, seven times slower than by itself.  Uses a
+ * context-owned scratch that grows on demand, in stream order (for pairs as large as q, k and
+ * v together; a larger one is twice the old one at least, which stays until the context goes):
+ * call once with a call's sizes before capturing it, and replay a captured call before the
+ * context is destroyed and in order with the context's other prompt attention calls. */
 int cw_prompt_attention(cw_ctx* ctx, const cw_prompt_attn_args* args);
 
 typedef struct {
@@ -479,9 +482,11 @@ typedef struct {
  *   n > 0 times behind `prompts`: x = (x - frequency * n) - presence
  *   t in the row's bias list:     x = x + bias (the last entry of t holds)
  *   t not allowed by the mask:    x = -inf
- * out = x rounded to the type; best = the lowest index of out's largest value, NaN
- * left out, 0 where none is above -3.402823e38 (as cw_argmax).  out may be the logits
- * themselves where their rows are contiguous, and may not overlap anything else.
+ * Biases come after the penalties: a token that is both repeated and biased gets its bias
+ * whole.  Of a row whose penalties are 1, 0, 0 the history is not read.  out = x rounded to
+ * the type; best = the lowest index of out's largest value, NaN left out, 0 where none is
+ * above -3.402823e38 (as cw_argmax).  out may be the logits themselves where their rows are
+ * contiguous, and may not overlap anything else.
  * Tokens outside the vocabulary, starts that descend or pass their buffer and mask rows
  * past n_masks are skipped and reported (a row with such a mask row has no mask). */
 int cw_adjust_logits(cw_ctx* ctx, const cw_adjust_logits_args* args);
