@@ -97,15 +97,15 @@ __device__ __forceinline__ void prompt_check(const PromptArgs& a, int tid, int t
     if (bad) prompt_bad(a);
 }
 
-// Operands as pairs: values are multiplied by 2^s so that the largest, `bits`, lies in
-// [2^14, 2^15).  What is not finite, or so large that products could leave f32's range, is
-// left to the f32 kernel.  So are a request and kv head with rows of k or v (a token's head)
-// whose largest values are more than PR_APART powers of two apart: a pair loses up to 2^-39
-// of the largest in sight or out of it, which is then 2^-27 of any row's own largest, and a
-// weight 2^-38 of the heaviest, which times any row of v is then below 2^-25 of the heaviest
-// key's row.  (Rows of zeros are exact.)
+// Operands as pairs h + l: values are multiplied by 2^s so that the largest, `bits`, lies in
+// [2^14, 2^15), and l is kept 2^11 times as large.  What is not finite, or so large that
+// products could leave f32's range, is left to the f32 kernel.  So are a request and kv head
+// with rows of k or v (a token's head) whose largest values are more than PR_APART powers of
+// two apart: a pair loses up to 2^-50 of the largest in sight or out of it, which is then
+// 2^-34 of any row's own largest, and a weight 2^-49 of the heaviest, which times any row of v
+// is then below 2^-32 of the heaviest key's row.  (Rows of zeros are exact.)
 constexpr uint32_t PR_ODD = (127u + 60) << 23;
-constexpr uint32_t PR_APART = 12;
+constexpr uint32_t PR_APART = 16;
 // 2^s is at most 2^100 (k's and q's are multiplied together), so what is smaller than this is
 // left out as well, but for zeros.
 constexpr uint32_t PR_TINY = (127u - 86) << 23;

@@ -33,7 +33,10 @@
 // count instructions, not one unit's time.
 //
 // f32 (head_dim <= 128): x 2^s = h + l, s by request and kv head (k, v) or by row and head
-// (q), and each product is h h + h l + l h.  The tensor cores cut their f32 sums at each step
+// (q), and each product is h h + h l + l h, with l held 2^11 times as large and the sum of the
+// small products divided by that when h h begins (a small element's l would sink into f16's
+// subnormals: 2^-9 of an element 2^-30 of the largest was lost, and 2^-20 is now; no time
+// was).  The tensor cores cut their f32 sums at each step
 // by what they have grown to, so the small products come first and a tile's sums are added
 // to the row's by the threads (error against 64 bits at 4096 keys 7.1e-6 without either,
 // 6.8e-7 with both; a plain f32 form has 1.2e-6).  Bound by shared memory and the tensor
@@ -184,6 +187,22 @@ __device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
         "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// The same products with what the accumulator held before divided by 2^PT_LOW first.
+constexpr int PT_LOW = 11;
+__device__ __forceinline__ void pt_mma_ss_low(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, %4;\n\t}" ::"r"(d), "l"(a), "l"(b),
+        "r"(idesc), "n"(PT_LOW)
+        : "memory");
+}
+__device__ __forceinline__ void pt_mma_ts_low(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.eq.b32 p, 0, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, %4;\n\t}" ::"r"(d), "r"(a), "l"(b),
+        "r"(idesc), "n"(PT_LOW)
         : "memory");
 }
 // 32 bytes at a 32-byte boundary.
@@ -537,15 +556,17 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                 const uint32_t d = tmem + b * TCOLS + (NB == 2 ? 0 : sb * PT_KEYS);
                 TtPlace x = k;
                 // half h of q's columns times the stage at place x
-                auto product = [&](int h, const TtPlace& x, uint32_t more) {
+                auto product = [&](int h, const TtPlace& x, uint32_t more, bool low) {
                     const uint64_t dk = kv0 + ((x.stage * STAGE) >> 4);
                     const uint64_t dq = q0 + ((b * Z::QBLOCK + h * COLS * Z::QCOL) >> 4);
 #pragma unroll
                     for (int s = 0; s < COLS * 4; s++)
-                        if ((PAIR ? 0 : h * 8) + s < steps)
-                            umma_f16(d, dq + (((s >> 2) * Z::QCOL + (s & 3) * 32) >> 4),
-                                     dk + (((s >> 2) * tile.col + (s & 3) * 32) >> 4), id_s,
-                                     s > 0 ? 1u : more);
+                        if ((PAIR ? 0 : h * 8) + s < steps) {
+                            const uint64_t sq = dq + (((s >> 2) * Z::QCOL + (s & 3) * 32) >> 4);
+                            const uint64_t sk = dk + (((s >> 2) * tile.col + (s & 3) * 32) >> 4);
+                            if (PAIR && low && s == 0) pt_mma_ss_low(d, sq, sk, id_s);
+                            else umma_f16(d, sq, sk, id_s, s > 0 ? 1u : more);
+                        }
                 };
 #pragma unroll
                 for (int h = 0; h < HALVES; h++) {
@@ -553,12 +574,12 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                     ok = ok && wait(&bars->full[x.stage], x.phase);
                     tc_fence_after();
                     // pairs: low parts of q times the high ones of k, high ones of q times the
-                    // low ones of k, and the high ones of both last, since a sum is cut at each
-                    // step by what it has grown to
-                    if (ok) product(PAIR ? 1 - h : h, x, h > 0);
+                    // low ones of k, both 2^PT_LOW too large, and the high ones of both last,
+                    // since a sum is cut at each step by what it has grown to
+                    if (ok) product(PAIR ? 1 - h : h, x, h > 0, false);
                     x.next(STAGES);
                 }
-                if (PAIR && ok) product(0, k, 1);
+                if (PAIR && ok) product(0, k, 1, true);
                 if (!ok) return;
                 tc_commit(&bars->s_full[sb]);
                 if (i + 1 == t.b[b].hi) tc_commit(&bars->q_empty[b]);
@@ -599,8 +620,9 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                     }
                     if (PAIR && part) {  // high times high last, as for the scores
                         const uint64_t dv = kv0 + ((v.stage * STAGE) >> 4);
+                        pt_mma_ts_low(o, p, dv, id_o[0]);
 #pragma unroll
-                        for (int s = 0; s < PT_KEYS / 16; s++)
+                        for (int s = 1; s < PT_KEYS / 16; s++)
                             pt_mma_ts(o, p + (s >> 2) * (PT_KEYS / 2) + (s & 3) * 8,
                                       dv + ((s * 2 * tile.group) >> 4), id_o[0], 1);
                     }
@@ -782,7 +804,7 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
         const float log2e = 1.44269504088896341f;
         // the reference lies LIFT below the largest score that it was taken from, which may
         // grow by GROWN before the sums are rescaled: weights stay below 2^15.  Of pairs the
-        // heaviest is 2^13 at least, so that the others lose at most 2^-38 of it
+        // heaviest is 2^13 at least, so that the others lose at most 2^-49 of it
         constexpr float LIFT = PAIR ? 13.f : TT_LIFT<BF>, GROWN = PAIR ? 2.f : 8.f;
         const bool cap = a.softcap > 0.f;
         const float c0 = cap ? log2e : a.scale * log2e;
@@ -923,7 +945,8 @@ __global__ void __launch_bounds__(PtShape<HD, sizeof(T) == 4>::THREADS, 1)
                         p[j >> 1] = pt_pack<BF>(y0, y1);
                         if constexpr (PAIR) {
                             const float2 h = __half22float2(*(const __half2*)&p[j >> 1]);
-                            low[j >> 1] = pt_pack<BF>(y0 - h.x, y1 - h.y);
+                            constexpr float up = 1 << PT_LOW;
+                            low[j >> 1] = pt_pack<BF>((y0 - h.x) * up, (y1 - h.y) * up);
                         }
                     }
                     // the second 32 keys come first, whose weights may go over the first ones'
@@ -1122,9 +1145,9 @@ static int pt_map(CUtensorMap* map, const void* base, bool bf, int dims_, int he
 }
 
 // ---- f32 operands as pairs ---------------------------------------------------------
-// x 2^s = h + l to 22 bits, h and l f16, s by request and kv head (k, v) or by row and head
-// (q).  With the largest in [2^14, 2^15), what l drops is at most 2^-39 of the largest, or
-// 2^-22 of the value itself (what that asks of the values: PR_APART).  A warp takes a head
+// x 2^s = h + l to 22 bits, h and l 2^PT_LOW f16, s by request and kv head (k, v) or by row and
+// head (q).  With the largest in [2^14, 2^15), what is dropped is at most 2^-50 of the largest,
+// or 2^-22 of the value itself (what that asks of the values: PR_APART).  A warp takes a head
 // row, or for the magnitudes 32 of them.  4096 tokens of 16/8 heads of 128: 28 us for the
 // magnitudes and 36 for the pairs of 252 (cold launches; 171 are the attention's, 6.5 the f32
 // kernel's look at what is left to it); both wait for their reads.
@@ -1230,7 +1253,7 @@ __global__ void __launch_bounds__(PS_WARPS * 32)
         float y = x[e] * by;
         if (!(fabsf(y) < 65504.f)) y = 0.f;  // not used: the f32 kernel's
         hi[e] = __float2half_rn(y);
-        lo[e] = __float2half_rn(y - __half2float(hi[e]));
+        lo[e] = __float2half_rn((y - __half2float(hi[e])) * (1 << PT_LOW));
     }
     __half* to = out + w * 2 * W + lane * N;
     if constexpr (N == 4) {

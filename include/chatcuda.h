@@ -447,10 +447,10 @@ typedef struct {
  * multiples of 16 bytes, with at most 128 query heads per kv head and a positive scale,
  * run on the tcgen05 tensor cores (there the softmax weights are rounded to the type
  * before the product with v).  f32 with head_dim <= 128 runs there as pairs of f16 where
- * there are keys enough, at f32 accuracy: a value loses less than 2^-22 of it or 2^-27 of the
+ * there are keys enough, at f32 accuracy: a value loses less than 2^-22 of it or 2^-34 of the
  * largest of its row and head.  Requests and kv heads that pairs cannot hold so (infinities,
  * NaN, magnitudes from 2^60 or below 2^-86, rows of k or v whose largest values are more
- * than 2^12 apart) run in f32 products, and so does everything else.  Starts that descend
+ * than 2^16 apart) run in f32 products, and so does everything else.  Starts that descend
  * or pass the buffers are cut to them and reported.  Which kernel a call takes goes by the mean
  * lengths of its requests, all that the host knows: an f32 call of one long prompt among many
  * short or empty requests runs in f32 products, seven times slower than by itself.  Uses a
