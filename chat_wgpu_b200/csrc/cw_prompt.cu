@@ -7,9 +7,9 @@
 // scales the latter two when the maximum grows.  256 threads hold 64 x 64 scores as 4 x 4
 // blocks and 64 x D sums as 4 rows by D / 16 columns.  It takes what the tensor cores do not:
 // short f32 prompts (17 tokens of 16/8 heads in 9.5 us, of which its launch is 3), few f32
-// rows over many keys (eight after 500 in 27 us), f32 past 128 dims (4000 tokens of 8/4 heads of 256 in 2.15 ms: 31
-// TFLOP/s, bound by the latency of its reads, two warps to a scheduler), 16-bit rows at odd
-// places, and requests whose f32 values do not fit pairs.
+// rows over many keys (eight after 500 in 27 us), f32 past 128 dims (4000 tokens of 8/4 heads
+// of 256 in 2.15 ms: 31 TFLOP/s, bound by the latency of its reads, two warps to a scheduler),
+// 16-bit rows at odd places, and requests whose f32 values do not fit pairs.
 #include <math.h>
 
 #include <algorithm>
